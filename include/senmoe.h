@@ -27,6 +27,10 @@
  *                              build's expert-contiguous permutation)
  *   senmoe_layer_destroy    <- Drop of the MLX Param<Array>s (deepseek_v2.rs:408-413)
  *   senmoe_last_error       <- Exception::custom(...) text, utils/moe.rs:66-74
+ *   senmoe_linear           <- nn::Linear::forward, for weights left in 16 bits
+ *                              (deepseek_v2.rs:528), with the activation and the residual
+ *                              add that follow it, dense or grouped by expert
+ *   senmoe_linear_backward  <- (no counterpart: the reference does not train)
  *
  * Weight layout is MLX's affine-quantized layout, unchanged
  * (src/engine/mlx_native.rs:3381-3389, 3473-3477): for a [E, out, in]
@@ -327,6 +331,111 @@ int senmoe_gather_qmm(const void* x, int64_t x_rows, const uint32_t* w, const vo
 int senmoe_quantized_linear(const void* x, int64_t num_tokens, const uint32_t* w, const void* scales,
                             const void* biases, int64_t in_features, int64_t out_features, int32_t group_size,
                             int32_t bits, void* y, senmoe_stream_t stream);
+
+/* ---- Linear products over 16-bit weights, dense or grouped by expert, with
+ * their gradients.
+ *
+ *   z[s, :] = x[s, :] @ weight[e(s)]^T + bias[e(s)]          (fp32)
+ *   y[s, :] = epilogue(z[s, :]) + residual[s, :]             (rounded once)
+ *
+ * Every tensor is bf16, or every tensor is fp16; sums are fp32.  Row s
+ * belongs to group e when offsets[e] <= s < offsets[e + 1]: x holds its rows
+ * in expert order and offsets is senmoe_dispatch's (or a slice of it, the
+ * range of a rank's experts).  offsets == NULL is the dense product: one
+ * group holding every row.  Groups may be empty; rows outside
+ * [offsets[0], offsets[num_groups]) come out as zero.  offsets must not
+ * decrease and must lie in [0, rows]: values that do not are clamped on the
+ * device, so that nothing outside the tensors is touched, and the outputs of
+ * such a call mean nothing. */
+typedef enum SenMoeDtype { SENMOE_BF16 = 0, SENMOE_FP16 = 1 } SenMoeDtype;
+
+typedef enum SenMoeEpilogue {
+  SENMOE_EPI_NONE = 0,
+  SENMOE_EPI_RELU = 1,
+  SENMOE_EPI_SILU = 2,
+  SENMOE_EPI_GELU = 3,      /* z * Phi(z) */
+  SENMOE_EPI_GELU_TANH = 4, /* gelu_approx */
+  /* gated pairs: weight (and bias, preact) hold 2 * out_features rows, the
+   * gate's first; y = silu(gate) * up, or gelu_approx(gate) * up */
+  SENMOE_EPI_SWIGLU = 5,
+  SENMOE_EPI_GEGLU = 6
+} SenMoeEpilogue;
+
+/* Kernels of a linear product: 0 picks by shape and alignment.  The tcgen05
+ * kernels read their operands with TMA, so these need 16-byte aligned bases
+ * and row strides of a multiple of 8 elements; other operands run on the
+ * warp-MMA kernels that copy element by element. */
+typedef enum SenMoeLinearPath {
+  SENMOE_LINEAR_AUTO = 0,
+  SENMOE_LINEAR_ANY = 1,    /* any strides and alignments */
+  SENMOE_LINEAR_TCGEN05 = 2 /* SENMOE_ERR_UNSUPPORTED where TMA cannot read the operands */
+} SenMoeLinearPath;
+
+/* Strides are in elements; the innermost dimension is contiguous.  wide =
+ * out_features, or 2 * out_features for a gated pair. */
+typedef struct SenMoeLinear {
+  int32_t dtype;               /* SenMoeDtype */
+  int32_t epilogue;            /* SenMoeEpilogue */
+  int32_t num_groups;          /* E <= 1024; 1 when offsets is NULL */
+  int32_t path;                /* SenMoeLinearPath */
+  int64_t rows;                /* S < 2^31 */
+  int64_t in_features;
+  int64_t out_features;
+  const void* x;               /* [S, in] */
+  int64_t x_stride;
+  const void* weight;          /* [E, wide, in] */
+  int64_t weight_stride;       /* between rows */
+  int64_t weight_group_stride; /* between groups */
+  const int32_t* offsets;      /* device int32 [E + 1], or NULL */
+  const void* bias;            /* [E, wide] contiguous, or NULL */
+  const void* residual;        /* [S, out], or NULL */
+  int64_t residual_stride;
+  void* y;                     /* [S, out] */
+  int64_t y_stride;
+  void* preact;                /* z [S, wide] for the backward pass, or NULL */
+  int64_t preact_stride;
+} SenMoeLinear;
+int senmoe_linear(const SenMoeLinear* product, senmoe_stream_t stream);
+
+/* Gradients of the product above from dy (residual's is dy itself):
+ *   dz = dy * epilogue'(preact)   (dy itself for SENMOE_EPI_NONE; gated: both
+ *                                  halves), rounded to the tensors' type
+ *   dx[s, :] = dz[s, :] @ weight[e(s)]
+ *   dweight[e] = sum over e's rows of dz[s, :]^T x[s, :]
+ *   dbias[e]   = sum over e's rows of dz[s, :]
+ * Any of dx, dweight and dbias may be NULL.  Groups without rows get zero
+ * dweight and dbias, rows outside the groups zero dx.  The sums are taken in a fixed order:
+ * the same call gives the same bits.  workspace: device memory of at least
+ * senmoe_linear_backward_workspace(grad) bytes (16-byte aligned; NULL when
+ * that is 0), in use until the call's work on the stream is done. */
+typedef struct SenMoeLinearGrad {
+  int32_t dtype, epilogue, num_groups, path;
+  int64_t rows, in_features, out_features;
+  const void* dy;              /* [S, out] */
+  int64_t dy_stride;
+  const void* x;               /* [S, in]; for dweight */
+  int64_t x_stride;
+  const void* weight;          /* [E, wide, in]; for dx */
+  int64_t weight_stride, weight_group_stride;
+  const int32_t* offsets;
+  const void* preact;          /* [S, wide]; NULL for SENMOE_EPI_NONE */
+  int64_t preact_stride;
+  void* dx;                    /* [S, in], or NULL */
+  int64_t dx_stride;
+  void* dweight;               /* [E, wide, in], or NULL */
+  int64_t dweight_stride, dweight_group_stride;
+  void* dbias;                 /* [E, wide] contiguous, or NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+} SenMoeLinearGrad;
+/* Bytes of workspace the call needs, or a negative status. */
+int64_t senmoe_linear_backward_workspace(const SenMoeLinearGrad* grad);
+int senmoe_linear_backward(const SenMoeLinearGrad* grad, senmoe_stream_t stream);
+
+/* Synchronises `stream` and reports a bounded wait of the linear kernels
+ * that ran out on the current device since the last check
+ * (SENMOE_ERR_TIMEOUT). */
+int senmoe_linear_check(senmoe_stream_t stream);
 
 /* Allocation-free forward (no counterpart in the reference; this build adds
  * it for callers that cannot allocate device memory at call time: code inside

@@ -369,6 +369,11 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
 // no attribute calls.
 cudaError_t ensure_dynamic_smem(const void* kernel, size_t bytes);
 
+// The message of the calling thread's last failing call (senmoe_last_error),
+// for entry points outside layer.cu; set_failure returns `status`.
+int set_failure(int status, const char* message);
+void clear_failure();
+
 // sigmoid of a per-token logit, in place.
 cudaError_t launch_sigmoid_inplace(float* v, int n, cudaStream_t st);
 

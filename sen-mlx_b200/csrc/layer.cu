@@ -54,6 +54,15 @@ int fail(int status, const char* fmt, ...) {
   return status;
 }
 
+}  // namespace
+
+namespace senmoe {
+int set_failure(int status, const char* message) { return fail(status, "%s", message); }
+void clear_failure() { g_last_error.clear(); }
+}  // namespace senmoe
+
+namespace {
+
 #define SENMOE_CUDA(call)                                                                            \
   do {                                                                                               \
     cudaError_t e_ = (call);                                                                         \

@@ -1,0 +1,258 @@
+// linear.cu -- the C ABI of the 16-bit linear products (include/senmoe.h):
+// argument checks, the choice of kernels, and the steps of the backward pass.
+
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdio>
+
+#include "../../include/senmoe.h"
+#include "kernels.h"
+#include "linear.cuh"
+
+using namespace senmoe;
+
+namespace {
+
+int reject(int status, const char* fmt, ...) {
+  char buf[384];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return set_failure(status, buf);
+}
+
+int cuda_status(const char* what, cudaError_t e) {
+  if (e == cudaSuccess) return SENMOE_OK;
+  return reject(e == cudaErrorNotSupported ? SENMOE_ERR_UNSUPPORTED : SENMOE_ERR_CUDA, "%s: %s", what,
+                cudaGetErrorString(e));
+}
+
+constexpr int64_t kMaxDim = int64_t(1) << 30;
+
+// A matrix operand: rows x cols, row stride in elements.
+int check_matrix(const char* call, const char* name, const void* p, int64_t stride, int64_t cols) {
+  if (!p) return reject(SENMOE_ERR_BAD_ARG, "%s: %s is NULL", call, name);
+  if (reinterpret_cast<uintptr_t>(p) & 1) return reject(SENMOE_ERR_BAD_ARG, "%s: %s is not 2-byte aligned", call, name);
+  if (stride < cols || stride > (int64_t(1) << 40))
+    return reject(SENMOE_ERR_BAD_ARG, "%s: %s row stride %lld for rows of %lld elements", call, name,
+                  (long long)stride, (long long)cols);
+  return SENMOE_OK;
+}
+
+int check_vector(const char* call, const char* name, const void* p) {
+  if (reinterpret_cast<uintptr_t>(p) & 1) return reject(SENMOE_ERR_BAD_ARG, "%s: %s is not 2-byte aligned", call, name);
+  return SENMOE_OK;
+}
+
+// What forward and backward have in common; wide: rows of W.
+int check_shape(const char* call, int32_t dtype, int32_t epilogue, int32_t groups, int32_t path, int64_t rows,
+                int64_t in, int64_t out, const int32_t* offsets, int64_t* wide) {
+  if (dtype != SENMOE_BF16 && dtype != SENMOE_FP16)
+    return reject(SENMOE_ERR_UNSUPPORTED, "%s: dtype %d (bf16 and fp16 are supported)", call, dtype);
+  if (epilogue < SENMOE_EPI_NONE || epilogue > SENMOE_EPI_GEGLU)
+    return reject(SENMOE_ERR_UNSUPPORTED, "%s: epilogue %d", call, epilogue);
+  if (path < SENMOE_LINEAR_AUTO || path > SENMOE_LINEAR_TCGEN05)
+    return reject(SENMOE_ERR_BAD_ARG, "%s: path %d", call, path);
+  if (groups < 1 || (!offsets && groups != 1))
+    return reject(SENMOE_ERR_BAD_ARG, "%s: num_groups=%d%s", call, groups, offsets ? "" : " without offsets");
+  if (groups > kMaxGroups) return reject(SENMOE_ERR_UNSUPPORTED, "%s: num_groups=%d (at most %d)", call, groups, kMaxGroups);
+  if (reinterpret_cast<uintptr_t>(offsets) & 3) return reject(SENMOE_ERR_BAD_ARG, "%s: offsets is not 4-byte aligned", call);
+  if (rows < 0 || rows >= (int64_t(1) << 31))
+    return reject(SENMOE_ERR_BAD_ARG, "%s: rows=%lld", call, (long long)rows);
+  *wide = epilogue >= SENMOE_EPI_SWIGLU ? 2 * out : out;
+  if (in < 1 || out < 1 || in > kMaxDim || *wide > kMaxDim)
+    return reject(SENMOE_ERR_BAD_ARG, "%s: in_features=%lld out_features=%lld", call, (long long)in, (long long)out);
+  // the kernels count tiles, of 16 rows at least, in 32 bits
+  const int64_t cols = *wide > in ? *wide : in;
+  if (((rows + 15) / 16 + groups) * ((cols + 63) / 64) >= (int64_t(1) << 31) ||
+      groups * ((*wide + 63) / 64) * ((in + 63) / 64) >= (int64_t(1) << 31))
+    return reject(SENMOE_ERR_UNSUPPORTED, "%s: rows=%lld in_features=%lld out_features=%lld is too large", call,
+                  (long long)rows, (long long)in, (long long)out);
+  return SENMOE_OK;
+}
+
+int check_group_stride(const char* call, const char* name, int64_t group_stride, int64_t stride, int64_t rows,
+                       int64_t cols, int groups) {
+  if (groups > 1 && (group_stride < (rows - 1) * stride + cols || group_stride > (int64_t(1) << 44)))
+    return reject(SENMOE_ERR_BAD_ARG, "%s: %s group stride %lld", call, name, (long long)group_stride);
+  return SENMOE_OK;
+}
+
+int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path, cudaStream_t st) {
+  if (path == SENMOE_LINEAR_TCGEN05) return reject(SENMOE_ERR_UNSUPPORTED, "%s: tcgen05 path", call);
+  return cuda_status(call, launch_linear_any(a, p, st));
+}
+
+int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
+
+// Rows of a group are summed in so many parts: one for every 256 rows of the
+// mean group, so that a long single group is not left to a few blocks.
+int bias_splits(int64_t rows, int groups) {
+  const int64_t s = rows / groups / 256;
+  return static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+struct GradLayout {
+  int64_t dz_stride = 0, dz_bytes = 0, partial_bytes = 0;
+  int splits = 1;
+  int64_t total() const { return dz_bytes + partial_bytes; }
+};
+
+GradLayout grad_layout(const SenMoeLinearGrad& g, int64_t wide) {
+  GradLayout l;
+  if (g.epilogue != SENMOE_EPI_NONE) {  // dz in rows that TMA can read
+    l.dz_stride = (wide + 7) & ~int64_t(7);
+    l.dz_bytes = round16(g.rows * l.dz_stride * 2);
+  }
+  if (g.dbias) {
+    l.splits = bias_splits(g.rows, g.num_groups);
+    if (l.splits > 1) l.partial_bytes = round16(int64_t(g.num_groups) * l.splits * wide * 4);
+  }
+  return l;
+}
+
+}  // namespace
+
+extern "C" {
+
+int senmoe_linear(const SenMoeLinear* q, senmoe_stream_t stream) {
+  clear_failure();
+  const char* call = "linear";
+  if (!q) return reject(SENMOE_ERR_BAD_ARG, "%s: product is NULL", call);
+  int64_t wide = 0;
+  int rc = check_shape(call, q->dtype, q->epilogue, q->num_groups, q->path, q->rows, q->in_features, q->out_features,
+                       q->offsets, &wide);
+  if (rc) return rc;
+  if (q->rows == 0) return SENMOE_OK;
+  if ((rc = check_matrix(call, "x", q->x, q->x_stride, q->in_features))) return rc;
+  if ((rc = check_matrix(call, "weight", q->weight, q->weight_stride, q->in_features))) return rc;
+  if ((rc = check_group_stride(call, "weight", q->weight_group_stride, q->weight_stride, wide, q->in_features,
+                               q->num_groups)))
+    return rc;
+  if ((rc = check_matrix(call, "y", q->y, q->y_stride, q->out_features))) return rc;
+  if (q->residual && (rc = check_matrix(call, "residual", q->residual, q->residual_stride, q->out_features))) return rc;
+  if (q->preact && (rc = check_matrix(call, "preact", q->preact, q->preact_stride, wide))) return rc;
+  if ((rc = check_vector(call, "bias", q->bias))) return rc;
+
+  LinearArgs a{};
+  a.a = q->x;
+  a.a_stride = q->x_stride;
+  a.b = q->weight;
+  a.b_stride = q->weight_stride;
+  a.b_group_stride = q->weight_group_stride;
+  a.offsets = q->offsets;
+  a.groups = q->num_groups;
+  a.rows = q->rows;
+  a.n = static_cast<int>(wide);
+  a.k = static_cast<int>(q->in_features);
+  a.act = q->epilogue;
+  a.bias = q->bias;
+  a.residual = q->residual;
+  a.residual_stride = q->residual_stride;
+  a.out = q->y;
+  a.out_stride = q->y_stride;
+  a.preact = q->preact;
+  a.preact_stride = q->preact_stride;
+  a.bf16 = q->dtype == SENMOE_BF16;
+  return run_product(call, a, kProdForward, q->path, stream);
+}
+
+static int check_grad(const SenMoeLinearGrad* g, int64_t* wide) {
+  const char* call = "linear_backward";
+  if (!g) return reject(SENMOE_ERR_BAD_ARG, "%s: grad is NULL", call);
+  return check_shape(call, g->dtype, g->epilogue, g->num_groups, g->path, g->rows, g->in_features, g->out_features,
+                     g->offsets, wide);
+}
+
+int64_t senmoe_linear_backward_workspace(const SenMoeLinearGrad* g) {
+  clear_failure();
+  int64_t wide = 0;
+  const int rc = check_grad(g, &wide);
+  return rc ? -int64_t(rc) : grad_layout(*g, wide).total();
+}
+
+int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
+  clear_failure();
+  const char* call = "linear_backward";
+  int64_t wide = 0;
+  int rc = check_grad(g, &wide);
+  if (rc) return rc;
+  const bool some = g->rows > 0, act = g->epilogue != SENMOE_EPI_NONE;
+  const int E = g->num_groups;
+  if (some && (rc = check_matrix(call, "dy", g->dy, g->dy_stride, g->out_features))) return rc;
+  if (some && act && (rc = check_matrix(call, "preact", g->preact, g->preact_stride, wide))) return rc;
+  if (some && g->dx) {
+    if ((rc = check_matrix(call, "dx", g->dx, g->dx_stride, g->in_features))) return rc;
+    if ((rc = check_matrix(call, "weight", g->weight, g->weight_stride, g->in_features))) return rc;
+    if ((rc = check_group_stride(call, "weight", g->weight_group_stride, g->weight_stride, wide, g->in_features, E)))
+      return rc;
+  }
+  if (g->dweight) {
+    if (some && (rc = check_matrix(call, "x", g->x, g->x_stride, g->in_features))) return rc;
+    if ((rc = check_matrix(call, "dweight", g->dweight, g->dweight_stride, g->in_features))) return rc;
+    if ((rc = check_group_stride(call, "dweight", g->dweight_group_stride, g->dweight_stride, wide, g->in_features, E)))
+      return rc;
+  }
+  if ((rc = check_vector(call, "dbias", g->dbias))) return rc;
+  const GradLayout l = grad_layout(*g, wide);
+  if (l.total() > 0 && (!g->workspace || g->workspace_bytes < l.total()))
+    return reject(SENMOE_ERR_BAD_ARG, "%s: workspace of %lld bytes, %lld needed", call,
+                  g->workspace ? (long long)g->workspace_bytes : 0ll, (long long)l.total());
+  if (reinterpret_cast<uintptr_t>(g->workspace) & 15)
+    return reject(SENMOE_ERR_BAD_ARG, "%s: workspace is not 16-byte aligned", call);
+
+  LinearGradArgs ga{};
+  ga.dy = g->dy;
+  ga.dy_stride = g->dy_stride;
+  ga.preact = act ? g->preact : nullptr;
+  ga.preact_stride = g->preact_stride;
+  ga.offsets = g->offsets;
+  ga.groups = E;
+  ga.rows = g->rows;
+  ga.n = static_cast<int>(wide);
+  ga.act = g->epilogue;
+  ga.dz = g->workspace;
+  ga.dz_stride = l.dz_stride;
+  ga.dbias = g->dbias;
+  ga.partial = reinterpret_cast<float*>(static_cast<char*>(g->workspace) + l.dz_bytes);
+  ga.splits = l.splits;
+  ga.bf16 = g->dtype == SENMOE_BF16;
+  if (some && act && (rc = cuda_status(call, launch_act_backward(ga, stream)))) return rc;
+
+  LinearArgs a{};
+  a.a = act ? ga.dz : g->dy;
+  a.a_stride = act ? l.dz_stride : g->dy_stride;
+  a.offsets = g->offsets;
+  a.groups = E;
+  a.rows = g->rows;
+  a.n = static_cast<int>(wide);
+  a.k = static_cast<int>(g->in_features);
+  a.bf16 = ga.bf16;
+  if (some && g->dx) {
+    a.b = g->weight;
+    a.b_stride = g->weight_stride;
+    a.b_group_stride = g->weight_group_stride;
+    a.out = g->dx;
+    a.out_stride = g->dx_stride;
+    if ((rc = run_product(call, a, kProdInput, g->path, stream))) return rc;
+  }
+  if (g->dweight) {
+    a.b = g->x;
+    a.b_stride = g->x_stride;
+    a.out = g->dweight;
+    a.out_stride = g->dweight_stride;
+    a.out_group_stride = g->dweight_group_stride;
+    if ((rc = run_product(call, a, kProdWeight, g->path, stream))) return rc;
+  }
+  if (g->dbias && (rc = cuda_status(call, launch_bias_grad(ga, stream)))) return rc;
+  return SENMOE_OK;
+}
+
+int senmoe_linear_check(senmoe_stream_t stream) {
+  clear_failure();
+  return cuda_status("linear_check", cudaStreamSynchronize(stream));
+}
+
+}  // extern "C"

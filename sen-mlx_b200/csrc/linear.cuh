@@ -1,0 +1,207 @@
+// linear.cuh -- what the 16-bit linear product kernels share: their
+// arguments, the epilogue's activations with their derivatives, and the table
+// of row groups.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace senmoe {
+
+// Values of SenMoeEpilogue (include/senmoe.h).
+enum LinearAct : int {
+  kActNone = 0,
+  kActRelu = 1,
+  kActSilu = 2,
+  kActGelu = 3,      // z * Phi(z)
+  kActGeluTanh = 4,  // its tanh form
+  kActSwiglu = 5,    // silu(gate) * up
+  kActGeglu = 6,     // tanh-form gelu(gate) * up
+};
+inline __host__ __device__ bool act_gated(int act) { return act >= kActSwiglu; }
+
+// The three products of a linear map, each C[i, j] = sum_k A(i, k) B(j, k):
+//   kProdForward  i = row of x,   j = row of W,    k = input feature
+//   kProdInput    i = row of dz,  j = input feature, k = row of W     (dx)
+//   kProdWeight   i = row of W,   j = input feature, k = row of the group (dW)
+enum LinearProduct : int { kProdForward = 0, kProdInput = 1, kProdWeight = 2 };
+
+constexpr int kMaxGroups = 1024;
+
+// One product.  a is x (forward) or dz; b is W (forward, dx) or x (dW); all
+// row-major with the given element strides between rows.  offsets null: one
+// group holding every row.
+struct LinearArgs {
+  const void* a;
+  const void* b;
+  int64_t a_stride, b_stride, b_group_stride;  // b_group_stride: W's, forward and dx
+  const int32_t* offsets;                      // [groups + 1]
+  int groups;
+  int64_t rows;                                // of x and dz
+  int n, k;                                    // W's rows (gate and up: both) and columns
+  int act;                                     // forward only
+  const void* bias;                            // [groups, n] or null
+  const void* residual;
+  int64_t residual_stride;
+  void* out;                                   // y, dx or dW
+  int64_t out_stride, out_group_stride;        // out_group_stride: dW's
+  void* preact;                                // forward: z before the activation, or null
+  int64_t preact_stride;
+  int bf16;                                    // 1: bf16, 0: fp16
+};
+
+// 16-bit values by their bit patterns.
+template <bool BF16> __device__ __forceinline__ float to_f32(uint16_t v) {
+  if constexpr (BF16) return bf16_bits_to_f32(v);
+  else return __half2float(__ushort_as_half(v));
+}
+template <bool BF16> __device__ __forceinline__ uint16_t from_f32(float v) {
+  if constexpr (BF16) return f32_to_bf16_bits(v);
+  else return __half_as_ushort(__float2half_rn(v));
+}
+
+// Activations in fp32.  The result is rounded once, to 16 bits, so the
+// intrinsics' few units in the last place of fp32 do not show.
+// gelu's tanh form 0.5 z (1 + tanh(a)) equals z / (1 + exp(-2a)), which has
+// one exponential and keeps its relative precision in the lower tail.
+__device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ float gelu_arg2(float z) {  // 2a, a = sqrt(2/pi) (z + 0.044715 z^3)
+  return 1.5957691216057308f * (z + 0.044715f * z * z * z);
+}
+__device__ __forceinline__ float act_value(int act, float z) {
+  switch (act) {
+    case kActRelu: return z > 0.0f ? z : (z != z ? z : 0.0f);
+    case kActSilu: case kActSwiglu: return __fdividef(z, 1.0f + __expf(-z));
+    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
+    case kActGeluTanh: case kActGeglu: return __fdividef(z, 1.0f + __expf(-gelu_arg2(z)));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_slope(int act, float z) {
+  switch (act) {
+    case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
+    case kActSilu: case kActSwiglu: {
+      const float s = logistic(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    case kActGelu:  // Phi(z) + z phi(z)
+      return 0.5f * (1.0f + erff(z * 0.7071067811865476f)) + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    case kActGeluTanh: case kActGeglu: {  // s = (1 + tanh a) / 2: s + 2 z s (1 - s) a'
+      const float s = logistic(gelu_arg2(z));
+      return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
+    }
+    default: return 1.0f;
+  }
+}
+
+// Row range of every group, made monotone and clamped to [0, rows] (whatever
+// offsets holds, no access leaves the operands), and the prefix sums of the
+// groups' chunks of `chunk` rows.  s_off and s_pre: groups + 1 ints of shared
+// memory each; s_tot: 64 ints.  Every thread of the block calls it; it ends
+// with __syncthreads.
+__device__ __forceinline__ void group_table(const int32_t* __restrict__ offsets, int groups, int64_t rows, int chunk,
+                                            int* s_off, int* s_pre, int* s_tot) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = (blockDim.x + 31) >> 5;
+  if (!offsets) {
+    if (tid == 0) {
+      s_off[0] = s_pre[0] = 0;
+      s_off[1] = static_cast<int>(rows);
+      s_pre[1] = static_cast<int>((rows + chunk - 1) / chunk);
+    }
+    __syncthreads();
+    return;
+  }
+  // one pass for the running maximum of the offsets, one for the chunk sums
+  const int n = groups + 1, per = (n + blockDim.x - 1) / blockDim.x;
+  const int first = min(tid * per, n), last = min(first + per, n);
+  const int cap = static_cast<int>(rows);
+  int m = 0;
+  for (int i = first; i < last; ++i) {
+    m = max(m, min(max(offsets[i], 0), cap));
+    s_off[i] = m;
+  }
+  int v = m;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = max(v, u);
+  }
+  if (lane == 31) s_tot[warp] = v;
+  int before = __shfl_up_sync(0xffffffffu, v, 1);
+  if (lane == 0) before = 0;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) before = max(before, s_tot[w]);
+  for (int i = first; i < last; ++i) s_off[i] = max(s_off[i], before);
+  __syncthreads();
+  int sum = 0;
+  for (int i = first; i < last; ++i) {
+    s_pre[i] = sum;  // chunks of this thread's groups before i
+    if (i < groups) sum += (s_off[i + 1] - s_off[i] + chunk - 1) / chunk;
+  }
+  v = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) s_tot[32 + warp] = v;
+  int base = v - sum;
+  __syncthreads();
+  for (int w = 0; w < warp && w < nw; ++w) base += s_tot[32 + w];
+  for (int i = first; i < last; ++i) s_pre[i] += base;
+  __syncthreads();
+}
+
+// The group whose chunks include chunk c: the last e with s_pre[e] <= c and chunks of its own.
+__device__ __forceinline__ int group_of(const int* s_pre, int groups, int c) {
+  int lo = 0, hi = groups;  // s_pre[lo] <= c < s_pre[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s_pre[mid] <= c) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Rows that no group holds (before the first offset, after the last) are
+// zero.  All threads of block `block` of `blocks`.
+__device__ __forceinline__ void zero_uncovered(const int* s_off, int groups, int64_t rows, uint16_t* out,
+                                               int64_t stride, int cols, int block, int blocks) {
+  const int64_t head = s_off[0], tail = s_off[groups];
+  const int64_t n = head + (rows - tail);
+  for (int64_t i = block; i < n; i += blocks) {
+    uint16_t* row = out + (i < head ? i : tail + (i - head)) * stride;
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) row[c] = 0;
+  }
+}
+
+// ------------------------------------------------------------ launchers
+// Any strides and alignments (linear_any.cu).
+cudaError_t launch_linear_any(const LinearArgs& a, LinearProduct p, cudaStream_t st);
+
+// dz = dy * act'(z) in 16 bits, and the row sums over each group (the bias
+// gradient); see linear_grad.cu.
+struct LinearGradArgs {
+  const void* dy;
+  int64_t dy_stride;
+  const void* preact;       // null: no activation, dz is dy
+  int64_t preact_stride;
+  const int32_t* offsets;
+  int groups;
+  int64_t rows;
+  int n;                    // columns of dz (gate and up: both)
+  int act;
+  void* dz;                 // [rows, dz_stride]
+  int64_t dz_stride;
+  void* dbias;              // [groups, n] or null
+  float* partial;           // [groups, splits, n] when splits > 1
+  int splits;
+  int bf16;
+};
+cudaError_t launch_act_backward(const LinearGradArgs& a, cudaStream_t st);
+cudaError_t launch_bias_grad(const LinearGradArgs& a, cudaStream_t st);
+
+}  // namespace senmoe

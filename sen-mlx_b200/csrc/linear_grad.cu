@@ -1,0 +1,189 @@
+// linear_grad.cu -- the elementwise and column-sum parts of the linear
+// products' backward pass.
+//
+// act_backward: dz = dy * act'(z) (gated: dg = dy * u * act'(g), du = dy *
+// act(g)), evaluated in fp32 and rounded once to the operands' 16-bit type,
+// because dz is an operand of both gradient products on the 16-bit tensor
+// cores.  The rounding (at most 2^-8 of the value in bf16, 2^-11 in fp16) is independent
+// from element to element and so adds to a gradient about as much as the
+// gradient's own rounding does.
+//
+// bias_grad: db[e] = sum of dz's rows of group e, in fp32 and in a fixed
+// order (rows strided over 8 warps, then warps, then splits), so repeated
+// calls agree bit for bit.
+
+#include "linear.cuh"
+
+namespace senmoe {
+namespace {
+
+constexpr int kActThreads = 256;
+
+template <bool BF16> __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = to_f32<BF16>(static_cast<uint16_t>(w[i]));
+    f[2 * i + 1] = to_f32<BF16>(static_cast<uint16_t>(w[i] >> 16));
+  }
+}
+template <bool BF16> __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = uint32_t(from_f32<BF16>(f[2 * i])) | (uint32_t(from_f32<BF16>(f[2 * i + 1])) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// V columns a thread: 8 (16-byte accesses) where every row starts on a
+// 16-byte boundary, else 1.
+template <bool BF16, int V>
+__global__ void __launch_bounds__(kActThreads) act_backward_kernel(const LinearGradArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const bool gated = act_gated(a.act);
+  const int cols = gated ? a.n / 2 : a.n, per_row = (cols + V - 1) / V;
+  const uint16_t* dy = static_cast<const uint16_t*>(a.dy);
+  const uint16_t* pre = static_cast<const uint16_t*>(a.preact);
+  uint16_t* dz = static_cast<uint16_t*>(a.dz);
+  const int64_t total = a.rows * per_row;
+  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kActThreads + threadIdx.x; it < total;
+       it += static_cast<int64_t>(gridDim.x) * kActThreads) {
+    const int64_t r = it / per_row;
+    const int c = static_cast<int>(it - r * per_row) * V;
+    const uint16_t* py = dy + r * a.dy_stride + c;
+    const uint16_t* pz = pre + r * a.preact_stride + c;
+    uint16_t* po = dz + r * a.dz_stride + c;
+    float d[V], z[V], u[V];
+    if constexpr (V == 8) {
+      const uint4 vy = *reinterpret_cast<const uint4*>(py), vz = *reinterpret_cast<const uint4*>(pz);
+      if (gated) {
+        const uint4 vu = *reinterpret_cast<const uint4*>(pz + cols);
+        unpack8<BF16>(vu, u);
+      }
+      unpack8<BF16>(vy, d);
+      unpack8<BF16>(vz, z);
+    } else {
+      d[0] = to_f32<BF16>(*py);
+      z[0] = to_f32<BF16>(*pz);
+      if (gated) u[0] = to_f32<BF16>(pz[cols]);
+    }
+    float g[V], du[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      g[i] = d[i] * act_slope(a.act, z[i]);
+      if (gated) {
+        g[i] = d[i] * u[i] * act_slope(a.act, z[i]);
+        du[i] = d[i] * act_value(a.act, z[i]);
+      }
+    }
+    if constexpr (V == 8) {
+      *reinterpret_cast<uint4*>(po) = pack8<BF16>(g);
+      if (gated) *reinterpret_cast<uint4*>(po + cols) = pack8<BF16>(du);
+    } else {
+      *po = from_f32<BF16>(g[0]);
+      if (gated) po[cols] = from_f32<BF16>(du[0]);
+    }
+  }
+}
+
+constexpr int kSumCols = 64;  // columns of a block: two a lane
+
+template <bool BF16>
+__global__ void __launch_bounds__(256) bias_grad_kernel(const LinearGradArgs a, const uint16_t* src, int64_t stride,
+                                                        bool pairs) {
+  __shared__ int s_off[kMaxGroups + 1], s_pre[kMaxGroups + 1], s_tot[64];
+  __shared__ float s_sum[8][kSumCols];
+  pdl_wait();
+  pdl_launch_dependents();
+  group_table(a.offsets, a.groups, a.rows, 1, s_off, s_pre, s_tot);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col_blocks = (a.n + kSumCols - 1) / kSumCols;
+  const int64_t items = static_cast<int64_t>(a.groups) * a.splits * col_blocks;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int cb = static_cast<int>(it % col_blocks);
+    const int es = static_cast<int>(it / col_blocks), e = es / a.splits, sp = es - e * a.splits;
+    const int cnt = s_off[e + 1] - s_off[e], per = (cnt + a.splits - 1) / a.splits;
+    const int r0 = min(sp * per, cnt), r1 = min(r0 + per, cnt);
+    const int c = cb * kSumCols + 2 * lane;
+    float x0 = 0.0f, x1 = 0.0f;
+    if (c < a.n) {
+      const uint16_t* p = src + static_cast<int64_t>(s_off[e]) * stride + c;
+      const bool two = c + 1 < a.n;
+#pragma unroll 4
+      for (int r = r0 + warp; r < r1; r += 8) {
+        const uint16_t* q = p + r * stride;
+        if (pairs && two) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(q);
+          x0 += to_f32<BF16>(static_cast<uint16_t>(w));
+          x1 += to_f32<BF16>(static_cast<uint16_t>(w >> 16));
+        } else {
+          x0 += to_f32<BF16>(q[0]);
+          if (two) x1 += to_f32<BF16>(q[1]);
+        }
+      }
+    }
+    s_sum[warp][2 * lane] = x0;
+    s_sum[warp][2 * lane + 1] = x1;
+    __syncthreads();
+    const int col = cb * kSumCols + threadIdx.x;
+    if (threadIdx.x < kSumCols && col < a.n) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) v += s_sum[w][threadIdx.x];
+      if (a.splits > 1)
+        a.partial[static_cast<int64_t>(es) * a.n + col] = v;
+      else
+        static_cast<uint16_t*>(a.dbias)[static_cast<int64_t>(e) * a.n + col] = from_f32<BF16>(v);
+    }
+    __syncthreads();
+  }
+}
+
+template <bool BF16> __global__ void __launch_bounds__(256) bias_join_kernel(const LinearGradArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t total = static_cast<int64_t>(a.groups) * a.n;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t e = i / a.n, c = i - e * a.n;
+    float v = 0.0f;
+    for (int s = 0; s < a.splits; ++s) v += a.partial[(e * a.splits + s) * a.n + c];
+    static_cast<uint16_t*>(a.dbias)[i] = from_f32<BF16>(v);
+  }
+}
+
+bool on16(const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 8 == 0; }
+
+unsigned grid_for(int64_t items, int64_t cap) {
+  const int64_t g = items < cap ? items : cap;
+  return static_cast<unsigned>(g < 1 ? 1 : g);
+}
+
+}  // namespace
+
+cudaError_t launch_act_backward(const LinearGradArgs& a, cudaStream_t st) {
+  const int cols = act_gated(a.act) ? a.n / 2 : a.n;
+  const bool wide = cols % 8 == 0 && on16(a.dy, a.dy_stride) && on16(a.preact, a.preact_stride) &&
+                    on16(a.dz, a.dz_stride);
+  const int64_t items = a.rows * ((cols + (wide ? 7 : 0)) / (wide ? 8 : 1));
+  const dim3 grid(grid_for((items + kActThreads - 1) / kActThreads, 148 * 8)), block(kActThreads);
+  auto kern = a.bf16 ? (wide ? act_backward_kernel<true, 8> : act_backward_kernel<true, 1>)
+                     : (wide ? act_backward_kernel<false, 8> : act_backward_kernel<false, 1>);
+  return launch_pdl(kern, grid, block, 0, st, a);
+}
+
+cudaError_t launch_bias_grad(const LinearGradArgs& a, cudaStream_t st) {
+  const uint16_t* src = static_cast<const uint16_t*>(a.preact ? a.dz : a.dy);
+  const int64_t stride = a.preact ? a.dz_stride : a.dy_stride;
+  const bool pairs = (reinterpret_cast<uintptr_t>(src) & 3) == 0 && stride % 2 == 0;
+  const int64_t items = static_cast<int64_t>(a.groups) * a.splits * ((a.n + kSumCols - 1) / kSumCols);
+  auto kern = a.bf16 ? bias_grad_kernel<true> : bias_grad_kernel<false>;
+  cudaError_t e = launch_pdl(kern, dim3(grid_for(items, 148 * 8)), dim3(256), 0, st, a, src, stride, pairs);
+  if (e != cudaSuccess || a.splits <= 1) return e;
+  auto join = a.bf16 ? bias_join_kernel<true> : bias_join_kernel<false>;
+  return launch_pdl(join, dim3(grid_for((static_cast<int64_t>(a.groups) * a.n + 255) / 256, 148 * 8)), dim3(256), 0,
+                    st, a);
+}
+
+}  // namespace senmoe

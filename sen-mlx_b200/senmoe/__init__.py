@@ -10,6 +10,9 @@ Mirrors the reference's MoE interfaces (paths inside the sen-mlx project):
   and ``x [..., K, 1, in]`` against ``[..., K]``).
 * ``SwitchLinear`` / ``DeepseekMoe`` -- src/engine/mlx_lm/models/deepseek_v2.rs:400-553;
   ``DeepseekMoe.forward(x [B, L, H]) -> [B, L, H]``.
+* ``linear`` / ``grouped_linear`` and their ``_backward`` -- linear products over
+  16-bit weights with the activation and residual in the product's launch,
+  dense or grouped by expert (products.py).
 * Failures raise ``SenMoeError`` carrying the C status and message, as the
   reference's shim turns a non-zero status into ``Exception::custom``
   (utils/moe.rs:66-74).
@@ -87,6 +90,26 @@ class SenMoePeerInfo(C.Structure):
                 ("device", C.c_int32), ("reserved", C.c_int32)]
 
 
+class SenMoeLinear(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("epilogue", C.c_int32), ("num_groups", C.c_int32), ("path", C.c_int32),
+                ("rows", C.c_int64), ("in_features", C.c_int64), ("out_features", C.c_int64),
+                ("x", _P), ("x_stride", C.c_int64),
+                ("weight", _P), ("weight_stride", C.c_int64), ("weight_group_stride", C.c_int64),
+                ("offsets", _P), ("bias", _P), ("residual", _P), ("residual_stride", C.c_int64),
+                ("y", _P), ("y_stride", C.c_int64), ("preact", _P), ("preact_stride", C.c_int64)]
+
+
+class SenMoeLinearGrad(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("epilogue", C.c_int32), ("num_groups", C.c_int32), ("path", C.c_int32),
+                ("rows", C.c_int64), ("in_features", C.c_int64), ("out_features", C.c_int64),
+                ("dy", _P), ("dy_stride", C.c_int64), ("x", _P), ("x_stride", C.c_int64),
+                ("weight", _P), ("weight_stride", C.c_int64), ("weight_group_stride", C.c_int64),
+                ("offsets", _P), ("preact", _P), ("preact_stride", C.c_int64),
+                ("dx", _P), ("dx_stride", C.c_int64),
+                ("dweight", _P), ("dweight_stride", C.c_int64), ("dweight_group_stride", C.c_int64),
+                ("dbias", _P), ("workspace", _P), ("workspace_bytes", C.c_int64)]
+
+
 # Every symbol include/senmoe.h declares, with its ctypes signature.
 _i64, _i32, _f32 = C.c_int64, C.c_int32, C.c_float
 SIGNATURES = {
@@ -112,6 +135,10 @@ SIGNATURES = {
     "senmoe_gemma_router": (C.c_int, [C.c_void_p, _P, _i64, _P, _P, _P]),
     "senmoe_quantized_linear": (C.c_int, [_P, _i64, _P, _P, _P, _i64, _i64, C.c_int32, C.c_int32, _P, _P]),
     "senmoe_layer_experts_forward": (C.c_int, [_P, _P, _i64, _P, _P, _P, _P]),
+    "senmoe_linear": (C.c_int, [_P, _P]),
+    "senmoe_linear_backward_workspace": (_i64, [_P]),
+    "senmoe_linear_backward": (C.c_int, [_P, _P]),
+    "senmoe_linear_check": (C.c_int, [_P]),
 }
 
 _lib = None
@@ -574,3 +601,7 @@ class MoeStack:
     def release(self) -> None:
         """Drops the captured graphs (before destroying layers or process groups)."""
         self.graphs.clear()
+
+
+from .products import (LINEAR_ANY, LINEAR_AUTO, LINEAR_TCGEN05, grouped_linear,  # noqa: E402
+                       grouped_linear_backward, linear, linear_backward, linear_check)
