@@ -825,6 +825,21 @@ cudaError_t make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner, uint64_t rows,
+                         uint64_t groups, uint64_t row_stride_bytes, uint64_t group_stride_bytes, uint32_t box_inner,
+                         uint32_t box_rows) {
+  auto enc = tmap_encoder();
+  if (!enc) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {inner, rows, groups};
+  const cuuint64_t strides[2] = {row_stride_bytes, group_stride_bytes};
+  const cuuint32_t box[3] = {box_inner, box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // Slot-ordered fp16 copy of the token rows (bf16 -> fp16 is exact in range),
 // k-permuted within each block of 8 columns like the dequantised weights
 // (kperm8), or in one of the warp-MMA kernel's orders (kperm256; kperm_g4,

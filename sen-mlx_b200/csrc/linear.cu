@@ -81,8 +81,11 @@ int check_group_stride(const char* call, const char* name, int64_t group_stride,
 }
 
 int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path, cudaStream_t st) {
-  if (path == SENMOE_LINEAR_TCGEN05) return reject(SENMOE_ERR_UNSUPPORTED, "%s: tcgen05 path", call);
-  return cuda_status(call, launch_linear_any(a, p, st));
+  const bool tc = path != SENMOE_LINEAR_ANY && linear_tc_supported(a, p);
+  if (path == SENMOE_LINEAR_TCGEN05 && !tc)
+    return reject(SENMOE_ERR_UNSUPPORTED, "%s: TMA needs 16-byte aligned operands, strides of a multiple of 8 elements",
+                  call);
+  return cuda_status(call, tc ? launch_linear_tc(a, p, st) : launch_linear_any(a, p, st));
 }
 
 int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
@@ -252,7 +255,11 @@ int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
 
 int senmoe_linear_check(senmoe_stream_t stream) {
   clear_failure();
-  return cuda_status("linear_check", cudaStreamSynchronize(stream));
+  int error = 0;
+  const int rc = cuda_status("linear_check", linear_device_error(stream, &error));
+  if (rc) return rc;
+  if (error == kDevWaitTimeout) return reject(SENMOE_ERR_TIMEOUT, "linear: a bounded wait on the device ran out");
+  return error ? reject(SENMOE_ERR_DEVICE, "linear: device error %d", error) : SENMOE_OK;
 }
 
 }  // extern "C"

@@ -181,6 +181,12 @@ __device__ __forceinline__ void zero_uncovered(const int* s_off, int groups, int
 // ------------------------------------------------------------ launchers
 // Any strides and alignments (linear_any.cu).
 cudaError_t launch_linear_any(const LinearArgs& a, LinearProduct p, cudaStream_t st);
+// tcgen05 (linear_tc.cu): operands that TMA can read, see linear_tc_supported.
+bool linear_tc_supported(const LinearArgs& a, LinearProduct p);
+cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, cudaStream_t st);
+// Waits for `st`, returns and clears the device error that the tcgen05
+// kernels recorded on the current device (DeviceError).
+cudaError_t linear_device_error(cudaStream_t st, int* error);
 
 // dz = dy * act'(z) in 16 bits, and the row sums over each group (the bias
 // gradient); see linear_grad.cu.
