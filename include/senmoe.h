@@ -378,7 +378,7 @@ typedef struct SenMoeLinear {
   int32_t epilogue;            /* SenMoeEpilogue */
   int32_t num_groups;          /* E <= 1024; 1 when offsets is NULL */
   int32_t path;                /* SenMoeLinearPath */
-  int64_t rows;                /* S < 2^31 */
+  int64_t rows;                /* S <= 2^31 - 1024 */
   int64_t in_features;
   int64_t out_features;
   const void* x;               /* [S, in] */

@@ -825,16 +825,15 @@ cudaError_t make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-cudaError_t make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner, uint64_t rows,
-                         uint64_t groups, uint64_t row_stride_bytes, uint64_t group_stride_bytes, uint32_t box_inner,
-                         uint32_t box_rows) {
+cudaError_t make_tmap_4d(CUtensorMap* map, const void* base, const uint64_t (&dims)[4],
+                         const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4]) {
   auto enc = tmap_encoder();
   if (!enc) return cudaErrorNotSupported;
-  const cuuint64_t dims[3] = {inner, rows, groups};
-  const cuuint64_t strides[2] = {row_stride_bytes, group_stride_bytes};
-  const cuuint32_t box[3] = {box_inner, box_rows, 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = enc(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr,
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+  const cuuint64_t s[3] = {stride_bytes[0], stride_bytes[1], stride_bytes[2]};
+  const cuuint32_t x[4] = {box[0], box[1], box[2], box[3]};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), d, s, x, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;

@@ -213,10 +213,9 @@ cudaError_t launch_tc_gemm(const CUtensorMap& tA0, const CUtensorMap& tA1, const
 cudaError_t make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner,
                          uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                          bool swizzle128);
-// The same with SWIZZLE_128B over [groups, rows, inner], each box in one group.
-cudaError_t make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner, uint64_t rows,
-                         uint64_t groups, uint64_t row_stride_bytes, uint64_t group_stride_bytes, uint32_t box_inner,
-                         uint32_t box_rows);
+// A 4-D tensor map of 16-bit elements with SWIZZLE_128B, innermost dimension first.
+cudaError_t make_tmap_4d(CUtensorMap* map, const void* base, const uint64_t (&dims)[4],
+                         const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4]);
 // x_sorted[s - s0, :] = fp16(x[perm[s] / k_div, :]) for s < num_slots (x bf16, rows of
 // `hidden`; s0 = offsets[eb], 0 without offsets); a value outside fp16 range
 // records kDevFp16Range in *err.  With slot_cap > 0 rows past it are skipped

@@ -30,6 +30,7 @@ int cuda_status(const char* what, cudaError_t e) {
 }
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024;  // row numbers, a tile past the last included, fit an int32
 
 // A matrix operand: rows x cols, row stride in elements.
 int check_matrix(const char* call, const char* name, const void* p, int64_t stride, int64_t cols) {
@@ -59,7 +60,7 @@ int check_shape(const char* call, int32_t dtype, int32_t epilogue, int32_t group
     return reject(SENMOE_ERR_BAD_ARG, "%s: num_groups=%d%s", call, groups, offsets ? "" : " without offsets");
   if (groups > kMaxGroups) return reject(SENMOE_ERR_UNSUPPORTED, "%s: num_groups=%d (at most %d)", call, groups, kMaxGroups);
   if (reinterpret_cast<uintptr_t>(offsets) & 3) return reject(SENMOE_ERR_BAD_ARG, "%s: offsets is not 4-byte aligned", call);
-  if (rows < 0 || rows >= (int64_t(1) << 31))
+  if (rows < 0 || rows > kMaxRows)
     return reject(SENMOE_ERR_BAD_ARG, "%s: rows=%lld", call, (long long)rows);
   *wide = epilogue >= SENMOE_EPI_SWIGLU ? 2 * out : out;
   if (in < 1 || out < 1 || in > kMaxDim || *wide > kMaxDim)
@@ -80,12 +81,13 @@ int check_group_stride(const char* call, const char* name, int64_t group_stride,
   return SENMOE_OK;
 }
 
-int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path, cudaStream_t st) {
+int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path, cudaStream_t st,
+                void* dbias = nullptr, bool* summed = nullptr) {
   const bool tc = path != SENMOE_LINEAR_ANY && linear_tc_supported(a, p);
   if (path == SENMOE_LINEAR_TCGEN05 && !tc)
     return reject(SENMOE_ERR_UNSUPPORTED, "%s: TMA needs 16-byte aligned operands, strides of a multiple of 8 elements",
                   call);
-  return cuda_status(call, tc ? launch_linear_tc(a, p, st) : launch_linear_any(a, p, st));
+  return cuda_status(call, tc ? launch_linear_tc(a, p, dbias, summed, st) : launch_linear_any(a, p, st));
 }
 
 int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
@@ -241,15 +243,16 @@ int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
     a.out_stride = g->dx_stride;
     if ((rc = run_product(call, a, kProdInput, g->path, stream))) return rc;
   }
+  bool summed = false;  // dbias came with dweight
   if (g->dweight) {
     a.b = g->x;
     a.b_stride = g->x_stride;
     a.out = g->dweight;
     a.out_stride = g->dweight_stride;
     a.out_group_stride = g->dweight_group_stride;
-    if ((rc = run_product(call, a, kProdWeight, g->path, stream))) return rc;
+    if ((rc = run_product(call, a, kProdWeight, g->path, stream, g->dbias, &summed))) return rc;
   }
-  if (g->dbias && (rc = cuda_status(call, launch_bias_grad(ga, stream)))) return rc;
+  if (g->dbias && !summed && (rc = cuda_status(call, launch_bias_grad(ga, stream)))) return rc;
   return SENMOE_OK;
 }
 

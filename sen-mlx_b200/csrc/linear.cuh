@@ -62,6 +62,15 @@ template <bool BF16> __device__ __forceinline__ uint16_t from_f32(float v) {
   if constexpr (BF16) return f32_to_bf16_bits(v);
   else return __half_as_ushort(__float2half_rn(v));
 }
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
 
 // Activations in fp32.  The result is rounded once, to 16 bits, so the
 // intrinsics' few units in the last place of fp32 do not show.
@@ -183,7 +192,9 @@ __device__ __forceinline__ void zero_uncovered(const int* s_off, int groups, int
 cudaError_t launch_linear_any(const LinearArgs& a, LinearProduct p, cudaStream_t st);
 // tcgen05 (linear_tc.cu): operands that TMA can read, see linear_tc_supported.
 bool linear_tc_supported(const LinearArgs& a, LinearProduct p);
-cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, cudaStream_t st);
+// dbias (dW only): also the column sums of dz, [groups, n] in the operands'
+// type, or null; *summed says whether this launch takes them.
+cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, void* dbias, bool* summed, cudaStream_t st);
 // Waits for `st`, returns and clears the device error that the tcgen05
 // kernels recorded on the current device (DeviceError).
 cudaError_t linear_device_error(cudaStream_t st, int* error);

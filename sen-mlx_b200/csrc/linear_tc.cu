@@ -1,11 +1,11 @@
 // linear_tc.cu -- the linear products on the 5th-generation tensor cores
 // (tcgen05, accumulators in TMEM, operands by TMA).
 //
-// One kernel for the three products.  A tile is D[128 features, w columns]:
-// the M side (128 lanes) always runs along the output's contiguous dimension
-// and the N side (w <= 256 columns, a multiple of 16 issued) along its rows,
-// so w follows a group's own row count and a small or ragged group costs
-// MMA time in proportion to its rows:
+// One kernel for the three products.  A tile is D[features, w columns]: the M
+// side (TMEM lanes) always runs along the output's contiguous dimension and
+// the N side (w <= 256 columns) along its rows, so w follows a group's own
+// row count and a small or ragged group costs MMA time in proportion to its
+// rows:
 //
 //   forward  M = rows of W (K-major), N = rows of x (K-major), K = in
 //   dx       M = in (W, MN-major),    N = rows of dz (K-major), K = rows of W
@@ -18,17 +18,27 @@
 // next multiple of 16 are zeroed in shared memory (in both operands, as the
 // strangers may hold infinities) and the MMAs stop there.
 //
-// Warp roles of a persistent CTA: warp 0 TMA producer, warp 1 MMA issuer (and
-// TMEM owner; it also zeroes dW's last rows), warps 4-11 epilogue (warps 2
-// and 3 only place these on the TMEM lane quarters).
-// Two accumulator sets in TMEM (2 x 256 columns) let the epilogue of a tile
-// run under the next tile's MMAs.  A gated pair keeps gate and up of the same
-// features as two accumulators of 128 columns, so its activation needs no
-// exchange between threads.
+// Three forms of a tile:
+//   * one CTA: 128 features;
+//   * a pair (cta_group::2): 256 features on two SMs, each holding half of
+//     the M operand and half of the N operand, so a tile's operands cross L2
+//     once for both;
+//   * a K split: the CTAs of a cluster take shares of one tile's K and add
+//     their fp32 accumulators over distributed shared memory in rank order
+//     (no atomics: the same bits every time), for products with fewer tiles
+//     than SMs.
+// A gated pair lays 64 gate rows over the same features' 64 up rows in the
+// 128 lanes; the epilogue warps of the two halves swap accumulators through
+// shared memory, each finishing half of the columns.
 //
-// Every wait is bounded (wait_or_abort): a role that gives up raises the
-// CTA's abort flag and records kDevWaitTimeout, the others follow, copies in
-// flight are awaited, and TMEM is freed.
+// Warp roles of a persistent CTA: warp 0 TMA producer, warp 1 MMA issuer (and
+// TMEM owner), warps 2-3 the bias gradient (dW), warps 4-11 epilogue.  Two
+// accumulator sets in TMEM (2 x 256 columns) let the epilogue of a tile run
+// under the next tile's MMAs.
+//
+// Every wait is bounded (wait_or_abort): a role that gives up raises the CTA's
+// abort flag and records kDevWaitTimeout, the others follow, copies in flight
+// are awaited, and TMEM is freed.
 
 #include <cuda.h>
 
@@ -39,35 +49,38 @@ namespace senmoe {
 namespace {
 
 constexpr int kBK = 64;                  // k of a stage: one 128-byte line
-constexpr int kBM = 128;
 constexpr int kEpiWarps = 8;
 constexpr int kEpiWarp0 = 4;
 constexpr int kTcThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr int kMaxStages = 10;
-constexpr uint32_t kMBytes = kBM * kBK * 2;  // one 128-feature operand tile
+constexpr uint32_t kMBytes = 128 * kBK * 2;  // a CTA's M operand of a stage
+constexpr uint32_t kBoxBytes = 64 * 128;     // an MN-major box: 64 features of 64 k
 constexpr int kTurnStride = 36;          // 32-bit words between column pairs of a warp's turning buffer
-constexpr uint32_t kRingBudget = 196608;
+constexpr uint32_t kRingBudget = 192 * 1024;
+constexpr uint32_t kRingBudgetGated = 176 * 1024;  // beside the gated exchange (16 KB)
+constexpr int kMaxSplit = 8;
 
 __device__ int g_linear_error;           // first device error of the linear kernels on this device
 
-enum Epilogue : int { kEpiPlain = 0, kEpiAct = 1, kEpiGated = 2 };
-
 struct TcArgs {
   LinearArgs l;
-  int bn;           // columns of a tile (N side), a multiple of 16
-  int box_rows;     // rows of an N-side K-major box
+  int bn;           // columns of a tile (N side)
+  int part;         // columns of a CTA's N operand: bn, or half of it in a pair
+  int m_pieces, n_pieces;  // MN-major: rows are whole 64-feature pieces (load_mn)
   int m_tiles;
   int n_tiles;      // dW: tiles along W's rows
   int stages;
-  uint32_t stage_bytes, n_offset;  // a stage, and where its N operand starts
+  int split;        // K split (one-CTA form): the cluster's size
+  uint32_t stage_bytes;  // a stage: the M operand, then the N operand
+  uint16_t* dbias;  // dW: column sums of dz, [groups, n], or null
 };
 
 // ------------------------------------------------------------ PTX wrappers
 // Shared-memory matrix descriptor, SWIZZLE_128B.  K-major: 8-row groups SBO =
 // 1024 bytes apart (LBO unused).  MN-major: 8-k groups SBO = 1024 bytes
-// apart, the next 64 features LBO = one box (64 x 128 bytes) on.
+// apart, the next 64 features LBO = one box on.
 template <bool MN> __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr) {
-  constexpr uint64_t lbo = MN ? (64 * 128) >> 4 : 1, sbo = 1024 >> 4;
+  constexpr uint64_t lbo = MN ? kBoxBytes >> 4 : 1, sbo = 1024 >> 4;
   return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (lbo << 16) | (sbo << 32) | (1ull << 46) | (2ull << 61);
 }
 // Instruction descriptor: D fp32, A and B fp16 (0) or bf16 (1), majors, N and M.
@@ -76,21 +89,52 @@ template <bool MN_A, bool MN_B> __device__ __forceinline__ uint32_t instr_desc(i
          (MN_A ? 1u << 15 : 0u) | (MN_B ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
+template <bool PAIR>
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+// Arrives on `bar` (a pair: on both CTAs' barrier at that offset) once every
+// MMA this thread issued has completed.
+template <bool PAIR> __device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t* dst) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t addr) {
+  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(addr) : "memory");
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
       "%15}, [%16];"
@@ -99,55 +143,139 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
-                                            uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-          "r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
-      : "memory");
+
+// TMA load of a box; PAIR: `bar` may be the other CTA's (a shared::cluster address).
+template <bool PAIR>
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                       uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, "
+        "%3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+        : "memory");
 }
-__device__ __forceinline__ void tma_load_2d_at(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+// An MN-major operand: `boxes` columns of 64 features from f0 on, 64 k rows
+// from k0.  Where the tensor's rows are whole 64-feature pieces the map has
+// these as a dimension and one load brings all (a load costs the TMA unit
+// some 100 cycles beside its bytes); otherwise one load a box.
+template <bool PAIR>
+__device__ __forceinline__ void load_mn(uint32_t dst, const CUtensorMap* map, bool pieces, int boxes, int f0, int k0,
+                                        int e, uint32_t bar) {
+  if (pieces) {
+    tma_4d<PAIR>(dst, map, 0, k0, f0 >> 6, e, bar);
+  } else {
+    for (int i = 0; i < boxes; ++i) tma_4d<PAIR>(dst + i * kBoxBytes, map, f0 + 64 * i, k0, 0, e, bar);
+  }
+}
+
+// ---- clusters
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, err));
+}
+
+// Named barrier of two warps (64 threads) that also joins a condition.
+__device__ __forceinline__ bool both_warps(int id, bool mine) {
+  uint32_t r;
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.aligned.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(mine ? 1u : 0u)
       : "memory");
+  return r != 0;
 }
 
 // ------------------------------------------------------------------ tiles
 struct Tile {
   int e;        // group
-  int m0;       // first feature (M side)
+  int m0;       // this CTA's first feature
   int c0;       // first column: a row of x / dz, or a row of W (dW)
   int w;        // columns, 1 .. bn
+  int n;        // columns of the MMA: w rounded up
+  int kb0, kb1; // this CTA's k blocks
   int k;        // extent of the contraction (dW: the group's rows, may be 0)
   int krow;     // dW: first row
 };
 
-template <int PROD>
-__device__ __forceinline__ Tile tile_at(const TcArgs& a, const int* s_off, const int* s_pre, int idx) {
+template <int PROD, bool GATED, bool PAIR>
+__device__ __forceinline__ Tile tile_at(const TcArgs& a, const int* s_off, const int* s_pre, int idx, int rank) {
+  constexpr int kFeat = GATED ? 64 : 128;
   Tile t;
   const int mt = idx % a.m_tiles, rest = idx / a.m_tiles;
-  t.m0 = mt * kBM;
+  t.m0 = PAIR ? (2 * mt + rank) * kFeat : mt * kFeat;
   if constexpr (PROD == kProdWeight) {
     t.e = rest / a.n_tiles;
     t.c0 = (rest - t.e * a.n_tiles) * a.bn;
     t.w = min(a.bn, a.l.n - t.c0);
+    t.n = PAIR ? (t.w + 127) & ~127 : (t.w + 15) & ~15;  // a pair: whole 64-feature boxes on each side
     t.krow = s_off[t.e];
     t.k = s_off[t.e + 1] - t.krow;
   } else {
     // a group's rows in equal chunks of at most bn, so that the last one is
-    // not a sliver (chunks are cheap in proportion to their width)
+    // not a sliver (a chunk costs time in proportion to its width)
+    constexpr int kStep = PAIR ? 32 : 16;
     t.e = group_of(s_pre, a.l.groups, rest);
     const int off = s_off[t.e], cnt = s_off[t.e + 1] - off, nch = s_pre[t.e + 1] - s_pre[t.e], j = rest - s_pre[t.e];
-    const int each = ((cnt + nch - 1) / nch + 15) & ~15;
+    const int each = ((cnt + nch - 1) / nch + kStep - 1) & ~(kStep - 1);
     t.c0 = off + j * each;
     t.w = min(each, cnt - j * each);
+    t.n = (t.w + kStep - 1) & ~(kStep - 1);
     t.k = PROD == kProdForward ? a.l.k : a.l.n;
     t.krow = 0;
   }
+  const int kb = (t.k + kBK - 1) / kBK;
+  t.kb0 = 0;
+  t.kb1 = kb;
+  if constexpr (!PAIR) {
+    if (a.split > 1) {
+      t.kb0 = static_cast<int>(static_cast<int64_t>(kb) * rank / a.split);
+      t.kb1 = static_cast<int>(static_cast<int64_t>(kb) * (rank + 1) / a.split);
+    }
+  }
   return t;
+}
+
+// The lines `left` up to the next multiple of 16 of a stage's MN-major boxes
+// (two of the M operand, n_boxes of the N operand behind it), one warp.
+__device__ __forceinline__ void zero_rows(unsigned char* stage, int left, int n_boxes, int lane) {
+  const int line = (16 - (left & 15)) * 8;  // 16-byte pieces of a box
+  for (int q = lane; q < (2 + n_boxes) * line; q += 32) {
+    const int box = q / line, in = q - box * line;
+    *reinterpret_cast<uint4*>(stage + box * kBoxBytes + left * 128 + in * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
 }
 
 template <int ACT> __device__ __forceinline__ void act_chunk(float (&z)[16]) {
@@ -168,16 +296,14 @@ __device__ __forceinline__ void act_chunk(int act, float (&z)[16]) {
 // values are rounded, turned in shared memory (two columns a word), and
 // leave as 16 bytes of one row a lane: lane 4p + o writes features 8o .. 8o +
 // 7 of columns 2p and 2p + 1.  Rows that cannot take 16-byte stores, and a
-// tile's last features, go one element at a time.
+// tile's last features, go one element at a time.  w columns and feats
+// features are valid (either may be 0 or less).
 template <bool BF16>
 __device__ __forceinline__ void store_chunk(const float (&v)[16], uint32_t* turn, uint16_t* out, int64_t stride, int w,
                                             int feats, bool vec, int lane) {
-  // out: first row and feature of the warp's block; w columns, feats features are valid
   if (vec) {
 #pragma unroll
-    for (int p = 0; p < 8; ++p)
-      turn[p * kTurnStride + lane] =
-          uint32_t(from_f32<BF16>(v[2 * p])) | (uint32_t(from_f32<BF16>(v[2 * p + 1])) << 16);
+    for (int p = 0; p < 8; ++p) turn[p * kTurnStride + lane] = pack2<BF16>(v[2 * p], v[2 * p + 1]);
     __syncwarp();
     const int p = lane >> 2, o = lane & 3;
     const uint4 a = *reinterpret_cast<const uint4*>(turn + p * kTurnStride + o * 8);
@@ -208,16 +334,67 @@ __device__ __forceinline__ void store_chunk(const float (&v)[16], uint32_t* turn
   }
 }
 
-template <int PROD, bool GATED, bool BF16>
+// What a warp needs to finish a tile's accumulators.
+template <int PROD, bool GATED, bool BF16> struct Finish {
+  const LinearArgs& l;
+  uint16_t *out, *pre;
+  int cols;           // features of the output
+  bool vec, pvec;
+  uint32_t* turn;
+  int lane;
+  __device__ __forceinline__ Finish(const LinearArgs& args, uint32_t* t, int ln) : l(args), turn(t), lane(ln) {
+    cols = PROD == kProdForward ? l.n / (GATED ? 2 : 1) : l.k;
+    out = static_cast<uint16_t*>(l.out);
+    pre = PROD == kProdForward ? static_cast<uint16_t*>(l.preact) : nullptr;
+    vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (l.out_stride & 7) == 0 &&
+          (PROD != kProdWeight || (l.out_group_stride & 7) == 0);
+    pvec = (reinterpret_cast<uintptr_t>(pre) & 15) == 0 && (l.preact_stride & 7) == 0 && (!GATED || (cols & 7) == 0);
+  }
+  __device__ __forceinline__ float bias(int e, int f, int lanes, int up) const {
+    if constexpr (PROD == kProdForward) {
+      if (l.bias && lane < lanes)
+        return to_f32<BF16>(static_cast<const uint16_t*>(l.bias)[static_cast<int64_t>(e) * l.n + up + f + lane]);
+    }
+    return 0.0f;
+  }
+  // z (bias added) of 16 columns -> preact, at column `at` of its rows
+  __device__ __forceinline__ void keep(const float (&z)[16], int64_t row, int at, int w, int feats) const {
+    if (PROD == kProdForward && pre)
+      store_chunk<BF16>(z, turn, pre + row * l.preact_stride + at, l.preact_stride, w, feats, pvec, lane);
+  }
+  // the activated values, + residual -> out
+  __device__ __forceinline__ void write(float (&y)[16], int e, int64_t row, int f, int w, int feats) const {
+    if constexpr (PROD == kProdForward) {
+      if (l.residual && lane < feats) {
+        const uint16_t* res = static_cast<const uint16_t*>(l.residual) + row * l.residual_stride + f + lane;
+        uint16_t r[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i] = i < w ? res[i * l.residual_stride] : uint16_t(0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] += to_f32<BF16>(r[i]);
+      }
+    }
+    uint16_t* dst = out + row * l.out_stride + f;
+    if constexpr (PROD == kProdWeight) dst += e * l.out_group_stride;
+    store_chunk<BF16>(y, turn, dst, l.out_stride, w, feats, vec, lane);
+  }
+};
+
+template <int PROD, bool GATED, bool BF16, bool PAIR>
 __global__ void __launch_bounds__(kTcThreads, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap tm_m, const __grid_constant__ CUtensorMap tm_n,
-                     const TcArgs a) {
+                     const __grid_constant__ CUtensorMap tm_half, const __grid_constant__ TcArgs a) {
   constexpr bool MN_M = PROD != kProdForward, MN_N = PROD == kProdWeight;
-  constexpr int NACC = GATED ? 2 : 1;
+  constexpr int kCtas = PAIR ? 2 : 1;
+  // dW in a pair: the second CTA's loads land on its own barrier (its warps 1
+  // to 3 work on them) and its warp 1 passes each on to the leader; elsewhere
+  // both CTAs' loads count on the leader's barrier
+  constexpr bool kRelay = PAIR && PROD == kProdWeight;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kMaxStages], bar_empty[kMaxStages], bar_accfull[2], bar_accempty[2],
       bar_drain;
   __shared__ __align__(16) uint32_t s_turn[kEpiWarps][8 * kTurnStride];
+  __shared__ __align__(16) float s_swap[GATED ? kEpiWarps : 1][GATED ? 16 * 32 : 1];
   __shared__ int s_off[kMaxGroups + 1], s_pre[kMaxGroups + 1], s_tot[64];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
@@ -228,35 +405,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t ring = (raw + 1023u) & ~1023u;
   unsigned char* ring_ptr = smem_raw + (ring - raw);
   const int stages = a.stages;
+  const int csize = PAIR ? 2 : a.split;  // CTAs of the cluster
+  const int rank = csize > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int unit = blockIdx.x / csize, units = gridDim.x / csize;
+  const bool sums = PROD == kProdWeight && a.dbias != nullptr;
 
   if (tid == 0) {
     for (int i = 0; i < stages; ++i) {
-      mbar_init(&bar_full[i], 1);
-      mbar_init(&bar_empty[i], 1);
+      mbar_init(&bar_full[i], kRelay && rank == 0 ? 2 : 1);
+      mbar_init(&bar_empty[i], sums ? 3 : 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_accfull[i], 1);
-      mbar_init(&bar_accempty[i], kEpiWarps);
+      mbar_init(&bar_accempty[i], kCtas * kEpiWarps);
     }
     mbar_init(&bar_drain, 1);
     s_abort = 0;
     fence_mbar_init();
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (warp == 1) tmem_alloc<PAIR>(&s_tmem);
   pdl_wait();
   pdl_launch_dependents();
   // chunks of bn rows; dW has no chunks, only the groups' row ranges
   group_table(a.l.offsets, a.l.groups, a.l.rows, PROD == kProdWeight ? 1 : a.bn, s_off, s_pre, s_tot);
   tc_fence_before();
   __syncthreads();
+  if (csize > 1) cluster_sync();  // the other CTAs' barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int tiles = a.m_tiles * (PROD == kProdWeight ? a.l.groups * a.n_tiles : s_pre[a.l.groups]);
-  const int grid = gridDim.x;
+  // shared by all roles: the tile's k blocks walk the ring in order
+  auto next = [stages](int& st, int& ph) {
+    if (++st == stages) { st = 0; ph ^= 1; }
+  };
 
   if (warp == 0) {
     // ============================================================ producer
@@ -264,198 +445,351 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint32_t issued = 0, parity = 0;  // by stage: loaded at least once, parity of the last load
       int st = 0, ph = 0;
       bool ok = true;
-      for (int idx = blockIdx.x; idx < tiles && ok; idx += grid) {
-        const Tile t = tile_at<PROD>(a, s_off, s_pre, idx);
-        const int kb = (t.k + kBK - 1) / kBK;
-        const int nbox = MN_N ? (t.w + 63) / 64 : (t.w + a.box_rows - 1) / a.box_rows;
-        const uint32_t box_bytes = MN_N ? 64 * 128 : a.box_rows * 128;
-        const uint32_t bytes = NACC * kMBytes + nbox * box_bytes;
-        for (int b = 0; b < kb; ++b) {
+      for (int idx = unit; idx < tiles && ok; idx += units) {
+        const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, idx, rank);
+        const int part = t.n / kCtas, col = t.c0 + (PAIR ? rank * part : 0);  // this CTA's share of the columns
+        // K-major columns: one load of a full part, or of half of one where that holds them
+        const bool small = !MN_N && 2 * part <= a.part && a.part >= 32;
+        const uint32_t bytes = kMBytes + (small ? a.part / 2 : a.part) * 128;
+        for (int b = t.kb0; b < t.kb1; ++b) {
           if (!(ok = wait_or_abort(&bar_empty[st], ph ^ 1, &s_abort, err))) break;
-          const uint32_t sm = ring + st * a.stage_bytes, sn = sm + a.n_offset;
-          uint64_t* full = &bar_full[st];
-          mbar_arrive_expect_tx(full, bytes);
-          const int k0 = t.krow + b * kBK;
-          if constexpr (PROD == kProdForward) {
-#pragma unroll
-            for (int h = 0; h < NACC; ++h)
-              tma_load_3d(sm + h * kMBytes, &tm_m, k0, t.m0 + h * (a.l.n / NACC), t.e, full);
-          } else if constexpr (PROD == kProdInput) {
-            tma_load_3d(sm, &tm_m, t.m0, k0, t.e, full);
-            tma_load_3d(sm + 64 * 128, &tm_m, t.m0 + 64, k0, t.e, full);
+          const uint32_t sm = ring + st * a.stage_bytes, sn = sm + kMBytes;
+          uint32_t full = smem_u32(&bar_full[st]);
+          if constexpr (PAIR && !kRelay) {
+            if (rank == 0) mbar_arrive_expect_tx(&bar_full[st], 2 * bytes);
+            full = map_rank(full, 0);
           } else {
-            tma_load_2d_at(sm, &tm_m, t.m0, k0, full);
-            tma_load_2d_at(sm + 64 * 128, &tm_m, t.m0 + 64, k0, full);
+            mbar_arrive_expect_tx(&bar_full[st], bytes);
           }
-          for (int i = 0; i < nbox; ++i) {
-            if constexpr (MN_N) tma_load_2d_at(sn + i * box_bytes, &tm_n, t.c0 + 64 * i, k0, full);
-            else tma_load_2d_at(sn + i * box_bytes, &tm_n, k0, t.c0 + a.box_rows * i, full);
-          }
+          const int k0 = t.krow + b * kBK;
+          if constexpr (PROD == kProdForward) tma_4d<PAIR>(sm, &tm_m, k0, t.m0, 0, t.e, full);
+          else load_mn<PAIR>(sm, &tm_m, a.m_pieces, 2, t.m0, k0, PROD == kProdInput ? t.e : 0, full);
+          if constexpr (MN_N) load_mn<PAIR>(sn, &tm_n, a.n_pieces, a.part / 64, col, k0, 0, full);
+          else tma_4d<PAIR>(sn, small ? &tm_half : &tm_n, k0, col, 0, 0, full);
           issued |= 1u << st;
           parity = (parity & ~(1u << st)) | (static_cast<uint32_t>(ph) << st);
-          if (++st == stages) { st = 0; ph ^= 1; }
+          next(st, ph);
         }
       }
-      if (!ok) {  // copies already issued: a bounded chance to land before the CTA leaves
-        volatile int never = 0;
-        for (int i = 0; i < stages; ++i)
-          if (issued >> i & 1) wait_or_abort(&bar_full[i], parity >> i & 1, &never, nullptr);
+      // the last loads of every stage have been consumed (a pair: so no
+      // arrival is still on its way when the CTA leaves)
+      volatile int never = 0;
+      for (int i = 0; i < stages; ++i) {
+        if (!(issued >> i & 1)) continue;
+        if (ok) ok = wait_or_abort(&bar_empty[i], parity >> i & 1, &s_abort, err);
+        // gave up: copies already issued get a bounded chance to land
+        if (!ok && (!PAIR || kRelay || rank == 0)) wait_or_abort(&bar_full[i], parity >> i & 1, &never, nullptr);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 && (!PAIR || rank == 0)) {
     // ========================================================== MMA issuer
     const bool leader = elect_one();
     bool ok = true;
     int st = 0, ph = 0, it = 0;
-    for (int idx = blockIdx.x; idx < tiles && ok; idx += grid, ++it) {
-      const Tile t = tile_at<PROD>(a, s_off, s_pre, idx);
+    for (int idx = unit; idx < tiles && ok; idx += units, ++it) {
+      const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, idx, rank);
       const int ab = it & 1, aph = (it >> 1) & 1;
-      if (!(ok = __all_sync(0xffffffffu, wait_or_abort(&bar_accempty[ab], aph ^ 1, &s_abort, err)))) break;
+      if (!(ok = warp_wait(&bar_accempty[ab], aph ^ 1, &s_abort, err))) break;
       tc_fence_after();
       const uint32_t d = tmem + ab * 256;
-      const uint32_t idesc = instr_desc<MN_M, MN_N>(a.l.bf16, (t.w + 15) & ~15, kBM);
-      const int kb = (t.k + kBK - 1) / kBK;
-      for (int b = 0; b < kb; ++b) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bar_full[st], ph, &s_abort, err));
-        if (!ok) break;
+      const uint32_t idesc = instr_desc<MN_M, MN_N>(a.l.bf16, t.n, 128 * kCtas);
+      for (int b = t.kb0; b < t.kb1; ++b) {
+        if (!(ok = warp_wait(&bar_full[st], ph, &s_abort, err))) break;
         const int left = t.k - b * kBK;
-        if (PROD == kProdWeight && left < kBK && (left & 15)) {
-          // the k rows after the group's last, up to the MMAs' next multiple
-          // of 16; the MMAs issued before run meanwhile
-          const int line = (16 - (left & 15)) * 8, boxes = 2 + (t.w + 63) / 64;  // 16-byte pieces of a box
-          unsigned char* p = ring_ptr + st * a.stage_bytes + left * 128;
-          for (int q = lane; q < boxes * line; q += 32) {
-            const int box = q / line, in = q - box * line;
-            *reinterpret_cast<uint4*>(p + (box < 2 ? box * 8192u : a.n_offset + (box - 2) * 8192u) + in * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
+        if (PROD == kProdWeight && left < kBK && (left & 15))
+          zero_rows(ring_ptr + st * a.stage_bytes, left, (t.n / kCtas + 63) / 64, lane);
         tc_fence_after();
         if (leader) {
-          const uint32_t sm = ring + st * a.stage_bytes, sn = sm + a.n_offset;
-          const uint64_t dm = smem_desc<MN_M>(sm), dn = smem_desc<MN_N>(sn);
+          const uint32_t sm = ring + st * a.stage_bytes;
+          const uint64_t dm = smem_desc<MN_M>(sm), dn = smem_desc<MN_N>(sm + kMBytes);
           const int ks = min(kBK, left + 15) >> 4;
           // 16 k: 32 bytes along a K-major line, 16 lines of an MN-major box
-          for (int s = 0; s < ks; ++s) {
-            const uint64_t am = dm + s * (MN_M ? 2048 >> 4 : 32 >> 4), an = dn + s * (MN_N ? 2048 >> 4 : 32 >> 4);
-#pragma unroll
-            for (int h = 0; h < NACC; ++h)
-              umma_ss(d + h * 128, am + h * (kMBytes >> 4), an, idesc, (b | s) != 0);
-          }
-          umma_commit(&bar_empty[st]);
+          for (int s = 0; s < ks; ++s)
+            umma_ss<PAIR>(d, dm + s * (MN_M ? 2048 >> 4 : 32 >> 4), dn + s * (MN_N ? 2048 >> 4 : 32 >> 4), idesc,
+                          (b > t.kb0 || s > 0) ? 1u : 0u);
+          umma_commit<PAIR>(&bar_empty[st]);
         }
         __syncwarp();
-        if (++st == stages) { st = 0; ph ^= 1; }
+        next(st, ph);
       }
-      if (ok && leader) umma_commit(&bar_accfull[ab]);
+      if (ok && leader) umma_commit<PAIR>(&bar_accfull[ab]);
       __syncwarp();
     }
-    if (leader) umma_commit(&bar_drain);  // every MMA issued has completed once this fires
+    // every MMA issued has completed once this fires
+    if (leader)
+      umma_commit<PAIR>(&bar_drain);
     __syncwarp();
     volatile int never = 0;
     wait_or_abort(&bar_drain, 0, &never, nullptr);
-  } else if (warp >= kEpiWarp0) {
+  } else if (warp == 1) {
+    // ====================== the pair's second CTA, dW: loads passed on
+    if constexpr (kRelay) {
+      bool ok = true;
+      int st = 0, ph = 0;
+      for (int idx = unit; idx < tiles && ok; idx += units) {
+        const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, idx, rank);
+        for (int b = t.kb0; b < t.kb1; ++b) {
+          if (!(ok = warp_wait(&bar_full[st], ph, &s_abort, err))) break;
+          const int left = t.k - b * kBK;
+          if (left < kBK && (left & 15)) zero_rows(ring_ptr + st * a.stage_bytes, left, t.n / 128, lane);
+          if (lane == 0) arrive_at(map_rank(smem_u32(&bar_full[st]), 0));
+          next(st, ph);
+        }
+      }
+    }
+    // (the leader's drain commit arrives here too)
+    volatile int never = 0;
+    wait_or_abort(&bar_drain, 0, &never, nullptr);
+  } else if (warp < kEpiWarp0) {
+    // ============================== dW: column sums of dz, the bias gradient
+    // Warp w takes the 64-column boxes w - 2, w, ... of this CTA's columns;
+    // lane 8r + c sums columns 8c .. 8c + 7 of rows r, r + 4, ...: rows in
+    // order, then the four lanes of a column, so a fixed order.  Only the
+    // first feature tile's CTAs sum; the others release the stages.
+    if constexpr (PROD == kProdWeight) {
+      if (sums) {
+        constexpr int kBoxes = PAIR ? 1 : 2;
+        bool ok = true;
+        int st = 0, ph = 0;
+        for (int idx = unit; idx < tiles && ok; idx += units) {
+          const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, idx, rank);
+          const int part = t.n / kCtas, col = t.c0 + (PAIR ? rank * part : 0);
+          const bool mine = idx % a.m_tiles == 0;
+          float acc[kBoxes][8] = {};
+          for (int b = t.kb0; b < t.kb1; ++b) {
+            if (!(ok = warp_wait(&bar_full[st], ph, &s_abort, err))) break;
+            if (mine) {
+              const int rows = min(kBK, t.k - b * kBK);
+#pragma unroll
+              for (int x = 0; x < kBoxes; ++x) {
+                const int box = warp - 2 + 2 * x;
+                if (box * 64 >= part) continue;
+                const unsigned char* p = ring_ptr + st * a.stage_bytes + kMBytes + box * kBoxBytes;
+                for (int r = lane >> 3; r < rows; r += 4) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(p + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                  const uint32_t wd[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    acc[x][2 * i] += to_f32<BF16>(static_cast<uint16_t>(wd[i]));
+                    acc[x][2 * i + 1] += to_f32<BF16>(static_cast<uint16_t>(wd[i] >> 16));
+                  }
+                }
+              }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_empty[st]);
+            next(st, ph);
+          }
+          if (mine && ok) {
+#pragma unroll
+            for (int x = 0; x < kBoxes; ++x) {
+              const int box = warp - 2 + 2 * x;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                float v = acc[x][i];
+                v += __shfl_xor_sync(0xffffffffu, v, 8);
+                v += __shfl_xor_sync(0xffffffffu, v, 16);
+                const int n = col + box * 64 + (lane & 7) * 8 + i;
+                if (lane < 8 && box * 64 < part && n < a.l.n)
+                  a.dbias[static_cast<int64_t>(t.e) * a.l.n + n] = from_f32<BF16>(v);
+              }
+            }
+          }
+        }
+      }
+    }
+  } else if (PAIR || a.split <= 1) {
     // ============================================================ epilogue
-    const int ew = warp - kEpiWarp0, q = warp & 3, half = ew >> 2;
-    uint32_t* turn = s_turn[ew];
-    const LinearArgs& l = a.l;
-    const int cols = PROD == kProdForward ? l.n / NACC : l.k;  // features of the output
-    uint16_t* out = static_cast<uint16_t*>(l.out);
-    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (l.out_stride & 7) == 0 &&
-                     (PROD != kProdWeight || (l.out_group_stride & 7) == 0);
-    uint16_t* pre = static_cast<uint16_t*>(l.preact);
-    const bool pvec = (reinterpret_cast<uintptr_t>(pre) & 15) == 0 && (l.preact_stride & 7) == 0 &&
-                      (NACC == 1 || (cols & 7) == 0);
+    // 32 columns at a time, the two warps of a lane quarter in turn
+    const int ew = warp - kEpiWarp0, q = warp & 3, turn2 = ew >> 2;
+    const Finish<PROD, GATED, BF16> fin(a.l, s_turn[ew], lane);
     int it = 0;
-    for (int idx = blockIdx.x; idx < tiles; idx += grid, ++it) {
-      const Tile t = tile_at<PROD>(a, s_off, s_pre, idx);
+    for (int idx = unit; idx < tiles; idx += units, ++it) {
+      const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, idx, rank);
       const int ab = it & 1, aph = (it >> 1) & 1;
-      if (!__all_sync(0xffffffffu, wait_or_abort(&bar_accfull[ab], aph, &s_abort, err))) break;
+      // a gated pair: quarters 0, 1 hold the gate of features 32 (q & 1) on, 2, 3 the up
+      const int f0 = t.m0 + (GATED ? q & 1 : q) * 32, feats = min(32, fin.cols - f0);
+      const int up = GATED && q >= 2 ? fin.cols : 0;
+      const float bias = fin.bias(t.e, f0, feats, up);
+      bool go = warp_wait(&bar_accfull[ab], aph, &s_abort, err);
+      // the two warps that swap leave together, or one would wait for the other
+      if constexpr (GATED) go = both_warps(1 + (turn2 * 2 + (q & 1)), go);
+      if (!go) break;
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + ab * 256;
-      const int f0 = t.m0 + q * 32, feats = min(32, cols - f0);  // this warp's features
-      float b0 = 0.0f, b1 = 0.0f;
-      if constexpr (PROD == kProdForward) {
-        if (l.bias && lane < feats) {
-          const uint16_t* bias = static_cast<const uint16_t*>(l.bias) + static_cast<int64_t>(t.e) * l.n + f0 + lane;
-          b0 = to_f32<BF16>(*bias);
-          if constexpr (GATED) b1 = to_f32<BF16>(bias[cols]);
+      const uint32_t release = PAIR ? map_rank(smem_u32(&bar_accempty[ab]), 0) : smem_u32(&bar_accempty[ab]);
+      bool released = false;
+      for (int c = turn2 * 32; c < t.w; c += 64) {
+        uint32_t r[32];
+        if (PROD == kProdWeight && t.k == 0) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0;
+        } else {
+          tmem_ld16(acc + c, r);
+          tmem_ld16(acc + c + 16, r + 16);
+          tmem_ld_wait();
+        }
+        if (c + 64 >= t.w) {  // this warp's last read of the accumulator
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(release);
+          released = true;
+        }
+        const int64_t row = t.c0 + c;
+        float z[2][16];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i >> 4][i & 15] = __uint_as_float(r[i]) + bias;
+        if constexpr (GATED) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) fin.keep(z[h], row + 16 * h, up + f0, t.w - c - 16 * h, feats);
+          // gate warps finish columns c .. c + 15 and hand the others over, up warps the reverse
+          const bool gate = q < 2;
+          float* mine = s_swap[ew];
+          const float* theirs = s_swap[ew ^ 2];
+          const int bar = 1 + (turn2 * 2 + (q & 1));
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mine[i * 32 + lane] = gate ? z[1][i] : z[0][i];
+          asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+          float y[16], u[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float v = theirs[i * 32 + lane];
+            y[i] = gate ? z[0][i] : v;
+            u[i] = gate ? v : z[1][i];
+          }
+          asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+          act_chunk(a.l.act, y);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] *= u[i];
+          const int h = gate ? 0 : 16;
+          fin.write(y, t.e, row + h, f0, t.w - c - h, feats);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int w = t.w - c - 16 * h;
+            if (w <= 0) break;
+            if constexpr (PROD == kProdForward) {
+              fin.keep(z[h], row + 16 * h, f0, w, feats);
+              act_chunk(a.l.act, z[h]);
+            }
+            fin.write(z[h], t.e, row + 16 * h, f0, w, feats);
+          }
         }
       }
-      if (feats > 0) {
-        for (int c = half * 16; c < t.w; c += 32) {
-          const int w = min(16, t.w - c);
-          uint32_t r0[16], r1[16];
-          float z[16];
-          if (PROD == kProdWeight && t.k == 0) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = 0.0f;
-          } else {
-            tmem_ld16(acc + c, r0);
-            if constexpr (GATED) tmem_ld16(acc + 128 + c, r1);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = __uint_as_float(r0[i]) + b0;
-          }
-          const int64_t row = t.c0 + c;
-          if constexpr (PROD == kProdForward) {
-            if (pre) store_chunk<BF16>(z, turn, pre + row * l.preact_stride + f0, l.preact_stride, w, feats, pvec, lane);
-            act_chunk(l.act, z);
-            if constexpr (GATED) {
-              float u[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) u[i] = __uint_as_float(r1[i]) + b1;
-              if (pre)
-                store_chunk<BF16>(u, turn, pre + row * l.preact_stride + cols + f0, l.preact_stride, w, feats, pvec,
-                                  lane);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) z[i] *= u[i];
-            }
-            if (l.residual && lane < feats) {
-              const uint16_t* res = static_cast<const uint16_t*>(l.residual) + row * l.residual_stride + f0 + lane;
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (i < w) z[i] += to_f32<BF16>(res[i * l.residual_stride]);
-            }
-          }
-          uint16_t* dst = out + row * l.out_stride + f0;
-          if constexpr (PROD == kProdWeight) dst += t.e * l.out_group_stride;
-          store_chunk<BF16>(z, turn, dst, l.out_stride, w, feats, vec, lane);
-        }
+      if (!released) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(release);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_accempty[ab]);
     }
-    if constexpr (PROD != kProdWeight) {
-      if (l.offsets) {  // rows of no group: zero
-        const int64_t head = s_off[0], tail = s_off[l.groups], n = head + (l.rows - tail);
-        for (int64_t i = blockIdx.x; i < n; i += grid) {
-          const int64_t r = i < head ? i : tail + (i - head);
-          for (int f = tid - kEpiWarp0 * 32; f < cols; f += kEpiWarps * 32) out[r * l.out_stride + f] = 0;
-          if (pre)
-            for (int f = tid - kEpiWarp0 * 32; f < l.n; f += kEpiWarps * 32) pre[r * l.preact_stride + f] = 0;
+  } else {
+    // ============== K split: this CTA's accumulator to shared memory (the
+    // ring, which the MMAs have read by then), [column][lane]
+    const int ew = warp - kEpiWarp0, q = warp & 3;
+    if (unit < tiles) {
+      const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
+      if (warp_wait(&bar_accfull[0], 0, &s_abort, err)) {
+        tc_fence_after();
+        const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16);
+        float* dst = reinterpret_cast<float*>(ring_ptr) + q * 32 + lane;
+        for (int c = (ew >> 2) * 16; c < t.w; c += 32) {
+          uint32_t r[16];
+          if (t.kb1 > t.kb0) {
+            tmem_ld16(acc + c, r);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = 0;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dst[(c + i) * 128] = __uint_as_float(r[i]);
         }
+        tc_fence_before();
+      }
+    }
+  }
+
+  __syncwarp();
+  if constexpr (!PAIR) {
+    if (csize > 1) {
+      cluster_sync();  // every share is in shared memory
+      if (warp >= kEpiWarp0 && unit < tiles) {
+        // chunks of 16 columns, dealt to the cluster's warps; shares added in rank order
+        const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
+        const int ew = warp - kEpiWarp0;
+        const Finish<PROD, GATED, BF16> fin(a.l, s_turn[ew], lane);
+        constexpr int kQuarters = GATED ? 2 : 4;
+        const int chunks = (t.w + 15) / 16 * kQuarters;
+        for (int i = ew * csize + rank; i < chunks; i += csize * kEpiWarps) {
+          const int q = i % kQuarters, c = i / kQuarters * 16, w = t.w - c;
+          const int f0 = t.m0 + q * 32, feats = min(32, fin.cols - f0);
+          float z[16], u[16];
+          const float b0 = fin.bias(t.e, f0, feats, 0), b1 = GATED ? fin.bias(t.e, f0, feats, fin.cols) : 0.0f;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) z[k] = u[k] = 0.0f;
+          for (int r = 0; r < csize; ++r) {
+            const uint32_t src = map_rank(ring + (c * 128 + q * 32 + lane) * 4, r);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              if (k < w) {
+                z[k] += ld_cluster(src + k * 512);
+                if constexpr (GATED) u[k] += ld_cluster(src + k * 512 + 256);
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 16; ++k) z[k] += b0;
+          if constexpr (PROD == kProdForward) {
+            const int64_t row = t.c0 + c;
+            fin.keep(z, row, f0, w, feats);
+            if constexpr (GATED) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) u[k] += b1;
+              fin.keep(u, row, fin.cols + f0, w, feats);
+            }
+            act_chunk(a.l.act, z);
+            if constexpr (GATED) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) z[k] *= u[k];
+            }
+          }
+          fin.write(z, t.e, t.c0 + c, f0, w, feats);
+        }
+      }
+    }
+  }
+  if constexpr (PROD != kProdWeight) {
+    if (a.l.offsets && warp >= kEpiWarp0) {  // rows of no group: zero
+      const LinearArgs& l = a.l;
+      uint16_t *out = static_cast<uint16_t*>(l.out), *pre = static_cast<uint16_t*>(l.preact);
+      const int cols = PROD == kProdForward ? l.n / (GATED ? 2 : 1) : l.k;
+      const int64_t head = s_off[0], tail = s_off[l.groups], n = head + (l.rows - tail);
+      for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
+        const int64_t r = i < head ? i : tail + (i - head);
+        for (int f = tid - kEpiWarp0 * 32; f < cols; f += kEpiWarps * 32) out[r * l.out_stride + f] = 0;
+        if (PROD == kProdForward && pre)
+          for (int f = tid - kEpiWarp0 * 32; f < l.n; f += kEpiWarps * 32) pre[r * l.preact_stride + f] = 0;
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
+  if (csize > 1) cluster_sync();  // nobody reads this CTA's shared memory or TMEM any more
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    tmem_free<PAIR>(tmem);
   }
 }
 
 // ------------------------------------------------------------- host side
 int tc_sm_count() {
+  static int counts[64] = {};  // by device; the same value whoever writes it
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-    n = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && counts[dev] > 0) return counts[dev];
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+  if (dev < 64) counts[dev] = n;
   return n;
 }
 
@@ -464,13 +798,111 @@ bool tma_ok(const void* p, int64_t stride, int64_t group_stride, int groups) {
          (groups <= 1 || (group_stride % 8 == 0 && group_stride < (int64_t(1) << 38)));
 }
 
-template <int PROD, bool GATED, bool BF16>
-cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const TcArgs& a, int grid, size_t smem,
+template <int PROD, bool GATED, bool BF16, bool PAIR>
+cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorMap& half, const TcArgs& a, int grid, size_t smem,
                      cudaStream_t st) {
-  auto kern = linear_tc_kernel<PROD, GATED, BF16>;
+  auto kern = linear_tc_kernel<PROD, GATED, BF16, PAIR>;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kern, dim3(grid), dim3(kTcThreads), smem, st, m, n, a);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = PAIR ? 2 : a.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR || a.split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, m, n, half, a);
+}
+
+template <bool PAIR, typename... A>
+cudaError_t launch_prod(LinearProduct p, bool gated, int bf16, const A&... args) {
+#define SENMOE_LINEAR_TC(P, G) (bf16 ? launch_t<P, G, true, PAIR>(args...) : launch_t<P, G, false, PAIR>(args...))
+  if (p == kProdInput) return SENMOE_LINEAR_TC(kProdInput, false);
+  if (p == kProdWeight) return SENMOE_LINEAR_TC(kProdWeight, false);
+  return gated ? SENMOE_LINEAR_TC(kProdForward, true) : SENMOE_LINEAR_TC(kProdForward, false);
+#undef SENMOE_LINEAR_TC
+}
+
+// The form of a product's tiles and its estimated time in SM cycles.
+struct Plan {
+  bool pair = false;
+  int bn = 16, split = 1;
+  int64_t tiles = 0;
+  double cycles = 0;
+};
+
+// Estimate of one form.  A k block of 64 costs the larger of its MMAs (8
+// cycles a 16-column step and K step of 16) and its operands' way from L2
+// (kL2Bytes a cycle and SM); tiles run in waves over the SMs.
+constexpr double kL2Bytes = 55, kTileCycles = 900, kSplitCycles = 1800;
+
+Plan make_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, bool pair, int bn, int split) {
+  Plan q;
+  q.pair = pair;
+  q.bn = bn;
+  q.split = split;
+  const int features = p == kProdForward ? (gated ? l.n / 2 : l.n) : l.k;
+  const int feat = (gated ? 64 : 128) * (pair ? 2 : 1);
+  const int64_t m_tiles = (features + feat - 1) / feat;
+  const double mean = static_cast<double>(l.rows) / l.groups;
+  double k, chunks, width;
+  if (p == kProdWeight) {
+    k = mean;
+    chunks = static_cast<double>(l.groups) * ((l.n + bn - 1) / bn);
+    width = l.n < bn ? l.n : bn;
+    q.tiles = static_cast<int64_t>(chunks) * m_tiles;
+  } else {
+    k = p == kProdForward ? l.k : l.n;
+    // no group has more chunks than rows
+    const int64_t upper = (l.rows + bn - 1) / bn + (l.offsets ? l.groups : 0);
+    q.tiles = (upper < l.rows ? upper : l.rows) * m_tiles;
+    if (l.offsets) {  // counts spread about the mean: a group near a multiple of bn takes one chunk more half the time
+      const double used = mean < 1 ? l.rows : l.groups;  // groups with rows, about
+      chunks = used * (mean < 1 ? 1.0 : static_cast<int64_t>(mean / bn + 0.5) < 1 ? 1.0 : mean / bn + 0.5);
+      width = mean < 1 ? 1 : l.rows / chunks;
+    } else {
+      chunks = static_cast<double>((l.rows + bn - 1) / bn);
+      width = l.rows / chunks;
+    }
+  }
+  const int step = pair ? (p == kProdWeight ? 128 : 32) : 16;
+  const double n = (static_cast<int64_t>(width + step - 1) / step) * step;
+  const double blocks = (k + kBK - 1) / kBK;
+  const double mma = 2.0 * n > 128 ? 2.0 * n : 128, load = 128.0 * (128 + (pair ? n / 2 : n)) / kL2Bytes;
+  const double per = mma > load ? mma : load;
+  const double slots = static_cast<double>(sms / ((pair ? 2 : 1) * split));
+  double waves = chunks * m_tiles / slots;
+  waves = waves < 8 ? static_cast<double>(static_cast<int64_t>(waves + 0.999)) : waves;
+  q.cycles = waves * (blocks / split * per + kTileCycles) + (split > 1 ? kSplitCycles : 0);
+  return q;
+}
+
+Plan choose_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms) {
+  static const int kWidths[] = {16, 32, 64, 128, 192, 256};
+  Plan best;
+  const int64_t rows = p == kProdWeight ? l.n : l.rows;
+  for (int w : kWidths) {
+    if (p == kProdWeight && w < 64) continue;
+    for (int pair = 0; pair < 2; ++pair) {
+      if (pair && (w < 64 || (p == kProdWeight && w < 256))) continue;
+      Plan q = make_plan(l, p, gated, sms, pair, w, 1);
+      if (best.cycles == 0 || q.cycles < best.cycles) best = q;
+      if (pair || best.cycles == 0) continue;
+      for (int s = 2; s <= kMaxSplit; s *= 2) {
+        if (q.tiles * s > sms) break;
+        const Plan t = make_plan(l, p, gated, sms, false, w, s);
+        if (t.cycles < best.cycles) best = t;
+      }
+    }
+    if (w >= rows) break;
+  }
+  return best;
 }
 
 }  // namespace
@@ -480,53 +912,62 @@ bool linear_tc_supported(const LinearArgs& a, LinearProduct p) {
   return a.rows > 0 && w_ok && tma_ok(a.a, a.a_stride, 0, 1);
 }
 
-cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, cudaStream_t st) {
+cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, void* dbias, bool* summed, cudaStream_t st) {
   const bool gated = p == kProdForward && act_gated(l.act);
+  const int sms = tc_sm_count();
+  const Plan plan = choose_plan(l, p, gated, sms);
   TcArgs a{};
   a.l = l;
+  // a K split leaves each CTA part of a column's rows: no sums there
+  a.dbias = p == kProdWeight && plan.split == 1 ? static_cast<uint16_t*>(dbias) : nullptr;
+  if (summed) *summed = a.dbias != nullptr;
+  a.bn = plan.bn;
+  a.split = plan.split;
   const int features = p == kProdForward ? (gated ? l.n / 2 : l.n) : l.k;
-  a.m_tiles = (features + kBM - 1) / kBM;
-  const int bn_max = gated ? 128 : 256;
-  int64_t tiles;
-  if (p == kProdWeight) {
-    a.bn = l.n >= 256 ? 256 : (l.n + 63) / 64 * 64;
-    a.n_tiles = (l.n + a.bn - 1) / a.bn;
-    tiles = static_cast<int64_t>(l.groups) * a.n_tiles * a.m_tiles;
-  } else {
-    // columns for the mean group with a quarter to spare
-    const int64_t mean = l.rows / l.groups, want = mean + mean / 4 + 1;
-    a.bn = want >= bn_max ? bn_max : want > 64 ? static_cast<int>((want + 63) / 64 * 64) : static_cast<int>((want + 15) / 16 * 16);
-    a.box_rows = a.bn < 64 ? a.bn : 64;
-    tiles = ((l.rows + a.bn - 1) / a.bn + (l.offsets ? l.groups : 0)) * a.m_tiles;
-  }
-  a.n_offset = (gated ? 2 : 1) * kMBytes;
-  a.stage_bytes = a.n_offset + a.bn * 128;
-  a.stages = static_cast<int>(kRingBudget / a.stage_bytes);
+  const int feat = (gated ? 64 : 128) * (plan.pair ? 2 : 1);
+  a.m_tiles = (features + feat - 1) / feat;
+  a.n_tiles = p == kProdWeight ? (l.n + a.bn - 1) / a.bn : 0;
+  a.part = plan.pair ? a.bn / 2 : a.bn;
+  a.stage_bytes = kMBytes + a.part * 128;
+  a.stages = static_cast<int>((gated ? kRingBudgetGated : kRingBudget) / a.stage_bytes);
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   const size_t smem = 1024 + static_cast<size_t>(a.stages) * a.stage_bytes;
 
-  // tensor maps: 16-bit patterns, 64-element boxes
-  CUtensorMap tm{}, tn{};
-  const auto dt = CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  CUtensorMap tm{}, tn{}, half{};
   cudaError_t e;
-  if (p == kProdWeight) {
-    e = make_tmap_2d(&tm, l.b, dt, l.k, l.rows, l.b_stride * 2, 64, 64, true);
-    if (e == cudaSuccess) e = make_tmap_2d(&tn, l.a, dt, l.n, l.rows, l.a_stride * 2, 64, 64, true);
+  // the M operand: W (forward, dx) or x (dW); the N operand: x, dz
+  const uint64_t b_row = l.b_stride * 2, a_row = l.a_stride * 2;
+  if (p == kProdForward) {
+    const uint64_t n = gated ? l.n / 2 : l.n, gs = l.groups > 1 ? l.b_group_stride * 2 : b_row * l.n;
+    e = make_tmap_4d(&tm, l.b, {uint64_t(l.k), n, gated ? 2u : 1u, uint64_t(l.groups)}, {b_row, n * b_row, gs},
+                     {64, gated ? 64u : 128u, gated ? 2u : 1u, 1});
   } else {
-    const int64_t gs = l.groups > 1 ? l.b_group_stride : l.b_stride * l.n;
-    e = make_tmap_3d(&tm, l.b, dt, l.k, l.n, l.groups, l.b_stride * 2, gs * 2, 64, p == kProdForward ? kBM : 64);
-    if (e == cudaSuccess)
-      e = make_tmap_2d(&tn, l.a, dt, p == kProdForward ? l.k : l.n, l.rows, l.a_stride * 2, 64, a.box_rows, true);
+    const uint64_t rows = p == kProdInput ? l.n : l.rows, groups = p == kProdInput ? l.groups : 1;
+    const uint64_t gs = groups > 1 ? l.b_group_stride * 2 : b_row * rows;
+    a.m_pieces = l.k % 64 == 0;
+    e = a.m_pieces ? make_tmap_4d(&tm, l.b, {64, rows, uint64_t(l.k / 64), groups}, {b_row, 128, gs}, {64, 64, 2, 1})
+                   : make_tmap_4d(&tm, l.b, {uint64_t(l.k), rows, 1, groups}, {b_row, b_row, gs}, {64, 64, 1, 1});
   }
   if (e != cudaSuccess) return e;
-  const int sms = tc_sm_count();
-  const int grid = static_cast<int>(tiles < 1 ? 1 : tiles < sms ? tiles : sms);
-#define SENMOE_LINEAR_TC(P, G)                                               \
-  (l.bf16 ? launch_t<P, G, true>(tm, tn, a, grid, smem, st) : launch_t<P, G, false>(tm, tn, a, grid, smem, st))
-  if (p == kProdInput) return SENMOE_LINEAR_TC(kProdInput, false);
-  if (p == kProdWeight) return SENMOE_LINEAR_TC(kProdWeight, false);
-  return gated ? SENMOE_LINEAR_TC(kProdForward, true) : SENMOE_LINEAR_TC(kProdForward, false);
-#undef SENMOE_LINEAR_TC
+  const uint64_t rows = l.rows;
+  if (p == kProdWeight) {
+    a.n_pieces = l.n % 64 == 0;
+    e = a.n_pieces ? make_tmap_4d(&tn, l.a, {64, rows, uint64_t(l.n / 64), 1}, {a_row, 128, a_row},
+                                  {64, 64, uint32_t(a.part / 64), 1})
+                   : make_tmap_4d(&tn, l.a, {uint64_t(l.n), rows, 1, 1}, {a_row, a_row, a_row}, {64, 64, 1, 1});
+    half = tn;
+  } else {
+    const uint64_t cols = p == kProdForward ? l.k : l.n;
+    e = make_tmap_4d(&tn, l.a, {cols, rows, 1, 1}, {a_row, a_row, a_row}, {64, uint32_t(a.part), 1, 1});
+    half = tn;
+    if (e == cudaSuccess && a.part >= 32)
+      e = make_tmap_4d(&half, l.a, {cols, rows, 1, 1}, {a_row, a_row, a_row}, {64, uint32_t(a.part / 2), 1, 1});
+  }
+  if (e != cudaSuccess) return e;
+  const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
+  const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
+  return plan.pair ? launch_prod<true>(p, gated, l.bf16, tm, tn, half, a, grid, smem, st)
+                   : launch_prod<false>(p, gated, l.bf16, tm, tn, half, a, grid, smem, st);
 }
 
 cudaError_t linear_device_error(cudaStream_t st, int* error) {
