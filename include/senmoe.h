@@ -363,12 +363,20 @@ typedef enum SenMoeEpilogue {
 
 /* Kernels of a linear product: 0 picks by shape and alignment.  The tcgen05
  * kernels read their operands with TMA, so these need 16-byte aligned bases
- * and row strides of a multiple of 8 elements; other operands run on the
+ * and row strides of a multiple of 8 elements; the few-row kernel (forward,
+ * decode) also in_features of a multiple of 8; anything else runs on the
  * warp-MMA kernels that copy element by element. */
 typedef enum SenMoeLinearPath {
   SENMOE_LINEAR_AUTO = 0,
-  SENMOE_LINEAR_ANY = 1,    /* any strides and alignments */
-  SENMOE_LINEAR_TCGEN05 = 2 /* SENMOE_ERR_UNSUPPORTED where TMA cannot read the operands */
+  SENMOE_LINEAR_ANY = 1,     /* any strides and alignments */
+  SENMOE_LINEAR_TCGEN05 = 2, /* SENMOE_ERR_UNSUPPORTED where TMA cannot read the operands */
+  SENMOE_LINEAR_SMALL = 3,   /* the few-row kernel (a backward call takes it as AUTO) */
+  /* one form of the tcgen05 tiles, for tests and measurements: one CTA, a CTA
+   * pair, K split over a cluster (SENMOE_ERR_UNSUPPORTED with more tiles than
+   * half the SMs) */
+  SENMOE_LINEAR_TCGEN05_ONE = 4,
+  SENMOE_LINEAR_TCGEN05_PAIR = 5,
+  SENMOE_LINEAR_TCGEN05_SPLIT = 6
 } SenMoeLinearPath;
 
 /* Strides are in elements; the innermost dimension is contiguous.  wide =

@@ -54,7 +54,7 @@ int check_shape(const char* call, int32_t dtype, int32_t epilogue, int32_t group
     return reject(SENMOE_ERR_UNSUPPORTED, "%s: dtype %d (bf16 and fp16 are supported)", call, dtype);
   if (epilogue < SENMOE_EPI_NONE || epilogue > SENMOE_EPI_GEGLU)
     return reject(SENMOE_ERR_UNSUPPORTED, "%s: epilogue %d", call, epilogue);
-  if (path < SENMOE_LINEAR_AUTO || path > SENMOE_LINEAR_TCGEN05)
+  if (path < SENMOE_LINEAR_AUTO || path > SENMOE_LINEAR_TCGEN05_SPLIT)
     return reject(SENMOE_ERR_BAD_ARG, "%s: path %d", call, path);
   if (groups < 1 || (!offsets && groups != 1))
     return reject(SENMOE_ERR_BAD_ARG, "%s: num_groups=%d%s", call, groups, offsets ? "" : " without offsets");
@@ -81,13 +81,32 @@ int check_group_stride(const char* call, const char* name, int64_t group_stride,
   return SENMOE_OK;
 }
 
+// The few-row kernel up to 64 rows of a dense product, and for grouped ones
+// while its small blocks (16 features of a group's rows) are few.
+constexpr int64_t kFewRows = 64, kFewBlocks = 148 * 8;
+bool few_rows(const LinearArgs& a) {
+  if (!a.offsets) return a.rows <= kFewRows;
+  const int64_t chunks = a.rows < a.groups ? a.rows : a.groups;
+  return a.rows <= kFewRows * a.groups && chunks * ((a.n + 15) / 16) <= kFewBlocks;
+}
+
 int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path, cudaStream_t st,
                 void* dbias = nullptr, bool* summed = nullptr) {
-  const bool tc = path != SENMOE_LINEAR_ANY && linear_tc_supported(a, p);
-  if (path == SENMOE_LINEAR_TCGEN05 && !tc)
+  if (path == SENMOE_LINEAR_ANY) return cuda_status(call, launch_linear_any(a, p, st));
+  const bool tc = linear_tc_supported(a, p);
+  const bool force_tc = path >= SENMOE_LINEAR_TCGEN05 && path != SENMOE_LINEAR_SMALL;
+  if (p == kProdForward && !force_tc) {
+    const bool small = linear_small_supported(a);
+    if (path == SENMOE_LINEAR_SMALL && !small)
+      return reject(SENMOE_ERR_UNSUPPORTED, "%s: the few-row kernels need 16-byte aligned operands, in_features and "
+                    "strides of a multiple of 8", call);
+    if (small && (path == SENMOE_LINEAR_SMALL || few_rows(a))) return cuda_status(call, launch_linear_small(a, st));
+  }
+  if (force_tc && !tc)
     return reject(SENMOE_ERR_UNSUPPORTED, "%s: TMA needs 16-byte aligned operands, strides of a multiple of 8 elements",
                   call);
-  return cuda_status(call, tc ? launch_linear_tc(a, p, dbias, summed, st) : launch_linear_any(a, p, st));
+  const int form = path > SENMOE_LINEAR_SMALL ? path - SENMOE_LINEAR_SMALL : kFormAuto;
+  return cuda_status(call, tc ? launch_linear_tc(a, p, form, dbias, summed, st) : launch_linear_any(a, p, st));
 }
 
 int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }

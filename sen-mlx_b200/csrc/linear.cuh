@@ -80,11 +80,20 @@ __device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0
 __device__ __forceinline__ float gelu_arg2(float z) {  // 2a, a = sqrt(2/pi) (z + 0.044715 z^3)
   return 1.5957691216057308f * (z + 0.044715f * z * z * z);
 }
+// Phi(z) through erfc's rational form of Abramowitz and Stegun, 7.1.26
+// (absolute error 1.5e-7, as much as erff's own rounding leaves of 1 + erf),
+// for a third of erff's instructions; e = exp(-z^2 / 2).
+__device__ __forceinline__ float normal_cdf(float z, float e) {
+  const float t = __fdividef(1.0f, 1.0f + 0.3275911f * 0.7071067811865476f * fabsf(z));
+  const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float q = 0.5f * p * e;
+  return z < 0.0f ? q : 1.0f - q;
+}
 __device__ __forceinline__ float act_value(int act, float z) {
   switch (act) {
     case kActRelu: return z > 0.0f ? z : (z != z ? z : 0.0f);
     case kActSilu: case kActSwiglu: return __fdividef(z, 1.0f + __expf(-z));
-    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
+    case kActGelu: return z * normal_cdf(z, __expf(-0.5f * z * z));
     case kActGeluTanh: case kActGeglu: return __fdividef(z, 1.0f + __expf(-gelu_arg2(z)));
     default: return z;
   }
@@ -96,8 +105,10 @@ __device__ __forceinline__ float act_slope(int act, float z) {
       const float s = logistic(z);
       return s * (1.0f + z * (1.0f - s));
     }
-    case kActGelu:  // Phi(z) + z phi(z)
-      return 0.5f * (1.0f + erff(z * 0.7071067811865476f)) + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    case kActGelu: {  // Phi(z) + z phi(z)
+      const float e = __expf(-0.5f * z * z);
+      return normal_cdf(z, e) + z * 0.3989422804014327f * e;
+    }
     case kActGeluTanh: case kActGeglu: {  // s = (1 + tanh a) / 2: s + 2 z s (1 - s) a'
       const float s = logistic(gelu_arg2(z));
       return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
@@ -190,11 +201,17 @@ __device__ __forceinline__ void zero_uncovered(const int* s_off, int groups, int
 // ------------------------------------------------------------ launchers
 // Any strides and alignments (linear_any.cu).
 cudaError_t launch_linear_any(const LinearArgs& a, LinearProduct p, cudaStream_t st);
+// Few rows, forward (linear_small.cu): 16-byte aligned rows of a multiple of 8 elements.
+bool linear_small_supported(const LinearArgs& a);
+cudaError_t launch_linear_small(const LinearArgs& a, cudaStream_t st);
 // tcgen05 (linear_tc.cu): operands that TMA can read, see linear_tc_supported.
 bool linear_tc_supported(const LinearArgs& a, LinearProduct p);
-// dbias (dW only): also the column sums of dz, [groups, n] in the operands'
-// type, or null; *summed says whether this launch takes them.
-cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, void* dbias, bool* summed, cudaStream_t st);
+// form: of the tiles, kFormAuto by estimated time.  dbias (dW only): also the
+// column sums of dz, [groups, n] in the operands' type, or null; *summed says
+// whether this launch takes them.
+enum LinearForm : int { kFormAuto = 0, kFormOne = 1, kFormPair = 2, kFormSplit = 3 };
+cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, int form, void* dbias, bool* summed,
+                             cudaStream_t st);
 // Waits for `st`, returns and clears the device error that the tcgen05
 // kernels recorded on the current device (DeviceError).
 cudaError_t linear_device_error(cudaStream_t st, int* error);

@@ -883,24 +883,27 @@ Plan make_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, bool p
   return q;
 }
 
-Plan choose_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms) {
+// form: kFormAuto, or the only form to consider.
+Plan choose_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, int form) {
   static const int kWidths[] = {16, 32, 64, 128, 192, 256};
   Plan best;
   const int64_t rows = p == kProdWeight ? l.n : l.rows;
   for (int w : kWidths) {
     if (p == kProdWeight && w < 64) continue;
     for (int pair = 0; pair < 2; ++pair) {
+      // a pair's CTAs hold at least 32 columns each, in dW two 64-feature boxes
       if (pair && (w < 64 || (p == kProdWeight && w < 256))) continue;
-      Plan q = make_plan(l, p, gated, sms, pair, w, 1);
-      if (best.cycles == 0 || q.cycles < best.cycles) best = q;
-      if (pair || best.cycles == 0) continue;
+      if (form == (pair ? kFormOne : kFormPair)) continue;
+      const Plan q = make_plan(l, p, gated, sms, pair, w, 1);
+      if (form != kFormSplit && (best.cycles == 0 || q.cycles < best.cycles)) best = q;
+      if (pair || form == kFormOne) continue;
       for (int s = 2; s <= kMaxSplit; s *= 2) {
         if (q.tiles * s > sms) break;
         const Plan t = make_plan(l, p, gated, sms, false, w, s);
-        if (t.cycles < best.cycles) best = t;
+        if (best.cycles == 0 || t.cycles < best.cycles) best = t;
       }
     }
-    if (w >= rows) break;
+    if (w >= rows && best.cycles > 0) break;
   }
   return best;
 }
@@ -912,10 +915,12 @@ bool linear_tc_supported(const LinearArgs& a, LinearProduct p) {
   return a.rows > 0 && w_ok && tma_ok(a.a, a.a_stride, 0, 1);
 }
 
-cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, void* dbias, bool* summed, cudaStream_t st) {
+cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, void* dbias, bool* summed,
+                             cudaStream_t st) {
   const bool gated = p == kProdForward && act_gated(l.act);
   const int sms = tc_sm_count();
-  const Plan plan = choose_plan(l, p, gated, sms);
+  const Plan plan = choose_plan(l, p, gated, sms, form);
+  if (plan.cycles == 0) return cudaErrorNotSupported;  // too many tiles for the K split asked for
   TcArgs a{};
   a.l = l;
   // a K split leaves each CTA part of a column's rows: no sums there

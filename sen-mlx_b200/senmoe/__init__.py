@@ -603,5 +603,6 @@ class MoeStack:
         self.graphs.clear()
 
 
-from .products import (LINEAR_ANY, LINEAR_AUTO, LINEAR_TCGEN05, grouped_linear,  # noqa: E402
-                       grouped_linear_backward, linear, linear_backward, linear_check)
+from .products import (LINEAR_ANY, LINEAR_AUTO, LINEAR_SMALL, LINEAR_TCGEN05, LINEAR_TCGEN05_ONE,  # noqa: E402
+                       LINEAR_TCGEN05_PAIR, LINEAR_TCGEN05_SPLIT, grouped_linear, grouped_linear_backward, linear,
+                       linear_backward, linear_check)

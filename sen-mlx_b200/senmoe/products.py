@@ -18,17 +18,29 @@ be captured into a CUDA graph.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import struct
 
 import torch
 
 from . import ERR_BAD_ARG, SenMoeError, SenMoeLinear, SenMoeLinearGrad, _check, lib
 
-LINEAR_AUTO, LINEAR_ANY, LINEAR_TCGEN05 = 0, 1, 2
+# SenMoeLinearPath
+LINEAR_AUTO, LINEAR_ANY, LINEAR_TCGEN05, LINEAR_SMALL = 0, 1, 2, 3
+LINEAR_TCGEN05_ONE, LINEAR_TCGEN05_PAIR, LINEAR_TCGEN05_SPLIT = 4, 5, 6
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "swiglu": 5, "geglu": 6}
 _GATED = 5  # from here on: gated pairs
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+# A decode step's product takes a few microseconds on the GPU, so the calls
+# keep their host side short: the argument structs are packed by one call
+# (their layout is the ctypes mirror's) and the current stream is read as the
+# handle that the C entry takes.
+_CODES = {C.c_int32: "i", C.c_int64: "q", C.c_void_p: "P"}
+_pack_linear = struct.Struct("".join(_CODES[t] for _, t in SenMoeLinear._fields_)).pack
+_pack_grad = struct.Struct("".join(_CODES[t] for _, t in SenMoeLinearGrad._fields_)).pack
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _bad(message: str) -> SenMoeError:
@@ -40,24 +52,21 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     n = t.shape[-1]
     if t.dim() != 2:
         t = t.reshape(-1, n)
-    if t.stride(1) != 1 and n > 1 or t.stride(0) < n and t.shape[0] > 1:
-        t = t.contiguous()
-    return t, max(t.stride(0), n)
+    s0, s1 = t.stride()
+    if s1 != 1 and n > 1 or s0 < n and t.shape[0] > 1:
+        return t.contiguous(), n
+    return t, s0 if s0 > n else n
 
 
 def _matrices(w: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """w [out, in] or [E, out, in]: (w, row stride, group stride)."""
     n, k = w.shape[-2], w.shape[-1]
-    if (w.stride(-1) != 1 and k > 1 or w.stride(-2) < k and n > 1
-            or w.dim() == 3 and w.shape[0] > 1 and w.stride(0) < n * w.stride(-2)):
+    s = w.stride()
+    if (s[-1] != 1 and k > 1 or s[-2] < k and n > 1
+            or len(s) == 3 and w.shape[0] > 1 and s[0] < n * s[-2]):
         w = w.contiguous()
-    stride = max(w.stride(-2), k)
-    return w, stride, w.stride(0) if w.dim() == 3 else 0
-
-
-def _on(stream):
-    """Where temporaries, outputs and launches go: the given stream, or the current one."""
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+        s = w.stride()
+    return w, s[-2] if s[-2] > k else k, s[0] if len(s) == 3 else 0
 
 
 def _activation(name: str) -> int:
@@ -67,72 +76,84 @@ def _activation(name: str) -> int:
         raise _bad(f"activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
 
 
-def _operands(first: torch.Tensor, *others) -> int:
-    """The common 16-bit dtype's code; every tensor on the current CUDA device."""
-    dtype, device = first.dtype, first.device
+def _operands(first: torch.Tensor, *others) -> tuple[int, int]:
+    """(the common 16-bit dtype's code, the device): every tensor on the current CUDA device."""
+    dtype, device = first.dtype, first.get_device()
     code = _DTYPES.get(dtype)
     if code is None:
         raise TypeError(f"tensors must be bfloat16 or float16, got {dtype}")
-    if not first.is_cuda:
+    if device < 0:
         raise TypeError("tensors must be CUDA tensors")
-    if device.index != torch.cuda.current_device():
-        raise _bad(f"tensors on {device}, current device is cuda:{torch.cuda.current_device()}")
     for t in others:
-        if t is not None and (t.dtype != dtype or t.device != device):
-            raise TypeError(f"tensors must share one dtype and device: {dtype} on {device}, {t.dtype} on {t.device}")
-    return code
+        if t is not None and (t.dtype is not dtype or t.get_device() != device):
+            raise TypeError(f"tensors must share one dtype and device: {dtype} on {first.device}, {t.dtype} on "
+                            f"{t.device}")
+    if device != _current_device():
+        raise _bad(f"tensors on {first.device}, current device is cuda:{_current_device()}")
+    return code, device
 
 
 def _groups(offsets: torch.Tensor, weight: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
     if weight.dim() != 3:
         raise _bad(f"weight must be [experts, out, in], got {tuple(weight.shape)}")
-    if offsets.dtype != torch.int32 or offsets.device != x.device:
+    if offsets.dtype is not torch.int32 or offsets.get_device() != x.get_device():
         raise TypeError(f"offsets must be int32 on {x.device}, got {offsets.dtype} on {offsets.device}")
-    if offsets.dim() != 1 or offsets.numel() != weight.shape[0] + 1:
+    if offsets.dim() != 1 or offsets.shape[0] != weight.shape[0] + 1:
         raise _bad(f"offsets {tuple(offsets.shape)} for {weight.shape[0]} experts")
     return offsets.contiguous()
 
 
 def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream, out, path):
+    if stream is not None:  # temporaries and outputs belong to the stream of the launch
+        with torch.cuda.stream(stream):
+            return _forward(x, weight, offsets, bias, residual, activation, save_preact, None, out, path)
     act = _activation(activation)
-    code = _operands(x, weight, bias, residual, out)
-    wide, k = weight.shape[-2], weight.shape[-1]
-    if x.dim() == 0 or x.shape[-1] != k:
-        raise _bad(f"x {tuple(x.shape)} against weight {tuple(weight.shape)}")
-    if act >= _GATED and wide % 2:
-        raise _bad(f"{activation}: weight has {wide} rows, gate and up need an even number")
-    n = wide // 2 if act >= _GATED else wide
-    groups = 1 if offsets is None else weight.shape[0]
+    code, device = _operands(x, weight, bias, residual, out)
+    wshape, xshape = weight.shape, x.shape
+    wide, k = wshape[-2], wshape[-1]
+    if not xshape or xshape[-1] != k:
+        raise _bad(f"x {tuple(xshape)} against weight {tuple(wshape)}")
+    n = wide
+    if act >= _GATED:
+        if wide % 2:
+            raise _bad(f"{activation}: weight has {wide} rows, gate and up need an even number")
+        n = wide // 2
+    groups = 1 if offsets is None else wshape[0]
+    pb = pr = pz = rs = 0
     if bias is not None:
         if bias.numel() != groups * wide or bias.shape[-1] != wide:
-            raise _bad(f"bias {tuple(bias.shape)} for weight {tuple(weight.shape)}")
-    shape = (*x.shape[:-1], n)
-    if residual is not None and tuple(residual.shape) != shape:
-        raise _bad(f"residual {tuple(residual.shape)}, the output is {shape}")
-    if out is not None and (tuple(out.shape) != shape or n > 1 and out.stride(-1) != 1):
-        raise _bad(f"out {tuple(out.shape)} strides {out.stride()}, the output is {shape}, its rows contiguous")
-    with _on(stream):
-        x2, xs = _rows(x)
-        rows = x2.shape[0]
-        w, ws, gs = _matrices(weight)
-        bias = bias if bias is None else bias.contiguous()
-        r, rs = (None, 0) if residual is None else _rows(residual)
-        if out is None:
-            y = torch.empty(shape, dtype=x.dtype, device=x.device)
-            y2, ys = y, n
-        else:
-            y = out
-            y2 = out if out.dim() == 2 else out.view(-1, n)
-            ys = y2.stride(0) if rows > 1 else n
-            if ys < n:
-                raise _bad(f"out strides {out.stride()}: its rows overlap")
-        z = torch.empty((*x.shape[:-1], wide), dtype=x.dtype, device=x.device) if save_preact else None
-        q = SenMoeLinear(code, act, groups, path, rows, k, n, x2.data_ptr(), xs, w.data_ptr(), ws, gs,
-                         None if offsets is None else offsets.data_ptr(),
-                         None if bias is None else bias.data_ptr(), None if r is None else r.data_ptr(), rs,
-                         y2.data_ptr(), ys, None if z is None else z.data_ptr(), wide)
-        _check(lib().senmoe_linear(C.byref(q), torch.cuda.current_stream().cuda_stream))
-    return (y, z) if save_preact else y
+            raise _bad(f"bias {tuple(bias.shape)} for weight {tuple(wshape)}")
+        bias = bias.contiguous()
+        pb = bias.data_ptr()
+    shape = (*xshape[:-1], n)
+    if residual is not None:
+        if residual.shape != shape:
+            raise _bad(f"residual {tuple(residual.shape)}, the output is {shape}")
+        residual, rs = _rows(residual)
+        pr = residual.data_ptr()
+    x2, xs = _rows(x)
+    rows = x2.shape[0]
+    w, ws, gs = _matrices(weight)
+    if out is None:
+        out = y = x2.new_empty(shape)
+        ys = n
+    else:
+        if out.shape != shape or n > 1 and out.stride(-1) != 1:
+            raise _bad(f"out {tuple(out.shape)} strides {out.stride()}, the output is {shape}, its rows contiguous")
+        y = out if out.dim() == 2 else out.view(-1, n)
+        ys = y.stride(0) if rows > 1 else n
+        if ys < n:
+            raise _bad(f"out strides {out.stride()}: its rows overlap")
+    if save_preact:
+        z = x2.new_empty((*xshape[:-1], wide))
+        pz = z.data_ptr()
+    status = lib().senmoe_linear(
+        _pack_linear(code, act, groups, path, rows, k, n, x2.data_ptr(), xs, w.data_ptr(), ws, gs,
+                     0 if offsets is None else offsets.data_ptr(), pb, pr, rs, y.data_ptr(), ys, pz, wide),
+        _current_stream(device))
+    if status:
+        _check(status)
+    return (out, z) if save_preact else out
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -161,39 +182,48 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
 
 
 def _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dweight, stream, path):
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dweight, None, path)
     act = _activation(activation)
-    code = _operands(dy, x, weight, preact)
-    wide, k = weight.shape[-2], weight.shape[-1]
-    if act >= _GATED and wide % 2:
-        raise _bad(f"{activation}: weight has {wide} rows, gate and up need an even number")
-    n = wide // 2 if act >= _GATED else wide
-    if x.dim() == 0 or x.shape[-1] != k or tuple(dy.shape) != (*x.shape[:-1], n):
-        raise _bad(f"dy {tuple(dy.shape)} and x {tuple(x.shape)} against weight {tuple(weight.shape)}")
-    if act and (preact is None or tuple(preact.shape) != (*x.shape[:-1], wide)):
-        raise _bad(f"{activation}: preact {None if preact is None else tuple(preact.shape)}, "
-                   f"{(*x.shape[:-1], wide)} wanted")
-    groups = 1 if offsets is None else weight.shape[0]
-    with _on(stream):
-        dy2, dys = _rows(dy)
-        x2, xs = _rows(x)
-        w, ws, gs = _matrices(weight)
-        z, zs = _rows(preact) if act else (None, 0)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
-        dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device) if need_dweight else None
-        db = torch.empty(weight.shape[:-1], dtype=x.dtype, device=x.device) if bias else None
-        g = SenMoeLinearGrad(code, act, groups, path, dy2.shape[0], k, n, dy2.data_ptr(), dys, x2.data_ptr(), xs,
-                             w.data_ptr(), ws, gs, None if offsets is None else offsets.data_ptr(),
-                             None if z is None else z.data_ptr(), zs, None if dx is None else dx.data_ptr(), k,
-                             None if dw is None else dw.data_ptr(), k, wide * k,
-                             None if db is None else db.data_ptr(), None, 0)
-        L, p = lib(), C.byref(g)
-        need = L.senmoe_linear_backward_workspace(p)
+    code, device = _operands(dy, x, weight, preact)
+    wshape, xshape = weight.shape, x.shape
+    wide, k = wshape[-2], wshape[-1]
+    n = wide
+    if act >= _GATED:
+        if wide % 2:
+            raise _bad(f"{activation}: weight has {wide} rows, gate and up need an even number")
+        n = wide // 2
+    if not xshape or xshape[-1] != k or dy.shape != (*xshape[:-1], n):
+        raise _bad(f"dy {tuple(dy.shape)} and x {tuple(xshape)} against weight {tuple(wshape)}")
+    z, pz, zs, pws, need = None, 0, 0, 0, 0
+    if act:
+        if preact is None or preact.shape != (*xshape[:-1], wide):
+            raise _bad(f"{activation}: preact {None if preact is None else tuple(preact.shape)}, "
+                       f"{(*xshape[:-1], wide)} wanted")
+        z, zs = _rows(preact)
+        pz = z.data_ptr()
+    groups = 1 if offsets is None else wshape[0]
+    dy2, dys = _rows(dy)
+    x2, xs = _rows(x)
+    w, ws, gs = _matrices(weight)
+    dx = x2.new_empty(xshape) if need_dx else None
+    dw = x2.new_empty(wshape) if need_dweight else None
+    db = x2.new_empty(wshape[:-1]) if bias else None
+    args = (code, act, groups, path, dy2.shape[0], k, n, dy2.data_ptr(), dys, x2.data_ptr(), xs, w.data_ptr(), ws, gs,
+            0 if offsets is None else offsets.data_ptr(), pz, zs, dx.data_ptr() if need_dx else 0, k,
+            dw.data_ptr() if need_dweight else 0, k, wide * k, db.data_ptr() if bias else 0)
+    L = lib()
+    if act or bias:
+        need = L.senmoe_linear_backward_workspace(_pack_grad(*args, 0, 0))
         if need < 0:
             _check(-need)
         if need:
-            ws_buf = torch.empty(need, dtype=torch.uint8, device=x.device)
-            g.workspace, g.workspace_bytes = ws_buf.data_ptr(), need
-        _check(L.senmoe_linear_backward(p, torch.cuda.current_stream().cuda_stream))
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+            pws = workspace.data_ptr()
+    status = L.senmoe_linear_backward(_pack_grad(*args, pws, need), _current_stream(device))
+    if status:
+        _check(status)
     return dx, dw, db
 
 

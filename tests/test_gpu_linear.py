@@ -415,3 +415,80 @@ def test_python_refusals(senmoe, torch):
         senmoe.linear_backward(s["dy"], s["x"], s["w"][0], activation="gelu")
     with pytest.raises(E):
         senmoe.linear_backward(s["dy"][:4], s["x"], s["w"][0])
+
+
+# Every kernel and tile form on shapes that each can take: rows and features
+# that end inside tiles, chunks and 64-element boxes, K shorter than a block
+# and not a multiple of one.
+FORM_SHAPES = [(1, 64, 128), (5, 8, 16), (16, 520, 136), (33, 72, 40), (64, 256, 264), (70, 264, 200), (161, 1032, 520),
+               (300, 192, 328)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", ["TCGEN05", "SMALL", "TCGEN05_ONE", "TCGEN05_PAIR", "TCGEN05_SPLIT"])
+@pytest.mark.parametrize("activation", ["none", "swiglu"])
+@pytest.mark.parametrize("rows,k,out", FORM_SHAPES)
+def test_every_form(senmoe, torch, form, rows, k, out, activation, dtype):
+    import linear_ref as R
+    form, wide = getattr(senmoe, "LINEAR_" + form), _wide(activation, out)
+    s = _make(torch, rows, k, wide, dtype)
+    r = s["r"][:, :out].contiguous()
+    y, z = senmoe.linear(s["x"], s["w"], bias=s["b"], residual=r, activation=activation, save_preact=True, path=form)
+    ref, bound, zr, zb = R.forward(s["x"], s["w"], None, s["b"], r, activation)
+    R.assert_within(z, zr, zb, "preact")
+    R.assert_within(y, ref, bound, "y")
+    dy, z = s["dy"][:, :out].contiguous(), None if activation == "none" else s["z"]
+    got = senmoe.linear_backward(dy, s["x"], s["w"], preact=z, activation=activation, bias=True, path=form)
+    for v, (ref, bound), what in zip(got, R.backward(dy, s["x"], s["w"], None, z, activation), ("dx", "dw", "db")):
+        R.assert_within(v, ref, bound, what)
+    senmoe.linear_check()
+
+
+@pytest.mark.parametrize("form", ["TCGEN05", "SMALL", "TCGEN05_ONE", "TCGEN05_PAIR"])
+@pytest.mark.parametrize("activation", ["none", "geglu"])
+@pytest.mark.parametrize("counts", GROUPS[:8], ids=lambda c: f"{len(c)}g{sum(c)}r")
+@pytest.mark.parametrize("k,out", [(72, 136), (256, 328)])
+def test_every_form_grouped(senmoe, torch, form, counts, k, out, activation):
+    import linear_ref as R
+    form, wide, rows = getattr(senmoe, "LINEAR_" + form), _wide(activation, out), sum(counts)
+    s = _make(torch, rows + 9, k, wide, "bfloat16", experts=len(counts))
+    off = _offsets(torch, counts, 4)  # rows 0-3 and the last 5 in no group
+    y = senmoe.grouped_linear(s["x"], s["w"], off, bias=s["b"], activation=activation, path=form)
+    ref, bound, _, _ = R.forward(s["x"], s["w"], off.tolist(), s["b"], None, activation)
+    assert (y[:4] == 0).all() and (y[4 + rows:] == 0).all()
+    R.assert_within(y[4:4 + rows], ref[4:4 + rows], bound[4:4 + rows], "y")
+    dy, z = s["dy"][:, :out].contiguous(), None if activation == "none" else s["z"]
+    got = senmoe.grouped_linear_backward(dy, s["x"], s["w"], off, preact=z, activation=activation, bias=True, path=form)
+    assert (got[0][:4] == 0).all() and (got[0][4 + rows:] == 0).all()
+    for v, (ref, bound), what in zip(got, R.backward(dy, s["x"], s["w"], off.tolist(), z, activation),
+                                     ("dx", "dw", "db")):
+        R.assert_within(v, ref, bound, what)
+    senmoe.linear_check()
+
+
+def test_k_split_over_a_group_that_is_empty_here(senmoe, torch):
+    """A K split's cluster whose tile has fewer K blocks than CTAs, and
+    clusters left without a tile by the groups' real counts."""
+    import linear_ref as R
+    s = _make(torch, 20, 72, 128, "bfloat16", experts=5)
+    off = _offsets(torch, [0, 19, 0, 1, 0])
+    y = senmoe.grouped_linear(s["x"], s["w"], off, bias=s["b"], path=senmoe.LINEAR_TCGEN05_SPLIT)
+    ref, bound, _, _ = R.forward(s["x"], s["w"], off.tolist(), s["b"])
+    R.assert_within(y, ref, bound, "y")
+    dx, dw, db = senmoe.grouped_linear_backward(s["dy"], s["x"], s["w"], off, bias=True,
+                                                path=senmoe.LINEAR_TCGEN05_SPLIT)
+    for v, (ref, bound), what in zip((dx, dw, db), R.backward(s["dy"], s["x"], s["w"], off.tolist()),
+                                     ("dx", "dw", "db")):
+        R.assert_within(v, ref, bound, what)
+
+
+def test_unsupported_forms(senmoe, torch):
+    s = _make(torch, 40, 33, 24, "bfloat16")
+    for form in (senmoe.LINEAR_TCGEN05, senmoe.LINEAR_TCGEN05_PAIR, senmoe.LINEAR_SMALL):
+        with pytest.raises(senmoe.SenMoeError) as e:
+            senmoe.linear(s["x"], s["w"], path=form)
+        assert e.value.status == senmoe.ERR_UNSUPPORTED
+    s = _make(torch, 4000, 64, 4096, "bfloat16")
+    with pytest.raises(senmoe.SenMoeError) as e:
+        senmoe.linear(s["x"], s["w"], path=senmoe.LINEAR_TCGEN05_SPLIT)
+    assert e.value.status == senmoe.ERR_UNSUPPORTED
