@@ -98,22 +98,30 @@ __device__ __forceinline__ float act_value(int act, float z) {
     default: return z;
   }
 }
-__device__ __forceinline__ float act_slope(int act, float z) {
+// act'(z), and act(z) in `value` (the two share their exponential).
+__device__ __forceinline__ float act_both(int act, float z, float& value) {
   switch (act) {
-    case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
+    case kActRelu:
+      value = z > 0.0f ? z : 0.0f;
+      return z > 0.0f ? 1.0f : 0.0f;
     case kActSilu: case kActSwiglu: {
       const float s = logistic(z);
+      value = z * s;
       return s * (1.0f + z * (1.0f - s));
     }
     case kActGelu: {  // Phi(z) + z phi(z)
-      const float e = __expf(-0.5f * z * z);
-      return normal_cdf(z, e) + z * 0.3989422804014327f * e;
+      const float e = __expf(-0.5f * z * z), c = normal_cdf(z, e);
+      value = z * c;
+      return c + z * 0.3989422804014327f * e;
     }
     case kActGeluTanh: case kActGeglu: {  // s = (1 + tanh a) / 2: s + 2 z s (1 - s) a'
       const float s = logistic(gelu_arg2(z));
+      value = z * s;
       return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
     }
-    default: return 1.0f;
+    default:
+      value = z;
+      return 1.0f;
   }
 }
 

@@ -28,62 +28,82 @@ template <bool BF16> __device__ __forceinline__ void unpack8(const uint4& v, flo
   }
 }
 template <bool BF16> __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = uint32_t(from_f32<BF16>(f[2 * i])) | (uint32_t(from_f32<BF16>(f[2 * i + 1])) << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
 }
 
-// V columns a thread: 8 (16-byte accesses) where every row starts on a
-// 16-byte boundary, else 1.
-template <bool BF16, int V>
+// A warp a row, V columns a lane and step: 8 (16-byte accesses) where every
+// row starts on a 16-byte boundary, else 1.  The loads of kUnroll steps are in
+// flight together.  Bound by HBM: dy and z read once, dz written once.
+template <bool BF16, int V, int ACT>
 __global__ void __launch_bounds__(kActThreads) act_backward_kernel(const LinearGradArgs a) {
+  constexpr bool kGated = ACT >= kActSwiglu;
+  constexpr int kUnroll = V == 8 ? 3 : 1;
   pdl_wait();
   pdl_launch_dependents();
-  const bool gated = act_gated(a.act);
-  const int cols = gated ? a.n / 2 : a.n, per_row = (cols + V - 1) / V;
-  const uint16_t* dy = static_cast<const uint16_t*>(a.dy);
-  const uint16_t* pre = static_cast<const uint16_t*>(a.preact);
-  uint16_t* dz = static_cast<uint16_t*>(a.dz);
-  const int64_t total = a.rows * per_row;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * kActThreads + threadIdx.x; it < total;
-       it += static_cast<int64_t>(gridDim.x) * kActThreads) {
-    const int64_t r = it / per_row;
-    const int c = static_cast<int>(it - r * per_row) * V;
-    const uint16_t* py = dy + r * a.dy_stride + c;
-    const uint16_t* pz = pre + r * a.preact_stride + c;
-    uint16_t* po = dz + r * a.dz_stride + c;
-    float d[V], z[V], u[V];
-    if constexpr (V == 8) {
-      const uint4 vy = *reinterpret_cast<const uint4*>(py), vz = *reinterpret_cast<const uint4*>(pz);
-      if (gated) {
-        const uint4 vu = *reinterpret_cast<const uint4*>(pz + cols);
-        unpack8<BF16>(vu, u);
-      }
-      unpack8<BF16>(vy, d);
-      unpack8<BF16>(vz, z);
-    } else {
-      d[0] = to_f32<BF16>(*py);
-      z[0] = to_f32<BF16>(*pz);
-      if (gated) u[0] = to_f32<BF16>(pz[cols]);
-    }
-    float g[V], du[V];
+  const int cols = kGated ? a.n / 2 : a.n;
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (kActThreads / 32);
+  for (int64_t r = blockIdx.x * (kActThreads / 32) + (threadIdx.x >> 5); r < a.rows; r += warps) {
+    const uint16_t* py = static_cast<const uint16_t*>(a.dy) + r * a.dy_stride;
+    const uint16_t* pz = static_cast<const uint16_t*>(a.preact) + r * a.preact_stride;
+    uint16_t* po = static_cast<uint16_t*>(a.dz) + r * a.dz_stride;
+    for (int c0 = lane * V; c0 < cols; c0 += 32 * V * kUnroll) {
+      uint4 vy[kUnroll], vz[kUnroll], vu[kUnroll];
+      if constexpr (V == 8) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      g[i] = d[i] * act_slope(a.act, z[i]);
-      if (gated) {
-        g[i] = d[i] * u[i] * act_slope(a.act, z[i]);
-        du[i] = d[i] * act_value(a.act, z[i]);
+        for (int j = 0; j < kUnroll; ++j) {
+          const int c = c0 + j * 256;
+          if (c < cols) {
+            vy[j] = *reinterpret_cast<const uint4*>(py + c);
+            vz[j] = *reinterpret_cast<const uint4*>(pz + c);
+            if constexpr (kGated) vu[j] = *reinterpret_cast<const uint4*>(pz + cols + c);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j) {
+        const int c = c0 + j * 32 * V;
+        if (c >= cols) break;
+        float d[V], z[V], u[V], g[V];
+        if constexpr (V == 8) {
+          unpack8<BF16>(vy[j], d);
+          unpack8<BF16>(vz[j], z);
+          if constexpr (kGated) unpack8<BF16>(vu[j], u);
+        } else {
+          d[0] = to_f32<BF16>(py[c]);
+          z[0] = to_f32<BF16>(pz[c]);
+          if constexpr (kGated) u[0] = to_f32<BF16>(pz[cols + c]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float value;
+          const float slope = act_both(ACT, z[i], value);
+          g[i] = d[i] * slope;
+          if constexpr (kGated) {
+            g[i] *= u[i];
+            u[i] = d[i] * value;
+          }
+        }
+        if constexpr (V == 8) {
+          *reinterpret_cast<uint4*>(po + c) = pack8<BF16>(g);
+          if constexpr (kGated) *reinterpret_cast<uint4*>(po + cols + c) = pack8<BF16>(u);
+        } else {
+          po[c] = from_f32<BF16>(g[0]);
+          if constexpr (kGated) po[cols + c] = from_f32<BF16>(u[0]);
+        }
       }
     }
-    if constexpr (V == 8) {
-      *reinterpret_cast<uint4*>(po) = pack8<BF16>(g);
-      if (gated) *reinterpret_cast<uint4*>(po + cols) = pack8<BF16>(du);
-    } else {
-      *po = from_f32<BF16>(g[0]);
-      if (gated) po[cols] = from_f32<BF16>(du[0]);
-    }
+  }
+}
+
+template <bool BF16, int V> auto act_backward_for(int act) {
+  switch (act) {
+    case kActRelu: return act_backward_kernel<BF16, V, kActRelu>;
+    case kActSilu: return act_backward_kernel<BF16, V, kActSilu>;
+    case kActGelu: return act_backward_kernel<BF16, V, kActGelu>;
+    case kActGeluTanh: return act_backward_kernel<BF16, V, kActGeluTanh>;
+    case kActSwiglu: return act_backward_kernel<BF16, V, kActSwiglu>;
+    case kActGeglu: return act_backward_kernel<BF16, V, kActGeglu>;
+    default: return act_backward_kernel<BF16, V, kActNone>;
   }
 }
 
@@ -166,10 +186,9 @@ cudaError_t launch_act_backward(const LinearGradArgs& a, cudaStream_t st) {
   const int cols = act_gated(a.act) ? a.n / 2 : a.n;
   const bool wide = cols % 8 == 0 && on16(a.dy, a.dy_stride) && on16(a.preact, a.preact_stride) &&
                     on16(a.dz, a.dz_stride);
-  const int64_t items = a.rows * ((cols + (wide ? 7 : 0)) / (wide ? 8 : 1));
-  const dim3 grid(grid_for((items + kActThreads - 1) / kActThreads, 148 * 8)), block(kActThreads);
-  auto kern = a.bf16 ? (wide ? act_backward_kernel<true, 8> : act_backward_kernel<true, 1>)
-                     : (wide ? act_backward_kernel<false, 8> : act_backward_kernel<false, 1>);
+  const dim3 grid(grid_for((a.rows + kActThreads / 32 - 1) / (kActThreads / 32), 148 * 8)), block(kActThreads);
+  auto kern = a.bf16 ? (wide ? act_backward_for<true, 8>(a.act) : act_backward_for<true, 1>(a.act))
+                     : (wide ? act_backward_for<false, 8>(a.act) : act_backward_for<false, 1>(a.act));
   return launch_pdl(kern, grid, block, 0, st, a);
 }
 

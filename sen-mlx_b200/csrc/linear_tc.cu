@@ -72,6 +72,7 @@ struct TcArgs {
   int stages;
   int split;        // K split (one-CTA form): the cluster's size
   uint32_t stage_bytes;  // a stage: the M operand, then the N operand
+  uint32_t tmem_cols;    // 512, or one accumulator where every CTA has one tile
   uint16_t* dbias;  // dW: column sums of dz, [groups, n], or null
 };
 
@@ -119,18 +120,22 @@ template <bool PAIR> __device__ __forceinline__ void umma_commit(uint64_t* bar) 
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
-template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t* dst) {
+template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
   if constexpr (PAIR) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
+                 : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   } else {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
+                 : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
 }
-template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t addr) {
-  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(addr) : "memory");
-  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(addr) : "memory");
+template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -160,6 +165,9 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int
         "[%6];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
         : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 // An MN-major operand: `boxes` columns of 64 features from f0 on, 64 k rows
 // from k0.  Where the tensor's rows are whole 64-feature pieces the map has
@@ -423,7 +431,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     s_abort = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc<PAIR>(&s_tmem);
+  if (warp == 0 && lane == 0) {  // kernel parameters: readable before the previous grid ends
+    prefetch_map(&tm_m);
+    prefetch_map(&tm_n);
+  }
+  if (warp == 1) tmem_alloc<PAIR>(&s_tmem, a.tmem_cols);
   pdl_wait();
   pdl_launch_dependents();
   // chunks of bn rows; dW has no chunks, only the groups' row ranges
@@ -714,43 +726,51 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (csize > 1) {
       cluster_sync();  // every share is in shared memory
       if (warp >= kEpiWarp0 && unit < tiles) {
-        // chunks of 16 columns, dealt to the cluster's warps; shares added in rank order
+        // items of four columns and 32 features, dealt to the cluster's warps;
+        // an item's loads are all in flight together, then added in rank order
         const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
         const int ew = warp - kEpiWarp0;
         const Finish<PROD, GATED, BF16> fin(a.l, s_turn[ew], lane);
         constexpr int kQuarters = GATED ? 2 : 4;
-        const int chunks = (t.w + 15) / 16 * kQuarters;
-        for (int i = ew * csize + rank; i < chunks; i += csize * kEpiWarps) {
-          const int q = i % kQuarters, c = i / kQuarters * 16, w = t.w - c;
+        const int items = (t.w + 3) / 4 * kQuarters;
+        for (int i = ew * csize + rank; i < items; i += csize * kEpiWarps) {
+          const int q = i % kQuarters, c = i / kQuarters * 4, w = min(4, t.w - c);
           const int f0 = t.m0 + q * 32, feats = min(32, fin.cols - f0);
-          float z[16], u[16];
           const float b0 = fin.bias(t.e, f0, feats, 0), b1 = GATED ? fin.bias(t.e, f0, feats, fin.cols) : 0.0f;
+          float v[kMaxSplit][GATED ? 8 : 4];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) z[k] = u[k] = 0.0f;
-          for (int r = 0; r < csize; ++r) {
+          for (int r = 0; r < kMaxSplit; ++r) {
+            if (r >= csize) break;
             const uint32_t src = map_rank(ring + (c * 128 + q * 32 + lane) * 4, r);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              if (k < w) {
-                z[k] += ld_cluster(src + k * 512);
-                if constexpr (GATED) u[k] += ld_cluster(src + k * 512 + 256);
-              }
+            for (int k = 0; k < 4; ++k) {
+              v[r][k] = k < w ? ld_cluster(src + k * 512) : 0.0f;
+              if constexpr (GATED) v[r][4 + k] = k < w ? ld_cluster(src + k * 512 + 256) : 0.0f;
+            }
+          }
+          float z[16] = {}, u[16] = {};
+#pragma unroll
+          for (int r = 0; r < kMaxSplit; ++r) {
+            if (r >= csize) break;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              z[k] += v[r][k];
+              if constexpr (GATED) u[k] += v[r][4 + k];
             }
           }
 #pragma unroll
-          for (int k = 0; k < 16; ++k) z[k] += b0;
+          for (int k = 0; k < 4; ++k) {
+            z[k] += b0;
+            u[k] += b1;
+          }
           if constexpr (PROD == kProdForward) {
             const int64_t row = t.c0 + c;
             fin.keep(z, row, f0, w, feats);
-            if constexpr (GATED) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k) u[k] += b1;
-              fin.keep(u, row, fin.cols + f0, w, feats);
-            }
+            if constexpr (GATED) fin.keep(u, row, fin.cols + f0, w, feats);
             act_chunk(a.l.act, z);
             if constexpr (GATED) {
 #pragma unroll
-              for (int k = 0; k < 16; ++k) z[k] *= u[k];
+              for (int k = 0; k < 4; ++k) z[k] *= u[k];
             }
           }
           fin.write(z, t.e, t.c0 + c, f0, w, feats);
@@ -778,7 +798,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (csize > 1) cluster_sync();  // nobody reads this CTA's shared memory or TMEM any more
   if (warp == 1) {
     tc_fence_after();
-    tmem_free<PAIR>(tmem);
+    tmem_free<PAIR>(tmem, a.tmem_cols);
   }
 }
 
@@ -936,6 +956,20 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, voi
   a.stage_bytes = kMBytes + a.part * 128;
   a.stages = static_cast<int>((gated ? kRingBudgetGated : kRingBudget) / a.stage_bytes);
   if (a.stages > kMaxStages) a.stages = kMaxStages;
+  a.tmem_cols = 512;
+  const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
+  const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
+  if (plan.tiles <= most) {
+    // One tile a CTA: no more stages than it has K blocks, one accumulator.
+    // What is left of the SM lets the next launch's CTA start its set-up.
+    const int64_t k = p == kProdForward ? l.k : p == kProdInput ? l.n : l.rows;
+    const int64_t blocks = ((k + kBK - 1) / kBK + plan.split - 1) / plan.split;
+    int need = static_cast<int>(blocks < a.stages ? blocks : a.stages);
+    const int room = static_cast<int>((a.bn * 512u + a.stage_bytes - 1) / a.stage_bytes);  // the split's sums lie there
+    if (plan.split > 1 && need < room) need = room;
+    if (need < a.stages) a.stages = need;
+    while (a.tmem_cols / 2 >= static_cast<uint32_t>(a.bn) && a.tmem_cols > 32) a.tmem_cols /= 2;
+  }
   const size_t smem = 1024 + static_cast<size_t>(a.stages) * a.stage_bytes;
 
   CUtensorMap tm{}, tn{}, half{};
@@ -969,8 +1003,6 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, voi
       e = make_tmap_4d(&half, l.a, {cols, rows, 1, 1}, {a_row, a_row, a_row}, {64, uint32_t(a.part / 2), 1, 1});
   }
   if (e != cudaSuccess) return e;
-  const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
-  const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
   return plan.pair ? launch_prod<true>(p, gated, l.bf16, tm, tn, half, a, grid, smem, st)
                    : launch_prod<false>(p, gated, l.bf16, tm, tn, half, a, grid, smem, st);
 }
