@@ -51,6 +51,11 @@ struct LinearArgs {
   void* preact;                                // forward: z before the activation, or null
   int64_t preact_stride;
   int bf16;                                    // 1: bf16, 0: fp16
+  // 1: the previous launch on the stream reads nothing of this one's outputs
+  // and writes nothing of its inputs, and waited for its own predecessor
+  // before it let dependents start: this launch need not wait for it before
+  // it starts, only before it ends (so that its end still means the other's).
+  int beside;
 };
 
 // 16-bit values by their bit patterns.
@@ -220,6 +225,8 @@ bool linear_tc_supported(const LinearArgs& a, LinearProduct p);
 enum LinearForm : int { kFormAuto = 0, kFormOne = 1, kFormPair = 2, kFormSplit = 3 };
 cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, int form, void* dbias, bool* summed,
                              cudaStream_t st);
+// The estimated time of launch_linear_tc, in SM cycles.
+double linear_tc_cycles(const LinearArgs& a, LinearProduct p);
 // Waits for `st`, returns and clears the device error that the tcgen05
 // kernels recorded on the current device (DeviceError).
 cudaError_t linear_device_error(cudaStream_t st, int* error);

@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     prefetch_map(&tm_n);
   }
   if (warp == 1) tmem_alloc<PAIR>(&s_tmem, a.tmem_cols);
-  pdl_wait();
+  if (!a.l.beside) pdl_wait();
   pdl_launch_dependents();
   // chunks of bn rows; dW has no chunks, only the groups' row ranges
   group_table(a.l.offsets, a.l.groups, a.l.rows, PROD == kProdWeight ? 1 : a.bn, s_off, s_pre, s_tot);
@@ -793,6 +793,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   }
 
+  if (a.l.beside) pdl_wait();
   tc_fence_before();
   __syncthreads();
   if (csize > 1) cluster_sync();  // nobody reads this CTA's shared memory or TMEM any more
@@ -929,6 +930,10 @@ Plan choose_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, int 
 }
 
 }  // namespace
+
+double linear_tc_cycles(const LinearArgs& l, LinearProduct p) {
+  return choose_plan(l, p, p == kProdForward && act_gated(l.act), tc_sm_count(), kFormAuto).cycles;
+}
 
 bool linear_tc_supported(const LinearArgs& a, LinearProduct p) {
   const bool w_ok = p == kProdWeight ? tma_ok(a.b, a.b_stride, 0, 1) : tma_ok(a.b, a.b_stride, a.b_group_stride, a.groups);

@@ -492,3 +492,23 @@ def test_unsupported_forms(senmoe, torch):
     with pytest.raises(senmoe.SenMoeError) as e:
         senmoe.linear(s["x"], s["w"], path=senmoe.LINEAR_TCGEN05_SPLIT)
     assert e.value.status == senmoe.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("activation", ["none", "geglu"])
+@pytest.mark.parametrize("rows", [257, 263, 320, 1031, 1088])
+def test_rows_past_whole_tiles(senmoe, torch, rows, activation):
+    """A few rows past a multiple of the widest tile, which may go to another
+    kernel; before and after other work on the stream."""
+    import linear_ref as R
+    k, out = 512, 2112
+    wide = _wide(activation, out)
+    s = _make(torch, rows, k, wide, "bfloat16")
+    r = s["r"][:, :out].contiguous()
+    ref, bound, zr, zb = R.forward(s["x"], s["w"], None, s["b"], r, activation)
+    for _ in range(3):
+        x = s["x"] + 0  # written just before the call, read and overwritten right after
+        y, z = senmoe.linear(x, s["w"], bias=s["b"], residual=r, activation=activation, save_preact=True)
+        x.zero_()
+        copy = y + 0
+        R.assert_within(z, zr, zb, "preact")
+        R.assert_within(copy, ref, bound, "y")
