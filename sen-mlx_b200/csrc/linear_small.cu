@@ -2,8 +2,9 @@
 // weights stream once from global memory into the registers of warp-level
 // MMAs, with no shared memory, barrier or TMEM between.
 //
-// A block computes 16 features (a gated pair: 16 gate and the same 16 up) of
-// one chunk of up to 8 * NT rows of one group; its eight warps take 32-column
+// A block computes 16 rows of W (a gated pair: 8 features' gate rows over
+// their 8 up rows, which leaves a feature's two sums in one thread) for one
+// chunk of up to 8 * NT rows of one group; its eight warps take 32-column
 // steps of K in turn.  In a step thread 4g + t of a warp loads the 8
 // consecutive columns 8t .. 8t + 7 of W's rows g and g + 8 and of the
 // chunk's rows g, g + 8, ...: 16 bytes each.  An m16n8k16 MMA wants k pairs
@@ -23,7 +24,7 @@ namespace senmoe {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kRows = 16;  // features of a block
+constexpr int kRows = 16;  // of W, a block
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -53,13 +54,13 @@ __device__ __forceinline__ uint4 load_x(const uint16_t* p, bool live) {
 
 template <bool BF16, bool GATED, int NT>
 __global__ void __launch_bounds__(kWarps * 32) linear_small_kernel(const __grid_constant__ LinearArgs a) {
-  constexpr int NB = GATED ? 2 : 1;
-  constexpr int kSteps = NT * NB > 8 ? 2 : 4;  // K steps whose loads are in flight together
-  __shared__ float s_part[kWarps / 2][NB][kRows][NT * 8 + 1];
+  constexpr int kFeat = GATED ? kRows / 2 : kRows;  // features of a block
+  constexpr int kSteps = 4;  // K steps whose loads are in flight together
+  __shared__ float s_part[kWarps / 2][kRows][NT * 8 + 1];
   __shared__ int s_sum[kWarps], s_tile[3];  // group, first row, rows
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   constexpr int kChunk = 8 * NT;
-  const int features = a.n / NB, f0 = blockIdx.x * kRows, want = blockIdx.y;
+  const int features = GATED ? a.n / 2 : a.n, f0 = blockIdx.x * kFeat, want = blockIdx.y;
   pdl_wait();
   pdl_launch_dependents();
 
@@ -111,13 +112,13 @@ __global__ void __launch_bounds__(kWarps * 32) linear_small_kernel(const __grid_
     // rows of no group: zero, this block's features of every gridDim.y-th
     const int head = min(max(a.offsets[0], 0), cap), tail = max(min(a.offsets[a.groups], cap), head);
     uint16_t *out = static_cast<uint16_t*>(a.out), *pre = static_cast<uint16_t*>(a.preact);
-    const int n = head + (cap - tail), f = f0 + (tid & 15);
-    for (int i = want + gridDim.y * (tid >> 4); i < n; i += gridDim.y * (kWarps * 2)) {
+    const int n = head + (cap - tail), f = f0 + tid % kFeat;
+    for (int i = want + gridDim.y * (tid / kFeat); i < n; i += gridDim.y * (kWarps * 32 / kFeat)) {
       const int64_t r = i < head ? i : tail + (i - head);
       if (f < features) {
         out[r * a.out_stride + f] = 0;
-        if (pre)
-          for (int h = 0; h < NB; ++h) pre[r * a.preact_stride + h * features + f] = 0;
+        if (pre) pre[r * a.preact_stride + f] = 0;
+        if (GATED && pre) pre[r * a.preact_stride + features + f] = 0;
       }
     }
     if (rows == 0) return;
@@ -126,23 +127,20 @@ __global__ void __launch_bounds__(kWarps * 32) linear_small_kernel(const __grid_
   }
 
   // ---- the products: warp w takes K steps w, w + 8, ...
+  // W's rows g and g + 8 of the block: features f0 + g and f0 + g + 8, or one feature's gate and up
   const uint16_t* w0 = static_cast<const uint16_t*>(a.b) + e * a.b_group_stride + (f0 + g) * a.b_stride + 8 * t4;
-  const uint16_t* w1 = w0 + 8 * a.b_stride;
-  const int64_t up = static_cast<int64_t>(features) * a.b_stride;
+  const uint16_t* w1 = w0 + (GATED ? features : 8) * a.b_stride;
   const uint16_t* x0 = static_cast<const uint16_t*>(a.a) + (row0 + g) * a.a_stride + 8 * t4;
-  const bool live0 = f0 + g < features, live1 = f0 + g + 8 < features;
-  float acc[NB][NT][4] = {};
+  const bool live0 = f0 + g < features, live1 = GATED ? live0 : f0 + g + 8 < features;
+  float acc[NT][4] = {};
   for (int s0 = warp * 32; s0 < a.k; s0 += kWarps * 32 * kSteps) {
-    uint4 wa[kSteps][NB][2], xb[kSteps];
+    uint4 wa[kSteps][2], xb[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int c = s0 + s * kWarps * 32;
       const bool in = c + 8 * t4 < a.k;
-#pragma unroll
-      for (int h = 0; h < NB; ++h) {
-        wa[s][h][0] = load_w(w0 + h * up + c, live0 && in);
-        wa[s][h][1] = load_w(w1 + h * up + c, live1 && in);
-      }
+      wa[s][0] = load_w(w0 + c, live0 && in);
+      wa[s][1] = load_w(w1 + c, live1 && in);
       xb[s] = load_x(x0 + c, g < rows && in);
     }
 #pragma unroll
@@ -153,11 +151,8 @@ __global__ void __launch_bounds__(kWarps * 32) linear_small_kernel(const __grid_
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const uint4 b = n == 0 ? xb[s] : load_x(x0 + n * 8 * a.a_stride + c, n * 8 + g < rows && in);
-#pragma unroll
-        for (int h = 0; h < NB; ++h) {
-          mma16816<BF16>(acc[h][n], wa[s][h][0].x, wa[s][h][1].x, wa[s][h][0].y, wa[s][h][1].y, b.x, b.y);
-          mma16816<BF16>(acc[h][n], wa[s][h][0].z, wa[s][h][1].z, wa[s][h][0].w, wa[s][h][1].w, b.z, b.w);
-        }
+        mma16816<BF16>(acc[n], wa[s][0].x, wa[s][1].x, wa[s][0].y, wa[s][1].y, b.x, b.y);
+        mma16816<BF16>(acc[n], wa[s][0].z, wa[s][1].z, wa[s][0].w, wa[s][1].w, b.z, b.w);
       }
     }
   }
@@ -165,35 +160,33 @@ __global__ void __launch_bounds__(kWarps * 32) linear_small_kernel(const __grid_
   // ---- partial sums: warps 4-7 hand over to 0-3, then the four are added
   auto each = [&](auto&& f) {
 #pragma unroll
-    for (int h = 0; h < NB; ++h)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) f(acc[h][n][q], s_part[warp & 3][h][g + (q >> 1) * 8][n * 8 + 2 * t4 + (q & 1)]);
+      for (int q = 0; q < 4; ++q) f(acc[n][q], s_part[warp & 3][g + (q >> 1) * 8][n * 8 + 2 * t4 + (q & 1)]);
   };
   if (warp >= kWarps / 2) each([](float& v, float& s) { s = v; });
   __syncthreads();
   if (warp < kWarps / 2) each([](float& v, float& s) { s += v; });
   __syncthreads();
 
-  // ---- epilogue: 16 features of a row at a time
+  // ---- epilogue: the block's features of a row at a time
   const uint16_t *bias = static_cast<const uint16_t*>(a.bias), *res = static_cast<const uint16_t*>(a.residual);
   uint16_t *out = static_cast<uint16_t*>(a.out), *pre = static_cast<uint16_t*>(a.preact);
-  const int f = f0 + (tid & 15), fi = tid & 15;
+  const int fi = tid % kFeat, f = f0 + fi;
   if (f >= features) return;
   const float b0 = bias ? to_f32<BF16>(bias[static_cast<int64_t>(e) * a.n + f]) : 0.0f;
   const float b1 = GATED && bias ? to_f32<BF16>(bias[static_cast<int64_t>(e) * a.n + features + f]) : 0.0f;
-  for (int r = tid >> 4; r < rows; r += kWarps * 2) {
+  for (int r = tid / kFeat; r < rows; r += kWarps * 32 / kFeat) {
     const int64_t row = row0 + r;
     float z = b0;
 #pragma unroll
-    for (int w = 0; w < kWarps / 2; ++w) z += s_part[w][0][fi][r];
+    for (int w = 0; w < kWarps / 2; ++w) z += s_part[w][fi][r];
     if (pre) pre[row * a.preact_stride + f] = from_f32<BF16>(z);
     float y = act_value(a.act, z);
     if constexpr (GATED) {
       float u = b1;
 #pragma unroll
-      for (int w = 0; w < kWarps / 2; ++w) u += s_part[w][1][fi][r];
+      for (int w = 0; w < kWarps / 2; ++w) u += s_part[w][fi + 8][r];
       if (pre) pre[row * a.preact_stride + features + f] = from_f32<BF16>(u);
       y *= u;
     }
@@ -225,7 +218,8 @@ cudaError_t launch_linear_small(const LinearArgs& a, cudaStream_t st) {
   const int nt = mean <= 8 ? 1 : mean <= 16 ? 2 : mean <= 32 ? 4 : 8;
   const int64_t most = (a.rows + 8 * nt - 1) / (8 * nt) + (a.offsets ? a.groups : 0);
   const int features = gated ? a.n / 2 : a.n;
-  const dim3 grid((features + kRows - 1) / kRows, static_cast<unsigned>(most < a.rows ? most : a.rows));
+  const int feat = gated ? kRows / 2 : kRows;
+  const dim3 grid((features + feat - 1) / feat, static_cast<unsigned>(most < a.rows ? most : a.rows));
   return a.bf16 ? (gated ? launch_t<true, true>(a, nt, grid, st) : launch_t<true, false>(a, nt, grid, st))
                 : (gated ? launch_t<false, true>(a, nt, grid, st) : launch_t<false, false>(a, nt, grid, st));
 }

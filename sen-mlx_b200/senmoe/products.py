@@ -47,9 +47,10 @@ def _bad(message: str) -> SenMoeError:
     return SenMoeError(ERR_BAD_ARG, message)
 
 
-def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """t [..., n] as (rows of n contiguous elements, their stride), a view where the strides allow one."""
-    n = t.shape[-1]
+def _rows(t: torch.Tensor, n: int) -> tuple[torch.Tensor, int]:
+    """t [..., n] as (rows of n contiguous elements, their stride), itself where the strides allow it."""
+    if t.is_contiguous():
+        return t, n
     if t.dim() != 2:
         t = t.reshape(-1, n)
     s0, s1 = t.stride()
@@ -58,15 +59,14 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     return t, s0 if s0 > n else n
 
 
-def _matrices(w: torch.Tensor) -> tuple[torch.Tensor, int, int]:
-    """w [out, in] or [E, out, in]: (w, row stride, group stride)."""
-    n, k = w.shape[-2], w.shape[-1]
-    s = w.stride()
-    if (s[-1] != 1 and k > 1 or s[-2] < k and n > 1
-            or len(s) == 3 and w.shape[0] > 1 and s[0] < n * s[-2]):
-        w = w.contiguous()
+def _matrices(w: torch.Tensor, n: int, k: int) -> tuple[torch.Tensor, int, int]:
+    """w [n, k] or [E, n, k]: (w, row stride, group stride)."""
+    if not w.is_contiguous():
         s = w.stride()
-    return w, s[-2] if s[-2] > k else k, s[0] if len(s) == 3 else 0
+        if not (s[-1] != 1 and k > 1 or s[-2] < k and n > 1 or len(s) == 3 and w.shape[0] > 1 and s[0] < n * s[-2]):
+            return w, s[-2] if s[-2] > k else k, s[0] if len(s) == 3 else 0
+        w = w.contiguous()
+    return w, k, n * k
 
 
 def _activation(name: str) -> int:
@@ -74,6 +74,11 @@ def _activation(name: str) -> int:
         return ACTIVATIONS[name]
     except KeyError:
         raise _bad(f"activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
+
+
+def _same(t: torch.Tensor, first: torch.Tensor, dtype, device: int) -> None:
+    if t.dtype is not dtype or t.get_device() != device:
+        raise TypeError(f"tensors must share one dtype and device: {dtype} on {first.device}, {t.dtype} on {t.device}")
 
 
 def _operands(first: torch.Tensor, *others) -> tuple[int, int]:
@@ -85,9 +90,7 @@ def _operands(first: torch.Tensor, *others) -> tuple[int, int]:
     if device < 0:
         raise TypeError("tensors must be CUDA tensors")
     for t in others:
-        if t is not None and (t.dtype is not dtype or t.get_device() != device):
-            raise TypeError(f"tensors must share one dtype and device: {dtype} on {first.device}, {t.dtype} on "
-                            f"{t.device}")
+        _same(t, first, dtype, device)
     if device != _current_device():
         raise _bad(f"tensors on {first.device}, current device is cuda:{_current_device()}")
     return code, device
@@ -108,11 +111,11 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
         with torch.cuda.stream(stream):
             return _forward(x, weight, offsets, bias, residual, activation, save_preact, None, out, path)
     act = _activation(activation)
-    code, device = _operands(x, weight, bias, residual, out)
-    wshape, xshape = weight.shape, x.shape
+    code, device = _operands(x, weight)
+    wshape, shape = weight.shape, x.shape
     wide, k = wshape[-2], wshape[-1]
-    if not xshape or xshape[-1] != k:
-        raise _bad(f"x {tuple(xshape)} against weight {tuple(wshape)}")
+    if not shape or shape[-1] != k:
+        raise _bad(f"x {tuple(shape)} against weight {tuple(wshape)}")
     n = wide
     if act >= _GATED:
         if wide % 2:
@@ -121,23 +124,27 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
     groups = 1 if offsets is None else wshape[0]
     pb = pr = pz = rs = 0
     if bias is not None:
+        _same(bias, x, x.dtype, device)
         if bias.numel() != groups * wide or bias.shape[-1] != wide:
             raise _bad(f"bias {tuple(bias.shape)} for weight {tuple(wshape)}")
-        bias = bias.contiguous()
+        bias = bias if bias.is_contiguous() else bias.contiguous()
         pb = bias.data_ptr()
-    shape = (*xshape[:-1], n)
+    lead = shape[:-1]
+    shape = (*lead, n)
     if residual is not None:
+        _same(residual, x, x.dtype, device)
         if residual.shape != shape:
             raise _bad(f"residual {tuple(residual.shape)}, the output is {shape}")
-        residual, rs = _rows(residual)
+        residual, rs = _rows(residual, n)
         pr = residual.data_ptr()
-    x2, xs = _rows(x)
-    rows = x2.shape[0]
-    w, ws, gs = _matrices(weight)
+    x, xs = _rows(x, k)
+    rows = x.numel() // k
+    weight, ws, gs = _matrices(weight, wide, k)
     if out is None:
-        out = y = x2.new_empty(shape)
+        out = y = x.new_empty(shape)
         ys = n
     else:
+        _same(out, x, x.dtype, device)
         if out.shape != shape or n > 1 and out.stride(-1) != 1:
             raise _bad(f"out {tuple(out.shape)} strides {out.stride()}, the output is {shape}, its rows contiguous")
         y = out if out.dim() == 2 else out.view(-1, n)
@@ -145,10 +152,10 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
         if ys < n:
             raise _bad(f"out strides {out.stride()}: its rows overlap")
     if save_preact:
-        z = x2.new_empty((*xshape[:-1], wide))
+        z = x.new_empty((*lead, wide))
         pz = z.data_ptr()
     status = lib().senmoe_linear(
-        _pack_linear(code, act, groups, path, rows, k, n, x2.data_ptr(), xs, w.data_ptr(), ws, gs,
+        _pack_linear(code, act, groups, path, rows, k, n, x.data_ptr(), xs, weight.data_ptr(), ws, gs,
                      0 if offsets is None else offsets.data_ptr(), pb, pr, rs, y.data_ptr(), ys, pz, wide),
         _current_stream(device))
     if status:
@@ -186,7 +193,7 @@ def _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dw
         with torch.cuda.stream(stream):
             return _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dweight, None, path)
     act = _activation(activation)
-    code, device = _operands(dy, x, weight, preact)
+    code, device = _operands(x, dy, weight)
     wshape, xshape = weight.shape, x.shape
     wide, k = wshape[-2], wshape[-1]
     n = wide
@@ -196,22 +203,23 @@ def _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dw
         n = wide // 2
     if not xshape or xshape[-1] != k or dy.shape != (*xshape[:-1], n):
         raise _bad(f"dy {tuple(dy.shape)} and x {tuple(xshape)} against weight {tuple(wshape)}")
-    z, pz, zs, pws, need = None, 0, 0, 0, 0
+    pz = zs = pws = need = 0
     if act:
         if preact is None or preact.shape != (*xshape[:-1], wide):
             raise _bad(f"{activation}: preact {None if preact is None else tuple(preact.shape)}, "
                        f"{(*xshape[:-1], wide)} wanted")
-        z, zs = _rows(preact)
-        pz = z.data_ptr()
+        _same(preact, x, x.dtype, device)
+        preact, zs = _rows(preact, wide)
+        pz = preact.data_ptr()
     groups = 1 if offsets is None else wshape[0]
-    dy2, dys = _rows(dy)
-    x2, xs = _rows(x)
-    w, ws, gs = _matrices(weight)
-    dx = x2.new_empty(xshape) if need_dx else None
-    dw = x2.new_empty(wshape) if need_dweight else None
-    db = x2.new_empty(wshape[:-1]) if bias else None
-    args = (code, act, groups, path, dy2.shape[0], k, n, dy2.data_ptr(), dys, x2.data_ptr(), xs, w.data_ptr(), ws, gs,
-            0 if offsets is None else offsets.data_ptr(), pz, zs, dx.data_ptr() if need_dx else 0, k,
+    dy, dys = _rows(dy, n)
+    x, xs = _rows(x, k)
+    weight, ws, gs = _matrices(weight, wide, k)
+    dx = x.new_empty(xshape) if need_dx else None
+    dw = x.new_empty(wshape) if need_dweight else None
+    db = x.new_empty(wshape[:-1]) if bias else None
+    args = (code, act, groups, path, x.numel() // k, k, n, dy.data_ptr(), dys, x.data_ptr(), xs, weight.data_ptr(), ws,
+            gs, 0 if offsets is None else offsets.data_ptr(), pz, zs, dx.data_ptr() if need_dx else 0, k,
             dw.data_ptr() if need_dweight else 0, k, wide * k, db.data_ptr() if bias else 0)
     L = lib()
     if act or bias:
