@@ -183,6 +183,26 @@ __device__ __forceinline__ void load_mn(uint32_t dst, const CUtensorMap* map, bo
   }
 }
 
+// ---- warp-level MMA (the bias gradient's column sums)
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t saddr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(saddr)
+               : "memory");
+}
+template <bool BF16> __device__ __forceinline__ void mma_ones(float (&d)[4], uint32_t one, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(one), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(one), "r"(b0), "r"(b1));
+}
+
 // ---- clusters
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -554,20 +574,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     wait_or_abort(&bar_drain, 0, &never, nullptr);
   } else if (warp < kEpiWarp0) {
     // ============================== dW: column sums of dz, the bias gradient
-    // Warp w takes the 64-column boxes w - 2, w, ... of this CTA's columns;
-    // lane 8r + c sums columns 8c .. 8c + 7 of rows r, r + 4, ...: rows in
-    // order, then the four lanes of a column, so a fixed order.  Only the
-    // first feature tile's CTAs sum; the others release the stages.
+    // Warp w takes the 64-column boxes w - 2, w, ... of this CTA's columns:
+    // ones (16 x 16) times 16 k rows on the warp-level MMA, accumulated in
+    // fp32 over the rows in order.  The rows of a last partial 16 are added
+    // one at a time (those after them may hold anything).  Only the first
+    // feature tile's CTAs sum; the others release the stages.
     if constexpr (PROD == kProdWeight) {
       if (sums) {
         constexpr int kBoxes = PAIR ? 1 : 2;
+        constexpr uint32_t kOnes = BF16 ? 0x3f803f80u : 0x3c003c00u;
         bool ok = true;
         int st = 0, ph = 0;
         for (int idx = unit; idx < tiles && ok; idx += units) {
           const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, idx, rank);
           const int part = t.n / kCtas, col = t.c0 + (PAIR ? rank * part : 0);
           const bool mine = idx % a.m_tiles == 0;
-          float acc[kBoxes][8] = {};
+          // acc[x][n]: columns 8n + 2 (lane & 3), + 1 of box x (the same in every
+          // row of the product); odd: column 2 lane, + 1 of the rows taken singly
+          float acc[kBoxes][8][4] = {}, odd[kBoxes][2] = {};
           for (int b = t.kb0; b < t.kb1; ++b) {
             if (!(ok = warp_wait(&bar_full[st], ph, &s_abort, err))) break;
             if (mine) {
@@ -576,15 +600,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               for (int x = 0; x < kBoxes; ++x) {
                 const int box = warp - 2 + 2 * x;
                 if (box * 64 >= part) continue;
-                const unsigned char* p = ring_ptr + st * a.stage_bytes + kMBytes + box * kBoxBytes;
-                for (int r = lane >> 3; r < rows; r += 4) {
-                  const uint4 v = *reinterpret_cast<const uint4*>(p + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-                  const uint32_t wd[4] = {v.x, v.y, v.z, v.w};
+                const uint32_t p = ring + st * a.stage_bytes + kMBytes + box * kBoxBytes;
+                for (int r0 = 0; r0 + 16 <= rows; r0 += 16) {
+                  const int r = r0 + (lane & 15);
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    acc[x][2 * i] += to_f32<BF16>(static_cast<uint16_t>(wd[i]));
-                    acc[x][2 * i + 1] += to_f32<BF16>(static_cast<uint16_t>(wd[i] >> 16));
+                  for (int n = 0; n < 4; ++n) {  // 16 columns: two matrices of each 8 rows
+                    uint32_t f[4];
+                    ldmatrix_trans(f, p + r * 128 + (((2 * n + (lane >> 4)) ^ (r & 7)) << 4));
+                    mma_ones<BF16>(acc[x][2 * n], kOnes, f[0], f[1]);
+                    mma_ones<BF16>(acc[x][2 * n + 1], kOnes, f[2], f[3]);
                   }
+                }
+                const unsigned char* q = ring_ptr + st * a.stage_bytes + kMBytes + box * kBoxBytes;
+                for (int r = rows & ~15; r < rows; ++r) {
+                  const uint32_t v = *reinterpret_cast<const uint32_t*>(q + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
+                                                                        (lane & 3) * 4);
+                  odd[x][0] += to_f32<BF16>(static_cast<uint16_t>(v));
+                  odd[x][1] += to_f32<BF16>(static_cast<uint16_t>(v >> 16));
                 }
               }
             }
@@ -596,14 +628,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int x = 0; x < kBoxes; ++x) {
               const int box = warp - 2 + 2 * x;
+              // lane 4n + j holds the columns 8n + 2j, + 1 of its group n
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                float v = acc[x][i];
-                v += __shfl_xor_sync(0xffffffffu, v, 8);
-                v += __shfl_xor_sync(0xffffffffu, v, 16);
-                const int n = col + box * 64 + (lane & 7) * 8 + i;
-                if (lane < 8 && box * 64 < part && n < a.l.n)
-                  a.dbias[static_cast<int64_t>(t.e) * a.l.n + n] = from_f32<BF16>(v);
+              for (int n = 0; n < 8; ++n) {
+                if (lane >> 2 == n) {
+                  odd[x][0] += acc[x][n][0];
+                  odd[x][1] += acc[x][n][1];
+                }
+              }
+              const int c = col + box * 64 + 2 * lane;
+              if (box * 64 < part) {
+                uint16_t* db = a.dbias + static_cast<int64_t>(t.e) * a.l.n + c;
+                if (c < a.l.n) db[0] = from_f32<BF16>(odd[x][0]);
+                if (c + 1 < a.l.n) db[1] = from_f32<BF16>(odd[x][1]);
               }
             }
           }
