@@ -107,11 +107,12 @@ template <bool BF16, int V> auto act_backward_for(int act) {
   }
 }
 
-constexpr int kSumCols = 64;  // columns of a block: two a lane
+constexpr int kSumCols = 256;  // columns of a block: eight a lane
 
+// vec: every row starts on a 16-byte boundary.
 template <bool BF16>
 __global__ void __launch_bounds__(256) bias_grad_kernel(const LinearGradArgs a, const uint16_t* src, int64_t stride,
-                                                        bool pairs) {
+                                                        bool vec) {
   __shared__ int s_off[kMaxGroups + 1], s_pre[kMaxGroups + 1], s_tot[64];
   __shared__ float s_sum[8][kSumCols];
   pdl_wait();
@@ -125,29 +126,28 @@ __global__ void __launch_bounds__(256) bias_grad_kernel(const LinearGradArgs a, 
     const int es = static_cast<int>(it / col_blocks), e = es / a.splits, sp = es - e * a.splits;
     const int cnt = s_off[e + 1] - s_off[e], per = (cnt + a.splits - 1) / a.splits;
     const int r0 = min(sp * per, cnt), r1 = min(r0 + per, cnt);
-    const int c = cb * kSumCols + 2 * lane;
-    float x0 = 0.0f, x1 = 0.0f;
-    if (c < a.n) {
-      const uint16_t* p = src + static_cast<int64_t>(s_off[e]) * stride + c;
-      const bool two = c + 1 < a.n;
+    const int c = cb * kSumCols + 8 * lane;
+    float x[8] = {};
+    const uint16_t* p = src + static_cast<int64_t>(s_off[e]) * stride + c;
+    if (vec && c + 8 <= a.n) {
 #pragma unroll 4
       for (int r = r0 + warp; r < r1; r += 8) {
-        const uint16_t* q = p + r * stride;
-        if (pairs && two) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(q);
-          x0 += to_f32<BF16>(static_cast<uint16_t>(w));
-          x1 += to_f32<BF16>(static_cast<uint16_t>(w >> 16));
-        } else {
-          x0 += to_f32<BF16>(q[0]);
-          if (two) x1 += to_f32<BF16>(q[1]);
-        }
+        float f[8];
+        unpack8<BF16>(*reinterpret_cast<const uint4*>(p + r * stride), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += f[i];
       }
+    } else {
+      for (int r = r0 + warp; r < r1; r += 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < a.n) x[i] += to_f32<BF16>(p[r * stride + i]);
     }
-    s_sum[warp][2 * lane] = x0;
-    s_sum[warp][2 * lane + 1] = x1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_sum[warp][8 * lane + i] = x[i];
     __syncthreads();
     const int col = cb * kSumCols + threadIdx.x;
-    if (threadIdx.x < kSumCols && col < a.n) {
+    if (col < a.n) {
       float v = 0.0f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) v += s_sum[w][threadIdx.x];
@@ -195,10 +195,9 @@ cudaError_t launch_act_backward(const LinearGradArgs& a, cudaStream_t st) {
 cudaError_t launch_bias_grad(const LinearGradArgs& a, cudaStream_t st) {
   const uint16_t* src = static_cast<const uint16_t*>(a.preact ? a.dz : a.dy);
   const int64_t stride = a.preact ? a.dz_stride : a.dy_stride;
-  const bool pairs = (reinterpret_cast<uintptr_t>(src) & 3) == 0 && stride % 2 == 0;
   const int64_t items = static_cast<int64_t>(a.groups) * a.splits * ((a.n + kSumCols - 1) / kSumCols);
   auto kern = a.bf16 ? bias_grad_kernel<true> : bias_grad_kernel<false>;
-  cudaError_t e = launch_pdl(kern, dim3(grid_for(items, 148 * 8)), dim3(256), 0, st, a, src, stride, pairs);
+  cudaError_t e = launch_pdl(kern, dim3(grid_for(items, 148 * 8)), dim3(256), 0, st, a, src, stride, on16(src, stride));
   if (e != cudaSuccess || a.splits <= 1) return e;
   auto join = a.bf16 ? bias_join_kernel<true> : bias_join_kernel<false>;
   return launch_pdl(join, dim3(grid_for((static_cast<int64_t>(a.groups) * a.n + 255) / 256, 148 * 8)), dim3(256), 0,

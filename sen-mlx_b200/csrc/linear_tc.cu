@@ -59,6 +59,7 @@ constexpr int kTurnStride = 36;          // 32-bit words between column pairs of
 constexpr uint32_t kRingBudget = 192 * 1024;
 constexpr uint32_t kRingBudgetGated = 176 * 1024;  // beside the gated exchange (16 KB)
 constexpr int kMaxSplit = 8;
+constexpr int kSumPieces = 4;  // bias gradient inside dW: most 8-column pieces of a warp
 
 __device__ int g_linear_error;           // first device error of the linear kernels on this device
 
@@ -181,26 +182,6 @@ __device__ __forceinline__ void load_mn(uint32_t dst, const CUtensorMap* map, bo
   } else {
     for (int i = 0; i < boxes; ++i) tma_4d<PAIR>(dst + i * kBoxBytes, map, f0 + 64 * i, k0, 0, e, bar);
   }
-}
-
-// ---- warp-level MMA (the bias gradient's column sums)
-__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t saddr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(saddr)
-               : "memory");
-}
-template <bool BF16> __device__ __forceinline__ void mma_ones(float (&d)[4], uint32_t one, uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, "
-                 "{%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(one), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%4,%4,%4}, {%5,%6}, "
-                 "{%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(one), "r"(b0), "r"(b1));
 }
 
 // ---- clusters
@@ -574,49 +555,43 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     wait_or_abort(&bar_drain, 0, &never, nullptr);
   } else if (warp < kEpiWarp0) {
     // ============================== dW: column sums of dz, the bias gradient
-    // Warp w takes the 64-column boxes w - 2, w, ... of this CTA's columns:
-    // ones (16 x 16) times 16 k rows on the warp-level MMA, accumulated in
-    // fp32 over the rows in order.  The rows of a last partial 16 are added
-    // one at a time (those after them may hold anything).  Only the first
-    // feature tile's CTAs sum; the others release the stages.
+    // Every feature tile of a column tile loads the same dz, so the column
+    // tile's 8-column pieces are dealt to its feature tiles (piece c to tile c
+    // mod m_tiles) and there to these two warps: a CTA adds few columns a
+    // block and keeps pace with the MMAs (one tile adding all of them took
+    // three times as long as its MMAs), and no sums cross CTAs.  Lane l adds
+    // rows l, l + 32, ... in fp32, then the lanes are added, all in a fixed
+    // order.  (As ones times dz on the warp-level MMA the sums held up the
+    // tcgen05 MMAs: 871 cycles a block of 64 rows instead of 535.)
     if constexpr (PROD == kProdWeight) {
       if (sums) {
-        constexpr int kBoxes = PAIR ? 1 : 2;
-        constexpr uint32_t kOnes = BF16 ? 0x3f803f80u : 0x3c003c00u;
         bool ok = true;
         int st = 0, ph = 0;
         for (int idx = unit; idx < tiles && ok; idx += units) {
           const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, idx, rank);
           const int part = t.n / kCtas, col = t.c0 + (PAIR ? rank * part : 0);
-          const bool mine = idx % a.m_tiles == 0;
-          // acc[x][n]: columns 8n + 2 (lane & 3), + 1 of box x (the same in every
-          // row of the product); odd: column 2 lane, + 1 of the rows taken singly
-          float acc[kBoxes][8][4] = {}, odd[kBoxes][2] = {};
+          const int c0 = idx % a.m_tiles + a.m_tiles * (warp - 2);  // first piece of this CTA's columns
+          float acc[kSumPieces][8] = {};
           for (int b = t.kb0; b < t.kb1; ++b) {
             if (!(ok = warp_wait(&bar_full[st], ph, &s_abort, err))) break;
-            if (mine) {
-              const int rows = min(kBK, t.k - b * kBK);
+            const int rows = min(kBK, t.k - b * kBK);
+            const unsigned char* base = ring_ptr + st * a.stage_bytes + kMBytes;
 #pragma unroll
-              for (int x = 0; x < kBoxes; ++x) {
-                const int box = warp - 2 + 2 * x;
-                if (box * 64 >= part) continue;
-                const uint32_t p = ring + st * a.stage_bytes + kMBytes + box * kBoxBytes;
-                for (int r0 = 0; r0 + 16 <= rows; r0 += 16) {
-                  const int r = r0 + (lane & 15);
+            for (int j = 0; j < kSumPieces; ++j) {
+              const int c = c0 + 2 * j * a.m_tiles;
+              if (8 * c >= part) break;
 #pragma unroll
-                  for (int n = 0; n < 4; ++n) {  // 16 columns: two matrices of each 8 rows
-                    uint32_t f[4];
-                    ldmatrix_trans(f, p + r * 128 + (((2 * n + (lane >> 4)) ^ (r & 7)) << 4));
-                    mma_ones<BF16>(acc[x][2 * n], kOnes, f[0], f[1]);
-                    mma_ones<BF16>(acc[x][2 * n + 1], kOnes, f[2], f[3]);
+              for (int h = 0; h < kBK / 32; ++h) {
+                const int r = 32 * h + lane;
+                if (r < rows) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(base + (c >> 3) * kBoxBytes + r * 128 +
+                                                                  (((c & 7) ^ (r & 7)) << 4));
+                  const uint32_t wd[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    acc[j][2 * i] += to_f32<BF16>(static_cast<uint16_t>(wd[i]));
+                    acc[j][2 * i + 1] += to_f32<BF16>(static_cast<uint16_t>(wd[i] >> 16));
                   }
-                }
-                const unsigned char* q = ring_ptr + st * a.stage_bytes + kMBytes + box * kBoxBytes;
-                for (int r = rows & ~15; r < rows; ++r) {
-                  const uint32_t v = *reinterpret_cast<const uint32_t*>(q + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
-                                                                        (lane & 3) * 4);
-                  odd[x][0] += to_f32<BF16>(static_cast<uint16_t>(v));
-                  odd[x][1] += to_f32<BF16>(static_cast<uint16_t>(v >> 16));
                 }
               }
             }
@@ -624,25 +599,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (lane == 0) mbar_arrive(&bar_empty[st]);
             next(st, ph);
           }
-          if (mine && ok) {
+          if (!ok) break;
 #pragma unroll
-            for (int x = 0; x < kBoxes; ++x) {
-              const int box = warp - 2 + 2 * x;
-              // lane 4n + j holds the columns 8n + 2j, + 1 of its group n
+          for (int j = 0; j < kSumPieces; ++j) {
+            const int c = c0 + 2 * j * a.m_tiles;
+            if (8 * c >= part) break;
+            // halves of the warp swap halves of the columns, until lane 4i has column i
+            float v4[4], v2[2];
 #pragma unroll
-              for (int n = 0; n < 8; ++n) {
-                if (lane >> 2 == n) {
-                  odd[x][0] += acc[x][n][0];
-                  odd[x][1] += acc[x][n][1];
-                }
-              }
-              const int c = col + box * 64 + 2 * lane;
-              if (box * 64 < part) {
-                uint16_t* db = a.dbias + static_cast<int64_t>(t.e) * a.l.n + c;
-                if (c < a.l.n) db[0] = from_f32<BF16>(odd[x][0]);
-                if (c + 1 < a.l.n) db[1] = from_f32<BF16>(odd[x][1]);
-              }
+            for (int i = 0; i < 4; ++i) {
+              const bool up = lane & 16;
+              v4[i] = (up ? acc[j][i + 4] : acc[j][i]) +
+                      __shfl_xor_sync(0xffffffffu, up ? acc[j][i] : acc[j][i + 4], 16);
             }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const bool up = lane & 8;
+              v2[i] = (up ? v4[i + 2] : v4[i]) + __shfl_xor_sync(0xffffffffu, up ? v4[i] : v4[i + 2], 8);
+            }
+            float v = (lane & 4 ? v2[1] : v2[0]) + __shfl_xor_sync(0xffffffffu, lane & 4 ? v2[0] : v2[1], 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            const int n = col + 8 * c + (lane >> 2);
+            if ((lane & 3) == 0 && n < a.l.n) a.dbias[static_cast<int64_t>(t.e) * a.l.n + n] = from_f32<BF16>(v);
           }
         }
       }
@@ -696,15 +675,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           float* mine = s_swap[ew];
           const float* theirs = s_swap[ew ^ 2];
           const int bar = 1 + (turn2 * 2 + (q & 1));
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mine[i * 32 + lane] = gate ? z[1][i] : z[0][i];
-          asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
           float y[16], u[16];
+          if (gate) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float v = theirs[i * 32 + lane];
-            y[i] = gate ? z[0][i] : v;
-            u[i] = gate ? v : z[1][i];
+            for (int i = 0; i < 16; ++i) mine[i * 32 + lane] = z[1][i];
+            asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              y[i] = z[0][i];
+              u[i] = theirs[i * 32 + lane];
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mine[i * 32 + lane] = z[0][i];
+            asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              y[i] = theirs[i * 32 + lane];
+              u[i] = z[1][i];
+            }
           }
           asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
           act_chunk(a.l.act, y);
@@ -733,7 +722,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else {
     // ============== K split: this CTA's accumulator to shared memory (the
-    // ring, which the MMAs have read by then), [column][lane]
+    // ring, which the MMAs have read by then), [column][lane]: a
+    // warp's loads of it from another CTA are whole lines
     const int ew = warp - kEpiWarp0, q = warp & 3;
     if (unit < tiles) {
       const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
@@ -763,42 +753,56 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (csize > 1) {
       cluster_sync();  // every share is in shared memory
       if (warp >= kEpiWarp0 && unit < tiles) {
-        // items of four columns and 32 features, dealt to the cluster's warps;
-        // an item's loads are all in flight together, then added in rank order
+        // items of 32 features and 16 columns, or 8 where that gives every warp
+        // of the cluster one at most; shares added in rank order
         const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
         const int ew = warp - kEpiWarp0;
         const Finish<PROD, GATED, BF16> fin(a.l, s_turn[ew], lane);
         constexpr int kQuarters = GATED ? 2 : 4;
-        const int items = (t.w + 3) / 4 * kQuarters;
+        const int step = (t.w + 7) / 8 * kQuarters <= csize * kEpiWarps ? 8 : 16;
+        const int items = (t.w + step - 1) / step * kQuarters;
         for (int i = ew * csize + rank; i < items; i += csize * kEpiWarps) {
-          const int q = i % kQuarters, c = i / kQuarters * 4, w = min(4, t.w - c);
+          const int q = i % kQuarters, c = i / kQuarters * step, w = min(step, t.w - c);
           const int f0 = t.m0 + q * 32, feats = min(32, fin.cols - f0);
           const float b0 = fin.bias(t.e, f0, feats, 0), b1 = GATED ? fin.bias(t.e, f0, feats, fin.cols) : 0.0f;
-          float v[kMaxSplit][GATED ? 8 : 4];
+          float z[16], u[16];
 #pragma unroll
-          for (int r = 0; r < kMaxSplit; ++r) {
-            if (r >= csize) break;
-            const uint32_t src = map_rank(ring + (c * 128 + q * 32 + lane) * 4, r);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              v[r][k] = k < w ? ld_cluster(src + k * 512) : 0.0f;
-              if constexpr (GATED) v[r][4 + k] = k < w ? ld_cluster(src + k * 512 + 256) : 0.0f;
-            }
+          for (int k = 0; k < 16; ++k) {
+            z[k] = b0;
+            u[k] = b1;
           }
-          float z[16] = {}, u[16] = {};
+          // 8 columns of every CTA in flight together (the rows past w are there, unused)
 #pragma unroll
-          for (int r = 0; r < kMaxSplit; ++r) {
-            if (r >= csize) break;
+          for (int k0 = 0; k0 < 16; k0 += 8) {
+            if (k0 >= w) break;
+            constexpr int kGroup = GATED ? 2 : 4;  // CTAs whose loads are in flight together
+            float sum[8] = {}, sum2[8] = {};
+            for (int r0 = 0; r0 < csize; r0 += kGroup) {
+              float v[kGroup][8], v2[GATED ? kGroup : 1][8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              z[k] += v[r][k];
-              if constexpr (GATED) u[k] += v[r][4 + k];
+              for (int r = 0; r < kGroup; ++r) {
+                const uint32_t src = map_rank(ring + ((c + k0) * 128 + q * 32 + lane) * 4, min(r0 + r, csize - 1));
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  v[r][k] = ld_cluster(src + k * 512);
+                  if constexpr (GATED) v2[r][k] = ld_cluster(src + k * 512 + 256);
+                }
+              }
+#pragma unroll
+              for (int r = 0; r < kGroup; ++r) {
+                if (r0 + r >= csize) break;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  sum[k] += v[r][k];
+                  if constexpr (GATED) sum2[k] += v2[r][k];
+                }
+              }
             }
-          }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            z[k] += b0;
-            u[k] += b1;
+            for (int k = 0; k < 8; ++k) {
+              z[k0 + k] += sum[k];
+              u[k0 + k] += sum2[k];
+            }
           }
           if constexpr (PROD == kProdForward) {
             const int64_t row = t.c0 + c;
@@ -807,7 +811,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             act_chunk(a.l.act, z);
             if constexpr (GATED) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) z[k] *= u[k];
+              for (int k = 0; k < 16; ++k) z[k] *= u[k];
             }
           }
           fin.write(z, t.e, t.c0 + c, f0, w, feats);
@@ -897,8 +901,9 @@ struct Plan {
 
 // Estimate of one form.  A k block of 64 costs the larger of its MMAs (8
 // cycles a 16-column step and K step of 16) and its operands' way from L2
-// (kL2Bytes a cycle and SM); tiles run in waves over the SMs.
-constexpr double kL2Bytes = 55, kTileCycles = 900, kSplitCycles = 1800;
+// (kL2Bytes a cycle and SM); tiles run in waves over the SMs.  A K split adds
+// a cluster's barriers and its shares' way between SMs.
+constexpr double kL2Bytes = 57, kTileCycles = 900, kSplitCycles = 2000, kSplitColumn = 20;
 
 Plan make_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, bool pair, int bn, int split) {
   Plan q;
@@ -937,7 +942,7 @@ Plan make_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, bool p
   const double slots = static_cast<double>(sms / ((pair ? 2 : 1) * split));
   double waves = chunks * m_tiles / slots;
   waves = waves < 8 ? static_cast<double>(static_cast<int64_t>(waves + 0.999)) : waves;
-  q.cycles = waves * (blocks / split * per + kTileCycles) + (split > 1 ? kSplitCycles : 0);
+  q.cycles = waves * (blocks / split * per + kTileCycles) + (split > 1 ? kSplitCycles + kSplitColumn * n : 0);
   return q;
 }
 
@@ -985,14 +990,14 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, voi
   if (plan.cycles == 0) return cudaErrorNotSupported;  // too many tiles for the K split asked for
   TcArgs a{};
   a.l = l;
-  // a K split leaves each CTA part of a column's rows: no sums there
-  a.dbias = p == kProdWeight && plan.split == 1 ? static_cast<uint16_t*>(dbias) : nullptr;
-  if (summed) *summed = a.dbias != nullptr;
   a.bn = plan.bn;
   a.split = plan.split;
   const int features = p == kProdForward ? (gated ? l.n / 2 : l.n) : l.k;
   const int feat = (gated ? 64 : 128) * (plan.pair ? 2 : 1);
   a.m_tiles = (features + feat - 1) / feat;
+  // a K split leaves each CTA part of a column's rows: no sums there
+  a.dbias = p == kProdWeight && plan.split == 1 && a.m_tiles * 2 * kSumPieces * 8 >= (plan.pair ? a.bn / 2 : a.bn) ? static_cast<uint16_t*>(dbias) : nullptr;
+  if (summed) *summed = a.dbias != nullptr;
   a.n_tiles = p == kProdWeight ? (l.n + a.bn - 1) / a.bn : 0;
   a.part = plan.pair ? a.bn / 2 : a.bn;
   a.stage_bytes = kMBytes + a.part * 128;
