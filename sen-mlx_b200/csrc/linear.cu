@@ -90,37 +90,6 @@ bool few_rows(const LinearArgs& a) {
   return a.rows <= kFewRows * a.groups && chunks * ((a.n + 15) / 16) <= kFewBlocks;
 }
 
-// Rows of a dense product that leave the tcgen05 tiles for the few-row kernel:
-// those past a multiple of 256, the widest tile, where the estimate says that
-// the wave of tiles they would start costs more than W's second way from L2
-// (kSmallBytes a cycle) and a launch.
-constexpr double kSmallBytes = 148 * 24.0, kSmallCycles = 4000;
-int64_t last_rows(const LinearArgs& a) {
-  const int64_t tail = a.rows % 256;
-  if (a.offsets || a.rows < 256 || tail == 0 || tail > kFewRows || !linear_small_supported(a)) return 0;
-  LinearArgs most = a;
-  most.rows -= tail;
-  const double small = kSmallCycles + 2.0 * a.n * a.k / kSmallBytes;
-  return linear_tc_cycles(most, kProdForward) + small < linear_tc_cycles(a, kProdForward) ? tail : 0;
-}
-
-int run_in_two(const char* call, const LinearArgs& a, int64_t tail, cudaStream_t st) {
-  LinearArgs most = a, last = a;
-  most.rows -= tail;
-  last.rows = tail;
-  const auto on = [&](const void* p, int64_t stride) {
-    return p ? static_cast<const char*>(p) + most.rows * stride * 2 : nullptr;
-  };
-  last.a = on(a.a, a.a_stride);
-  last.out = const_cast<char*>(on(a.out, a.out_stride));
-  last.residual = on(a.residual, a.residual_stride);
-  last.preact = const_cast<char*>(on(a.preact, a.preact_stride));
-  const int rc = cuda_status(call, launch_linear_small(last, st));
-  if (rc) return rc;
-  most.beside = 1;  // other rows of the same tensors
-  return cuda_status(call, launch_linear_tc(most, kProdForward, kFormAuto, nullptr, nullptr, st));
-}
-
 int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path, cudaStream_t st,
                 void* dbias = nullptr, bool* summed = nullptr) {
   if (path == SENMOE_LINEAR_ANY) return cuda_status(call, launch_linear_any(a, p, st));
@@ -136,10 +105,6 @@ int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path
   if (force_tc && !tc)
     return reject(SENMOE_ERR_UNSUPPORTED, "%s: TMA needs 16-byte aligned operands, strides of a multiple of 8 elements",
                   call);
-  if (p == kProdForward && path == SENMOE_LINEAR_AUTO && tc) {
-    const int64_t tail = last_rows(a);
-    if (tail > 0) return run_in_two(call, a, tail, st);
-  }
   const int form = path > SENMOE_LINEAR_SMALL ? path - SENMOE_LINEAR_SMALL : kFormAuto;
   return cuda_status(call, tc ? launch_linear_tc(a, p, form, dbias, summed, st) : launch_linear_any(a, p, st));
 }

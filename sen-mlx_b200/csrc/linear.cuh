@@ -225,8 +225,6 @@ bool linear_tc_supported(const LinearArgs& a, LinearProduct p);
 enum LinearForm : int { kFormAuto = 0, kFormOne = 1, kFormPair = 2, kFormSplit = 3 };
 cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, int form, void* dbias, bool* summed,
                              cudaStream_t st);
-// The estimated time of launch_linear_tc, in SM cycles.
-double linear_tc_cycles(const LinearArgs& a, LinearProduct p);
 // Waits for `st`, returns and clears the device error that the tcgen05
 // kernels recorded on the current device (DeviceError).
 cudaError_t linear_device_error(cudaStream_t st, int* error);

@@ -56,8 +56,14 @@ constexpr int kMaxStages = 10;
 constexpr uint32_t kMBytes = 128 * kBK * 2;  // a CTA's M operand of a stage
 constexpr uint32_t kBoxBytes = 64 * 128;     // an MN-major box: 64 features of 64 k
 constexpr int kTurnStride = 36;          // 32-bit words between column pairs of a warp's turning buffer
-constexpr uint32_t kRingBudget = 192 * 1024;
-constexpr uint32_t kRingBudgetGated = 176 * 1024;  // beside the gated exchange (16 KB)
+// Dynamic shared memory: the ring, then each epilogue warp's turning buffer,
+// then (gated) its half of the swap; beside them the static row-group tables
+// and barriers and the ring's alignment.
+constexpr uint32_t kTurnBytes = 8 * kTurnStride * 4, kSwapBytes = 16 * 32 * 4;
+constexpr uint32_t kStaticBytes = 9 * 1024 + 1024;
+constexpr uint32_t epilogue_bytes(bool gated) { return kEpiWarps * (kTurnBytes + (gated ? kSwapBytes : 0)); }
+constexpr uint32_t ring_budget(bool gated) { return 227 * 1024 - kStaticBytes - epilogue_bytes(gated); }
+constexpr int kColStep = kEpiWarps / 4 * 32;  // columns the epilogue warps take between them
 constexpr int kMaxSplit = 8;
 constexpr int kSumPieces = 4;  // bias gradient inside dW: most 8-column pieces of a warp
 
@@ -402,8 +408,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kMaxStages], bar_empty[kMaxStages], bar_accfull[2], bar_accempty[2],
       bar_drain;
-  __shared__ __align__(16) uint32_t s_turn[kEpiWarps][8 * kTurnStride];
-  __shared__ __align__(16) float s_swap[GATED ? kEpiWarps : 1][GATED ? 16 * 32 : 1];
   __shared__ int s_off[kMaxGroups + 1], s_pre[kMaxGroups + 1], s_tot[64];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
@@ -414,6 +418,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t ring = (raw + 1023u) & ~1023u;
   unsigned char* ring_ptr = smem_raw + (ring - raw);
   const int stages = a.stages;
+  unsigned char* epi_ptr = ring_ptr + stages * a.stage_bytes;
+  const auto turn_of = [&](int ew) { return reinterpret_cast<uint32_t*>(epi_ptr + ew * kTurnBytes); };
+  const auto swap_of = [&](int ew) { return reinterpret_cast<float*>(epi_ptr + kEpiWarps * kTurnBytes + ew * kSwapBytes); };
   const int csize = PAIR ? 2 : a.split;  // CTAs of the cluster
   const int rank = csize > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int unit = blockIdx.x / csize, units = gridDim.x / csize;
@@ -628,9 +635,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else if (PAIR || a.split <= 1) {
     // ============================================================ epilogue
-    // 32 columns at a time, the two warps of a lane quarter in turn
+    // 32 columns at a time, the warps of a lane quarter in turn
     const int ew = warp - kEpiWarp0, q = warp & 3, turn2 = ew >> 2;
-    const Finish<PROD, GATED, BF16> fin(a.l, s_turn[ew], lane);
+    const Finish<PROD, GATED, BF16> fin(a.l, turn_of(ew), lane);
     int it = 0;
     for (int idx = unit; idx < tiles; idx += units, ++it) {
       const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, idx, rank);
@@ -647,7 +654,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + ab * 256;
       const uint32_t release = PAIR ? map_rank(smem_u32(&bar_accempty[ab]), 0) : smem_u32(&bar_accempty[ab]);
       bool released = false;
-      for (int c = turn2 * 32; c < t.w; c += 64) {
+      for (int c = turn2 * 32; c < t.w; c += kColStep) {
         uint32_t r[32];
         if (PROD == kProdWeight && t.k == 0) {
 #pragma unroll
@@ -657,7 +664,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tmem_ld16(acc + c + 16, r + 16);
           tmem_ld_wait();
         }
-        if (c + 64 >= t.w) {  // this warp's last read of the accumulator
+        if (c + kColStep >= t.w) {  // this warp's last read of the accumulator
           tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_at(release);
@@ -672,8 +679,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int h = 0; h < 2; ++h) fin.keep(z[h], row + 16 * h, up + f0, t.w - c - 16 * h, feats);
           // gate warps finish columns c .. c + 15 and hand the others over, up warps the reverse
           const bool gate = q < 2;
-          float* mine = s_swap[ew];
-          const float* theirs = s_swap[ew ^ 2];
+          float* mine = swap_of(ew);
+          const float* theirs = swap_of(ew ^ 2);
           const int bar = 1 + (turn2 * 2 + (q & 1));
           float y[16], u[16];
           if (gate) {
@@ -731,7 +738,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_after();
         const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16);
         float* dst = reinterpret_cast<float*>(ring_ptr) + q * 32 + lane;
-        for (int c = (ew >> 2) * 16; c < t.w; c += 32) {
+        for (int c = (ew >> 2) * 16; c < t.w; c += kColStep / 2) {
           uint32_t r[16];
           if (t.kb1 > t.kb0) {
             tmem_ld16(acc + c, r);
@@ -757,7 +764,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // of the cluster one at most; shares added in rank order
         const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
         const int ew = warp - kEpiWarp0;
-        const Finish<PROD, GATED, BF16> fin(a.l, s_turn[ew], lane);
+        const Finish<PROD, GATED, BF16> fin(a.l, turn_of(ew), lane);
         constexpr int kQuarters = GATED ? 2 : 4;
         const int step = (t.w + 7) / 8 * kQuarters <= csize * kEpiWarps ? 8 : 16;
         const int items = (t.w + step - 1) / step * kQuarters;
@@ -973,10 +980,6 @@ Plan choose_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, int 
 
 }  // namespace
 
-double linear_tc_cycles(const LinearArgs& l, LinearProduct p) {
-  return choose_plan(l, p, p == kProdForward && act_gated(l.act), tc_sm_count(), kFormAuto).cycles;
-}
-
 bool linear_tc_supported(const LinearArgs& a, LinearProduct p) {
   const bool w_ok = p == kProdWeight ? tma_ok(a.b, a.b_stride, 0, 1) : tma_ok(a.b, a.b_stride, a.b_group_stride, a.groups);
   return a.rows > 0 && w_ok && tma_ok(a.a, a.a_stride, 0, 1);
@@ -1001,7 +1004,7 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, voi
   a.n_tiles = p == kProdWeight ? (l.n + a.bn - 1) / a.bn : 0;
   a.part = plan.pair ? a.bn / 2 : a.bn;
   a.stage_bytes = kMBytes + a.part * 128;
-  a.stages = static_cast<int>((gated ? kRingBudgetGated : kRingBudget) / a.stage_bytes);
+  a.stages = static_cast<int>(ring_budget(gated) / a.stage_bytes);
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   a.tmem_cols = 512;
   const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
@@ -1017,7 +1020,7 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, voi
     if (need < a.stages) a.stages = need;
     while (a.tmem_cols / 2 >= static_cast<uint32_t>(a.bn) && a.tmem_cols > 32) a.tmem_cols /= 2;
   }
-  const size_t smem = 1024 + static_cast<size_t>(a.stages) * a.stage_bytes;
+  const size_t smem = 1024 + static_cast<size_t>(a.stages) * a.stage_bytes + epilogue_bytes(gated);
 
   CUtensorMap tm{}, tn{}, half{};
   cudaError_t e;
