@@ -55,7 +55,7 @@ __device__ __forceinline__ uint4 load_x(const uint16_t* p, bool live) {
 template <bool BF16, bool GATED, int NT>
 __global__ void __launch_bounds__(kWarps * 32) linear_small_kernel(const __grid_constant__ LinearArgs a) {
   constexpr int kFeat = GATED ? kRows / 2 : kRows;  // features of a block
-  constexpr int kSteps = 4;  // K steps whose loads are in flight together
+  constexpr int kSteps = NT > 2 ? 2 : 4;  // K steps whose loads, of W and of the rows, are in flight together
   __shared__ float s_part[kWarps / 2][kRows][NT * 8 + 1];
   __shared__ int s_sum[kWarps], s_tile[3];  // group, first row, rows
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -134,23 +134,23 @@ __global__ void __launch_bounds__(kWarps * 32) linear_small_kernel(const __grid_
   const bool live0 = f0 + g < features, live1 = GATED ? live0 : f0 + g + 8 < features;
   float acc[NT][4] = {};
   for (int s0 = warp * 32; s0 < a.k; s0 += kWarps * 32 * kSteps) {
-    uint4 wa[kSteps][2], xb[kSteps];
+    uint4 wa[kSteps][2], xb[kSteps][NT];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int c = s0 + s * kWarps * 32;
       const bool in = c + 8 * t4 < a.k;
       wa[s][0] = load_w(w0 + c, live0 && in);
       wa[s][1] = load_w(w1 + c, live1 && in);
-      xb[s] = load_x(x0 + c, g < rows && in);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) xb[s][n] = load_x(x0 + n * 8 * a.a_stride + c, n * 8 + g < rows && in);
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int c = s0 + s * kWarps * 32;
       if (c >= a.k) break;
-      const bool in = c + 8 * t4 < a.k;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const uint4 b = n == 0 ? xb[s] : load_x(x0 + n * 8 * a.a_stride + c, n * 8 + g < rows && in);
+        const uint4 b = xb[s][n];
         mma16816<BF16>(acc[n], wa[s][0].x, wa[s][1].x, wa[s][0].y, wa[s][1].y, b.x, b.y);
         mma16816<BF16>(acc[n], wa[s][0].z, wa[s][1].z, wa[s][0].w, wa[s][1].w, b.z, b.w);
       }

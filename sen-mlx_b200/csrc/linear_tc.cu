@@ -64,7 +64,10 @@ constexpr uint32_t kStaticBytes = 9 * 1024 + 1024;
 constexpr uint32_t epilogue_bytes(bool gated) { return kEpiWarps * (kTurnBytes + (gated ? kSwapBytes : 0)); }
 constexpr uint32_t ring_budget(bool gated) { return 227 * 1024 - kStaticBytes - epilogue_bytes(gated); }
 constexpr int kColStep = kEpiWarps / 4 * 32;  // columns the epilogue warps take between them
-constexpr int kMaxSplit = 8;
+// Largest K split, and how many clusters of that size are resident at once
+// (of 148 SMs; cudaOccupancyMaxActiveClusters): one more would wait for a
+// whole round.  Clusters of 8 (15 at once) were slower than 4 wherever both fit.
+constexpr int kMaxSplit = 4, kMaxQuads = 33;
 constexpr int kSumPieces = 4;  // bias gradient inside dW: most 8-column pieces of a warp
 
 __device__ int g_linear_error;           // first device error of the linear kernels on this device
@@ -968,7 +971,7 @@ Plan choose_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, int 
       if (form != kFormSplit && (best.cycles == 0 || q.cycles < best.cycles)) best = q;
       if (pair || form == kFormOne) continue;
       for (int s = 2; s <= kMaxSplit; s *= 2) {
-        if (q.tiles * s > sms) break;
+        if (q.tiles > (s == 2 ? sms / 2 : kMaxQuads * sms / 148)) break;
         const Plan t = make_plan(l, p, gated, sms, false, w, s);
         if (best.cycles == 0 || t.cycles < best.cycles) best = t;
       }
