@@ -273,8 +273,6 @@ int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
   }
   bool summed = false;  // dbias came with dweight
   if (g->dweight) {
-    // dW reads what dx reads and writes apart from it; dx waited for dz
-    a.beside = some && g->dx && a.rows > 0;
     a.b = g->x;
     a.b_stride = g->x_stride;
     a.out = g->dweight;

@@ -51,11 +51,6 @@ struct LinearArgs {
   void* preact;                                // forward: z before the activation, or null
   int64_t preact_stride;
   int bf16;                                    // 1: bf16, 0: fp16
-  // 1: the previous launch on the stream reads nothing of this one's outputs
-  // and writes nothing of its inputs, and waited for its own predecessor
-  // before it let dependents start: this launch need not wait for it before
-  // it starts, only before it ends (so that its end still means the other's).
-  int beside;
 };
 
 // 16-bit values by their bit patterns.

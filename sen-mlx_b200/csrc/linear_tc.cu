@@ -82,7 +82,6 @@ struct TcArgs {
   int stages;
   int split;        // K split (one-CTA form): the cluster's size
   uint32_t stage_bytes;  // a stage: the M operand, then the N operand
-  uint32_t tmem_cols;    // 512, or one accumulator where every CTA has one tile
   uint16_t* dbias;  // dW: column sums of dz, [groups, n], or null
 };
 
@@ -130,22 +129,19 @@ template <bool PAIR> __device__ __forceinline__ void umma_commit(uint64_t* bar) 
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
-template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
+// All 512 columns: the ring leaves no room for a second CTA on the SM.
+template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t* dst) {
   if constexpr (PAIR) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
-                 : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   } else {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
-                 : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
 }
-template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
-  if constexpr (PAIR)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
-  else
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t addr) {
+  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(addr) : "memory");
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -446,14 +442,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     prefetch_map(&tm_m);
     prefetch_map(&tm_n);
   }
-  if (warp == 1) tmem_alloc<PAIR>(&s_tmem, a.tmem_cols);
-  if (!a.l.beside) pdl_wait();
-  pdl_launch_dependents();
+  if (warp == 1) tmem_alloc<PAIR>(&s_tmem);
+  pdl_wait();
   // chunks of bn rows; dW has no chunks, only the groups' row ranges
   group_table(a.l.offsets, a.l.groups, a.l.rows, PROD == kProdWeight ? 1 : a.bn, s_off, s_pre, s_tot);
   tc_fence_before();
   __syncthreads();
   if (csize > 1) cluster_sync();  // the other CTAs' barriers exist before anything arrives on them
+  // only now, with this CTA's (or pair's) TMEM held: a dependent's CTA never asks for it first
+  pdl_launch_dependents();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int tiles = a.m_tiles * (PROD == kProdWeight ? a.l.groups * a.n_tiles : s_pre[a.l.groups]);
@@ -844,14 +841,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   }
 
-  if (a.l.beside) pdl_wait();
   tc_fence_before();
   __syncthreads();
   if (csize > 1) cluster_sync();  // nobody reads this CTA's shared memory or TMEM any more
   if (warp == 1) {
     tc_fence_after();
-    tmem_free<PAIR>(tmem, a.tmem_cols);
+    tmem_free<PAIR>(tmem);
   }
+  // A pair frees its TMEM together: neither CTA leaves before both have, or
+  // the SM of the first could take another kernel's CTA, and its allocation,
+  // with the pair's still half undone.
+  __syncwarp();
+  if constexpr (PAIR) cluster_sync();
 }
 
 // ------------------------------------------------------------- host side
@@ -1009,20 +1010,8 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, voi
   a.stage_bytes = kMBytes + a.part * 128;
   a.stages = static_cast<int>(ring_budget(gated) / a.stage_bytes);
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  a.tmem_cols = 512;
   const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
   const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
-  if (plan.tiles <= most) {
-    // One tile a CTA: no more stages than it has K blocks, one accumulator.
-    // What is left of the SM lets the next launch's CTA start its set-up.
-    const int64_t k = p == kProdForward ? l.k : p == kProdInput ? l.n : l.rows;
-    const int64_t blocks = ((k + kBK - 1) / kBK + plan.split - 1) / plan.split;
-    int need = static_cast<int>(blocks < a.stages ? blocks : a.stages);
-    const int room = static_cast<int>((a.bn * 512u + a.stage_bytes - 1) / a.stage_bytes);  // the split's sums lie there
-    if (plan.split > 1 && need < room) need = room;
-    if (need < a.stages) a.stages = need;
-    while (a.tmem_cols / 2 >= static_cast<uint32_t>(a.bn) && a.tmem_cols > 32) a.tmem_cols /= 2;
-  }
   const size_t smem = 1024 + static_cast<size_t>(a.stages) * a.stage_bytes + epilogue_bytes(gated);
 
   CUtensorMap tm{}, tn{}, half{};
