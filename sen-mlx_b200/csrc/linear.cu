@@ -65,10 +65,10 @@ int check_shape(const char* call, int32_t dtype, int32_t epilogue, int32_t group
   *wide = epilogue >= SENMOE_EPI_SWIGLU ? 2 * out : out;
   if (in < 1 || out < 1 || in > kMaxDim || *wide > kMaxDim)
     return reject(SENMOE_ERR_BAD_ARG, "%s: in_features=%lld out_features=%lld", call, (long long)in, (long long)out);
-  // the kernels count tiles, of 16 rows at least, in 32 bits
+  // the kernels count tiles, of 16 rows at least, in 32 bits, a grid past the last one included
   const int64_t cols = *wide > in ? *wide : in;
-  if (((rows + 15) / 16 + groups) * ((cols + 63) / 64) >= (int64_t(1) << 31) ||
-      groups * ((*wide + 63) / 64) * ((in + 63) / 64) >= (int64_t(1) << 31))
+  if (((rows + 15) / 16 + groups) * ((cols + 63) / 64) >= (int64_t(1) << 30) ||
+      groups * ((*wide + 63) / 64) * ((in + 63) / 64) >= (int64_t(1) << 30))
     return reject(SENMOE_ERR_UNSUPPORTED, "%s: rows=%lld in_features=%lld out_features=%lld is too large", call,
                   (long long)rows, (long long)in, (long long)out);
   return SENMOE_OK;
