@@ -39,6 +39,7 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _CODES = {C.c_int32: "i", C.c_int64: "q", C.c_void_p: "P"}
 _pack_linear = struct.Struct("".join(_CODES[t] for _, t in SenMoeLinear._fields_)).pack
 _pack_grad = struct.Struct("".join(_CODES[t] for _, t in SenMoeLinearGrad._fields_)).pack
+_c_linear = None  # the library's entry, once it is loaded
 _current_device = torch._C._cuda_getDevice
 _current_stream = torch._C._cuda_getCurrentRawStream
 
@@ -48,9 +49,7 @@ def _bad(message: str) -> SenMoeError:
 
 
 def _rows(t: torch.Tensor, n: int) -> tuple[torch.Tensor, int]:
-    """t [..., n] as (rows of n contiguous elements, their stride), itself where the strides allow it."""
-    if t.is_contiguous():
-        return t, n
+    """t [..., n] as (rows of n contiguous elements, their stride), a view where the strides allow one."""
     if t.dim() != 2:
         t = t.reshape(-1, n)
     s0, s1 = t.stride()
@@ -61,19 +60,14 @@ def _rows(t: torch.Tensor, n: int) -> tuple[torch.Tensor, int]:
 
 def _matrices(w: torch.Tensor, n: int, k: int) -> tuple[torch.Tensor, int, int]:
     """w [n, k] or [E, n, k]: (w, row stride, group stride)."""
-    if not w.is_contiguous():
-        s = w.stride()
-        if not (s[-1] != 1 and k > 1 or s[-2] < k and n > 1 or len(s) == 3 and w.shape[0] > 1 and s[0] < n * s[-2]):
-            return w, s[-2] if s[-2] > k else k, s[0] if len(s) == 3 else 0
-        w = w.contiguous()
-    return w, k, n * k
+    s = w.stride()
+    if not (s[-1] != 1 and k > 1 or s[-2] < k and n > 1 or len(s) == 3 and w.shape[0] > 1 and s[0] < n * s[-2]):
+        return w, s[-2] if s[-2] > k else k, s[0] if len(s) == 3 else 0
+    return w.contiguous(), k, n * k
 
 
-def _activation(name: str) -> int:
-    try:
-        return ACTIVATIONS[name]
-    except KeyError:
-        raise _bad(f"activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
+def _no_activation(name) -> SenMoeError:
+    return _bad(f"activation {name!r}: one of {', '.join(ACTIVATIONS)}")
 
 
 def _same(t: torch.Tensor, first: torch.Tensor, dtype, device: int) -> None:
@@ -110,7 +104,9 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
     if stream is not None:  # temporaries and outputs belong to the stream of the launch
         with torch.cuda.stream(stream):
             return _forward(x, weight, offsets, bias, residual, activation, save_preact, None, out, path)
-    act = _activation(activation)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise _no_activation(activation)
     code, device = _operands(x, weight)
     wshape, shape = weight.shape, x.shape
     wide, k = wshape[-2], wshape[-1]
@@ -135,11 +131,17 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
         _same(residual, x, x.dtype, device)
         if residual.shape != shape:
             raise _bad(f"residual {tuple(residual.shape)}, the output is {shape}")
-        residual, rs = _rows(residual, n)
+        rs = n
+        if not residual.is_contiguous():
+            residual, rs = _rows(residual, n)
         pr = residual.data_ptr()
-    x, xs = _rows(x, k)
+    xs = ws = k
+    gs = wide * k
+    if not x.is_contiguous():
+        x, xs = _rows(x, k)
+    if not weight.is_contiguous():
+        weight, ws, gs = _matrices(weight, wide, k)
     rows = x.numel() // k
-    weight, ws, gs = _matrices(weight, wide, k)
     if out is None:
         out = y = x.new_empty(shape)
         ys = n
@@ -154,7 +156,10 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
     if save_preact:
         z = x.new_empty((*lead, wide))
         pz = z.data_ptr()
-    status = lib().senmoe_linear(
+    global _c_linear
+    if _c_linear is None:
+        _c_linear = lib().senmoe_linear
+    status = _c_linear(
         _pack_linear(code, act, groups, path, rows, k, n, x.data_ptr(), xs, weight.data_ptr(), ws, gs,
                      0 if offsets is None else offsets.data_ptr(), pb, pr, rs, y.data_ptr(), ys, pz, wide),
         _current_stream(device))
@@ -192,7 +197,9 @@ def _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dw
     if stream is not None:
         with torch.cuda.stream(stream):
             return _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dweight, None, path)
-    act = _activation(activation)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise _no_activation(activation)
     code, device = _operands(x, dy, weight)
     wshape, xshape = weight.shape, x.shape
     wide, k = wshape[-2], wshape[-1]
