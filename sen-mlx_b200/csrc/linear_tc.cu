@@ -969,11 +969,11 @@ Plan make_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, bool p
 
 // form: kFormAuto, or the only form to consider.
 Plan choose_plan(const LinearArgs& l, LinearProduct p, bool gated, int sms, int form) {
-  static const int kWidths[] = {16, 32, 64, 128, 192, 256};
+  static const int kWidths[] = {16, 32, 64, 96, 128, 160, 192, 224, 256};  // dW: whole 64-feature boxes
   Plan best;
   const int64_t rows = p == kProdWeight ? l.n : l.rows;
   for (int w : kWidths) {
-    if (p == kProdWeight && w < 64) continue;
+    if (p == kProdWeight && w % 64 != 0) continue;
     for (int pair = 0; pair < 2; ++pair) {
       // a pair's CTAs hold at least 32 columns each, in dW two 64-feature boxes
       if (pair && (w < 64 || (p == kProdWeight && w < 256))) continue;
