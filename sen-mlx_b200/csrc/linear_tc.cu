@@ -213,10 +213,8 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -448,19 +446,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     s_abort = 0;
     fence_mbar_init();
   }
-  if (warp == 0 && lane == 0) {  // kernel parameters: readable before the previous grid ends
+  if (warp == 0 && lane == 0) {
     prefetch_map(&tm_m);
     prefetch_map(&tm_n);
   }
-  if (warp == 1) tmem_alloc<PAIR>(&s_tmem);
-  pdl_wait();
   // chunks of bn rows; dW has no chunks, only the groups' row ranges
   group_table(a.l.offsets, a.l.groups, a.l.rows, PROD == kProdWeight ? 1 : a.bn, s_off, s_pre, s_tot);
+  __syncthreads();
+  // the other CTAs run and their barriers exist before anything arrives on
+  // them, and before a pair asks for its TMEM on both SMs
+  if (csize > 1) cluster_sync();
+  if (warp == 1) tmem_alloc<PAIR>(&s_tmem);
   tc_fence_before();
   __syncthreads();
-  if (csize > 1) cluster_sync();  // the other CTAs' barriers exist before anything arrives on them
-  // only now, with this CTA's (or pair's) TMEM held: a dependent's CTA never asks for it first
-  pdl_launch_dependents();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int tiles = a.m_tiles * (PROD == kProdWeight ? a.l.groups * a.n_tiles : s_pre[a.l.groups]);
@@ -738,88 +736,68 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
   } else {
-    // ============== K split: this CTA's accumulator to shared memory (the
-    // ring, which the MMAs have read by then), [column][lane]: a
-    // warp's loads of it from another CTA are whole lines
-    const int ew = warp - kEpiWarp0, q = warp & 3;
-    if (unit < tiles) {
-      const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
-      if (warp_wait(&bar_accfull[0], 0, &s_abort, err)) {
-        tc_fence_after();
-        const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16);
-        float* dst = reinterpret_cast<float*>(ring_ptr) + q * 32 + lane;
-        for (int c = (ew >> 2) * 16; c < t.w; c += kColStep / 2) {
-          uint32_t r[16];
-          if (t.kb1 > t.kb0) {
-            tmem_ld16(acc + c, r);
-            tmem_ld_wait();
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] = 0;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dst[(c + i) * 128] = __uint_as_float(r[i]);
-        }
-        tc_fence_before();
-      }
-    }
+    // =========================== K split: this CTA's accumulator is ready
+    if (unit < tiles) warp_wait(&bar_accfull[0], 0, &s_abort, err);
+    tc_fence_after();
   }
 
   __syncwarp();
   if constexpr (!PAIR) {
     if (csize > 1) {
-      cluster_sync();  // every share is in shared memory
-      if (warp >= kEpiWarp0 && unit < tiles) {
-        // items of 32 features and 16 columns, or 8 where that gives every warp
-        // of the cluster one at most; shares added in rank order
-        const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
-        const int ew = warp - kEpiWarp0;
+      // Chunks of 16 columns are dealt to the cluster's CTAs.  Every CTA sends
+      // its share of a chunk to the chunk's owner, whose ring is free by then
+      // (stores, so nothing waits for a trip between SMs; a warp's 32 lanes
+      // are one line), and the owner adds the shares in rank order:
+      // [its chunk][rank][column][lane].
+      cluster_sync();
+      const bool epi = warp >= kEpiWarp0 && unit < tiles;
+      const int ew = warp - kEpiWarp0;
+      Tile t{};
+      if (epi) t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
+      const int chunks = (t.w + 15) / 16;
+      if (epi) {
+        const int q = warp & 3;
+        const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16);
+        for (int c = ew >> 2; c < chunks; c += kEpiWarps / 4) {
+          uint32_t r[16];
+          if (t.kb1 > t.kb0) {
+            tmem_ld16(acc + 16 * c, r);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = 0;
+          }
+          const uint32_t dst =
+              map_rank(ring + (((c / csize) * csize + rank) * 16 * 128 + q * 32 + lane) * 4, c % csize);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st_cluster(dst + i * 512, r[i]);
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      cluster_sync();  // every share is where it is added
+      if (epi) {
         const Finish<PROD, GATED, BF16> fin(a.l, turn_of(ew), lane);
         constexpr int kQuarters = GATED ? 2 : 4;
-        const int step = (t.w + 7) / 8 * kQuarters <= csize * kEpiWarps ? 8 : 16;
-        const int items = (t.w + step - 1) / step * kQuarters;
-        for (int i = ew * csize + rank; i < items; i += csize * kEpiWarps) {
-          const int q = i % kQuarters, c = i / kQuarters * step, w = min(step, t.w - c);
+        const int mine = chunks > rank ? (chunks - rank + csize - 1) / csize : 0;  // chunks rank, rank + csize, ...
+        for (int i = ew; i < mine * kQuarters; i += kEpiWarps) {
+          const int q = i % kQuarters, slot = i / kQuarters, c = (slot * csize + rank) * 16, w = t.w - c;
           const int f0 = t.m0 + q * 32, feats = min(32, fin.cols - f0);
           const float b0 = fin.bias(t.e, f0, feats, 0), b1 = GATED ? fin.bias(t.e, f0, feats, fin.cols) : 0.0f;
+          const float* src = reinterpret_cast<const float*>(ring_ptr) + slot * csize * 16 * 128 + q * 32 + lane;
           float z[16], u[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            z[k] = b0;
-            u[k] = b1;
-          }
-          // 8 columns of every CTA in flight together (the rows past w are there, unused)
+            float v = 0.0f, v2 = 0.0f;
 #pragma unroll
-          for (int k0 = 0; k0 < 16; k0 += 8) {
-            if (k0 >= w) break;
-            constexpr int kGroup = GATED ? 2 : 4;  // CTAs whose loads are in flight together
-            float sum[8] = {}, sum2[8] = {};
-            for (int r0 = 0; r0 < csize; r0 += kGroup) {
-              float v[kGroup][8], v2[GATED ? kGroup : 1][8];
-#pragma unroll
-              for (int r = 0; r < kGroup; ++r) {
-                const uint32_t src = map_rank(ring + ((c + k0) * 128 + q * 32 + lane) * 4, min(r0 + r, csize - 1));
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  v[r][k] = ld_cluster(src + k * 512);
-                  if constexpr (GATED) v2[r][k] = ld_cluster(src + k * 512 + 256);
-                }
-              }
-#pragma unroll
-              for (int r = 0; r < kGroup; ++r) {
-                if (r0 + r >= csize) break;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  sum[k] += v[r][k];
-                  if constexpr (GATED) sum2[k] += v2[r][k];
-                }
+            for (int r = 0; r < kMaxSplit; ++r) {
+              if (r < csize) {
+                v += src[(r * 16 + k) * 128];
+                if constexpr (GATED) v2 += src[(r * 16 + k) * 128 + 64];
               }
             }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              z[k0 + k] += sum[k];
-              u[k0 + k] += sum2[k];
-            }
+            z[k] = v + b0;
+            u[k] = v2 + b1;
           }
           if constexpr (PROD == kProdForward) {
             const int64_t row = t.c0 + c;
@@ -834,6 +812,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           fin.write(z, t.e, t.c0 + c, f0, w, feats);
         }
       }
+      __syncwarp();
     }
   }
   if constexpr (PROD != kProdWeight) {
@@ -887,19 +866,20 @@ cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorM
   auto kern = linear_tc_kernel<PROD, GATED, BF16, PAIR>;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = PAIR ? 2 : a.split;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  // Launched in plain stream order, unlike the other kernels here: this one
+  // takes the whole SM, TMEM included, so a dependent started early would gain
+  // nothing but a place to wait in.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : a.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kTcThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR || a.split > 1 ? 2 : 1;
+  cfg.numAttrs = PAIR || a.split > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, m, n, half, a);
 }
 
