@@ -83,17 +83,18 @@ int check_group_stride(const char* call, const char* name, int64_t group_stride,
 
 // Whether the few-row kernel is the faster one.  Measured against the tcgen05
 // tiles (us, W from HBM; bf16):
-//   dense 2048 x 2048        8 rows 4.6 / 8.8   32 rows 7.0 / 9.0   64 rows 9.5 / 9.5
-//   dense 2048 x 8192        8 rows 9.0 / 13.2  16 rows 11.1 / 13.3  32 rows 15.0 / 13.2
-//   dense 512 x 2048         64 rows 4.6 / 6.1  96 rows 7.3 / 6.2
+//   dense 2048 x 2048        8 rows 4.6 / 10.5   32 rows 7.0 / 10.7   64 rows 9.5 / 10.7
+//   dense 2048 x 8192        8 rows 9.0 / 15.0   16 rows 11.1 / 14.9  32 rows 15.0 / 15.2
+//   dense 2816 x 2112        32 rows 9.2 / 12.8  64 rows 12.2 / 12.6  96 rows 18.9 / 12.8
+//   dense 512 x 2048         64 rows 4.6 / 7.5   96 rows 7.3 / 7.6
 // Every 16-feature block reads all rows, so rows x W bounds it from 9 rows on.
-//   128 experts, 2048 x 1536 swiglu:  8 rows 12.0 / 17.4  64 rows 59 / 62  128 rows 100 / 86
-//   32 experts, the same:             128 rows 39.8 / 41.6  256 rows 52 / 42
-//   128 experts, 768 x 2048:          8 rows 10.8 / 11.2  16 rows 17.4 / 15.3
+//   128 experts, 2048 x 1536 swiglu:  8 rows 12.1 / 18.0  64 rows 59 / 63  128 rows 100 / 87
+//   32 experts, the same:             128 rows 40.1 / 42.4  256 rows 52 / 42
+//   128 experts, 768 x 2048:          8 rows 10.6 / 11.9  16 rows 17.4 / 16.1
 // Grouped: with few rows a group, while the blocks are few or long (K).
 bool few_rows(const LinearArgs& a) {
   if (!a.offsets)
-    return a.rows <= 8 || (a.rows <= 64 && static_cast<int64_t>(a.n) * a.k * a.rows <= (int64_t(1) << 28));
+    return a.rows <= 8 || (a.rows <= 64 && static_cast<int64_t>(a.n) * a.k * a.rows <= 400000000);
   if (a.rows > 64 && a.rows > 4 * a.groups) return false;
   const int64_t chunks = a.rows < a.groups ? a.rows : a.groups;
   return chunks * ((a.n + 15) / 16) <= (a.k >= 1024 ? 148 * 40 : 148 * 8);

@@ -512,3 +512,20 @@ def test_rows_past_whole_tiles(senmoe, torch, rows, activation):
         copy = y + 0
         R.assert_within(z, zr, zb, "preact")
         R.assert_within(copy, ref, bound, "y")
+
+
+def test_a_long_chain_of_calls(senmoe, torch):
+    """A thousand calls of several kernels each, queued without waiting: the
+    last one's results are the first one's."""
+    s = _make(torch, 1500, 512, 1088, "bfloat16")
+    t = _make(torch, 40, 1024, 512, "bfloat16")
+
+    def calls():
+        y, z = senmoe.linear(s["x"], s["w"], bias=s["b"], activation="gelu", save_preact=True)
+        g = senmoe.linear_backward(s["dy"], s["x"], s["w"], preact=s["z"], activation="gelu", bias=True)
+        return (y, z, *g, senmoe.linear(t["x"], t["w"]), *senmoe.linear_backward(t["dy"], t["x"], t["w"])[:2])
+    first = calls()
+    for _ in range(1000):
+        last = calls()
+    senmoe.linear_check()
+    assert all(torch.equal(a, b) for a, b in zip(first, last))
