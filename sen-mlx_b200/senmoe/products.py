@@ -90,14 +90,13 @@ def _operands(first: torch.Tensor, *others) -> tuple[int, int]:
     return code, device
 
 
-def _groups(offsets: torch.Tensor, weight: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+def _check_groups(offsets: torch.Tensor, weight: torch.Tensor, x: torch.Tensor) -> None:
     if weight.dim() != 3:
         raise _bad(f"weight must be [experts, out, in], got {tuple(weight.shape)}")
     if offsets.dtype is not torch.int32 or offsets.get_device() != x.get_device():
         raise TypeError(f"offsets must be int32 on {x.device}, got {offsets.dtype} on {offsets.device}")
     if offsets.dim() != 1 or offsets.shape[0] != weight.shape[0] + 1:
         raise _bad(f"offsets {tuple(offsets.shape)} for {weight.shape[0]} experts")
-    return offsets.contiguous()
 
 
 def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream, out, path):
@@ -117,7 +116,9 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
         if wide % 2:
             raise _bad(f"{activation}: weight has {wide} rows, gate and up need an even number")
         n = wide // 2
-    groups = 1 if offsets is None else wshape[0]
+    groups = 1
+    if offsets is not None:
+        groups, offsets = wshape[0], offsets.contiguous()
     pb = pr = pz = rs = 0
     if bias is not None:
         _same(bias, x, x.dtype, device)
@@ -189,7 +190,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     [offsets[0], offsets[E]) come out as zero."""
     if x.dim() != 2:
         raise _bad(f"x must be [rows, in], got {tuple(x.shape)}")
-    offsets = _groups(offsets, weight, x)
+    _check_groups(offsets, weight, x)
     return _forward(x, weight, offsets, bias, None, activation, save_preact, stream, out, path)
 
 
@@ -218,7 +219,9 @@ def _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dw
         _same(preact, x, x.dtype, device)
         preact, zs = _rows(preact, wide)
         pz = preact.data_ptr()
-    groups = 1 if offsets is None else wshape[0]
+    groups = 1
+    if offsets is not None:
+        groups, offsets = wshape[0], offsets.contiguous()
     dy, dys = _rows(dy, n)
     x, xs = _rows(x, k)
     weight, ws, gs = _matrices(weight, wide, k)
@@ -260,7 +263,7 @@ def grouped_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Ten
     ``grouped_linear`` from dy [S, out].  Experts without rows get zeros."""
     if x.dim() != 2:
         raise _bad(f"x must be [rows, in], got {tuple(x.shape)}")
-    offsets = _groups(offsets, weight, x)
+    _check_groups(offsets, weight, x)
     return _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dweight, stream, path)
 
 

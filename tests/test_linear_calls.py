@@ -1,0 +1,55 @@
+"""CPU tests of what the linear products' calls do before anything is launched."""
+import contextlib
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def senmoe():
+    import build as b
+    b.build()
+    import senmoe as s
+    return s
+
+
+class _Copied(Exception):
+    pass
+
+
+class _StridedOffsets:
+    """Stands for int32 offsets that are not contiguous: says where they are copied."""
+
+    def __init__(self, torch, inside):
+        self.dtype, self.device, self.shape, self.inside = torch.int32, "cpu", (2,), inside
+
+    def dim(self):
+        return 1
+
+    def get_device(self):
+        return -1
+
+    def contiguous(self):
+        raise _Copied(list(self.inside))
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_offsets_are_copied_on_the_launch_stream(senmoe, monkeypatch, backward):
+    import torch
+    from senmoe import products
+    inside = []
+
+    @contextlib.contextmanager
+    def stream(s):
+        inside.append(s)
+        yield
+        inside.pop()
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(products, "_operands", lambda *t: (0, -1))
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(1, 32, 64, dtype=torch.bfloat16)
+    off = _StridedOffsets(torch, inside)
+    with pytest.raises(_Copied) as e:
+        if backward:
+            senmoe.grouped_linear_backward(torch.zeros(4, 32, dtype=torch.bfloat16), x, w, off, stream="launch")
+        else:
+            senmoe.grouped_linear(x, w, off, stream="launch")
+    assert e.value.args[0] == ["launch"]
