@@ -40,8 +40,9 @@ _CODES = {C.c_int32: "i", C.c_int64: "q", C.c_void_p: "P"}
 _pack_linear = struct.Struct("".join(_CODES[t] for _, t in SenMoeLinear._fields_)).pack
 _pack_grad = struct.Struct("".join(_CODES[t] for _, t in SenMoeLinearGrad._fields_)).pack
 _c_linear = None  # the library's entry, once it is loaded
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
+# (None in a torch without CUDA, which has no tensor that gets as far.)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _bad(message: str) -> SenMoeError:

@@ -53,3 +53,15 @@ def test_offsets_are_copied_on_the_launch_stream(senmoe, monkeypatch, backward):
         else:
             senmoe.grouped_linear(x, w, off, stream="launch")
     assert e.value.args[0] == ["launch"]
+
+
+def test_import_without_a_cuda_build_of_torch():
+    """The loader and the synthetic weights are used on hosts whose torch has no CUDA build."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "sen-mlx_b200")
+    prog = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]: delattr(torch._C, n)\n"
+            "import senmoe, senmoe.loader, senmoe.synth\n")
+    subprocess.run([sys.executable, "-c", prog], check=True, cwd=root, timeout=300)
