@@ -112,6 +112,8 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
     wide, k = wshape[-2], wshape[-1]
     if not shape or shape[-1] != k:
         raise _bad(f"x {tuple(shape)} against weight {tuple(wshape)}")
+    if wide < 1 or k < 1:
+        raise _bad(f"weight {tuple(wshape)}: in_features={k} out_features={wide}")
     n = wide
     if act >= _GATED:
         if wide % 2:
@@ -123,7 +125,7 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
     pb = pr = pz = rs = 0
     if bias is not None:
         _same(bias, x, x.dtype, device)
-        if bias.numel() != groups * wide or bias.shape[-1] != wide:
+        if bias.numel() != groups * wide or not bias.dim() or bias.shape[-1] != wide:
             raise _bad(f"bias {tuple(bias.shape)} for weight {tuple(wshape)}")
         bias = bias if bias.is_contiguous() else bias.contiguous()
         pb = bias.data_ptr()
@@ -151,7 +153,10 @@ def _forward(x, weight, offsets, bias, residual, activation, save_preact, stream
         _same(out, x, x.dtype, device)
         if out.shape != shape or n > 1 and out.stride(-1) != 1:
             raise _bad(f"out {tuple(out.shape)} strides {out.stride()}, the output is {shape}, its rows contiguous")
-        y = out if out.dim() == 2 else out.view(-1, n)
+        try:
+            y = out if out.dim() == 2 else out.view(-1, n)
+        except RuntimeError:
+            raise _bad(f"out strides {out.stride()}: its rows have no common stride") from None
         ys = y.stride(0) if rows > 1 else n
         if ys < n:
             raise _bad(f"out strides {out.stride()}: its rows overlap")
@@ -205,6 +210,8 @@ def _backward(dy, x, weight, offsets, preact, activation, bias, need_dx, need_dw
     code, device = _operands(x, dy, weight)
     wshape, xshape = weight.shape, x.shape
     wide, k = wshape[-2], wshape[-1]
+    if wide < 1 or k < 1:
+        raise _bad(f"weight {tuple(wshape)}: in_features={k} out_features={wide}")
     n = wide
     if act >= _GATED:
         if wide % 2:

@@ -65,3 +65,24 @@ def test_import_without_a_cuda_build_of_torch():
             "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]: delattr(torch._C, n)\n"
             "import senmoe, senmoe.loader, senmoe.synth\n")
     subprocess.run([sys.executable, "-c", prog], check=True, cwd=root, timeout=300)
+
+
+def _bf16(*shape):
+    import torch
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("call,word", [
+    (lambda m: m.linear(_bf16(4, 0), _bf16(8, 0)), "in_features=0"),
+    (lambda m: m.linear(_bf16(4, 8), _bf16(0, 8), activation="swiglu"), "out_features=0"),
+    (lambda m: m.linear_backward(_bf16(4, 8), _bf16(4, 0), _bf16(8, 0)), "in_features=0"),
+    (lambda m: m.linear_backward(_bf16(2, 2, 0), _bf16(2, 2, 8), _bf16(0, 8)), "out_features=0"),
+    (lambda m: m.linear(_bf16(4, 8), _bf16(1, 8), bias=_bf16(())), "bias"),
+    (lambda m: m.linear(_bf16(2, 3, 8), _bf16(8, 8), out=_bf16(3, 2, 8).transpose(0, 1)), "out"),
+])
+def test_bad_shapes_are_refused_in_the_packages_manner(senmoe, monkeypatch, call, word):
+    from senmoe import products
+    monkeypatch.setattr(products, "_operands", lambda *t: (0, -1))
+    with pytest.raises(senmoe.SenMoeError, match=word) as e:
+        call(senmoe)
+    assert e.value.status == senmoe.ERR_BAD_ARG
