@@ -102,7 +102,8 @@ bool few_rows(const LinearArgs& a) {
 
 int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path, cudaStream_t st,
                 void* dbias = nullptr, bool* summed = nullptr) {
-  if (path == SENMOE_LINEAR_ANY) return cuda_status(call, launch_linear_any(a, p, st));
+  // (no rows: dW's zeros, which no tile form is needed for)
+  if (path == SENMOE_LINEAR_ANY || a.rows == 0) return cuda_status(call, launch_linear_any(a, p, st));
   const bool tc = linear_tc_supported(a, p);
   const bool force_tc = path >= SENMOE_LINEAR_TCGEN05 && path != SENMOE_LINEAR_SMALL;
   if (p == kProdForward && !force_tc) {

@@ -50,3 +50,10 @@ def test_strided_offsets_on_another_stream(senmoe, torch):
         assert torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(got, grads))
         torch.cuda.synchronize()
         del junk
+
+
+@pytest.mark.parametrize("form", ["TCGEN05", "TCGEN05_ONE", "TCGEN05_PAIR", "TCGEN05_SPLIT"])
+def test_gradients_of_no_rows_in_every_form(senmoe, torch, form):
+    x, w, dy = _normal(torch, 1, 0, 64), _normal(torch, 2, 48, 64), _normal(torch, 3, 0, 48)
+    dx, dw, db = senmoe.linear_backward(dy, x, w, bias=True, path=getattr(senmoe, "LINEAR_" + form))
+    assert dx.shape == (0, 64) and dw.shape == w.shape and (dw == 0).all() and (db == 0).all()
