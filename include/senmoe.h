@@ -445,6 +445,10 @@ int senmoe_linear_backward(const SenMoeLinearGrad* grad, senmoe_stream_t stream)
  * (SENMOE_ERR_TIMEOUT). */
 int senmoe_linear_check(senmoe_stream_t stream);
 
+/* Test of the above: launches a kernel on `stream` whose one wait runs out
+ * after its limit (about 2 s), as the kernels' waits would. */
+int senmoe_selftest_linear_wait(senmoe_stream_t stream);
+
 /* Allocation-free forward (no counterpart in the reference; this build adds
  * it for callers that cannot allocate device memory at call time: code inside
  * an open CUDA stream capture, serving loops whose HBM another allocator has

@@ -295,4 +295,9 @@ int senmoe_linear_check(senmoe_stream_t stream) {
   return error ? reject(SENMOE_ERR_DEVICE, "linear: device error %d", error) : SENMOE_OK;
 }
 
+int senmoe_selftest_linear_wait(senmoe_stream_t stream) {
+  clear_failure();
+  return cuda_status("selftest_linear_wait", selftest_linear_wait(stream));
+}
+
 }  // extern "C"

@@ -223,6 +223,8 @@ cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, int form, voi
 // Waits for `st`, returns and clears the device error that the tcgen05
 // kernels recorded on the current device (DeviceError).
 cudaError_t linear_device_error(cudaStream_t st, int* error);
+// A kernel whose only wait runs out (about 2 s) and is recorded.
+cudaError_t selftest_linear_wait(cudaStream_t st);
 
 // dz = dy * act'(z) in 16 bits, and the row sums over each group (the bias
 // gradient); see linear_grad.cu.

@@ -52,6 +52,8 @@
 
 #include <cuda.h>
 
+#include <mutex>
+
 #include "kernels.h"
 #include "linear.cuh"
 
@@ -82,6 +84,7 @@ constexpr int kMaxSplit = 4, kMaxQuads = 33;
 constexpr int kSumPieces = 4;  // bias gradient inside dW: most 8-column pieces of a warp
 
 __device__ int g_linear_error;           // first device error of the linear kernels on this device
+__device__ int g_linear_taken;           // what the last check found there
 
 struct TcArgs {
   LinearArgs l;
@@ -845,6 +848,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if constexpr (PAIR) cluster_sync();
 }
 
+// Reads and clears in one step: an error that a kernel on another stream
+// records meanwhile is this check's or the next one's.
+__global__ void take_error_kernel() { g_linear_taken = atomicExch(&g_linear_error, 0); }
+
+// A wait that nothing ends, through its limit.
+__global__ void selftest_wait_kernel() {
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ volatile int abort_flag;
+  mbar_init(&bar, 1);
+  fence_mbar_init();
+  abort_flag = 0;
+  wait_or_abort(&bar, 0, &abort_flag, &g_linear_error);
+}
+
 // ------------------------------------------------------------- host side
 int tc_sm_count() {
   static int counts[64] = {};  // by device; the same value whoever writes it
@@ -1040,13 +1057,18 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, voi
                    : launch_prod<false>(p, gated, l.bf16, tm, tn, half, a, grid, smem, st);
 }
 
+cudaError_t selftest_linear_wait(cudaStream_t st) {
+  return cudaLaunchKernel(reinterpret_cast<const void*>(selftest_wait_kernel), dim3(1), dim3(1), nullptr, 0, st);
+}
+
 cudaError_t linear_device_error(cudaStream_t st, int* error) {
+  static std::mutex once;  // g_linear_taken is one word a device
+  const std::lock_guard<std::mutex> hold(once);
   *error = 0;
-  cudaError_t e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(error, g_linear_error, sizeof(int));
-  const int zero = 0;
-  if (e == cudaSuccess && *error) e = cudaMemcpyToSymbol(g_linear_error, &zero, sizeof(int));
-  return e;
+  cudaError_t e = cudaLaunchKernel(reinterpret_cast<const void*>(take_error_kernel), dim3(1), dim3(1), nullptr, 0, st);
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(error, g_linear_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  const cudaError_t done = cudaStreamSynchronize(st);
+  return e != cudaSuccess ? e : done;
 }
 
 }  // namespace senmoe

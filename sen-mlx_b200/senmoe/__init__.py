@@ -139,6 +139,7 @@ SIGNATURES = {
     "senmoe_linear_backward_workspace": (_i64, [_P]),
     "senmoe_linear_backward": (C.c_int, [_P, _P]),
     "senmoe_linear_check": (C.c_int, [_P]),
+    "senmoe_selftest_linear_wait": (C.c_int, [_P]),
 }
 
 _lib = None

@@ -57,3 +57,20 @@ def test_gradients_of_no_rows_in_every_form(senmoe, torch, form):
     x, w, dy = _normal(torch, 1, 0, 64), _normal(torch, 2, 48, 64), _normal(torch, 3, 0, 48)
     dx, dw, db = senmoe.linear_backward(dy, x, w, bias=True, path=getattr(senmoe, "LINEAR_" + form))
     assert dx.shape == (0, 64) and dw.shape == w.shape and (dw == 0).all() and (db == 0).all()
+
+
+def test_a_wait_that_runs_out_is_reported_once(senmoe, torch):
+    """Recorded on one stream, reported and cleared by the first check after it
+    on any stream; later calls and checks are right."""
+    senmoe.linear_check()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    assert senmoe.lib().senmoe_selftest_linear_wait(a.cuda_stream) == 0
+    senmoe.linear_check(b)  # not there yet
+    with pytest.raises(senmoe.SenMoeError, match="ran out") as e:
+        senmoe.linear_check(a)
+    assert e.value.status == senmoe.ERR_TIMEOUT
+    senmoe.linear_check(a)
+    senmoe.linear_check(b)
+    x, w = _normal(torch, 1, 300, 128), _normal(torch, 2, 96, 128)
+    assert torch.isfinite(senmoe.linear(x, w)).all()
+    senmoe.linear_check()
