@@ -11,6 +11,7 @@ import sys
 import torch
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "sen-mlx_b200"))
+import senmoe  # noqa: E402
 from senmoe.block16 import Moe16, Moe16Weights  # noqa: E402
 
 
@@ -26,7 +27,8 @@ def make_block(hidden, intermediate, experts, top_k, shared, seed, device="cuda"
 
 
 def train(block, teacher, x, steps, lr):
-    """Plain gradient steps on fp32 copies of the weights; the loss of each."""
+    """Plain gradient steps on fp32 copies of the weights; the loss of each.
+    A step whose kernels gave up a wait raises before it is taken."""
     names = ("gate_up", "down", "shared_gate_up", "shared_down")
     master = {n: getattr(block.w, n).float() for n in names}
     target = teacher.forward(x).float()
@@ -36,6 +38,7 @@ def train(block, teacher, x, steps, lr):
         off = h.float() - target
         losses.append(float(off.square().mean()))
         _, grads = block.backward((off * (2.0 / x.shape[0])).to(h.dtype), saved)
+        senmoe.linear_check()
         for n in names:
             master[n] -= lr * grads[n].float()
             getattr(block.w, n).copy_(master[n])

@@ -26,7 +26,11 @@ class Moe16Weights:
 
 
 class Moe16:
-    """h = x + sum_k w_k expert_k(x) + shared(x), x [T, H] bf16."""
+    """h = x + sum_k w_k expert_k(x) + shared(x), x [T, H] bf16.
+
+    Nothing here waits for the device, so a bounded wait that ran out in a
+    product shows only in ``senmoe.linear_check``: call it where the host waits
+    anyway, in training before a step's gradients are used."""
 
     def __init__(self, weights: Moe16Weights, top_k: int, norm_topk_prob: bool = True):
         self.w, self.top_k, self.norm = weights, top_k, norm_topk_prob

@@ -86,3 +86,26 @@ def test_bad_shapes_are_refused_in_the_packages_manner(senmoe, monkeypatch, call
     with pytest.raises(senmoe.SenMoeError, match=word) as e:
         call(senmoe)
     assert e.value.status == senmoe.ERR_BAD_ARG
+
+
+def test_finetuning_stops_before_a_failed_step_is_taken(senmoe, monkeypatch):
+    """A wait that ran out leaves garbage gradients: no weight takes them."""
+    import os
+    import sys
+    import types
+
+    import torch
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples"))
+    import moe_finetune
+    names = ("gate_up", "down", "shared_gate_up", "shared_down")
+    w = types.SimpleNamespace(**{n: torch.ones(2, 2, dtype=torch.bfloat16) for n in names})
+    x = torch.ones(3, 2, dtype=torch.bfloat16)
+    block = types.SimpleNamespace(w=w, forward=lambda x, train=False: (2 * x, None) if train else x,
+                                  backward=lambda dh, saved: (dh, {n: torch.ones(2, 2) for n in names}))
+
+    def ran_out(stream=None):
+        raise senmoe.SenMoeError(senmoe.ERR_TIMEOUT, "a wait ran out")
+    monkeypatch.setattr(senmoe, "linear_check", ran_out)
+    with pytest.raises(senmoe.SenMoeError):
+        moe_finetune.train(block, block, x, steps=2, lr=0.5)
+    assert all((getattr(w, n) == 1).all() for n in names)
