@@ -74,3 +74,53 @@ def test_a_wait_that_runs_out_is_reported_once(senmoe, torch):
     x, w = _normal(torch, 1, 300, 128), _normal(torch, 2, 96, 128)
     assert torch.isfinite(senmoe.linear(x, w)).all()
     senmoe.linear_check()
+
+
+def _tail(torch, dtype):
+    """Values from -12 to 6 that the type holds exactly, as z = x w with one nonzero column, and x, w."""
+    dt = getattr(torch, dtype)
+    z = torch.linspace(-12, 6, 3001, device="cuda").to(dt)
+    x = torch.zeros(z.numel(), 8, dtype=dt, device="cuda")
+    x[:, 0] = z
+    w = torch.zeros(8, 8, dtype=dt, device="cuda")
+    w[:, 0] = 1
+    return x, w, z.double()
+
+
+def _cdf(torch, z):
+    """Phi(z); erfc keeps the lower tail's relative precision, which special.ndtr on the GPU does not (0 from -8.4 on)."""
+    return 0.5 * torch.special.erfc(-z * 0.5 ** 0.5)
+
+
+# The activations' relative error: __expf's 2 + 1.17 |a| units at a = -72 (z =
+# -12) 1.0e-5, the argument's rounding |a| 2^-24 = 4e-6, the division, the
+# polynomial and the product a few units: 2^-15 covers them.
+@pytest.mark.parametrize("form", ["ANY", "SMALL", "TCGEN05_ONE", "TCGEN05_PAIR", "TCGEN05_SPLIT"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_gelu_keeps_its_relative_precision_in_the_lower_tail(senmoe, torch, form, dtype):
+    import linear_ref as R
+    x, w, z = _tail(torch, dtype)
+    if form == "TCGEN05_SPLIT":  # few tiles only
+        x, z = x[:500].contiguous(), z[:500]
+    y = senmoe.linear(x, w, activation="gelu", path=getattr(senmoe, "LINEAR_" + form))
+    ref = (z * _cdf(torch, z))[:, None].expand(-1, 8)
+    u, tiny = R.HALF_UNIT[x.dtype], R.TINY[x.dtype]
+    R.assert_within(y, ref, (u + 2.0 ** -15) * ref.abs() + tiny, "gelu")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_gelu_slope_keeps_its_relative_precision_in_the_lower_tail(senmoe, torch, dtype):
+    """dx = (dy act'(z)) W with one nonzero weight: dy's products alone, rounded to 16 bits
+    at most twice.  Phi(z) and z phi(z) cancel near -0.75, so each of the two counts."""
+    import linear_ref as R
+    x, w, z = _tail(torch, dtype)
+    rows = z.numel()
+    dy = torch.zeros(rows, 8, dtype=x.dtype, device="cuda")
+    dy[:, 0] = 1
+    pre = z.to(x.dtype)[:, None].expand(rows, 8).contiguous()
+    dx = senmoe.linear_backward(dy, x, w, preact=pre, activation="gelu", need_dweight=False)[0][:, 0]
+    phi = torch.exp(-0.5 * z * z) * 0.3989422804014327
+    cdf = _cdf(torch, z)
+    ref = cdf + z * phi
+    u, tiny = R.HALF_UNIT[x.dtype], R.TINY[x.dtype]
+    R.assert_within(dx, ref, 2.01 * u * ref.abs() + 2.0 ** -15 * (cdf + z.abs() * phi) + 2 * tiny, "slope")
