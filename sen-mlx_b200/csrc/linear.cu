@@ -101,7 +101,7 @@ bool few_rows(const LinearArgs& a) {
 }
 
 int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path, cudaStream_t st,
-                void* dbias = nullptr, bool* summed = nullptr) {
+                const BiasJoin* bias = nullptr, bool* summed = nullptr) {
   // (no rows: dW's zeros, which no tile form is needed for)
   if (path == SENMOE_LINEAR_ANY || a.rows == 0) return cuda_status(call, launch_linear_any(a, p, st));
   const bool tc = linear_tc_supported(a, p);
@@ -117,21 +117,13 @@ int run_product(const char* call, const LinearArgs& a, LinearProduct p, int path
     return reject(SENMOE_ERR_UNSUPPORTED, "%s: TMA needs 16-byte aligned operands, strides of a multiple of 8 elements",
                   call);
   const int form = path > SENMOE_LINEAR_SMALL ? path - SENMOE_LINEAR_SMALL : kFormAuto;
-  return cuda_status(call, tc ? launch_linear_tc(a, p, form, dbias, summed, st) : launch_linear_any(a, p, st));
+  return cuda_status(call, tc ? launch_linear_tc(a, p, form, bias, summed, st) : launch_linear_any(a, p, st));
 }
 
 int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
 
-// Rows of a group are summed in so many parts: one for every 256 rows of the
-// mean group, so that a long single group is not left to a few blocks.
-int bias_splits(int64_t rows, int groups) {
-  const int64_t s = rows / groups / 256;
-  return static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
-}
-
 struct GradLayout {
   int64_t dz_stride = 0, dz_bytes = 0, partial_bytes = 0;
-  int splits = 1;
   int64_t total() const { return dz_bytes + partial_bytes; }
 };
 
@@ -141,10 +133,7 @@ GradLayout grad_layout(const SenMoeLinearGrad& g, int64_t wide) {
     l.dz_stride = (wide + 7) & ~int64_t(7);
     l.dz_bytes = round16(g.rows * l.dz_stride * 2);
   }
-  if (g.dbias) {
-    l.splits = bias_splits(g.rows, g.num_groups);
-    if (l.splits > 1) l.partial_bytes = round16(int64_t(g.num_groups) * l.splits * wide * 4);
-  }
+  if (g.dbias) l.partial_bytes = round16(dz_slots(g.rows, g.num_groups, g.offsets, dz_run(g.epilogue)) * wide * 4);
   return l;
 }
 
@@ -241,7 +230,7 @@ int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
   LinearGradArgs ga{};
   ga.dy = g->dy;
   ga.dy_stride = g->dy_stride;
-  ga.preact = act ? g->preact : nullptr;
+  ga.preact = g->preact;
   ga.preact_stride = g->preact_stride;
   ga.offsets = g->offsets;
   ga.groups = E;
@@ -251,10 +240,11 @@ int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
   ga.dz = g->workspace;
   ga.dz_stride = l.dz_stride;
   ga.dbias = g->dbias;
-  ga.partial = reinterpret_cast<float*>(static_cast<char*>(g->workspace) + l.dz_bytes);
-  ga.splits = l.splits;
+  if (l.partial_bytes) ga.partial = reinterpret_cast<float*>(static_cast<char*>(g->workspace) + l.dz_bytes);
   ga.bf16 = g->dtype == SENMOE_BF16;
-  if (some && act && (rc = cuda_status(call, launch_act_backward(ga, stream)))) return rc;
+  if (act && (rc = cuda_status(call, launch_dz(ga, stream)))) return rc;
+  BiasJoin join{act ? ga.partial : nullptr, g->offsets, E, dz_run(g->epilogue), ga.n, g->rows, g->dbias};
+  bool summed = !g->dbias || (act && some && !ga.partial);  // no bias gradient, or there already
 
   LinearArgs a{};
   a.a = act ? ga.dz : g->dy;
@@ -273,16 +263,19 @@ int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
     a.out_stride = g->dx_stride;
     if ((rc = run_product(call, a, kProdInput, g->path, stream))) return rc;
   }
-  bool summed = false;  // dbias came with dweight
   if (g->dweight) {
     a.b = g->x;
     a.b_stride = g->x_stride;
     a.out = g->dweight;
     a.out_stride = g->dweight_stride;
     a.out_group_stride = g->dweight_group_stride;
-    if ((rc = run_product(call, a, kProdWeight, g->path, stream, g->dbias, &summed))) return rc;
+    if ((rc = run_product(call, a, kProdWeight, g->path, stream, summed ? nullptr : &join, &summed))) return rc;
   }
-  if (g->dbias && !summed && (rc = cuda_status(call, launch_bias_grad(ga, stream)))) return rc;
+  if (!summed) {  // no dweight, or a form that does not take it
+    if (!act && (rc = cuda_status(call, launch_dz(ga, stream)))) return rc;
+    join.partial = ga.partial;
+    if ((act || ga.partial || !some) && (rc = cuda_status(call, launch_bias_join(join, ga.bf16, stream)))) return rc;
+  }
   return SENMOE_OK;
 }
 

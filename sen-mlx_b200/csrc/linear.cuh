@@ -220,11 +220,12 @@ bool linear_small_supported(const LinearArgs& a);
 cudaError_t launch_linear_small(const LinearArgs& a, cudaStream_t st);
 // tcgen05 (linear_tc.cu): operands that TMA can read, see linear_tc_supported.
 bool linear_tc_supported(const LinearArgs& a, LinearProduct p);
-// form: of the tiles, kFormAuto by estimated time.  dbias (dW only): also the
-// column sums of dz, [groups, n] in the operands' type, or null; *summed says
-// whether this launch takes them.
+// form: of the tiles, kFormAuto by estimated time.  bias (dW only, or null):
+// also the bias gradient, from its parts, or without parts as the column sums
+// of dz where this form can take them; *summed says whether it does.
+struct BiasJoin;
 enum LinearForm : int { kFormAuto = 0, kFormOne = 1, kFormPair = 2, kFormSplit = 3 };
-cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, int form, void* dbias, bool* summed,
+cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, int form, const BiasJoin* bias, bool* summed,
                              cudaStream_t st);
 // Waits for `st`, returns and clears the device error that the tcgen05
 // kernels recorded on the current device (DeviceError).
@@ -232,26 +233,75 @@ cudaError_t linear_device_error(cudaStream_t st, int* error);
 // A kernel whose only wait runs out (about 2 s) and is recorded.
 cudaError_t selftest_linear_wait(cudaStream_t st);
 
-// dz = dy * act'(z) in 16 bits, and the row sums over each group (the bias
-// gradient); see linear_grad.cu.
+// dz = dy * act'(z) in 16 bits, and its column sums over each group (the bias
+// gradient) from the fp32 values; see linear_grad.cu.
 struct LinearGradArgs {
   const void* dy;
   int64_t dy_stride;
-  const void* preact;       // null: no activation, dz is dy
+  const void* preact;       // not read for kActNone
   int64_t preact_stride;
   const int32_t* offsets;
   int groups;
   int64_t rows;
   int n;                    // columns of dz (gate and up: both)
-  int act;
+  int act;                  // kActNone: dz is dy and is not stored
   void* dz;                 // [rows, dz_stride]
   int64_t dz_stride;
   void* dbias;              // [groups, n] or null
-  float* partial;           // [groups, splits, n] when splits > 1
-  int splits;
+  float* partial;           // [dz_slots, n]: the sums' parts; null where there is one run
   int bf16;
 };
-cudaError_t launch_act_backward(const LinearGradArgs& a, cudaStream_t st);
-cudaError_t launch_bias_grad(const LinearGradArgs& a, cudaStream_t st);
+// Rows of a run, and the slots that the sums of all runs and groups take (0:
+// the one run of a dense product goes straight to dbias).
+constexpr int dz_run_rows(bool gated) { return gated ? 2 : 4; }  // of one warp
+int dz_run(int act);
+int64_t dz_slots(int64_t rows, int groups, bool grouped, int run);
+cudaError_t launch_dz(const LinearGradArgs& a, cudaStream_t st);
+
+// dbias[e] = the sum of group e's slots.
+struct BiasJoin {
+  const float* partial;     // [dz_slots, n]
+  const int32_t* offsets;
+  int groups, run, n;
+  int64_t rows;
+  void* dbias;              // [groups, n]
+};
+// A warp takes 32 columns of a group or, where groups have many runs, 8
+// columns whose four lanes take every fourth slot.
+__host__ __device__ inline int bias_join_cols(const BiasJoin& j) { return j.rows / j.groups > 16 * j.run ? 8 : 32; }
+__host__ __device__ inline int64_t bias_join_items(const BiasJoin& j) {
+  const int w = bias_join_cols(j);
+  return static_cast<int64_t>(j.groups) * ((j.n + w - 1) / w);
+}
+// Warp `warp` of `warps`; every lane calls it.
+template <bool BF16> __device__ __forceinline__ void join_bias(const BiasJoin& j, int warp, int warps) {
+  const int rows = static_cast<int>(j.rows), lane = threadIdx.x & 31;
+  const int width = bias_join_cols(j), slices = 32 / width, slice = lane / width, col_blocks = (j.n + width - 1) / width;
+  const int64_t items = bias_join_items(j);
+  for (int64_t it = warp; it < items; it += warps) {
+    const int e = static_cast<int>(it / col_blocks);
+    const int c = static_cast<int>(it - static_cast<int64_t>(e) * col_blocks) * width + lane % width;
+    float v = 0.0f;
+    if (c < j.n) {
+      const int o0 = j.offsets ? min(max(j.offsets[e], 0), rows) : 0;
+      const int o1 = j.offsets ? min(max(j.offsets[e + 1], 0), rows) : rows;
+      const float* p = j.partial + static_cast<int64_t>(e) * j.n + c;
+      const int last = o1 > o0 ? (o1 - 1) / j.run : -1;
+      for (int run = o0 / j.run + slice; run <= last; run += 8 * slices) {  // eight loads in flight, none waits for an add
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = run + i * slices <= last ? p[static_cast<int64_t>(run + i * slices) * j.n] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v += t[i];
+      }
+    }
+    if (slices > 1) {
+      v += __shfl_xor_sync(0xffffffffu, v, 8);
+      v += __shfl_xor_sync(0xffffffffu, v, 16);
+    }
+    if (slice == 0 && c < j.n) static_cast<uint16_t*>(j.dbias)[static_cast<int64_t>(e) * j.n + c] = from_f32<BF16>(v);
+  }
+}
+cudaError_t launch_bias_join(const BiasJoin& j, bool bf16, cudaStream_t st);
 
 }  // namespace senmoe

@@ -1,27 +1,26 @@
 // linear_grad.cu -- the elementwise and column-sum parts of the linear
 // products' backward pass.
 //
-// act_backward: dz = dy * act'(z) (gated: dg = dy * u * act'(g), du = dy *
-// act(g)), evaluated in fp32 and rounded once to the operands' 16-bit type,
-// because dz is an operand of both gradient products on the 16-bit tensor
-// cores.  The rounding (at most 2^-8 of the value in bf16, 2^-11 in fp16) is
-// independent from element to element and so adds to a gradient about as much
-// as the gradient's own rounding does: 0.0023 of a gradient's norm in bf16
+// dz = dy * act'(z) (gated: dg = dy * u * act'(g), du = dy * act(g)),
+// evaluated in fp32.  The bias gradient, the sum of each group's dz, is taken
+// here from the fp32 values.  dz itself is rounded once to the operands' 16-bit
+// type, because it is an operand of both gradient products on the 16-bit
+// tensor cores.  That rounding (at most 2^-8 of the value in bf16, 2^-11 in
+// fp16) is independent from element to element and so adds to dx and dW about
+// as much as their own rounding does: 0.0023 of a gradient's norm in bf16
 // against 0.0017 for fp32 sums of an unrounded dz.  Over some 10,000 random
-// sizes the ratio was 1.4, and up to 1.8 where a few large elements decide
-// (a handful of rows, short bias gradients).  Carrying dz in two 16-bit parts
-// would bring it to 1 for twice the products.
-//
-// bias_grad: db[e] = sum of dz's rows of group e, in fp32 and in a fixed
-// order (rows strided over 8 warps, then warps, then splits), so repeated
-// calls agree bit for bit.
+// sizes the ratio was 1.4, and up to 1.8 where a few large elements decide (a
+// handful of rows).  Carrying dz in two 16-bit parts would bring it to 1 for
+// twice the products.
+
+#include <type_traits>
 
 #include "linear.cuh"
 
 namespace senmoe {
 namespace {
 
-constexpr int kActThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 
 template <bool BF16> __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -35,151 +34,211 @@ template <bool BF16> __device__ __forceinline__ uint4 pack8(const float (&f)[8])
   return make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
 }
 
-// A warp a piece of a row (kUnroll steps), V columns a lane and step: 8 (16-byte accesses) where every
+// One row's V columns (gated: the gate's and the up's) as loaded, and dz of them.
+template <bool BF16, int V, int ACT> struct Piece {
+  static constexpr bool kGated = ACT >= kActSwiglu, kStore = ACT != kActNone;  // none: dz is dy
+  using Raw = std::conditional_t<V == 8, uint4, uint16_t>;
+  Raw y, z, u;
+  static __device__ __forceinline__ void unpack(const Raw& v, float (&f)[V]) {
+    if constexpr (V == 8) unpack8<BF16>(v, f);
+    else f[0] = to_f32<BF16>(v);
+  }
+  static __device__ __forceinline__ void store(uint16_t* p, const float (&f)[V]) {
+    if constexpr (V == 8) *reinterpret_cast<uint4*>(p) = pack8<BF16>(f);
+    else *p = from_f32<BF16>(f[0]);
+  }
+  __device__ __forceinline__ void load(const uint16_t* dy, const uint16_t* pre, int cols) {
+    y = *reinterpret_cast<const Raw*>(dy);
+    if constexpr (kStore) z = *reinterpret_cast<const Raw*>(pre);
+    if constexpr (kGated) u = *reinterpret_cast<const Raw*>(pre + cols);
+  }
+  // g: dz, or its gate half; up: its up half
+  __device__ __forceinline__ void gradient(float (&g)[V], float (&up)[V]) const {
+    unpack(y, g);
+    if constexpr (kStore) {
+      float zf[V];
+      unpack(z, zf);
+      if constexpr (kGated) unpack(u, up);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float value;
+        const float d = g[i];
+        g[i] = d * act_both(ACT, zf[i], value);
+        if constexpr (kGated) {
+          g[i] *= up[i];
+          up[i] = d * value;
+        }
+      }
+    }
+  }
+};
+
+// dz alone.  A warp a piece of a row (kUnroll steps), V columns a lane and step: 8 (16-byte accesses) where every
 // row starts on a 16-byte boundary, else 1.  The loads of kUnroll steps are in
 // flight together.  Bound by HBM: dy and z read once, dz written once; 36 us
 // for 32768 rows of 2 x 768 (252 MB, 7.0 TB/s with part of the writes still in
 // L2; 82 us with a thread an element group and a division each).
 template <bool BF16, int V, int ACT>
-__global__ void __launch_bounds__(kActThreads) act_backward_kernel(const LinearGradArgs a) {
-  constexpr bool kGated = ACT >= kActSwiglu;
+__global__ void __launch_bounds__(kThreads) dz_kernel(const LinearGradArgs a) {
+  using P = Piece<BF16, V, ACT>;
   constexpr int kUnroll = V == 8 ? 3 : 1;
   pdl_wait();
   pdl_launch_dependents();
-  const int cols = kGated ? a.n / 2 : a.n;
+  const int cols = P::kGated ? a.n / 2 : a.n;
   const int lane = threadIdx.x & 31;
   const unsigned pieces = (cols + 32 * V * kUnroll - 1) / (32 * V * kUnroll);
-  const int64_t items = a.rows * pieces, warps = gridDim.x * (kActThreads / 32);
-  for (int64_t it = blockIdx.x * (kActThreads / 32) + (threadIdx.x >> 5); it < items; it += warps) {
+  const int64_t items = a.rows * pieces, warps = gridDim.x * kWarps;
+  for (int64_t it = blockIdx.x * kWarps + (threadIdx.x >> 5); it < items; it += warps) {
     const int64_t r = it < 0xffffffffll ? static_cast<unsigned>(it) / pieces : it / pieces;
-    const uint16_t* py = static_cast<const uint16_t*>(a.dy) + r * a.dy_stride;
-    const uint16_t* pz = static_cast<const uint16_t*>(a.preact) + r * a.preact_stride;
-    uint16_t* po = static_cast<uint16_t*>(a.dz) + r * a.dz_stride;
+    const uint16_t* dy = static_cast<const uint16_t*>(a.dy) + r * a.dy_stride;
+    const uint16_t* pre = static_cast<const uint16_t*>(a.preact) + r * a.preact_stride;
+    uint16_t* dz = static_cast<uint16_t*>(a.dz) + r * a.dz_stride;
     const int c0 = static_cast<int>(it - r * pieces) * 32 * V * kUnroll + lane * V;
-    uint4 vy[kUnroll], vz[kUnroll], vu[kUnroll];
-    if constexpr (V == 8) {
+    P piece[kUnroll];
 #pragma unroll
-      for (int j = 0; j < kUnroll; ++j) {
-        const int c = c0 + j * 256;
-        if (c < cols) {
-          vy[j] = *reinterpret_cast<const uint4*>(py + c);
-          vz[j] = *reinterpret_cast<const uint4*>(pz + c);
-          if constexpr (kGated) vu[j] = *reinterpret_cast<const uint4*>(pz + cols + c);
-        }
-      }
-    }
+    for (int j = 0; j < kUnroll; ++j)
+      if (c0 + j * 32 * V < cols) piece[j].load(dy + c0 + j * 32 * V, pre + c0 + j * 32 * V, cols);
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       const int c = c0 + j * 32 * V;
       if (c >= cols) break;
-      float d[V], z[V], u[V], g[V];
-      if constexpr (V == 8) {
-        unpack8<BF16>(vy[j], d);
-        unpack8<BF16>(vz[j], z);
-        if constexpr (kGated) unpack8<BF16>(vu[j], u);
-      } else {
-        d[0] = to_f32<BF16>(py[c]);
-        z[0] = to_f32<BF16>(pz[c]);
-        if constexpr (kGated) u[0] = to_f32<BF16>(pz[cols + c]);
-      }
+      float g[V], up[V];
+      piece[j].gradient(g, up);
+      P::store(dz + c, g);
+      if constexpr (P::kGated) P::store(dz + cols + c, up);
+    }
+  }
+}
+
+// dz and its column sums; for ACT none the sums alone.  A block takes a run of
+// kWarps * kRows rows and 32 * V columns, each warp kRows of the rows with all
+// their loads in flight together, and the warps' fp32 sums meet in shared
+// memory.  Each group's part of a run goes to slot (run + group) of `partial`:
+// along the rows every new pair of run and group raises that number, so no two
+// share a slot, and a group's slots follow from its offsets alone.  A dense
+// product of one run goes straight to dbias.  The order of every sum is fixed.
+// 57 us for 32768 rows of 2 x 768 in 128 groups, 18 for 4096 x 2112 (dz alone
+// 38.5 and 11), a join kernel included; dW's launch joins the parts for nothing.
+// 16 or 32 rows a run with all loads out at once: with a block's rows in a loop, or
+// more than 85 registers (two blocks an SM), it took 72 and 20.
+template <bool BF16, int V, int ACT>
+__global__ void __launch_bounds__(kThreads, 3) dz_sums_kernel(const LinearGradArgs a) {
+  using P = Piece<BF16, V, ACT>;
+  constexpr int kRows = dz_run_rows(P::kGated), kRun = kRows * kWarps, kHalves = P::kGated ? 2 : 1;
+  __shared__ int s_off[kMaxGroups + 1];
+  __shared__ __align__(16) float s_sum[2][kWarps][kHalves][32 * V];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int rows = static_cast<int>(a.rows), groups = a.groups;
+  const int cols = P::kGated ? a.n / 2 : a.n;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col_blocks = (cols + 32 * V - 1) / (32 * V);
+  const int64_t items = static_cast<int64_t>((rows + kRun - 1) / kRun) * col_blocks;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int run = static_cast<int>(it / col_blocks), cb = static_cast<int>(it - static_cast<int64_t>(run) * col_blocks);
+    const int r0 = run * kRun, r1 = min(r0 + kRun, rows), mine = r0 + warp * kRows, c = (cb * 32 + lane) * V;
+    const bool live = c < cols;
+    P piece[kRows];
+    const uint16_t* dy = static_cast<const uint16_t*>(a.dy) + mine * a.dy_stride + c;
+    const uint16_t* pre = static_cast<const uint16_t*>(a.preact) + mine * a.preact_stride + c;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float value;
-        const float slope = act_both(ACT, z[i], value);
-        g[i] = d[i] * slope;
-        if constexpr (kGated) {
-          g[i] *= u[i];
-          u[i] = d[i] * value;
+    for (int j = 0; j < kRows; ++j)
+      if (live && mine + j < r1) piece[j].load(dy + j * a.dy_stride, pre + j * a.preact_stride, cols);
+    if (a.offsets && it == blockIdx.x)  // the groups, while the loads are on their way
+      for (int i = threadIdx.x; i <= groups; i += kThreads) s_off[i] = min(max(a.offsets[i], 0), rows);
+    // the run's parts, one a group; s_sum takes turns, so a part needs one barrier
+    if (a.offsets) __syncthreads();
+    int e = 0;
+    if (a.offsets) {  // the last i with s_off[i] <= r0, or -1
+      int lo = -1, hi = groups + 1;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_off[mid] <= r0) lo = mid;
+        else hi = mid;
+      }
+      e = lo;
+    }
+    for (int from = r0, to, turn = 0; from < r1; from = to) {
+      to = r1;
+      if (a.offsets) {
+        while (e < groups && s_off[e + 1] <= from) ++e;
+        if (e < groups) to = min(r1, s_off[e + 1]);
+        if (e < 0 || e >= groups) continue;  // rows of no group
+      }
+      float sum[kHalves][V] = {};
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        if (!live || mine + j < from || mine + j >= to) continue;
+        float g[V], up[V];
+        piece[j].gradient(g, up);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          sum[0][i] += g[i];
+          if constexpr (P::kGated) sum[1][i] += up[i];
+        }
+        if constexpr (P::kStore) {
+          uint16_t* p = static_cast<uint16_t*>(a.dz) + (mine + j) * a.dz_stride + c;
+          P::store(p, g);
+          if constexpr (P::kGated) P::store(p + cols, up);
         }
       }
-      if constexpr (V == 8) {
-        *reinterpret_cast<uint4*>(po + c) = pack8<BF16>(g);
-        if constexpr (kGated) *reinterpret_cast<uint4*>(po + cols + c) = pack8<BF16>(u);
-      } else {
-        po[c] = from_f32<BF16>(g[0]);
-        if constexpr (kGated) po[cols + c] = from_f32<BF16>(u[0]);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        if constexpr (V == 8) {
+          float4* p = reinterpret_cast<float4*>(&s_sum[turn][warp][h][8 * lane]);
+          p[0] = make_float4(sum[h][0], sum[h][1], sum[h][2], sum[h][3]);
+          p[1] = make_float4(sum[h][4], sum[h][5], sum[h][6], sum[h][7]);
+        } else {
+          s_sum[turn][warp][h][lane] = sum[h][0];
+        }
       }
-    }
-  }
-}
-
-template <bool BF16, int V> auto act_backward_for(int act) {
-  switch (act) {
-    case kActRelu: return act_backward_kernel<BF16, V, kActRelu>;
-    case kActSilu: return act_backward_kernel<BF16, V, kActSilu>;
-    case kActGelu: return act_backward_kernel<BF16, V, kActGelu>;
-    case kActGeluTanh: return act_backward_kernel<BF16, V, kActGeluTanh>;
-    case kActSwiglu: return act_backward_kernel<BF16, V, kActSwiglu>;
-    case kActGeglu: return act_backward_kernel<BF16, V, kActGeglu>;
-    default: return act_backward_kernel<BF16, V, kActNone>;
-  }
-}
-
-constexpr int kSumCols = 256;  // columns of a block: eight a lane
-
-// vec: every row starts on a 16-byte boundary.
-template <bool BF16>
-__global__ void __launch_bounds__(256) bias_grad_kernel(const LinearGradArgs a, const uint16_t* src, int64_t stride,
-                                                        bool vec) {
-  __shared__ int s_off[kMaxGroups + 1], s_pre[kMaxGroups + 1], s_tot[64];
-  __shared__ float s_sum[8][kSumCols];
-  pdl_wait();
-  pdl_launch_dependents();
-  group_table(a.offsets, a.groups, a.rows, 1, s_off, s_pre, s_tot);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col_blocks = (a.n + kSumCols - 1) / kSumCols;
-  const int64_t items = static_cast<int64_t>(a.groups) * a.splits * col_blocks;
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int cb = static_cast<int>(it % col_blocks);
-    const int es = static_cast<int>(it / col_blocks), e = es / a.splits, sp = es - e * a.splits;
-    const int cnt = s_off[e + 1] - s_off[e], per = (cnt + a.splits - 1) / a.splits;
-    const int r0 = min(sp * per, cnt), r1 = min(r0 + per, cnt);
-    const int c = cb * kSumCols + 8 * lane;
-    float x[8] = {};
-    const uint16_t* p = src + static_cast<int64_t>(s_off[e]) * stride + c;
-    if (vec && c + 8 <= a.n) {
-#pragma unroll 4
-      for (int r = r0 + warp; r < r1; r += 8) {
-        float f[8];
-        unpack8<BF16>(*reinterpret_cast<const uint4*>(p + r * stride), f);
+      __syncthreads();
+      for (int t = threadIdx.x; t < kHalves * 32 * V; t += kThreads) {
+        const int h = t / (32 * V), col = cb * 32 * V + t % (32 * V);
+        float v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += f[i];
+        for (int w = 0; w < kWarps; ++w) v += s_sum[turn][w][h][t % (32 * V)];
+        if (col >= cols) continue;
+        if (a.partial) a.partial[static_cast<int64_t>(run + e) * a.n + h * cols + col] = v;
+        else static_cast<uint16_t*>(a.dbias)[h * cols + col] = from_f32<BF16>(v);
       }
-    } else {
-      for (int r = r0 + warp; r < r1; r += 8)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c + i < a.n) x[i] += to_f32<BF16>(p[r * stride + i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s_sum[warp][8 * lane + i] = x[i];
-    __syncthreads();
-    const int col = cb * kSumCols + threadIdx.x;
-    if (col < a.n) {
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) v += s_sum[w][threadIdx.x];
-      if (a.splits > 1)
-        a.partial[static_cast<int64_t>(es) * a.n + col] = v;
-      else
-        static_cast<uint16_t*>(a.dbias)[static_cast<int64_t>(e) * a.n + col] = from_f32<BF16>(v);
+      turn ^= 1;
     }
     __syncthreads();
   }
 }
 
-template <bool BF16> __global__ void __launch_bounds__(256) bias_join_kernel(const LinearGradArgs a) {
+template <bool BF16> __global__ void __launch_bounds__(kThreads) join_kernel(const BiasJoin j) {
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t total = static_cast<int64_t>(a.groups) * a.n;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t e = i / a.n, c = i - e * a.n;
-    float v = 0.0f;
-    for (int s = 0; s < a.splits; ++s) v += a.partial[(e * a.splits + s) * a.n + c];
-    static_cast<uint16_t*>(a.dbias)[i] = from_f32<BF16>(v);
-  }
+  join_bias<BF16>(j, blockIdx.x * kWarps + (threadIdx.x >> 5), gridDim.x * kWarps);
 }
+
+template <bool BF16, int V> struct Dz {
+  static auto of(int act) {
+    switch (act) {
+      case kActRelu: return dz_kernel<BF16, V, kActRelu>;
+      case kActSilu: return dz_kernel<BF16, V, kActSilu>;
+      case kActGelu: return dz_kernel<BF16, V, kActGelu>;
+      case kActGeluTanh: return dz_kernel<BF16, V, kActGeluTanh>;
+      case kActSwiglu: return dz_kernel<BF16, V, kActSwiglu>;
+      default: return dz_kernel<BF16, V, kActGeglu>;
+    }
+  }
+};
+template <bool BF16, int V> struct DzSums {
+  static auto of(int act) {
+    switch (act) {
+      case kActRelu: return dz_sums_kernel<BF16, V, kActRelu>;
+      case kActSilu: return dz_sums_kernel<BF16, V, kActSilu>;
+      case kActGelu: return dz_sums_kernel<BF16, V, kActGelu>;
+      case kActGeluTanh: return dz_sums_kernel<BF16, V, kActGeluTanh>;
+      case kActSwiglu: return dz_sums_kernel<BF16, V, kActSwiglu>;
+      case kActGeglu: return dz_sums_kernel<BF16, V, kActGeglu>;
+      default: return dz_sums_kernel<BF16, V, kActNone>;
+    }
+  }
+};
 
 bool on16(const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 8 == 0; }
 
@@ -190,27 +249,37 @@ unsigned grid_for(int64_t items, int64_t cap) {
 
 }  // namespace
 
-cudaError_t launch_act_backward(const LinearGradArgs& a, cudaStream_t st) {
-  const int cols = act_gated(a.act) ? a.n / 2 : a.n;
-  const bool wide = cols % 8 == 0 && on16(a.dy, a.dy_stride) && on16(a.preact, a.preact_stride) &&
-                    on16(a.dz, a.dz_stride);
-  const int64_t items = a.rows * ((cols + (wide ? 767 : 31)) / (wide ? 768 : 32));
-  const dim3 grid(grid_for((items + kActThreads / 32 - 1) / (kActThreads / 32), 148 * 16)), block(kActThreads);
-  auto kern = a.bf16 ? (wide ? act_backward_for<true, 8>(a.act) : act_backward_for<true, 1>(a.act))
-                     : (wide ? act_backward_for<false, 8>(a.act) : act_backward_for<false, 1>(a.act));
-  return launch_pdl(kern, grid, block, 0, st, a);
+int dz_run(int act) { return kWarps * dz_run_rows(act_gated(act)); }
+
+int64_t dz_slots(int64_t rows, int groups, bool grouped, int run) {
+  if (rows == 0 || (!grouped && rows <= run)) return 0;
+  return (rows + run - 1) / run + (grouped ? groups : 0);
 }
 
-cudaError_t launch_bias_grad(const LinearGradArgs& a, cudaStream_t st) {
-  const uint16_t* src = static_cast<const uint16_t*>(a.preact ? a.dz : a.dy);
-  const int64_t stride = a.preact ? a.dz_stride : a.dy_stride;
-  const int64_t items = static_cast<int64_t>(a.groups) * a.splits * ((a.n + kSumCols - 1) / kSumCols);
-  auto kern = a.bf16 ? bias_grad_kernel<true> : bias_grad_kernel<false>;
-  cudaError_t e = launch_pdl(kern, dim3(grid_for(items, 148 * 8)), dim3(256), 0, st, a, src, stride, on16(src, stride));
-  if (e != cudaSuccess || a.splits <= 1) return e;
-  auto join = a.bf16 ? bias_join_kernel<true> : bias_join_kernel<false>;
-  return launch_pdl(join, dim3(grid_for((static_cast<int64_t>(a.groups) * a.n + 255) / 256, 148 * 8)), dim3(256), 0,
-                    st, a);
+template <template <bool, int> class F> static auto pick(bool bf16, bool wide, int act) {
+  return bf16 ? (wide ? F<true, 8>::of(act) : F<true, 1>::of(act)) : (wide ? F<false, 8>::of(act) : F<false, 1>::of(act));
+}
+
+cudaError_t launch_dz(const LinearGradArgs& a, cudaStream_t st) {
+  if (a.rows == 0) return cudaSuccess;
+  const int cols = act_gated(a.act) ? a.n / 2 : a.n;
+  const bool act = a.act != kActNone;
+  const bool wide = cols % 8 == 0 && on16(a.dy, a.dy_stride) &&
+                    (!act || (on16(a.preact, a.preact_stride) && on16(a.dz, a.dz_stride)));
+  const dim3 block(kThreads);
+  if (!a.dbias) {
+    const int64_t items = a.rows * ((cols + (wide ? 767 : 31)) / (wide ? 768 : 32));
+    return launch_pdl(pick<Dz>(a.bf16, wide, a.act), dim3(grid_for((items + kWarps - 1) / kWarps, 148 * 16)), block, 0, st, a);
+  }
+  const int run = dz_run(a.act);
+  const int64_t items = (a.rows + run - 1) / run * ((cols + (wide ? 255 : 31)) / (wide ? 256 : 32));
+  return launch_pdl(pick<DzSums>(a.bf16, wide, a.act), dim3(grid_for(items, 148 * 64)), block, 0, st, a);
+}
+
+cudaError_t launch_bias_join(const BiasJoin& j, bool bf16, cudaStream_t st) {
+  const int64_t warps = bias_join_items(j);
+  return launch_pdl(bf16 ? join_kernel<true> : join_kernel<false>, dim3(grid_for((warps + kWarps - 1) / kWarps, 148 * 8)),
+                    dim3(kThreads), 0, st, j);
 }
 
 }  // namespace senmoe

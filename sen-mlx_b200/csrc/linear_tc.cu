@@ -97,6 +97,7 @@ struct TcArgs {
   int split;        // K split (one-CTA form): the cluster's size
   uint32_t stage_bytes;  // a stage: the M operand, then the N operand
   uint16_t* dbias;  // dW: column sums of dz, [groups, n], or null
+  BiasJoin join;    // dW: the bias gradient from its parts; partial null: not here
 };
 
 // ------------------------------------------------------------ PTX wrappers
@@ -582,7 +583,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // rows l, l + 32, ... in fp32, then the lanes are added, all in a fixed
     // order.  (As ones times dz on the warp-level MMA the sums held up the
     // tcgen05 MMAs: 871 cycles a block of 64 rows instead of 535.)
+    // With an activation the sums come from the fp32 dz, in parts, which these
+    // warps join while the tiles run.
     if constexpr (PROD == kProdWeight) {
+      if (a.join.partial) join_bias<BF16>(a.join, blockIdx.x * 2 + warp - 2, gridDim.x * 2);
       if (sums) {
         bool ok = true;
         int st = 0, ph = 0;
@@ -997,7 +1001,7 @@ bool linear_tc_supported(const LinearArgs& a, LinearProduct p) {
   return a.rows > 0 && w_ok && tma_ok(a.a, a.a_stride, 0, 1);
 }
 
-cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, void* dbias, bool* summed,
+cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, const BiasJoin* bias, bool* summed,
                              cudaStream_t st) {
   const bool gated = p == kProdForward && act_gated(l.act);
   const int sms = tc_sm_count();
@@ -1010,9 +1014,14 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, voi
   const int features = p == kProdForward ? (gated ? l.n / 2 : l.n) : l.k;
   const int feat = (gated ? 64 : 128) * (plan.pair ? 2 : 1);
   a.m_tiles = (features + feat - 1) / feat;
-  // a K split leaves each CTA part of a column's rows: no sums there
-  a.dbias = p == kProdWeight && plan.split == 1 && a.m_tiles * 2 * kSumPieces * 8 >= (plan.pair ? a.bn / 2 : a.bn) ? static_cast<uint16_t*>(dbias) : nullptr;
-  if (summed) *summed = a.dbias != nullptr;
+  if (bias && bias->partial) {
+    a.join = *bias;
+    *summed = true;
+  } else if (bias && plan.split == 1 && a.m_tiles * 2 * kSumPieces * 8 >= (plan.pair ? a.bn / 2 : a.bn)) {
+    // (a K split leaves each CTA part of a column's rows: no sums there)
+    a.dbias = static_cast<uint16_t*>(bias->dbias);
+    *summed = true;
+  }
   a.n_tiles = p == kProdWeight ? (l.n + a.bn - 1) / a.bn : 0;
   a.part = plan.pair ? a.bn / 2 : a.bn;
   a.stage_bytes = kMBytes + a.part * 128;

@@ -124,3 +124,39 @@ def test_gelu_slope_keeps_its_relative_precision_in_the_lower_tail(senmoe, torch
     ref = cdf + z * phi
     u, tiny = R.HALF_UNIT[x.dtype], R.TINY[x.dtype]
     R.assert_within(dx, ref, 2.01 * u * ref.abs() + 2.0 ** -15 * (cdf + z.abs() * phi) + 2 * tiny, "slope")
+
+
+def _dz_and_size(torch, dy, z, activation):
+    """dz in float64 and the size that the intrinsics' error, 2^-17, goes with."""
+    import linear_ref as R
+    size = dy.double().abs()
+    if activation in R.GATED:
+        g, up = z.double().chunk(2, -1)
+        size = torch.cat([size * up.abs(), size * g.abs()], -1)
+    else:
+        size = size * (1 + z.double().abs())
+    return R.slope_dz(dy, z, activation), size
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("activation", ["relu", "silu", "gelu", "gelu_tanh", "swiglu", "geglu"])
+@pytest.mark.parametrize("counts,out", [([3], 136), ([19], 33), ([333], 200), ([5000], 64), ([0, 2, 40, 0, 300, 1], 72),
+                                        ([70, 0, 9], 35)])
+def test_bias_gradient_sums_unrounded_terms(senmoe, torch, counts, out, activation, dtype):
+    """dbias is the sum of dy act'(z) held in 32 bits, rounded once: its bound
+    has no term for a rounding of dz to 16 bits."""
+    import linear_ref as R
+    rows, wide, k = sum(counts), out * (2 if activation in R.GATED else 1), 40
+    x, dy, z = (_normal(torch, i, rows, n, dtype=dtype) for i, n in ((1, k), (2, out), (3, wide)))
+    if len(counts) == 1:
+        w, off = _normal(torch, 4, wide, k, dtype=dtype, scale=k ** -0.5), None
+        db = senmoe.linear_backward(dy, x, w, preact=z, activation=activation, bias=True)[2][None]
+    else:
+        w = _normal(torch, 4, len(counts), wide, k, dtype=dtype, scale=k ** -0.5)
+        off = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+        db = senmoe.grouped_linear_backward(dy, x, w, off, preact=z, activation=activation, bias=True)[2]
+    dz, size = _dz_and_size(torch, dy, z, activation)
+    for e, a, b in R.groups(None if off is None else off.tolist(), rows):
+        ref, err = dz[a:b].sum(0), 2.0 ** -17 * size[a:b].sum(0)
+        err = err + (b - a + 8) * 2.0 ** -23 * dz[a:b].abs().sum(0)
+        R.assert_within(db[e], ref, err + R.HALF_UNIT[x.dtype] * (ref.abs() + err) + R.TINY[x.dtype], f"db {e}")
