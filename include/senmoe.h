@@ -407,12 +407,16 @@ int senmoe_linear(const SenMoeLinear* product, senmoe_stream_t stream);
 
 /* Gradients of the product above from dy (residual's is dy itself):
  *   dz = dy * epilogue'(preact)   (dy itself for SENMOE_EPI_NONE; gated: both
- *                                  halves), rounded to the tensors' type
+ *                                  halves), rounded to the tensors' type for
+ *                                  dx and dweight, kept in fp32 for dbias
  *   dx[s, :] = dz[s, :] @ weight[e(s)]
  *   dweight[e] = sum over e's rows of dz[s, :]^T x[s, :]
  *   dbias[e]   = sum over e's rows of dz[s, :]
  * Any of dx, dweight and dbias may be NULL.  Groups without rows get zero
- * dweight and dbias, rows outside the groups zero dx.  The sums are taken in a fixed order:
+ * dweight and dbias, rows outside the groups zero dx.  An fp16 dz that leaves
+ * fp16's range (a gated pair's may reach 2^32) is held by a power of two of its
+ * group's, which dx and dweight take back before they are rounded: what is
+ * smaller than 2^-39 of the group's largest is lost then.  The sums are taken in a fixed order:
  * the same call gives the same bits.  workspace: device memory of at least
  * senmoe_linear_backward_workspace(grad) bytes (16-byte aligned; NULL when
  * that is 0), in use until the call's work on the stream is done. */

@@ -51,7 +51,21 @@ struct LinearArgs {
   void* preact;                                // forward: z before the activation, or null
   int64_t preact_stride;
   int bf16;                                    // 1: bf16, 0: fp16
+  const unsigned* dz_max;                      // dx, dW: the groups' scales of an fp16 dz (dz_exponent), or null
 };
+
+// fp16 holds 2^-14 to 65504 in full precision, less than |dy u act'(z)| may
+// span.  So an fp16 dz is stored times 2^-x, with x from its group's largest
+// finite |dz| (as the bits of a float), and the gradients' epilogues multiply
+// by 2^x: 0 where that is between 2^-6 and 65504, so that the terms that
+// decide a sum are in range as they are, otherwise the x that takes it into
+// [2^14, 2^15).  Elements under 2^-39 of a group's largest are lost.
+__host__ __device__ inline int dz_exponent(unsigned max_bits) {
+  const int x = static_cast<int>(max_bits >> 23) - 127;
+  if (max_bits == 0 || (x >= -6 && max_bits <= 0x477fe000u)) return 0;
+  return (x > -100 ? x : -100) - 14;
+}
+__device__ __forceinline__ float power_of_two(int x) { return __int_as_float((x + 127) << 23); }
 
 // 16-bit values by their bit patterns.
 template <bool BF16> __device__ __forceinline__ float to_f32(uint16_t v) {
@@ -249,6 +263,7 @@ struct LinearGradArgs {
   int64_t dz_stride;
   void* dbias;              // [groups, n] or null
   float* partial;           // [dz_slots, n]: the sums' parts; null where there is one run
+  unsigned* dz_max;         // fp16: [groups], the largest finite |dz| (see dz_exponent); null: dz is not scaled
   int bf16;
 };
 // Rows of a run, and the slots that the sums of all runs and groups take (0:

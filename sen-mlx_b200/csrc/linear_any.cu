@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(kThreads) linear_any_kernel(const LinearArgs a
           const int i = wi + m * 16 + g + (q >> 1) * 8, j = wj + n * 8 + 2 * t4 + (q & 1);
           if (i >= ni || j >= nj) continue;
           float z = acc[0][m][n][q];
+          if (PROD != kProdForward && a.dz_max) z *= power_of_two(dz_exponent(a.dz_max[e]));
           if constexpr (PROD == kProdForward) {
             const int64_t row = i0 + i;
             const int64_t bcol = static_cast<int64_t>(e) * a.n + j0 + j;

@@ -362,7 +362,7 @@ __device__ __forceinline__ void store_chunk(const float (&v)[16], uint32_t* turn
 }
 
 // What a warp needs to finish a tile's accumulators.
-template <int PROD, bool GATED, bool BF16> struct Finish {
+template <int PROD, bool GATED, bool BF16, bool SCALED> struct Finish {
   const LinearArgs& l;
   uint16_t *out, *pre;
   int cols;           // features of the output
@@ -384,13 +384,17 @@ template <int PROD, bool GATED, bool BF16> struct Finish {
     }
     return 0.0f;
   }
+  // dz's scale, undone in its products
+  __device__ __forceinline__ float scale(int e) const {
+    return SCALED ? power_of_two(dz_exponent(l.dz_max[e])) : 1.0f;
+  }
   // z (bias added) of 16 columns -> preact, at column `at` of its rows
   __device__ __forceinline__ void keep(const float (&z)[16], int64_t row, int at, int w, int feats) const {
     if (PROD == kProdForward && pre)
       store_chunk<BF16>(z, turn, pre + row * l.preact_stride + at, l.preact_stride, w, feats, pvec, lane);
   }
-  // the activated values, + residual -> out
-  __device__ __forceinline__ void write(float (&y)[16], int e, int64_t row, int f, int w, int feats) const {
+  // the activated values, + residual (gradients: times dz's scale) -> out
+  __device__ __forceinline__ void write(float (&y)[16], float scale, int e, int64_t row, int f, int w, int feats) const {
     if constexpr (PROD == kProdForward) {
       if (l.residual && lane < feats) {
         const uint16_t* res = static_cast<const uint16_t*>(l.residual) + row * l.residual_stride + f + lane;
@@ -401,13 +405,20 @@ template <int PROD, bool GATED, bool BF16> struct Finish {
         for (int i = 0; i < 16; ++i) y[i] += to_f32<BF16>(r[i]);
       }
     }
+    if constexpr (SCALED) {  // (a branch: mostly 1, and a dW of few rows is bound by its epilogue)
+      if (scale != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] *= scale;
+      }
+    }
     uint16_t* dst = out + row * l.out_stride + f;
     if constexpr (PROD == kProdWeight) dst += e * l.out_group_stride;
     store_chunk<BF16>(y, turn, dst, l.out_stride, w, feats, vec, lane);
   }
 };
 
-template <int PROD, bool GATED, bool BF16, bool PAIR>
+// SCALED: dx or dW of an fp16 dz stored by a power of two a group (dz_exponent).
+template <int PROD, bool GATED, bool BF16, bool PAIR, bool SCALED>
 __global__ void __launch_bounds__(kTcThreads, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap tm_m, const __grid_constant__ CUtensorMap tm_n,
                      const __grid_constant__ CUtensorMap tm_half, const __grid_constant__ TcArgs a) {
@@ -653,7 +664,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ============================================================ epilogue
     // 32 columns at a time, the warps of a lane quarter in turn
     const int ew = warp - kEpiWarp0, q = warp & 3, turn2 = ew >> 2;
-    const Finish<PROD, GATED, BF16> fin(a.l, turn_of(ew), lane);
+    const Finish<PROD, GATED, BF16, SCALED> fin(a.l, turn_of(ew), lane);
     int it = 0;
     for (int idx = unit; idx < tiles; idx += units, ++it) {
       const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, idx, rank);
@@ -661,7 +672,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // a gated pair: quarters 0, 1 hold the gate of features 32 (q & 1) on, 2, 3 the up
       const int f0 = t.m0 + (GATED ? q & 1 : q) * 32, feats = min(32, fin.cols - f0);
       const int up = GATED && q >= 2 ? fin.cols : 0;
-      const float bias = fin.bias(t.e, f0, feats, up);
+      const float bias = fin.bias(t.e, f0, feats, up), scale = fin.scale(t.e);
       bool go = warp_wait(&bar_accfull[ab], aph, &s_abort, err);
       // the two warps that swap leave together, or one would wait for the other
       if constexpr (GATED) go = both_warps(1 + (turn2 * 2 + (q & 1)), go);
@@ -723,7 +734,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i] *= u[i];
           const int h = gate ? 0 : 16;
-          fin.write(y, t.e, row + h, f0, t.w - c - h, feats);
+          fin.write(y, scale, t.e, row + h, f0, t.w - c - h, feats);
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -733,7 +744,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               fin.keep(z[h], row + 16 * h, f0, w, feats);
               act_chunk(a.l.act, z[h]);
             }
-            fin.write(z[h], t.e, row + 16 * h, f0, w, feats);
+            fin.write(z[h], scale, t.e, row + 16 * h, f0, w, feats);
           }
         }
       }
@@ -785,7 +796,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       __syncwarp();
       cluster_sync();  // every share is where it is added
       if (epi) {
-        const Finish<PROD, GATED, BF16> fin(a.l, turn_of(ew), lane);
+        const Finish<PROD, GATED, BF16, SCALED> fin(a.l, turn_of(ew), lane);
+        const float scale = fin.scale(t.e);
         constexpr int kQuarters = GATED ? 2 : 4;
         const int mine = chunks > rank ? (chunks - rank + csize - 1) / csize : 0;  // chunks rank, rank + csize, ...
         for (int i = ew; i < mine * kQuarters; i += kEpiWarps) {
@@ -817,7 +829,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               for (int k = 0; k < 16; ++k) z[k] *= u[k];
             }
           }
-          fin.write(z, t.e, t.c0 + c, f0, w, feats);
+          fin.write(z, scale, t.e, t.c0 + c, f0, w, feats);
         }
       }
       __syncwarp();
@@ -882,10 +894,10 @@ bool tma_ok(const void* p, int64_t stride, int64_t group_stride, int groups) {
          (groups <= 1 || (group_stride % 8 == 0 && group_stride < (int64_t(1) << 38)));
 }
 
-template <int PROD, bool GATED, bool BF16, bool PAIR>
+template <int PROD, bool GATED, bool BF16, bool PAIR, bool SCALED>
 cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorMap& half, const TcArgs& a, int grid, size_t smem,
                      cudaStream_t st) {
-  auto kern = linear_tc_kernel<PROD, GATED, BF16, PAIR>;
+  auto kern = linear_tc_kernel<PROD, GATED, BF16, PAIR, SCALED>;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   // Launched in plain stream order, unlike the other kernels here: this one
@@ -906,11 +918,14 @@ cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorM
 }
 
 template <bool PAIR, typename... A>
-cudaError_t launch_prod(LinearProduct p, bool gated, int bf16, const A&... args) {
-#define SENMOE_LINEAR_TC(P, G) (bf16 ? launch_t<P, G, true, PAIR>(args...) : launch_t<P, G, false, PAIR>(args...))
-  if (p == kProdInput) return SENMOE_LINEAR_TC(kProdInput, false);
-  if (p == kProdWeight) return SENMOE_LINEAR_TC(kProdWeight, false);
-  return gated ? SENMOE_LINEAR_TC(kProdForward, true) : SENMOE_LINEAR_TC(kProdForward, false);
+cudaError_t launch_prod(LinearProduct p, bool gated, const LinearArgs& l, const A&... args) {
+#define SENMOE_LINEAR_TC(P, G, S) \
+  (l.bf16 ? launch_t<P, G, true, PAIR, false>(args...) : launch_t<P, G, false, PAIR, S>(args...))
+  if (l.dz_max)
+    return p == kProdInput ? SENMOE_LINEAR_TC(kProdInput, false, true) : SENMOE_LINEAR_TC(kProdWeight, false, true);
+  if (p == kProdInput) return SENMOE_LINEAR_TC(kProdInput, false, false);
+  if (p == kProdWeight) return SENMOE_LINEAR_TC(kProdWeight, false, false);
+  return gated ? SENMOE_LINEAR_TC(kProdForward, true, false) : SENMOE_LINEAR_TC(kProdForward, false, false);
 #undef SENMOE_LINEAR_TC
 }
 
@@ -1062,8 +1077,8 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, con
       e = make_tmap_4d(&half, l.a, {cols, rows, 1, 1}, {a_row, a_row, a_row}, {64, uint32_t(a.part / 2), 1, 1});
   }
   if (e != cudaSuccess) return e;
-  return plan.pair ? launch_prod<true>(p, gated, l.bf16, tm, tn, half, a, grid, smem, st)
-                   : launch_prod<false>(p, gated, l.bf16, tm, tn, half, a, grid, smem, st);
+  return plan.pair ? launch_prod<true>(p, gated, l, tm, tn, half, a, grid, smem, st)
+                   : launch_prod<false>(p, gated, l, tm, tn, half, a, grid, smem, st);
 }
 
 cudaError_t selftest_linear_wait(cudaStream_t st) {

@@ -160,3 +160,99 @@ def test_bias_gradient_sums_unrounded_terms(senmoe, torch, counts, out, activati
         ref, err = dz[a:b].sum(0), 2.0 ** -17 * size[a:b].sum(0)
         err = err + (b - a + 8) * 2.0 ** -23 * dz[a:b].abs().sum(0)
         R.assert_within(db[e], ref, err + R.HALF_UNIT[x.dtype] * (ref.abs() + err) + R.TINY[x.dtype], f"db {e}")
+
+
+def _gradients(torch, dy, x, w, off, z, activation):
+    """(ref, bound) of dx, dw and db for fp16.  dz is held to 16 bits at a power
+    of two of each group's choice: to half a unit of itself, and to half of
+    fp16's smallest step, 2^-25, which is taken as it is where the group's
+    largest |dz| is between 2^-6 and 65504 and otherwise is at most 2^-39 of it."""
+    import linear_ref as R
+    u, tiny = R.HALF_UNIT[x.dtype], R.TINY[x.dtype]
+    dz, size = _dz_and_size(torch, dy, z, activation)
+    w3 = w if w.dim() == 3 else w[None]
+    E, n, k = w3.shape
+    out = [torch.zeros(s, dtype=torch.float64, device="cuda") for s in (x.shape, (E, n, k), (E, n)) for _ in range(2)]
+    dx, bx, dw, bw, db, bb = out
+    for e, a, b in R.groups(None if off is None else off.tolist(), x.shape[0]):
+        if a == b:
+            continue
+        d, xe, we = dz[a:b], x[a:b].double(), w3[e].double()
+        m = float(d.abs()[d.isfinite()].max())
+        step = max(2.0 ** -39 * m, tiny if 2.0 ** -6.01 <= m <= 65600 else 0.0)
+        near = 2.0 ** -17 * size[a:b]
+        er = u * d.abs() + near + step
+        dx[a:b], dw[e], db[e] = d @ we, d.t() @ xe, d.sum(0)
+        bx[a:b] = er @ we.abs() + (n + 8) * 2.0 ** -23 * ((d.abs() + er) @ we.abs())
+        bw[e] = er.t() @ xe.abs() + (b - a + 8) * 2.0 ** -23 * ((d.abs() + er).t() @ xe.abs())
+        bb[e] = near.sum(0) + (b - a + 8) * 2.0 ** -23 * (d.abs() + near).sum(0)
+    if w.dim() == 2:
+        dw, bw, db, bb = dw[0], bw[0], db[0], bb[0]
+    return [(v, bd + u * (v.abs() + bd) + tiny) for v, bd in ((dx, bx), (dw, bw), (db, bb))]
+
+
+# dy, z, weight and x scales: dz far over 65504, dz of fp16's subnormals, and
+# gradients that fit fp16 in both
+RANGES = {"large": (300.0, 400.0, 1e-3, 1e-2), "small": (2.0 ** -20, 1.0, 20.0, 50.0), "unit": (0.5, 1.0, 0.1, 1.0)}
+
+
+@pytest.mark.parametrize("form", ["AUTO", "ANY", "TCGEN05_ONE", "TCGEN05_PAIR", "TCGEN05_SPLIT"])
+@pytest.mark.parametrize("activation,size", [("swiglu", "large"), ("geglu", "large"), ("swiglu", "small"),
+                                             ("silu", "small"), ("gelu", "small"), ("relu", "small")])
+@pytest.mark.parametrize("rows,k,out", [(5, 72, 40), (150, 136, 72), (70, 41, 33)])
+def test_fp16_gradients_whose_dz_leaves_the_range(senmoe, torch, form, activation, size, rows, k, out):
+    import linear_ref as R
+    if k % 8 and form.startswith("TCGEN05"):
+        pytest.skip("not on TMA's grid")
+    wide = out * (2 if activation in R.GATED else 1)
+    sy, sz, sw, sx = RANGES[size]
+    dy, z = _normal(torch, 1, rows, out, dtype="float16", scale=sy), _normal(torch, 2, rows, wide, dtype="float16", scale=sz)
+    w, x = _normal(torch, 3, wide, k, dtype="float16", scale=sw), _normal(torch, 4, rows, k, dtype="float16", scale=sx)
+    got = senmoe.linear_backward(dy, x, w, preact=z, activation=activation, bias=rows != 5,
+                                 path=getattr(senmoe, "LINEAR_" + form))
+    refs = _gradients(torch, dy, x, w, None, z, activation)
+    for v, (ref, bound), what in zip(got, refs, ("dx", "dw", "db")):
+        if v is not None:
+            keep = ref.abs() < 60000  # (an output past fp16's range is an infinity)
+            assert keep.float().mean() > 0.9 or what == "db"  # (the large dbias is past fp16's range)
+            R.assert_within(v[keep], ref[keep], bound[keep], what)
+    senmoe.linear_check()
+
+
+@pytest.mark.parametrize("form", ["AUTO", "ANY", "TCGEN05_ONE", "TCGEN05_PAIR", "TCGEN05_SPLIT"])
+def test_fp16_groups_of_different_ranges(senmoe, torch, form):
+    """Each group has its own power of two; one with an infinity keeps its other rows' dx."""
+    import linear_ref as R
+    counts, k, out, first = [40, 0, 33, 70, 1, 20], 72, 48, 3
+    sizes = ["large", "unit", "small", "unit", "small", "large"]
+    rows = sum(counts) + first + 5
+    x = torch.full((rows, k), float("nan"), dtype=torch.float16, device="cuda")
+    dy = torch.full((rows, out), float("inf"), dtype=torch.float16, device="cuda")
+    z = torch.full((rows, 2 * out), 60000.0, dtype=torch.float16, device="cuda")
+    w = torch.zeros(len(counts), 2 * out, k, dtype=torch.float16, device="cuda")
+    o = [first]
+    for e, (n, size) in enumerate(zip(counts, sizes)):
+        sy, sz, sw, sx = RANGES[size]
+        a, b = o[-1], o[-1] + n
+        dy[a:b], z[a:b] = _normal(torch, 10 + e, n, out, scale=sy), _normal(torch, 20 + e, n, 2 * out, scale=sz)
+        w[e], x[a:b] = _normal(torch, 30 + e, 2 * out, k, scale=sw), _normal(torch, 40 + e, n, k, scale=sx)
+        o.append(b)
+    off = torch.tensor(o, dtype=torch.int32, device="cuda")
+    path = getattr(senmoe, "LINEAR_" + form)
+    inner = slice(first, o[-1])
+    loc = off - first
+    for broken in (False, True):
+        if broken:
+            dy[o[5] + 7, 3] = float("inf")
+        dx, dw, db = senmoe.grouped_linear_backward(dy, x, w, off, preact=z, activation="swiglu", bias=True, path=path)
+        refs = _gradients(torch, dy[inner], x[inner], w, loc, z[inner], "swiglu")
+        rows_ok = [i for i in range(o[-1] - first) if not broken or i != o[5] + 7 - first]
+        groups_ok = [e for e in range(6) if not broken or e != 5]
+        assert (dx[:first] == 0).all() and (dx[o[-1]:] == 0).all()
+        for v, (ref, bound), keep, what in ((dx[inner], refs[0], rows_ok, "dx"), (dw, refs[1], groups_ok, "dw"),
+                                            (db, refs[2], groups_ok, "db")):
+            v, ref, bound = v[keep], ref[keep], bound[keep]
+            fits = ref.abs() < 60000
+            assert fits.float().mean() > 0.8 or what == "db"  # (the large groups' dbias is past fp16's range)
+            R.assert_within(v[fits], ref[fits], bound[fits], what)
+    senmoe.linear_check()
