@@ -581,9 +581,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
     }
-    // (the leader's drain commit arrives here too)
-    volatile int never = 0;
-    wait_or_abort(&bar_drain, 0, &never, nullptr);
   } else if (warp < kEpiWarp0) {
     // ============================== dW: column sums of dz, the bias gradient
     // Every feature tile of a column tile loads the same dz, so the column
@@ -852,6 +849,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   tc_fence_before();
   __syncthreads();
+  if (PAIR && rank == 1 && warp == 1) {
+    // The leader's drain commit arrives here too.  Waited for only now, with
+    // this CTA's tiles finished, so that the limit does not run from the
+    // kernel's start and a long kernel's CTA cannot leave before the arrival.
+    volatile int never = 0;
+    wait_or_abort(&bar_drain, 0, &never, nullptr);
+    __syncwarp();
+  }
   if (csize > 1) cluster_sync();  // nobody reads this CTA's shared memory or TMEM any more
   if (warp == 1) {
     tc_fence_after();
