@@ -225,9 +225,12 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
-  return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, err));
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
+                                          long long limit = kWaitLimitCycles) {
+  return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, err, limit));
 }
+// Limit of a wait for `blocks` k blocks of a tile, of some 600 cycles each.
+__device__ __forceinline__ long long blocks_limit(int blocks) { return kWaitLimitCycles + 2048ll * blocks; }
 
 // Named barrier of two warps (64 threads) that also joins a condition.
 __device__ __forceinline__ bool both_warps(int id, bool mine) {
@@ -670,7 +673,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int f0 = t.m0 + (GATED ? q & 1 : q) * 32, feats = min(32, fin.cols - f0);
       const int up = GATED && q >= 2 ? fin.cols : 0;
       const float bias = fin.bias(t.e, f0, feats, up), scale = fin.scale(t.e);
-      bool go = warp_wait(&bar_accfull[ab], aph, &s_abort, err);
+      bool go = warp_wait(&bar_accfull[ab], aph, &s_abort, err, blocks_limit(t.kb1 - t.kb0));
       // the two warps that swap leave together, or one would wait for the other
       if constexpr (GATED) go = both_warps(1 + (turn2 * 2 + (q & 1)), go);
       if (!go) break;
@@ -753,7 +756,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else {
     // =========================== K split: this CTA's accumulator is ready
-    if (unit < tiles) warp_wait(&bar_accfull[0], 0, &s_abort, err);
+    if (unit < tiles) {
+      const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
+      warp_wait(&bar_accfull[0], 0, &s_abort, err, blocks_limit(t.kb1 - t.kb0));
+    }
     tc_fence_after();
   }
 

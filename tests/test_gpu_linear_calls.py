@@ -256,3 +256,23 @@ def test_fp16_groups_of_different_ranges(senmoe, torch, form):
             assert fits.float().mean() > 0.8 or what == "db"  # (the large groups' dbias is past fp16's range)
             R.assert_within(v[fits], ref[fits], bound[fits], what)
     senmoe.linear_check()
+
+
+def test_a_tile_that_takes_longer_than_a_wait_may(senmoe, torch):
+    """2^29 rows summed by one tile of one CTA: some 3 s, while a wait that
+    nothing ends gives up after 2 s.  All but a few hundred rows are zero."""
+    import linear_ref as R
+    rows, k, out = 1 << 29, 16, 16
+    if torch.cuda.mem_get_info()[0] < 45 << 30:
+        pytest.skip("needs 34 GB")
+    at = torch.cat([torch.arange(100), torch.arange(rows // 2, rows // 2 + 100), torch.arange(rows - 100, rows)]).cuda()
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros(rows, out, dtype=torch.bfloat16, device="cuda")
+    x[at], dy[at] = _normal(torch, 1, 300, k), _normal(torch, 2, 300, out)
+    w = _normal(torch, 3, out, k)
+    dw = senmoe.linear_backward(dy, x, w, need_dx=False, path=senmoe.LINEAR_TCGEN05_ONE)[1]
+    senmoe.linear_check()
+    (_, _), (ref, bound), (_, _) = R.backward(dy[at], x[at], w)
+    R.assert_within(dw, ref, bound, "dw")  # (a zero row rounds nothing)
+    del x, dy
+    torch.cuda.empty_cache()
