@@ -46,9 +46,18 @@
 // 4096 tokens swiglu 210 us for 1.09 GB and 206 GFLOP.  dW is bound by its
 // writes: 246 us for 805 MB, which a memset writes in 207.
 //
-// Every wait is bounded (wait_or_abort): a role that gives up raises the CTA's
-// abort flag and records kDevWaitTimeout, the others follow, copies in flight
-// are awaited, and TMEM is freed.
+// Waits.  Every wait on an mbarrier is bounded (wait_or_abort): a role that
+// gives up raises the CTA's abort flag and records kDevWaitTimeout, the others
+// follow, copies in flight are awaited, and TMEM is freed.  Three kinds of wait
+// have no limit, and need none as long as these hold:
+//   * barrier.cluster and the block's barriers: every thread arrives at each,
+//     whatever its role's waits returned (a cluster's CTAs run together);
+//   * the named barriers of a gated pair: its two warps first agree on whether
+//     they go on (both_warps) and then take the same steps;
+//   * tcgen05.alloc: only one of this package's CTAs that use TMEM fits an SM
+//     at a time (one_cta_an_sm), on whichever stream, and none leaves before its TMEM is
+//     free, a pair's CTAs together; and a pair asks only when both CTAs run.
+// So launches on several streams wait for one another's SMs and nothing else.
 
 #include <cuda.h>
 
@@ -905,6 +914,24 @@ bool tma_ok(const void* p, int64_t stride, int64_t group_stride, int groups) {
          (groups <= 1 || (group_stride % 8 == 0 && group_stride < (int64_t(1) << 38)));
 }
 
+// Stages of the ring, as many as fit.
+constexpr uint32_t stage_bytes_for(int part) { return kMBytes + part * 128; }
+constexpr int stages_for(bool gated, int part) {
+  const int fit = static_cast<int>(ring_budget(gated) / stage_bytes_for(part));
+  return fit < kMaxStages ? fit : kMaxStages;
+}
+constexpr size_t tc_smem(bool gated, int part) {
+  return 1024 + static_cast<size_t>(stages_for(gated, part)) * stage_bytes_for(part) + epilogue_bytes(gated);
+}
+// More than half an SM, and more than the quantized experts' tcgen05 kernels
+// (169 KB at least) leave: no two CTAs that use TMEM share one.
+constexpr bool one_cta_an_sm() {
+  for (int part = 16; part <= 256; part += 16)
+    if (tc_smem(false, part) < 120 * 1024 || tc_smem(true, part) < 120 * 1024) return false;
+  return true;
+}
+static_assert(one_cta_an_sm(), "tcgen05.alloc would wait for the CTA beside");
+
 template <int PROD, bool GATED, bool BF16, bool PAIR, bool SCALED>
 cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorMap& half, const TcArgs& a, int grid, size_t smem,
                      cudaStream_t st) {
@@ -1050,12 +1077,11 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, con
   }
   a.n_tiles = p == kProdWeight ? (l.n + a.bn - 1) / a.bn : 0;
   a.part = plan.pair ? a.bn / 2 : a.bn;
-  a.stage_bytes = kMBytes + a.part * 128;
-  a.stages = static_cast<int>(ring_budget(gated) / a.stage_bytes);
-  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  a.stage_bytes = stage_bytes_for(a.part);
+  a.stages = stages_for(gated, a.part);
   const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
   const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
-  const size_t smem = 1024 + static_cast<size_t>(a.stages) * a.stage_bytes + epilogue_bytes(gated);
+  const size_t smem = tc_smem(gated, a.part);
 
   CUtensorMap tm{}, tn{}, half{};
   cudaError_t e;

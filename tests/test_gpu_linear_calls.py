@@ -276,3 +276,35 @@ def test_a_tile_that_takes_longer_than_a_wait_may(senmoe, torch):
     R.assert_within(dw, ref, bound, "dw")  # (a zero row rounds nothing)
     del x, dy
     torch.cuda.empty_cache()
+
+
+def test_products_on_two_streams_at_once(senmoe, torch):
+    """Every tile form and the elementwise kernels queued on two streams side by
+    side, other sizes on each: the bits of the same calls one after the other."""
+    def calls(seed, rows, k, out, stream=None):
+        s = [_normal(torch, seed + i, *shape, scale=sc) for i, (shape, sc) in enumerate(
+            [((rows, k), 1), ((2 * out, k), k ** -0.5), ((rows, out), 0.5), ((rows, 2 * out), 1), ((4, out, k), k ** -0.5)])]
+        off = torch.tensor([0, rows // 3, rows // 3, rows - 5, rows], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+
+        def run(stream):
+            got = []
+            for path in (senmoe.LINEAR_AUTO, senmoe.LINEAR_TCGEN05_ONE, senmoe.LINEAR_TCGEN05_PAIR):
+                got.append(senmoe.linear(s[0], s[1], activation="swiglu", path=path, stream=stream))
+                got += senmoe.linear_backward(s[2], s[0], s[1], preact=s[3], activation="swiglu", bias=True, path=path,
+                                              stream=stream)
+                got.append(senmoe.grouped_linear(s[0], s[4], off, path=path, stream=stream))
+                got += senmoe.grouped_linear_backward(s[2], s[0], s[4], off, bias=True, path=path, stream=stream)
+            return got
+        return run
+    a, b = calls(1, 1300, 512, 320), calls(7, 210, 1024, 264)
+    want = a(None), b(None)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = a(sa), b(sb)
+    sa.synchronize()
+    sb.synchronize()
+    senmoe.linear_check()
+    for w, g in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(w, g))
