@@ -124,6 +124,7 @@ int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
 
 struct GradLayout {
   int64_t dz_stride = 0, dz_bytes = 0, partial_bytes = 0, max_bytes = 0;
+  int run = 0;
   int64_t total() const { return dz_bytes + partial_bytes + max_bytes; }
 };
 
@@ -134,7 +135,8 @@ GradLayout grad_layout(const SenMoeLinearGrad& g, int64_t wide) {
     l.dz_bytes = round16(g.rows * l.dz_stride * 2);
     if (g.dtype == SENMOE_FP16 && g.rows > 0) l.max_bytes = round16(int64_t(g.num_groups) * 4);
   }
-  if (g.dbias) l.partial_bytes = round16(dz_slots(g.rows, g.num_groups, g.offsets, dz_run(g.epilogue)) * wide * 4);
+  l.run = dz_run(g.rows, g.offsets, g.epilogue);
+  if (g.dbias) l.partial_bytes = round16(dz_slots(g.rows, g.num_groups, g.offsets, l.run) * wide * 4);
   return l;
 }
 
@@ -241,12 +243,13 @@ int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
   ga.dz = g->workspace;
   ga.dz_stride = l.dz_stride;
   ga.dbias = g->dbias;
+  ga.run = l.run;
   if (l.partial_bytes) ga.partial = reinterpret_cast<float*>(static_cast<char*>(g->workspace) + l.dz_bytes);
   if (l.max_bytes && (g->dx || g->dweight))
     ga.dz_max = reinterpret_cast<unsigned*>(static_cast<char*>(g->workspace) + l.dz_bytes + l.partial_bytes);
   ga.bf16 = g->dtype == SENMOE_BF16;
   if (act && (rc = cuda_status(call, launch_dz(ga, stream)))) return rc;
-  BiasJoin join{act ? ga.partial : nullptr, g->offsets, E, dz_run(g->epilogue), ga.n, g->rows, g->dbias};
+  BiasJoin join{act ? ga.partial : nullptr, g->offsets, E, l.run, ga.n, g->rows, g->dbias};
   bool summed = !g->dbias || (act && some && !ga.partial);  // no bias gradient, or there already
 
   LinearArgs a{};

@@ -263,13 +263,14 @@ struct LinearGradArgs {
   int64_t dz_stride;
   void* dbias;              // [groups, n] or null
   float* partial;           // [dz_slots, n]: the sums' parts; null where there is one run
+  int run;                  // dz_run's
   unsigned* dz_max;         // fp16: [groups], the largest finite |dz| (see dz_exponent); null: dz is not scaled
   int bf16;
 };
 // Rows of a run, and the slots that the sums of all runs and groups take (0:
 // the one run of a dense product goes straight to dbias).
 constexpr int dz_run_rows(bool gated) { return gated ? 2 : 4; }  // of one warp
-int dz_run(int act);
+int dz_run(int64_t rows, bool grouped, int act);
 int64_t dz_slots(int64_t rows, int groups, bool grouped, int run);
 cudaError_t launch_dz(const LinearGradArgs& a, cudaStream_t st);
 

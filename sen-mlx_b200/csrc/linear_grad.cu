@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(kThreads) dz_kernel(const LinearGradArgs a) {
 // memory.  Each group's part of a run goes to slot (run + group) of `partial`:
 // along the rows every new pair of run and group raises that number, so no two
 // share a slot, and a group's slots follow from its offsets alone.  A dense
-// product of one run goes straight to dbias.  The order of every sum is fixed.
+// product of one run goes straight to dbias (without an activation up to 512
+// rows do, read in turns: no workspace, no join).  The order of every sum is fixed.
 // 57 us for 32768 rows of 2 x 768 in 128 groups, 18 for 4096 x 2112 (dz alone
 // 38.5 and 11), a join kernel included; dW's launch joins the parts for nothing.
 // 16 or 32 rows a run with all loads out at once: with a block's rows in a loop, or
@@ -140,7 +141,8 @@ __global__ void __launch_bounds__(kThreads, 3) dz_sums_kernel(const LinearGradAr
   const int cols = P::kGated ? a.n / 2 : a.n;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col_blocks = (cols + 32 * V - 1) / (32 * V);
-  const int64_t items = static_cast<int64_t>((rows + kRun - 1) / kRun) * col_blocks;
+  const int length = P::kStore ? kRun : a.run;  // rows of a run
+  const int64_t items = static_cast<int64_t>((rows + length - 1) / length) * col_blocks;
   if constexpr (SCALED) {
     int some = 0;
     for (int i = threadIdx.x; i < groups; i += kThreads) some |= dz_exponent(a.dz_max[i]);
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 3) dz_sums_kernel(const LinearGradAr
   }
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
     const int run = static_cast<int>(it / col_blocks), cb = static_cast<int>(it - static_cast<int64_t>(run) * col_blocks);
-    const int r0 = run * kRun, r1 = min(r0 + kRun, rows), mine = r0 + warp * kRows, c = (cb * 32 + lane) * V;
+    const int r0 = run * length, r1 = min(r0 + length, rows), mine = r0 + warp * kRows, c = (cb * 32 + lane) * V;
     const bool live = c < cols;
     P piece[kRows];
     const uint16_t* dy = static_cast<const uint16_t*>(a.dy) + mine * a.dy_stride + c;
@@ -206,6 +208,23 @@ __global__ void __launch_bounds__(kThreads, 3) dz_sums_kernel(const LinearGradAr
           uint16_t* p = static_cast<uint16_t*>(a.dz) + (mine + j) * a.dz_stride + c;
           P::store(p, g);
           if constexpr (P::kGated) P::store(p + cols, up);
+        }
+      }
+      if constexpr (!P::kStore) {
+        for (int row = mine + kRun; row < r1 && live; row += kRun) {  // a dense run's further rows
+          const int64_t at = row - mine;
+          P more[kRows];
+#pragma unroll
+          for (int j = 0; j < kRows; ++j)
+            if (row + j < r1) more[j].load(dy + (at + j) * a.dy_stride, nullptr, cols);
+#pragma unroll
+          for (int j = 0; j < kRows; ++j) {
+            if (row + j >= r1) break;
+            float g[V], up[V];
+            more[j].gradient(g, up);
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[0][i] += g[i];
+          }
         }
       }
       if constexpr (SCALED) continue;
@@ -305,7 +324,10 @@ unsigned grid_for(int64_t items, int64_t cap) {
 
 }  // namespace
 
-int dz_run(int act) { return kWarps * dz_run_rows(act_gated(act)); }
+int dz_run(int64_t rows, bool grouped, int act) {
+  if (act == kActNone && !grouped && rows <= 512) return 512;
+  return kWarps * dz_run_rows(act_gated(act));
+}
 
 int64_t dz_slots(int64_t rows, int groups, bool grouped, int run) {
   if (rows == 0 || (!grouped && rows <= run)) return 0;
@@ -327,8 +349,7 @@ cudaError_t launch_dz(const LinearGradArgs& a, cudaStream_t st) {
     const int64_t items = a.rows * ((cols + (wide ? 767 : 31)) / (wide ? 768 : 32));
     return launch_pdl(pick<Dz>(a.bf16, wide, a.act), dim3(grid_for((items + kWarps - 1) / kWarps, 148 * 16)), block, 0, st, a);
   }
-  const int run = dz_run(a.act);
-  const int64_t items = (a.rows + run - 1) / run * ((cols + (wide ? 255 : 31)) / (wide ? 256 : 32));
+  const int64_t items = (a.rows + a.run - 1) / a.run * ((cols + (wide ? 255 : 31)) / (wide ? 256 : 32));
   const dim3 grid(grid_for(items, 148 * 64));
   if (a.dz_max) {
     const cudaError_t e = launch_pdl(clear_kernel, dim3(1), block, 0, st, a.dz_max, a.groups);

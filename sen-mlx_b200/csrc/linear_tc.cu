@@ -105,8 +105,9 @@ struct TcArgs {
   int stages;
   int split;        // K split (one-CTA form): the cluster's size
   uint32_t stage_bytes;  // a stage: the M operand, then the N operand
+  long long tile_limit;  // of the wait for a tile's accumulators, cycles
   uint16_t* dbias;  // dW: column sums of dz, [groups, n], or null
-  BiasJoin join;    // dW: the bias gradient from its parts; partial null: not here
+  BiasJoin join;    // dW: the bias gradient from its parts
 };
 
 // ------------------------------------------------------------ PTX wrappers
@@ -238,8 +239,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
                                           long long limit = kWaitLimitCycles) {
   return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, err, limit));
 }
-// Limit of a wait for `blocks` k blocks of a tile, of some 600 cycles each.
-__device__ __forceinline__ long long blocks_limit(int blocks) { return kWaitLimitCycles + 2048ll * blocks; }
 
 // Named barrier of two warps (64 threads) that also joins a condition.
 __device__ __forceinline__ bool both_warps(int id, bool mine) {
@@ -430,7 +429,9 @@ template <int PROD, bool GATED, bool BF16, bool SCALED> struct Finish {
 };
 
 // SCALED: dx or dW of an fp16 dz stored by a power of two a group (dz_exponent).
-template <int PROD, bool GATED, bool BF16, bool PAIR, bool SCALED>
+// JOIN: dW that also joins the parts of the bias gradient.  (Instances of their
+// own: in every dW's code either costs the shortest launches 2 to 4 %.)
+template <int PROD, bool GATED, bool BF16, bool PAIR, bool SCALED, bool JOIN>
 __global__ void __launch_bounds__(kTcThreads, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap tm_m, const __grid_constant__ CUtensorMap tm_n,
                      const __grid_constant__ CUtensorMap tm_half, const __grid_constant__ TcArgs a) {
@@ -606,7 +607,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // With an activation the sums come from the fp32 dz, in parts, which these
     // warps join while the tiles run.
     if constexpr (PROD == kProdWeight) {
-      if (a.join.partial) join_bias<BF16>(a.join, blockIdx.x * 2 + warp - 2, gridDim.x * 2);
+      if constexpr (JOIN) join_bias<BF16>(a.join, blockIdx.x * 2 + warp - 2, gridDim.x * 2);
       if (sums) {
         bool ok = true;
         int st = 0, ph = 0;
@@ -682,7 +683,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int f0 = t.m0 + (GATED ? q & 1 : q) * 32, feats = min(32, fin.cols - f0);
       const int up = GATED && q >= 2 ? fin.cols : 0;
       const float bias = fin.bias(t.e, f0, feats, up), scale = fin.scale(t.e);
-      bool go = warp_wait(&bar_accfull[ab], aph, &s_abort, err, blocks_limit(t.kb1 - t.kb0));
+      bool go = warp_wait(&bar_accfull[ab], aph, &s_abort, err, a.tile_limit);
       // the two warps that swap leave together, or one would wait for the other
       if constexpr (GATED) go = both_warps(1 + (turn2 * 2 + (q & 1)), go);
       if (!go) break;
@@ -765,10 +766,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else {
     // =========================== K split: this CTA's accumulator is ready
-    if (unit < tiles) {
-      const Tile t = tile_at<PROD, GATED, PAIR>(a, s_off, s_pre, unit, rank);
-      warp_wait(&bar_accfull[0], 0, &s_abort, err, blocks_limit(t.kb1 - t.kb0));
-    }
+    if (unit < tiles) warp_wait(&bar_accfull[0], 0, &s_abort, err, a.tile_limit);
     tc_fence_after();
   }
 
@@ -932,10 +930,10 @@ constexpr bool one_cta_an_sm() {
 }
 static_assert(one_cta_an_sm(), "tcgen05.alloc would wait for the CTA beside");
 
-template <int PROD, bool GATED, bool BF16, bool PAIR, bool SCALED>
+template <int PROD, bool GATED, bool BF16, bool PAIR, bool SCALED, bool JOIN>
 cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorMap& half, const TcArgs& a, int grid, size_t smem,
                      cudaStream_t st) {
-  auto kern = linear_tc_kernel<PROD, GATED, BF16, PAIR, SCALED>;
+  auto kern = linear_tc_kernel<PROD, GATED, BF16, PAIR, SCALED, JOIN>;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   // Launched in plain stream order, unlike the other kernels here: this one
@@ -956,14 +954,13 @@ cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorM
 }
 
 template <bool PAIR, typename... A>
-cudaError_t launch_prod(LinearProduct p, bool gated, const LinearArgs& l, const A&... args) {
-#define SENMOE_LINEAR_TC(P, G, S) \
-  (l.bf16 ? launch_t<P, G, true, PAIR, false>(args...) : launch_t<P, G, false, PAIR, S>(args...))
-  if (l.dz_max)
-    return p == kProdInput ? SENMOE_LINEAR_TC(kProdInput, false, true) : SENMOE_LINEAR_TC(kProdWeight, false, true);
-  if (p == kProdInput) return SENMOE_LINEAR_TC(kProdInput, false, false);
-  if (p == kProdWeight) return SENMOE_LINEAR_TC(kProdWeight, false, false);
-  return gated ? SENMOE_LINEAR_TC(kProdForward, true, false) : SENMOE_LINEAR_TC(kProdForward, false, false);
+cudaError_t launch_prod(LinearProduct p, bool gated, const LinearArgs& l, bool join, const A&... args) {
+#define SENMOE_LINEAR_TC(P, G, S, J) \
+  (l.bf16 ? launch_t<P, G, true, PAIR, false, J>(args...) : launch_t<P, G, false, PAIR, S, J>(args...))
+  if (p == kProdInput) return l.dz_max ? SENMOE_LINEAR_TC(kProdInput, false, true, false) : SENMOE_LINEAR_TC(kProdInput, false, false, false);
+  if (p == kProdWeight && join) return SENMOE_LINEAR_TC(kProdWeight, false, true, true);  // (an fp16 dz with parts has scales)
+  if (p == kProdWeight) return l.dz_max ? SENMOE_LINEAR_TC(kProdWeight, false, true, false) : SENMOE_LINEAR_TC(kProdWeight, false, false, false);
+  return gated ? SENMOE_LINEAR_TC(kProdForward, true, false, false) : SENMOE_LINEAR_TC(kProdForward, false, false, false);
 #undef SENMOE_LINEAR_TC
 }
 
@@ -1078,6 +1075,9 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, con
   a.n_tiles = p == kProdWeight ? (l.n + a.bn - 1) / a.bn : 0;
   a.part = plan.pair ? a.bn / 2 : a.bn;
   a.stage_bytes = stage_bytes_for(a.part);
+  // a k block takes some 600 cycles; dW: a group may hold every row
+  const int64_t k = p == kProdForward ? l.k : p == kProdInput ? l.n : l.rows;
+  a.tile_limit = kWaitLimitCycles + 2048ll * ((k + kBK - 1) / kBK);
   a.stages = stages_for(gated, a.part);
   const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
   const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
@@ -1114,8 +1114,8 @@ cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, con
       e = make_tmap_4d(&half, l.a, {cols, rows, 1, 1}, {a_row, a_row, a_row}, {64, uint32_t(a.part / 2), 1, 1});
   }
   if (e != cudaSuccess) return e;
-  return plan.pair ? launch_prod<true>(p, gated, l, tm, tn, half, a, grid, smem, st)
-                   : launch_prod<false>(p, gated, l, tm, tn, half, a, grid, smem, st);
+  return plan.pair ? launch_prod<true>(p, gated, l, a.join.partial, tm, tn, half, a, grid, smem, st)
+                   : launch_prod<false>(p, gated, l, a.join.partial, tm, tn, half, a, grid, smem, st);
 }
 
 cudaError_t selftest_linear_wait(cudaStream_t st) {
