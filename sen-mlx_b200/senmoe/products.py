@@ -15,6 +15,10 @@ gated pairs ``swiglu`` (silu) and ``geglu`` (tanh gelu), whose weight, bias and
 pre-activation hold ``2 * out`` rows, the gate's first.  Sums are fp32 and the
 result is rounded once.  Nothing synchronises with the host, so the calls can
 be captured into a CUDA graph.
+
+The calls record nothing for autograd: what they return has no ``grad_fn``,
+whatever their arguments require.  Training calls the ``_backward`` functions,
+or wraps a pair in a ``torch.autograd.Function``.
 """
 from __future__ import annotations
 
