@@ -40,11 +40,11 @@
 // products stand between the tensor pipe, the operands' way from L2 (a pair's
 // 256 x 256 tile asks for 64 bytes a cycle and SM of MMA time) and shared
 // memory, whose bandwidth operands, TMA and the epilogue's turning share:
-// 8192 x 2048 -> 8192 gelu with z kept 204 us = 1345 TFLOP/s, 81 % tensor pipe
+// 8192 x 2048 -> 8192 gelu with z kept 206 us = 1334 TFLOP/s, 78 % tensor pipe
 // (153 with neither loads nor epilogue, 171 without the epilogue).  Experts'
 // weights come from HBM once: 64 tokens down over 128 experts 69 us = 5.8 TB/s;
 // 4096 tokens swiglu 210 us for 1.09 GB and 206 GFLOP.  dW is bound by its
-// writes: 246 us for 805 MB, which a memset writes in 207.
+// writes: 247 us for 805 MB, which a memset writes in 204.
 //
 // Waits.  Every wait on an mbarrier is bounded (wait_or_abort): a role that
 // gives up raises the CTA's abort flag and records kDevWaitTimeout, the others
