@@ -308,3 +308,20 @@ def test_products_on_two_streams_at_once(senmoe, torch):
     senmoe.linear_check()
     for w, g in zip(want, got):
         assert all(torch.equal(p, q) for p, q in zip(w, g))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("rows", [1, 31, 33, 511, 512, 513, 769, 16384, 16385, 40001])
+@pytest.mark.parametrize("out,stride", [(136, 136), (33, 40), (257, 257)])
+def test_bias_gradient_without_an_activation(senmoe, torch, rows, out, stride, dtype):
+    """Where dW does not take the sums: not asked for, or on the copying kernels."""
+    import linear_ref as R
+    k = 24
+    dy = _normal(torch, 1, rows, stride, dtype=dtype)[:, :out]
+    x, w = _normal(torch, 2, rows, k, dtype=dtype), _normal(torch, 3, out, k, dtype=dtype)
+    ref, size = dy.double().sum(0), dy.double().abs().sum(0)
+    err = (rows + 8) * 2.0 ** -23 * size
+    bound = err + R.HALF_UNIT[x.dtype] * (ref.abs() + err) + R.TINY[x.dtype]
+    for path, dw in ((senmoe.LINEAR_AUTO, False), (senmoe.LINEAR_ANY, True), (senmoe.LINEAR_AUTO, True)):
+        db = senmoe.linear_backward(dy, x, w, bias=True, need_dx=False, need_dweight=dw, path=path)[2]
+        R.assert_within(db, ref, bound, "db")
