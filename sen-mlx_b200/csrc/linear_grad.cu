@@ -6,12 +6,12 @@
 // here from the fp32 values.  dz itself is rounded once to the operands' 16-bit
 // type, because it is an operand of both gradient products on the 16-bit
 // tensor cores.  That rounding (at most 2^-8 of the value in bf16, 2^-11 in
-// fp16, whose range dz_exponent extends) is independent from element to element and so adds to dx and dW about
-// as much as their own rounding does: 0.0023 of a gradient's norm in bf16
-// against 0.0017 for fp32 sums of an unrounded dz.  Over some 10,000 random
-// sizes the ratio was 1.4, and up to 1.8 where a few large elements decide (a
-// handful of rows).  Carrying dz in two 16-bit parts would bring it to 1 for
-// twice the products.
+// fp16, whose range dz_exponent extends) is independent from element to
+// element and so adds to dx and dW about as much as their own rounding does:
+// 0.0023 of a gradient's norm in bf16 against 0.0017 for fp32 sums of an
+// unrounded dz.  Over some 10,000 random sizes the ratio was 1.4, and up to 1.8
+// where a few large elements decide (a handful of rows).  Carrying dz in two
+// 16-bit parts would bring it to 1 for twice the products.
 
 #include <type_traits>
 
@@ -74,9 +74,9 @@ template <bool BF16, int V, int ACT> struct Piece {
   }
 };
 
-// dz alone.  A warp a piece of a row (kUnroll steps), V columns a lane and step: 8 (16-byte accesses) where every
-// row starts on a 16-byte boundary, else 1.  The loads of kUnroll steps are in
-// flight together.  Bound by HBM: dy and z read once, dz written once; 36 us
+// dz alone.  A warp takes a piece of a row (kUnroll steps), V columns a lane
+// and step: 8 (16-byte accesses) where every row starts on a 16-byte boundary,
+// else 1.  The loads of kUnroll steps are in flight together.  Bound by HBM: dy and z read once, dz written once; 36 us
 // for 32768 rows of 2 x 768 (252 MB, 7.0 TB/s with part of the writes still in
 // L2; 82 us with a thread an element group and a division each).
 template <bool BF16, int V, int ACT>
@@ -117,17 +117,20 @@ __global__ void __launch_bounds__(kThreads) dz_kernel(const LinearGradArgs a) {
 // memory.  Each group's part of a run goes to slot (run + group) of `partial`:
 // along the rows every new pair of run and group raises that number, so no two
 // share a slot, and a group's slots follow from its offsets alone.  A dense
-// product of one run goes straight to dbias (without an activation its runs are
-// longer, read in turns, for a small workspace: dW mostly takes these sums).  The order of every sum is fixed.
+// product of one run goes straight to dbias (without an activation its runs
+// are longer, read in turns, for a small workspace: dW mostly takes these
+// sums).  The order of every sum is fixed.
+//
 // 57 us for 32768 rows of 2 x 768 in 128 groups, 18 for 4096 x 2112 (dz alone
-// 38.5 and 11), a join kernel included; dW's launch joins the parts for nothing.
-// 16 or 32 rows a run with all loads out at once: with a block's rows in a loop, or
-// more than 85 registers (two blocks an SM), it took 72 and 20.
+// 38.5 and 11), a join kernel included; dW's launch joins the parts for
+// nothing.  With a block's rows in a loop, or more than 85 registers (two
+// blocks an SM), it took 72 and 20.
+//
 // fp16 (with or without a bias gradient): a first launch stores dz as it is and
 // raises each group's dz_max to its largest finite |dz|; a second one (SCALED)
-// stores the groups again that need a scale (dz_exponent).  Where none does, the
-// maxima and that launch cost 3 us (333 x 2048 -> 2048 silu, 23.7 -> 26.4) to a
-// tenth of the backward pass (512 rows in 128 groups, 150 -> 163).
+// stores the groups again that need a scale (dz_exponent).  Where none does,
+// the maxima and that launch cost 3 us (333 x 2048 -> 2048 silu, 23.7 -> 26.4)
+// to a tenth of the backward pass (512 rows in 128 groups, 150 -> 163).
 template <bool BF16, int V, int ACT, bool SCALED>
 __global__ void __launch_bounds__(kThreads, 3) dz_sums_kernel(const LinearGradArgs a) {
   using P = Piece<BF16, V, ACT>;
