@@ -31,6 +31,10 @@
  *                              (deepseek_v2.rs:528), with the activation and the residual
  *                              add that follow it, dense or grouped by expert
  *   senmoe_linear_backward  <- (no counterpart: the reference does not train)
+ *   senmoe_rms_norm         <- the residual add and the norm before the block, h = x + r and
+ *                              post_attention_layernorm(h) (deepseek_v2.rs:613-620)
+ *   senmoe_quantize8, senmoe_linear8
+ *                           <- (no counterpart: MLX quantizes weights only)
  *
  * Weight layout is MLX's affine-quantized layout, unchanged
  * (src/engine/mlx_native.rs:3381-3389, 3473-3477): for a [E, out, in]
@@ -452,6 +456,132 @@ int senmoe_linear_check(senmoe_stream_t stream);
 /* Test of the above: launches a kernel on `stream` whose one wait runs out
  * after its limit (about 2 s), as the kernels' waits would. */
 int senmoe_selftest_linear_wait(senmoe_stream_t stream);
+
+/* ---- RMS norm, with the residual's addition and an output in 8 bits.
+ *
+ *   h = x + residual                          (rounded to the tensors' type; x itself without one)
+ *   y = h / sqrt(mean(h^2) + eps) * g         g = weight, or 1 + weight with unit_offset
+ *
+ * in 16 bits (y), in 8 bits with scales (codes, scales; see "rows in 8 bits"
+ * below), or both.  x, residual, h and y are bf16, or all are fp16; weight is
+ * of their type, or fp32.  Sums are fp32, every output is rounded once.
+ * Strides are in elements; the innermost dimension is contiguous.  Rows on a
+ * 16-byte grid (bases, row strides) of a multiple of 8 elements, up to 16384,
+ * are read once; others element by element.  h may be x's or the residual's
+ * rows (same base and stride); no other output may overlap an input. */
+typedef struct SenMoeNorm {
+  int32_t dtype;         /* SenMoeDtype */
+  int32_t weight_fp32;   /* weight is fp32 */
+  int32_t unit_offset;   /* weights are stored around zero */
+  float eps;
+  int64_t rows, hidden;
+  const void* x;         /* [rows, hidden] */
+  int64_t x_stride;
+  const void* residual;  /* [rows, hidden], or NULL */
+  int64_t residual_stride;
+  const void* weight;    /* [hidden] */
+  void* h;               /* x + residual, or NULL */
+  int64_t h_stride;
+  void* y;               /* or NULL */
+  int64_t y_stride;
+  void* codes;           /* [rows, hidden], or NULL; then hidden is a multiple of 32 */
+  int64_t codes_stride;
+  void* scales;          /* [rows, hidden / 32] */
+  int64_t scales_stride;
+} SenMoeNorm;
+int senmoe_rms_norm(const SenMoeNorm* norm, senmoe_stream_t stream);
+
+/* Gradients of the norm above from dy; with dn = dy g, r = 1 / sqrt(mean(h^2) + eps):
+ *   dx = r (dn - h r^2 mean(dn h)) + dh       (the residual's gradient as well)
+ *   dweight = sum over the rows of dy h r
+ * dh is the gradient that reaches h beside the norm (the residual stream's),
+ * or NULL.  dx and dweight may each be NULL.  dweight has weight's type; the
+ * same call gives the same bits.  workspace: device memory of at least
+ * senmoe_rms_norm_backward_workspace(grad) bytes (16-byte aligned; NULL when
+ * that is 0), in use until the call's work on the stream is done. */
+typedef struct SenMoeNormGrad {
+  int32_t dtype, weight_fp32, unit_offset;
+  float eps;
+  int64_t rows, hidden;
+  const void* dy;
+  int64_t dy_stride;
+  const void* h;
+  int64_t h_stride;
+  const void* weight;
+  const void* dh;
+  int64_t dh_stride;
+  void* dx;
+  int64_t dx_stride;
+  void* dweight;         /* [hidden] */
+  void* workspace;
+  int64_t workspace_bytes;
+} SenMoeNormGrad;
+/* Bytes of workspace the call needs on the current device, or a negative status. */
+int64_t senmoe_rms_norm_backward_workspace(const SenMoeNormGrad* grad);
+int senmoe_rms_norm_backward(const SenMoeNormGrad* grad, senmoe_stream_t stream);
+
+/* ---- Rows in 8 bits: e4m3 elements (codes, a byte each) and for every 32
+ * consecutive ones of a row a scale 2^(byte - 127) (scales, a byte each; 255 is
+ * NaN), the smallest with which the 32 are at most 448 = e4m3's largest.  An
+ * element is rounded once, to nearest even.  A block that holds an infinity or
+ * a NaN reads as NaN.  The kernels read codes with TMA: bases and row strides
+ * are multiples of 16.
+ *
+ * senmoe_quantize8: codes [rows, wide] of x [rows, n] (SENMOE_EPI_NONE, wide =
+ * n), or of dz = x * epilogue'(preact) (as in senmoe_linear_backward, from
+ * fp32 values, wide = 2 * n for a gated pair), n a multiple of 32. */
+typedef struct SenMoeQuantize8 {
+  int32_t dtype;         /* SenMoeDtype of x and preact */
+  int32_t epilogue;      /* SenMoeEpilogue */
+  int64_t rows, n;
+  const void* x;         /* [rows, n] */
+  int64_t x_stride;
+  const void* preact;    /* [rows, wide]; NULL for SENMOE_EPI_NONE */
+  int64_t preact_stride;
+  void* codes;           /* [rows, wide] */
+  int64_t codes_stride;
+  void* scales;          /* [rows, wide / 32] */
+  int64_t scales_stride;
+} SenMoeQuantize8;
+int senmoe_quantize8(const SenMoeQuantize8* quantize, senmoe_stream_t stream);
+
+/* The linear product above over x and weight in 8 bits, dense or grouped by
+ * expert:
+ *   z[s, :] = x[s, :] @ weight[e(s)]^T + bias[e(s)]          (fp32)
+ *   y[s, :] = epilogue(z[s, :]) + residual[s, :]
+ * in_features is a multiple of 32.  Products and sums are those of the values
+ * the bytes stand for, in fp32.  y comes out in 16 bits (y) or in 8 bits with
+ * scales (y_codes, y_scales; out_features a multiple of 32), one of the two,
+ * rounded once.  bias, residual, y and preact are bf16, or all are fp16.
+ * offsets, groups, uncovered rows (zeros; in 8 bits both bytes) and overlaps
+ * as in senmoe_linear.  path: SENMOE_LINEAR_ANY is not offered
+ * (SENMOE_ERR_UNSUPPORTED), the others as there.  senmoe_linear_check reports
+ * these kernels' waits too. */
+typedef struct SenMoeLinear8 {
+  int32_t dtype, epilogue, num_groups, path;
+  int64_t rows, in_features, out_features;
+  const void* x;               /* codes [S, in] */
+  int64_t x_stride;
+  const void* x_scales;        /* [S, in / 32] */
+  int64_t x_scales_stride;
+  const void* weight;          /* codes [E, wide, in] */
+  int64_t weight_stride, weight_group_stride;
+  const void* weight_scales;   /* [E, wide, in / 32] */
+  int64_t weight_scales_stride, weight_scales_group_stride;
+  const int32_t* offsets;      /* device int32 [E + 1], or NULL */
+  const void* bias;            /* [E, wide] contiguous, or NULL */
+  const void* residual;        /* [S, out], or NULL */
+  int64_t residual_stride;
+  void* y;                     /* [S, out], or NULL */
+  int64_t y_stride;
+  void* y_codes;               /* [S, out], or NULL */
+  int64_t y_codes_stride;
+  void* y_scales;              /* [S, out / 32] */
+  int64_t y_scales_stride;
+  void* preact;                /* z [S, wide], or NULL */
+  int64_t preact_stride;
+} SenMoeLinear8;
+int senmoe_linear8(const SenMoeLinear8* product, senmoe_stream_t stream);
 
 /* Allocation-free forward (no counterpart in the reference; this build adds
  * it for callers that cannot allocate device memory at call time: code inside

@@ -3,31 +3,15 @@
 
 #include <cuda_runtime.h>
 
-#include <cstdarg>
-#include <cstdio>
-
 #include "../../include/senmoe.h"
+#include "checks.h"
 #include "kernels.h"
 #include "linear.cuh"
+#include "linear8.cuh"
 
 using namespace senmoe;
 
 namespace {
-
-int reject(int status, const char* fmt, ...) {
-  char buf[384];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  return set_failure(status, buf);
-}
-
-int cuda_status(const char* what, cudaError_t e) {
-  if (e == cudaSuccess) return SENMOE_OK;
-  return reject(e == cudaErrorNotSupported ? SENMOE_ERR_UNSUPPORTED : SENMOE_ERR_CUDA, "%s: %s", what,
-                cudaGetErrorString(e));
-}
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024;  // row numbers, a tile past the last included, fit an int32
@@ -288,9 +272,11 @@ int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
 
 int senmoe_linear_check(senmoe_stream_t stream) {
   clear_failure();
-  int error = 0;
-  const int rc = cuda_status("linear_check", linear_device_error(stream, &error));
+  int error = 0, error8 = 0;
+  int rc = cuda_status("linear_check", linear_device_error(stream, &error));
   if (rc) return rc;
+  if ((rc = cuda_status("linear_check", linear8_device_error(stream, &error8)))) return rc;
+  if (!error) error = error8;
   if (error == kDevWaitTimeout) return reject(SENMOE_ERR_TIMEOUT, "linear: a bounded wait on the device ran out");
   return error ? reject(SENMOE_ERR_DEVICE, "linear: device error %d", error) : SENMOE_OK;
 }

@@ -86,6 +86,18 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float h
   }
 }
 
+template <bool BF16> __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = to_f32<BF16>(static_cast<uint16_t>(w[i]));
+    f[2 * i + 1] = to_f32<BF16>(static_cast<uint16_t>(w[i] >> 16));
+  }
+}
+template <bool BF16> __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
+}
+
 // Activations in fp32, rounded once, to 16 bits.  The intrinsics' error (a few
 // units in the last place, __expf one more for every unit of its argument: below
 // 2^-15 of the value down to z = -12) is far below a 16-bit unit.  Where its

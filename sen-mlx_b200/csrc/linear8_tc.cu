@@ -1,0 +1,818 @@
+// linear8_tc.cu -- the products over 8-bit rows on the 5th-generation tensor
+// cores: tcgen05.mma kind::mxf8f6f4 with block scales, accumulators in TMEM.
+//
+// A tile is D[features, w columns] as in linear_tc.cu: M (TMEM lanes) runs
+// along W's rows, N (w <= 224 columns) along the rows of x, so that a ragged
+// group costs MMA time in proportion to its rows.  A stage holds 128 k: the
+// operands as 128-byte-swizzled boxes by TMA, one byte an element, and their
+// scales, 4 bytes a row.  The tensor core multiplies by the scales itself:
+//
+//   D += sum over blocks b of 32 k:  2^(sw[m, b] + sx[n, b])  sum_k W[m, k] x[n, k]
+//
+// with fp32 sums.  It reads the scales from TMEM, where row r of an operand is
+// lane r mod 32 (the same in each quarter of the lanes) and column r / 32, the
+// four bytes of a word being four consecutive blocks.  Warps 2 and 3 bring
+// them there: a lane loads the words of rows l, l + 32, l + 64, l + 96 of 128
+// rows (16 bytes of a row, 4 stages, at a time where rows are aligned for it,
+// the next 4 stages' in flight), which side by side are the 16 bytes that
+// tcgen05.cp 32x128b wants for lane l, and the MMA warp issues the copies
+// ahead of a stage's MMAs.  Copies and MMAs of one thread run in order; two
+// sets of scale columns alternate all the same, so that a copy need not wait
+// for the MMAs before it.
+//
+// Forms of a tile: one CTA (128 features), a pair (cta_group::2, 256 features
+// on two SMs, each holding half of the columns' codes and all of their
+// scales), or a K split over a cluster; gated pairs lay 64 gate rows over the
+// same features' 64 up rows.  Waits are bounded, and those without a limit
+// need none, as in linear_tc.cu.
+//
+// 8-bit output: a warp's 32 lanes are 32 consecutive features, one block of a
+// row of y, so the block's largest is one warp reduction a column.
+
+#include <cuda.h>
+
+#include <mutex>
+
+#include "kernels.h"
+#include "linear8.cuh"
+#include "linear_tiles.cuh"
+
+namespace senmoe {
+namespace {
+
+constexpr int kBK8 = 128;                      // k of a stage: one 128-byte line
+constexpr uint32_t kMBytes8 = 128 * kBK8;      // a CTA's M operand of a stage
+constexpr int kMaxWidth = 224;                 // columns of a tile: two accumulators and two sets of scales in 512
+constexpr uint32_t kAccColumn = 256;           // from one accumulator to the other
+constexpr uint32_t kScaleColumn = 240;         // of the scales, behind each accumulator
+constexpr uint32_t kAtomBytes = 512;           // 128 rows' scales of a stage
+constexpr uint32_t kScaleBytes = 3 * kAtomBytes;  // W's rows, then up to 256 columns
+constexpr uint32_t kStaticBytes8 = 9 * 1024 + 1024;
+constexpr uint32_t epilogue_bytes8(bool gated) { return kEpiWarps * (kTurnBytes + (gated ? kSwapBytes : 0)); }
+constexpr uint32_t ring_budget8(bool gated) { return 227 * 1024 - kStaticBytes8 - epilogue_bytes8(gated); }
+
+__device__ int g_linear8_error;  // first device error of these kernels on this device
+__device__ int g_linear8_taken;  // what the last check found there
+
+struct Tc8Args {
+  Linear8Args l;
+  int bn, part;          // columns of a tile, and of a CTA's N operand (half of it in a pair)
+  int m_tiles, stages, split;
+  uint32_t stage_bytes;  // a stage's operands
+  int w_load, x_load;    // bytes of a scale row in one load: 16, 8, 4 or 1
+  long long tile_limit;  // of the wait for a tile's accumulators, cycles
+};
+
+// Instruction descriptor, block-scaled 8-bit kinds: e4m3 x e4m3 (0, 0), both
+// K-major, N / 8 from bit 17, scales in e8m0 (bit 23), M / 128 from bit 27.
+// The byte of a scale word that an MMA of 32 k takes is in bits 4 (B) and 29 (A).
+__device__ __forceinline__ uint32_t instr_desc8(int n, int m) {
+  return (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 7) << 27);
+}
+template <bool PAIR>
+__device__ __forceinline__ void umma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                            uint32_t accumulate) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+// 32 rows of 16 bytes at saddr -> 4 TMEM columns, the same in every quarter of
+// the lanes.  Unswizzled descriptor: 8-row groups 128 bytes apart.
+template <bool PAIR> __device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
+  const uint64_t desc = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
+  if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// (release at cluster scope: what the lanes wrote to their own shared memory
+// is read by MMAs that the other CTA issues)
+__device__ __forceinline__ void arrive_release_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// ------------------------------------------------------------------ tiles
+struct Tile8 {
+  int e;         // group
+  int m0;        // this CTA's first feature
+  int c0, w, n;  // first column (a row of x), columns, columns of the MMA
+  int kb0, kb1;  // this CTA's k blocks
+};
+
+template <bool GATED, bool PAIR>
+__device__ __forceinline__ Tile8 tile_at8(const Tc8Args& a, const int* s_off, const int* s_pre, int idx, int rank) {
+  constexpr int kFeat = GATED ? 64 : 128, kStep = PAIR ? 32 : 16;
+  Tile8 t;
+  const int mt = idx % a.m_tiles, rest = idx / a.m_tiles;
+  t.m0 = PAIR ? (2 * mt + rank) * kFeat : mt * kFeat;
+  // a group's rows in equal chunks of at most bn
+  t.e = group_of(s_pre, a.l.groups, rest);
+  const int off = s_off[t.e], cnt = s_off[t.e + 1] - off, nch = s_pre[t.e + 1] - s_pre[t.e], j = rest - s_pre[t.e];
+  const int each = ((cnt + nch - 1) / nch + kStep - 1) & ~(kStep - 1);
+  t.c0 = off + j * each;
+  t.w = min(each, cnt - j * each);
+  t.n = (t.w + kStep - 1) & ~(kStep - 1);
+  const int kb = (a.l.k + kBK8 - 1) / kBK8;
+  t.kb0 = 0;
+  t.kb1 = kb;
+  if constexpr (!PAIR) {
+    if (a.split > 1) {
+      t.kb0 = static_cast<int>(static_cast<int64_t>(kb) * rank / a.split);
+      t.kb1 = static_cast<int>(static_cast<int64_t>(kb) * (rank + 1) / a.split);
+    }
+  }
+  return t;
+}
+
+// The scales of a row's blocks 16 q .. 16 q + 15 (four stages), row at p, `have`
+// blocks in all: `load` bytes at a time; what lies past the row reads as 2^0
+// (no MMA takes it).
+__device__ __forceinline__ uint4 load_scales(const uint8_t* p, int q, int have, int load) {
+  uint32_t w[4] = {0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+  const int at = 16 * q;
+  p += at;
+  if (load == 16) {
+    if (at < have) return *reinterpret_cast<const uint4*>(p);
+  } else if (load == 8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (at + 8 * i < have) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p + 8 * i);
+        w[2 * i] = v.x;
+        w[2 * i + 1] = v.y;
+      }
+    }
+  } else if (load == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + 4 * i < have) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (at + i < have) w[i >> 2] = (w[i >> 2] & ~(0xffu << 8 * (i & 3))) | static_cast<uint32_t>(p[i]) << 8 * (i & 3);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// ---------------------------------------------------------------- epilogue
+// 16 columns x 32 features, a feature a lane -> 8 bits: each column's 32
+// values are one block of a row of y.
+__device__ __forceinline__ void store_chunk8(const float (&v)[16], uint32_t* turn, uint8_t* codes, int64_t stride,
+                                             uint8_t* scales, int64_t scales_stride, int w, int lane) {
+  uint8_t* t8 = reinterpret_cast<uint8_t*>(turn);
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    uint32_t byte;
+    t8[i * 32 + lane] = pack8_warp(v[i], byte);
+    if (lane == i) mine = byte;
+  }
+  __syncwarp();
+  const int c = lane >> 1, half = lane & 1;
+  const uint4 q = *reinterpret_cast<const uint4*>(t8 + c * 32 + half * 16);
+  __syncwarp();
+  if (c < w) *reinterpret_cast<uint4*>(codes + c * stride + half * 16) = q;
+  if (lane < w && lane < 16) scales[lane * scales_stride] = static_cast<uint8_t>(mine);
+}
+
+// What a warp needs to finish a tile's accumulators.
+template <bool GATED, bool BF16, bool EIGHT> struct Finish8 {
+  const Linear8Args& l;
+  uint16_t *out, *pre;
+  int cols;  // features of the output
+  bool vec, pvec;
+  uint32_t* turn;
+  int lane;
+  __device__ __forceinline__ Finish8(const Linear8Args& args, uint32_t* t, int ln) : l(args), turn(t), lane(ln) {
+    cols = l.n / (GATED ? 2 : 1);
+    out = static_cast<uint16_t*>(l.y);
+    pre = static_cast<uint16_t*>(l.preact);
+    vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (l.y_stride & 7) == 0;
+    pvec = (reinterpret_cast<uintptr_t>(pre) & 15) == 0 && (l.preact_stride & 7) == 0 && (!GATED || (cols & 7) == 0);
+  }
+  __device__ __forceinline__ float bias(int e, int f, int lanes, int up) const {
+    if (l.bias && lane < lanes)
+      return to_f32<BF16>(static_cast<const uint16_t*>(l.bias)[static_cast<int64_t>(e) * l.n + up + f + lane]);
+    return 0.0f;
+  }
+  // z (bias added) of 16 columns -> preact, at column `at` of its rows
+  __device__ __forceinline__ void keep(const float (&z)[16], int64_t row, int at, int w, int feats) const {
+    if (pre) store_chunk<BF16>(z, turn, pre + row * l.preact_stride + at, l.preact_stride, w, feats, pvec, lane);
+  }
+  // the activated values, + residual -> y
+  __device__ __forceinline__ void write(float (&y)[16], int64_t row, int f, int w, int feats) const {
+    if (l.residual && lane < feats) {
+      const uint16_t* res = static_cast<const uint16_t*>(l.residual) + row * l.residual_stride + f + lane;
+      uint16_t r[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r[i] = i < w ? res[i * l.residual_stride] : uint16_t(0);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] += to_f32<BF16>(r[i]);
+    }
+    if constexpr (EIGHT) {
+      if (feats > 0)  // whole blocks: 32 features or none
+        store_chunk8(y, turn, l.codes + row * l.codes_stride + f, l.codes_stride,
+                     l.scales + row * l.scales_stride + f / kBlock8, l.scales_stride, w, lane);
+    } else {
+      store_chunk<BF16>(y, turn, out + row * l.y_stride + f, l.y_stride, w, feats, vec, lane);
+    }
+  }
+};
+
+template <bool GATED, bool BF16, bool PAIR, bool EIGHT>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    linear8_tc_kernel(const __grid_constant__ CUtensorMap tm_m, const __grid_constant__ CUtensorMap tm_n,
+                      const __grid_constant__ CUtensorMap tm_half, const __grid_constant__ Tc8Args a) {
+  constexpr int kCtas = PAIR ? 2 : 1;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t bar_full[kMaxStages], bar_empty[kMaxStages], bar_accfull[2], bar_accempty[2],
+      bar_drain;
+  __shared__ int s_off[kMaxGroups + 1], s_pre[kMaxGroups + 1], s_tot[64];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_abort;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int* err = &g_linear8_error;
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t ring = (raw + 1023u) & ~1023u;
+  unsigned char* ring_ptr = smem_raw + (ring - raw);
+  const int stages = a.stages;
+  const uint32_t scale_base = ring + stages * a.stage_bytes;  // [stage][W's rows, columns 0-127, columns 128 on]
+  unsigned char* scale_ptr = ring_ptr + stages * a.stage_bytes;
+  unsigned char* epi_ptr = scale_ptr + stages * kScaleBytes;
+  const auto turn_of = [&](int ew) { return reinterpret_cast<uint32_t*>(epi_ptr + ew * kTurnBytes); };
+  const auto swap_of = [&](int ew) { return reinterpret_cast<float*>(epi_ptr + kEpiWarps * kTurnBytes + ew * kSwapBytes); };
+  const int csize = PAIR ? 2 : a.split;  // CTAs of the cluster
+  const int rank = csize > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int unit = blockIdx.x / csize, units = gridDim.x / csize;
+
+  if (tid == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&bar_full[i], 1 + 2 * kCtas);  // the loads, and the scale warps of both CTAs
+      mbar_init(&bar_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar_accfull[i], 1);
+      mbar_init(&bar_accempty[i], kCtas * kEpiWarps);
+    }
+    mbar_init(&bar_drain, 1);
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_map(&tm_m);
+    prefetch_map(&tm_n);
+  }
+  group_table(a.l.offsets, a.l.groups, a.l.rows, a.bn, s_off, s_pre, s_tot);
+  __syncthreads();
+  // the other CTAs run and their barriers exist before anything arrives on
+  // them, and before a pair asks for its TMEM on both SMs
+  if (csize > 1) cluster_sync();
+  if (warp == 1) tmem_alloc<PAIR>(&s_tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int tiles = a.m_tiles * s_pre[a.l.groups];
+  // shared by all roles: the tile's k blocks walk the ring in order
+  auto next = [stages](int& st, int& ph) {
+    if (++st == stages) { st = 0; ph ^= 1; }
+  };
+
+  if (warp == 0) {
+    // ============================================================ producer
+    if (lane == 0) {
+      uint32_t issued = 0, parity = 0;  // by stage: loaded at least once, parity of the last load
+      int st = 0, ph = 0;
+      bool ok = true;
+      for (int idx = unit; idx < tiles && ok; idx += units) {
+        const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
+        const int part = t.n / kCtas, col = t.c0 + (PAIR ? rank * part : 0);  // this CTA's share of the columns
+        // one load of a full part, or of half of one where that holds the columns
+        const bool small = 2 * part <= a.part && a.part >= 32;
+        const uint32_t bytes = kMBytes8 + (small ? a.part / 2 : a.part) * kBK8;
+        for (int b = t.kb0; b < t.kb1; ++b) {
+          if (!(ok = wait_or_abort(&bar_empty[st], ph ^ 1, &s_abort, err))) break;
+          const uint32_t sm = ring + st * a.stage_bytes, sn = sm + kMBytes8;
+          uint32_t full = smem_u32(&bar_full[st]);
+          if constexpr (PAIR) {
+            if (rank == 0) mbar_arrive_expect_tx(&bar_full[st], 2 * bytes);
+            full = map_rank(full, 0);
+          } else {
+            mbar_arrive_expect_tx(&bar_full[st], bytes);
+          }
+          const int k0 = b * (kBK8 / 2);  // the maps count pairs of elements
+          tma_4d<PAIR>(sm, &tm_m, k0, t.m0, 0, t.e, full);
+          tma_4d<PAIR>(sn, small ? &tm_half : &tm_n, k0, col, 0, 0, full);
+          issued |= 1u << st;
+          parity = (parity & ~(1u << st)) | (static_cast<uint32_t>(ph) << st);
+          next(st, ph);
+        }
+      }
+      // the last loads of every stage have been consumed (a pair: so no
+      // arrival is still on its way when the CTA leaves)
+      volatile int never = 0;
+      for (int i = 0; i < stages; ++i) {
+        if (!(issued >> i & 1)) continue;
+        if (ok) ok = wait_or_abort(&bar_empty[i], parity >> i & 1, &s_abort, err);
+        // gave up: copies already issued get a bounded chance to land
+        if (!ok && (!PAIR || rank == 0)) wait_or_abort(&bar_full[i], parity >> i & 1, &never, nullptr);
+      }
+    }
+  } else if (warp == 1 && (!PAIR || rank == 0)) {
+    // ========================================================== MMA issuer
+    const bool leader = elect_one();
+    bool ok = true;
+    int st = 0, ph = 0, it = 0;
+    uint32_t set = 0;  // of scale columns
+    for (int idx = unit; idx < tiles && ok; idx += units, ++it) {
+      const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
+      const int ab = it & 1, aph = (it >> 1) & 1;
+      if (!(ok = warp_wait(&bar_accempty[ab], aph ^ 1, &s_abort, err))) break;
+      tc_fence_after();
+      const uint32_t d = tmem + ab * kAccColumn;
+      const uint32_t idesc = instr_desc8(t.n, 128 * kCtas);
+      for (int b = t.kb0; b < t.kb1; ++b) {
+        if (!(ok = warp_wait(&bar_full[st], ph, &s_abort, err))) break;
+        tc_fence_after();
+        if (leader) {
+          const uint32_t sm = ring + st * a.stage_bytes, sc = scale_base + st * kScaleBytes;
+          const uint32_t sa = tmem + kScaleColumn + set * kAccColumn, sb = sa + 4;
+          copy_scales<PAIR>(sa, sc);
+          copy_scales<PAIR>(sb, sc + kAtomBytes);
+          if (t.n > 128) copy_scales<PAIR>(sb + 4, sc + 2 * kAtomBytes);
+          const uint64_t dm = smem_desc<false>(sm), dn = smem_desc<false>(sm + kMBytes8);
+          const int ks = min(kBK8, a.l.k - b * kBK8) / kBlock8;
+          for (int s = 0; s < ks; ++s)  // 32 k: 32 bytes along a line
+            umma_scaled<PAIR>(d, dm + s * (32 >> 4), dn + s * (32 >> 4), idesc | (s << 4) | (s << 29), sa, sb,
+                              (b > t.kb0 || s > 0) ? 1u : 0u);
+          umma_commit<PAIR>(&bar_empty[st]);
+        }
+        __syncwarp();
+        set ^= 1;
+        next(st, ph);
+      }
+      if (ok && leader) umma_commit<PAIR>(&bar_accfull[ab]);
+      __syncwarp();
+    }
+    // every MMA issued has completed once this fires
+    if (leader) umma_commit<PAIR>(&bar_drain);
+    __syncwarp();
+    volatile int never = 0;
+    wait_or_abort(&bar_drain, 0, &never, nullptr);
+  } else if (warp == 2 || warp == 3) {
+    // ============================================================== scales
+    // warp 2: W's 128 rows of the tile; warp 3: the columns, 128 at a time
+    const Linear8Args& l = a.l;
+    const int blocks = l.k / kBlock8, cap = static_cast<int>(l.rows) - 1;
+    const int load = warp == 2 ? a.w_load : a.x_load;
+    int st = 0, ph = 0;
+    bool ok = true;
+    for (int idx = unit; idx < tiles && ok; idx += units) {
+      const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
+      const int atoms = warp == 2 ? 1 : (t.n + 127) / 128;
+      // this lane's rows; past the last one, that one (no result is of it)
+      const uint8_t* p[2][4];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 32 + lane;
+          if (warp == 2) {
+            const int half = GATED ? l.n / 2 : l.n, f = GATED ? t.m0 + (r & 63) : t.m0 + r;
+            const int64_t row = min(f, half - 1) + (GATED && r >= 64 ? half : 0);
+            p[g][i] = l.w_scales + t.e * l.w_scales_group_stride + row * l.w_scales_stride;
+          } else {
+            p[g][i] = l.x_scales + static_cast<int64_t>(min(t.c0 + g * 128 + r, cap)) * l.x_scales_stride;
+          }
+        }
+      }
+      uint4 now[2][4], then[2][4];
+      const auto fetch = [&](uint4 (&v)[2][4], int q) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (g < atoms) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[g][i] = load_scales(p[g][i], q, blocks, load);
+          }
+        }
+      };
+      const int q0 = t.kb0 / 4, q1 = (t.kb1 + 3) / 4;
+      if (q0 < q1) fetch(now, q0);
+      for (int q = q0; q < q1 && ok; ++q) {
+        if (q + 1 < q1) fetch(then, q + 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int b = 4 * q + j;
+          if (b < t.kb0 || b >= t.kb1 || !ok) continue;
+          if (!(ok = warp_wait(&bar_empty[st], ph ^ 1, &s_abort, err))) continue;
+          unsigned char* dst = scale_ptr + st * kScaleBytes + (warp == 2 ? 0 : kAtomBytes) + lane * 16;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (g < atoms)
+              *reinterpret_cast<uint4*>(dst + g * kAtomBytes) = make_uint4(word_of(now[g][0], j), word_of(now[g][1], j),
+                                                                         word_of(now[g][2], j), word_of(now[g][3], j));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) arrive_release_at(PAIR ? map_rank(smem_u32(&bar_full[st]), 0) : smem_u32(&bar_full[st]));
+          next(st, ph);
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) now[g][i] = then[g][i];
+        }
+      }
+    }
+  } else if (warp >= kEpiWarp0 && (PAIR || a.split <= 1)) {
+    // ============================================================ epilogue
+    // 32 columns at a time, the warps of a lane quarter in turn
+    const int ew = warp - kEpiWarp0, q = warp & 3, turn2 = ew >> 2;
+    const Finish8<GATED, BF16, EIGHT> fin(a.l, turn_of(ew), lane);
+    int it = 0;
+    for (int idx = unit; idx < tiles; idx += units, ++it) {
+      const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
+      const int ab = it & 1, aph = (it >> 1) & 1;
+      // a gated pair: quarters 0, 1 hold the gate of features 32 (q & 1) on, 2, 3 the up
+      const int f0 = t.m0 + (GATED ? q & 1 : q) * 32, feats = min(32, fin.cols - f0);
+      const int up = GATED && q >= 2 ? fin.cols : 0;
+      const float bias = fin.bias(t.e, f0, feats, up);
+      bool go = warp_wait(&bar_accfull[ab], aph, &s_abort, err, a.tile_limit);
+      // the two warps that swap leave together, or one would wait for the other
+      if constexpr (GATED) go = both_warps(1 + (turn2 * 2 + (q & 1)), go);
+      if (!go) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + ab * kAccColumn;
+      const uint32_t release = PAIR ? map_rank(smem_u32(&bar_accempty[ab]), 0) : smem_u32(&bar_accempty[ab]);
+      bool released = false;
+      for (int c = turn2 * 32; c < t.w; c += kColStep) {
+        uint32_t r[32];
+        tmem_ld16(acc + c, r);
+        tmem_ld16(acc + c + 16, r + 16);
+        tmem_ld_wait();
+        if (c + kColStep >= t.w) {  // this warp's last read of the accumulator
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(release);
+          released = true;
+        }
+        const int64_t row = t.c0 + c;
+        float z[2][16];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i >> 4][i & 15] = __uint_as_float(r[i]) + bias;
+        if constexpr (GATED) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) fin.keep(z[h], row + 16 * h, up + f0, t.w - c - 16 * h, feats);
+          // gate warps finish columns c .. c + 15 and hand the others over, up warps the reverse
+          const bool gate = q < 2;
+          float* mine = swap_of(ew);
+          const float* theirs = swap_of(ew ^ 2);
+          const int bar = 1 + (turn2 * 2 + (q & 1));
+          float y[16], u[16];
+          if (gate) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mine[i * 32 + lane] = z[1][i];
+            asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              y[i] = z[0][i];
+              u[i] = theirs[i * 32 + lane];
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mine[i * 32 + lane] = z[0][i];
+            asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              y[i] = theirs[i * 32 + lane];
+              u[i] = z[1][i];
+            }
+          }
+          asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
+          act_chunk(a.l.act, y);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] *= u[i];
+          const int h = gate ? 0 : 16;
+          fin.write(y, row + h, f0, t.w - c - h, feats);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int w = t.w - c - 16 * h;
+            if (w <= 0) break;
+            fin.keep(z[h], row + 16 * h, f0, w, feats);
+            act_chunk(a.l.act, z[h]);
+            fin.write(z[h], row + 16 * h, f0, w, feats);
+          }
+        }
+      }
+      if (!released) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(release);
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    // =========================== K split: this CTA's accumulator is ready
+    if (unit < tiles) warp_wait(&bar_accfull[0], 0, &s_abort, err, a.tile_limit);
+    tc_fence_after();
+  }
+
+  __syncwarp();
+  if constexpr (!PAIR) {
+    if (csize > 1) {
+      // Chunks of 16 columns are dealt to the cluster's CTAs; every CTA sends
+      // its share of a chunk to the chunk's owner, whose ring is free by then,
+      // and the owner adds the shares in rank order: [its chunk][rank][column][lane].
+      cluster_sync();
+      const bool epi = warp >= kEpiWarp0 && unit < tiles;
+      const int ew = warp - kEpiWarp0;
+      Tile8 t{};
+      if (epi) t = tile_at8<GATED, PAIR>(a, s_off, s_pre, unit, rank);
+      const int chunks = (t.w + 15) / 16;
+      if (epi) {
+        const int q = warp & 3;
+        const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16);
+        for (int c = ew >> 2; c < chunks; c += kEpiWarps / 4) {
+          uint32_t r[16];
+          if (t.kb1 > t.kb0) {
+            tmem_ld16(acc + 16 * c, r);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = 0;
+          }
+          const uint32_t dst =
+              map_rank(ring + (((c / csize) * csize + rank) * 16 * 128 + q * 32 + lane) * 4, c % csize);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st_cluster(dst + i * 512, r[i]);
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      cluster_sync();  // every share is where it is added
+      if (epi) {
+        const Finish8<GATED, BF16, EIGHT> fin(a.l, turn_of(ew), lane);
+        constexpr int kQuarters = GATED ? 2 : 4;
+        const int mine = chunks > rank ? (chunks - rank + csize - 1) / csize : 0;  // chunks rank, rank + csize, ...
+        for (int i = ew; i < mine * kQuarters; i += kEpiWarps) {
+          const int q = i % kQuarters, slot = i / kQuarters, c = (slot * csize + rank) * 16, w = t.w - c;
+          const int f0 = t.m0 + q * 32, feats = min(32, fin.cols - f0);
+          const float b0 = fin.bias(t.e, f0, feats, 0), b1 = GATED ? fin.bias(t.e, f0, feats, fin.cols) : 0.0f;
+          const float* src = reinterpret_cast<const float*>(ring_ptr) + slot * csize * 16 * 128 + q * 32 + lane;
+          float z[16], u[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float v = 0.0f, v2 = 0.0f;
+#pragma unroll
+            for (int r = 0; r < kMaxSplit; ++r) {
+              if (r < csize) {
+                v += src[(r * 16 + k) * 128];
+                if constexpr (GATED) v2 += src[(r * 16 + k) * 128 + 64];
+              }
+            }
+            z[k] = v + b0;
+            u[k] = v2 + b1;
+          }
+          const int64_t row = t.c0 + c;
+          fin.keep(z, row, f0, w, feats);
+          if constexpr (GATED) fin.keep(u, row, fin.cols + f0, w, feats);
+          act_chunk(a.l.act, z);
+          if constexpr (GATED) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) z[k] *= u[k];
+          }
+          fin.write(z, row, f0, w, feats);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  if (a.l.offsets && warp >= kEpiWarp0) {  // rows of no group: zero
+    const Linear8Args& l = a.l;
+    uint16_t *out = static_cast<uint16_t*>(l.y), *pre = static_cast<uint16_t*>(l.preact);
+    const int cols = l.n / (GATED ? 2 : 1), first = tid - kEpiWarp0 * 32;
+    const int64_t head = s_off[0], tail = s_off[l.groups], n = head + (l.rows - tail);
+    for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
+      const int64_t r = i < head ? i : tail + (i - head);
+      if constexpr (EIGHT) {
+        for (int f = first; f < cols; f += kEpiWarps * 32) l.codes[r * l.codes_stride + f] = 0;
+        for (int f = first; f < cols / kBlock8; f += kEpiWarps * 32) l.scales[r * l.scales_stride + f] = 0;
+      } else {
+        for (int f = first; f < cols; f += kEpiWarps * 32) out[r * l.y_stride + f] = 0;
+      }
+      if (pre)
+        for (int f = first; f < l.n; f += kEpiWarps * 32) pre[r * l.preact_stride + f] = 0;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR && rank == 1 && warp == 1) {
+    // The leader's drain commit arrives here too: waited for with this CTA's
+    // tiles finished, so that the limit does not run from the kernel's start.
+    volatile int never = 0;
+    wait_or_abort(&bar_drain, 0, &never, nullptr);
+    __syncwarp();
+  }
+  if (csize > 1) cluster_sync();  // nobody reads this CTA's shared memory or TMEM any more
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free<PAIR>(tmem);
+  }
+  // A pair frees its TMEM together, see linear_tc.cu.
+  __syncwarp();
+  if constexpr (PAIR) cluster_sync();
+}
+
+__global__ void take_error8_kernel() { g_linear8_taken = atomicExch(&g_linear8_error, 0); }
+
+// ------------------------------------------------------------- host side
+int tc8_sm_count() {
+  static int counts[64] = {};  // by device; the same value whoever writes it
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && counts[dev] > 0) return counts[dev];
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+  if (dev < 64) counts[dev] = n;
+  return n;
+}
+
+constexpr uint32_t stage_bytes8(int part) { return kMBytes8 + part * kBK8; }
+constexpr int stages8(bool gated, int part) {
+  const int fit = static_cast<int>(ring_budget8(gated) / (stage_bytes8(part) + kScaleBytes));
+  return fit < kMaxStages ? fit : kMaxStages;
+}
+constexpr size_t smem8(bool gated, int part) {
+  return 1024 + static_cast<size_t>(stages8(gated, part)) * (stage_bytes8(part) + kScaleBytes) + epilogue_bytes8(gated);
+}
+// As in linear_tc.cu: no two CTAs that use TMEM share an SM.
+constexpr bool one_cta_an_sm8() {
+  for (int part = 16; part <= kMaxWidth; part += 16)
+    if (smem8(false, part) < 120 * 1024 || smem8(true, part) < 120 * 1024) return false;
+  return true;
+}
+static_assert(one_cta_an_sm8(), "tcgen05.alloc would wait for the CTA beside");
+
+// Bytes of scale rows that one load may take: the rows' alignment allows it,
+// and rows are whole loads, so that none passes the last row's end.
+int scale_load(const void* p, int64_t stride, int64_t group_stride, int k) {
+  for (int n = 16; n > 1; n /= 2)
+    if (n != 2 && reinterpret_cast<uintptr_t>(p) % n == 0 && stride % n == 0 && group_stride % n == 0 &&
+        k / kBlock8 % n == 0)
+      return n;
+  return 1;
+}
+
+template <bool GATED, bool BF16, bool PAIR, bool EIGHT>
+cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorMap& half, const Tc8Args& a, int grid,
+                     size_t smem, cudaStream_t st) {
+  auto kern = linear8_tc_kernel<GATED, BF16, PAIR, EIGHT>;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
+  if (e != cudaSuccess) return e;
+  // in plain stream order: the kernel takes the whole SM, TMEM included
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : a.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR || a.split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, m, n, half, a);
+}
+
+// The form of a product's tiles and its estimated time in SM cycles.
+struct Plan8 {
+  bool pair = false;
+  int bn = 16, split = 1;
+  int64_t tiles = 0;
+  double cycles = 0;
+};
+
+// As in linear_tc.cu, with a k block of 128: the same bytes and MMA cycles as
+// 64 16-bit k.
+constexpr double kL2Bytes8 = 57, kTileCycles8 = 900, kSplitCycles8 = 2000, kSplitColumn8 = 20;
+
+Plan8 make_plan8(const Linear8Args& l, bool gated, int sms, bool pair, int bn, int split) {
+  Plan8 q;
+  q.pair = pair;
+  q.bn = bn;
+  q.split = split;
+  const int features = gated ? l.n / 2 : l.n, feat = (gated ? 64 : 128) * (pair ? 2 : 1);
+  const int64_t m_tiles = (features + feat - 1) / feat;
+  const double mean = static_cast<double>(l.rows) / l.groups;
+  // no group has more chunks than rows
+  const int64_t upper = (l.rows + bn - 1) / bn + (l.offsets ? l.groups : 0);
+  q.tiles = (upper < l.rows ? upper : l.rows) * m_tiles;
+  double chunks = static_cast<double>((l.rows + bn - 1) / bn), width = l.rows / chunks;
+  if (l.offsets) {  // counts spread about the mean: a group near a multiple of bn takes one chunk more half the time
+    const double used = mean < 1 ? l.rows : l.groups;  // groups with rows, about
+    chunks = used * (mean < 1 ? 1.0 : static_cast<int64_t>(mean / bn + 0.5) < 1 ? 1.0 : mean / bn + 0.5);
+    width = mean < 1 ? 1 : l.rows / chunks;
+  }
+  const int step = pair ? 32 : 16;
+  const double n = (static_cast<int64_t>(width + step - 1) / step) * step;
+  const double blocks = (l.k + kBK8 - 1) / kBK8;
+  const double mma = 2.0 * n > 128 ? 2.0 * n : 128, load = 128.0 * (128 + (pair ? n / 2 : n)) / kL2Bytes8;
+  const double per = mma > load ? mma : load;
+  const double slots = static_cast<double>(sms / ((pair ? 2 : 1) * split));
+  double waves = chunks * m_tiles / slots;
+  waves = waves < 8 ? static_cast<double>(static_cast<int64_t>(waves + 0.999)) : waves;
+  q.cycles = waves * (blocks / split * per + kTileCycles8) + (split > 1 ? kSplitCycles8 + kSplitColumn8 * n : 0);
+  return q;
+}
+
+// form: kFormAuto, or the only form to consider.
+Plan8 choose_plan8(const Linear8Args& l, bool gated, int sms, int form) {
+  static const int kWidths[] = {16, 32, 64, 96, 128, 160, 192, 224};
+  Plan8 best;
+  for (int w : kWidths) {
+    for (int pair = 0; pair < 2; ++pair) {
+      if (pair && w < 64) continue;  // a pair's CTAs hold at least 32 columns each
+      if (form == (pair ? kFormOne : kFormPair)) continue;
+      const Plan8 q = make_plan8(l, gated, sms, pair, w, 1);
+      if (form != kFormSplit && (best.cycles == 0 || q.cycles < best.cycles)) best = q;
+      if (pair || form == kFormOne) continue;
+      for (int s = 2; s <= kMaxSplit; s *= 2) {
+        if (q.tiles > (s == 2 ? sms / 2 : kMaxQuads * sms / 148)) break;
+        const Plan8 t = make_plan8(l, gated, sms, false, w, s);
+        if (best.cycles == 0 || t.cycles < best.cycles) best = t;
+      }
+    }
+    if (w >= l.rows && best.cycles > 0) break;
+  }
+  return best;
+}
+
+template <bool PAIR, bool EIGHT, typename... A>
+cudaError_t launch_form(bool gated, bool bf16, const A&... args) {
+  if (gated) return bf16 ? launch_t<true, true, PAIR, EIGHT>(args...) : launch_t<true, false, PAIR, EIGHT>(args...);
+  return bf16 ? launch_t<false, true, PAIR, EIGHT>(args...) : launch_t<false, false, PAIR, EIGHT>(args...);
+}
+
+}  // namespace
+
+cudaError_t launch_linear8_tc(const Linear8Args& l, int form, cudaStream_t st) {
+  const bool gated = act_gated(l.act);
+  const int sms = tc8_sm_count();
+  const Plan8 plan = choose_plan8(l, gated, sms, form);
+  if (plan.cycles == 0) return cudaErrorNotSupported;  // too many tiles for the K split asked for
+  Tc8Args a{};
+  a.l = l;
+  a.bn = plan.bn;
+  a.split = plan.split;
+  const int features = gated ? l.n / 2 : l.n, feat = (gated ? 64 : 128) * (plan.pair ? 2 : 1);
+  a.m_tiles = (features + feat - 1) / feat;
+  a.part = plan.pair ? a.bn / 2 : a.bn;
+  a.stage_bytes = stage_bytes8(a.part);
+  a.w_load = scale_load(l.w_scales, l.w_scales_stride, l.groups > 1 ? l.w_scales_group_stride : 0, l.k);
+  a.x_load = scale_load(l.x_scales, l.x_scales_stride, 0, l.k);
+  a.tile_limit = kWaitLimitCycles + 2048ll * ((l.k + kBK8 - 1) / kBK8);
+  a.stages = stages8(gated, a.part);
+  const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
+  const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
+  const size_t smem = smem8(gated, a.part);
+
+  // two elements a 16-bit unit of the maps
+  CUtensorMap tm{}, tn{}, half{};
+  const uint64_t w_row = l.w_stride, x_row = l.x_stride, n = features, k2 = l.k / 2, rows = l.rows;
+  const uint64_t gs = l.groups > 1 ? l.w_group_stride : w_row * l.n;
+  cudaError_t e = make_tmap_4d(&tm, l.w, {k2, n, gated ? 2u : 1u, uint64_t(l.groups)}, {w_row, n * w_row, gs},
+                               {64, gated ? 64u : 128u, gated ? 2u : 1u, 1});
+  if (e == cudaSuccess) e = make_tmap_4d(&tn, l.x, {k2, rows, 1, 1}, {x_row, x_row, x_row}, {64, uint32_t(a.part), 1, 1});
+  half = tn;
+  if (e == cudaSuccess && a.part >= 32)
+    e = make_tmap_4d(&half, l.x, {k2, rows, 1, 1}, {x_row, x_row, x_row}, {64, uint32_t(a.part / 2), 1, 1});
+  if (e != cudaSuccess) return e;
+  if (plan.pair)
+    return l.codes ? launch_form<true, true>(gated, l.bf16, tm, tn, half, a, grid, smem, st)
+                   : launch_form<true, false>(gated, l.bf16, tm, tn, half, a, grid, smem, st);
+  return l.codes ? launch_form<false, true>(gated, l.bf16, tm, tn, half, a, grid, smem, st)
+                 : launch_form<false, false>(gated, l.bf16, tm, tn, half, a, grid, smem, st);
+}
+
+cudaError_t linear8_device_error(cudaStream_t st, int* error) {
+  static std::mutex once;  // g_linear8_taken is one word a device
+  const std::lock_guard<std::mutex> hold(once);
+  *error = 0;
+  cudaError_t e = cudaLaunchKernel(reinterpret_cast<const void*>(take_error8_kernel), dim3(1), dim3(1), nullptr, 0, st);
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(error, g_linear8_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  const cudaError_t done = cudaStreamSynchronize(st);
+  return e != cudaSuccess ? e : done;
+}
+
+}  // namespace senmoe

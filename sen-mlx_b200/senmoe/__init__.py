@@ -13,6 +13,10 @@ Mirrors the reference's MoE interfaces (paths inside the sen-mlx project):
 * ``linear`` / ``grouped_linear`` and their ``_backward`` -- linear products over
   16-bit weights with the activation and residual in the product's launch,
   dense or grouped by expert (products.py).
+* ``rms_norm`` and its ``_backward`` -- the norm before the block, with the
+  residual's addition and an output in 8 bits (norm.py); ``quantize8``,
+  ``linear8`` / ``grouped_linear8`` and their ``_input_grad`` -- the linear
+  products over 8-bit rows with scales (products8.py).
 * Failures raise ``SenMoeError`` carrying the C status and message, as the
   reference's shim turns a non-zero status into ``Exception::custom``
   (utils/moe.rs:66-74).
@@ -110,6 +114,39 @@ class SenMoeLinearGrad(C.Structure):
                 ("dbias", _P), ("workspace", _P), ("workspace_bytes", C.c_int64)]
 
 
+class SenMoeNorm(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("weight_fp32", C.c_int32), ("unit_offset", C.c_int32), ("eps", C.c_float),
+                ("rows", C.c_int64), ("hidden", C.c_int64), ("x", _P), ("x_stride", C.c_int64),
+                ("residual", _P), ("residual_stride", C.c_int64), ("weight", _P), ("h", _P), ("h_stride", C.c_int64),
+                ("y", _P), ("y_stride", C.c_int64), ("codes", _P), ("codes_stride", C.c_int64),
+                ("scales", _P), ("scales_stride", C.c_int64)]
+
+
+class SenMoeNormGrad(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("weight_fp32", C.c_int32), ("unit_offset", C.c_int32), ("eps", C.c_float),
+                ("rows", C.c_int64), ("hidden", C.c_int64), ("dy", _P), ("dy_stride", C.c_int64),
+                ("h", _P), ("h_stride", C.c_int64), ("weight", _P), ("dh", _P), ("dh_stride", C.c_int64),
+                ("dx", _P), ("dx_stride", C.c_int64), ("dweight", _P), ("workspace", _P),
+                ("workspace_bytes", C.c_int64)]
+
+
+class SenMoeQuantize8(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("epilogue", C.c_int32), ("rows", C.c_int64), ("n", C.c_int64),
+                ("x", _P), ("x_stride", C.c_int64), ("preact", _P), ("preact_stride", C.c_int64),
+                ("codes", _P), ("codes_stride", C.c_int64), ("scales", _P), ("scales_stride", C.c_int64)]
+
+
+class SenMoeLinear8(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("epilogue", C.c_int32), ("num_groups", C.c_int32), ("path", C.c_int32),
+                ("rows", C.c_int64), ("in_features", C.c_int64), ("out_features", C.c_int64),
+                ("x", _P), ("x_stride", C.c_int64), ("x_scales", _P), ("x_scales_stride", C.c_int64),
+                ("weight", _P), ("weight_stride", C.c_int64), ("weight_group_stride", C.c_int64),
+                ("weight_scales", _P), ("weight_scales_stride", C.c_int64), ("weight_scales_group_stride", C.c_int64),
+                ("offsets", _P), ("bias", _P), ("residual", _P), ("residual_stride", C.c_int64),
+                ("y", _P), ("y_stride", C.c_int64), ("y_codes", _P), ("y_codes_stride", C.c_int64),
+                ("y_scales", _P), ("y_scales_stride", C.c_int64), ("preact", _P), ("preact_stride", C.c_int64)]
+
+
 # Every symbol include/senmoe.h declares, with its ctypes signature.
 _i64, _i32, _f32 = C.c_int64, C.c_int32, C.c_float
 SIGNATURES = {
@@ -140,6 +177,11 @@ SIGNATURES = {
     "senmoe_linear_backward": (C.c_int, [_P, _P]),
     "senmoe_linear_check": (C.c_int, [_P]),
     "senmoe_selftest_linear_wait": (C.c_int, [_P]),
+    "senmoe_rms_norm": (C.c_int, [_P, _P]),
+    "senmoe_rms_norm_backward_workspace": (_i64, [_P]),
+    "senmoe_rms_norm_backward": (C.c_int, [_P, _P]),
+    "senmoe_quantize8": (C.c_int, [_P, _P]),
+    "senmoe_linear8": (C.c_int, [_P, _P]),
 }
 
 _lib = None
@@ -607,3 +649,6 @@ class MoeStack:
 from .products import (LINEAR_ANY, LINEAR_AUTO, LINEAR_SMALL, LINEAR_TCGEN05, LINEAR_TCGEN05_ONE,  # noqa: E402
                        LINEAR_TCGEN05_PAIR, LINEAR_TCGEN05_SPLIT, grouped_linear, grouped_linear_backward, linear,
                        linear_backward, linear_check)
+from .products8 import (Rows8, grouped_linear8, grouped_linear8_input_grad, linear8, linear8_input_grad,  # noqa: E402
+                        quantize8)
+from .norm import Normed, rms_norm, rms_norm_backward  # noqa: E402
