@@ -94,12 +94,6 @@ template <bool PAIR> __device__ __forceinline__ void copy_scales(uint32_t taddr,
   if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
   else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-// (release at cluster scope: what the lanes wrote to their own shared memory
-// is read by MMAs that the other CTA issues)
-__device__ __forceinline__ void arrive_release_at(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
 // ------------------------------------------------------------------ tiles
 struct Tile8 {
   int e;         // group
@@ -425,7 +419,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) arrive_release_at(PAIR ? map_rank(smem_u32(&bar_full[st]), 0) : smem_u32(&bar_full[st]));
+          // (to the other CTA too with the plain arrive: what it guards is this
+          // SM's shared memory, which the proxy fence has ordered; with
+          // .release.cluster a stage took 1600 cycles)
+          if (lane == 0) arrive_at(PAIR ? map_rank(smem_u32(&bar_full[st]), 0) : smem_u32(&bar_full[st]));
           next(st, ph);
         }
 #pragma unroll
