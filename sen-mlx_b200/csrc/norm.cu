@@ -12,10 +12,13 @@
 // taken of the rounded h, which is what the layers after it and the backward
 // pass have.
 //
-// Bound by HBM: a row is read once into registers, 16 bytes a lane and load,
-// and everything is written from there.  A row takes 1 to 16 warps: enough
-// that a lane holds at most four pieces, and with few rows as many as shorten
-// the one trip to memory and back that such a call is.
+// Bound by HBM.  A row takes 1 to 16 warps: enough that a lane holds at most
+// four pieces of 16 bytes (backward, with its sums for dweight, two), and with
+// few rows as many as shorten the one trip to memory and back that such a call
+// is.  Rows are read once, each lane its own pieces with cp.async into its own
+// places of shared memory, from where it takes them into registers: no barrier
+// but the one of the row's sum, and with many rows a row's warps have the next
+// rows' loads in flight, more bytes than registers would hold.
 
 #include <cuda_runtime.h>
 
@@ -28,9 +31,16 @@ namespace senmoe {
 namespace {
 
 constexpr int kNormThreads = 256;
-constexpr int kNormIter = 4;           // most pieces of 8 elements a lane holds
-constexpr int kNormWarps = 16;         // most warps of a row
+constexpr int kNormIter = 4;    // most pieces of 8 elements a lane holds
+constexpr int kGradIter = 2;    // wanted at most in the backward pass: 8 sums for dweight a piece
+constexpr int kNormWarps = 16;  // most warps of a row
 constexpr int kNormWide = kNormIter * kNormWarps * 32 * 8;  // longest row held in registers
+// With many rows: rows of a row's warps in shared memory, and blocks of 256
+// threads an SM.  32767 rows of 2816 fp16 (369 MB) forward 64.7 us with 2 rows,
+// 66.2 with 3, 70.9 with 4; 80.7 us with 2 blocks, 79.2 with 3, 67.8 with 6.
+// 32768 rows of 2048 backward (537 MB) 90 us with 2 rows, 104 with 3, 108 with
+// 4; 158 us with 1 block, 110 with 3; 104 with 4 pieces a lane, 116 with 1.
+constexpr int kDepth = 2, kNormBlocks = 4, kGradBlocks = 2;
 
 struct NormArgs {
   const void *x, *residual, *weight;
@@ -56,12 +66,12 @@ struct NormGradArgs {
   float eps, offset;
 };
 
-// Read once: past L1.
-__device__ __forceinline__ uint4 load_once(const uint16_t* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+// 16 bytes global -> shared, past L1.
+__device__ __forceinline__ void cp_async_16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // g of 8 consecutive columns
 template <bool BF16> __device__ __forceinline__ void gain8(const void* weight, int fp32, float offset, int c, float (&g)[8]) {
   if (fp32) {
@@ -102,63 +112,94 @@ template <int WARPS, int N> __device__ __forceinline__ void row_sums(float (&v)[
 
 template <int WARPS> constexpr int norm_threads() { return WARPS * 32 > kNormThreads ? WARPS * 32 : kNormThreads; }
 
-template <bool BF16, int WARPS, int ITER>
-__global__ void __launch_bounds__(norm_threads<WARPS>()) norm_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int kLanes = WARPS * 32, kRows = norm_threads<WARPS>() / kLanes;
-  __shared__ float s_sum[kRows][WARPS][1];
+// Rows on their way: DEPTH slots of a row's STREAMS operands in shared memory,
+// a lane's pieces in its own places.
+template <int WARPS, int ITER, int DEPTH> struct RowRing {
+  static constexpr int kThreads = norm_threads<WARPS>(), kLanes = WARPS * 32, kRows = kThreads / kLanes;
+  uint4* mine;  // [DEPTH][streams][ITER][threads]
+  int streams;
+  __device__ __forceinline__ RowRing(unsigned char* smem, int n) : mine(reinterpret_cast<uint4*>(smem) + threadIdx.x), streams(n) {}
+  __device__ __forceinline__ uint4* at(int slot, int stream, int i) const {
+    return mine + ((slot * streams + stream) * ITER + i) * kThreads;
+  }
+  // row: one operand's row, or past the last one null
+  __device__ __forceinline__ void fetch(int slot, int stream, const uint16_t* row, int hidden) const {
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (threadIdx.x % kLanes + i * kLanes) * 8;
+      if (row && c < hidden) cp_async_16(at(slot, stream, i), row + c);
+    }
+  }
+};
+constexpr size_t ring_bytes(int threads, int iter, int depth, int streams) { return size_t(threads) * iter * depth * streams * 16; }
+
+template <bool BF16, int WARPS, int ITER, int DEPTH>
+__global__ void __launch_bounds__(norm_threads<WARPS>(), 1024 / norm_threads<WARPS>())
+    norm_kernel(const __grid_constant__ NormArgs a) {
+  using Ring = RowRing<WARPS, ITER, DEPTH>;
+  constexpr int kLanes = Ring::kLanes, kRows = Ring::kRows;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ float s_sum[2][kRows][WARPS][1];
   const int sub = threadIdx.x / kLanes, t = threadIdx.x % kLanes;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub;
+  const Ring ring(smem_raw, a.residual ? 2 : 1);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub;
   pdl_wait();
   pdl_launch_dependents();
-  if (row >= a.rows) return;  // a row's warps together
-  const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.x_stride;
-  const uint16_t* res = static_cast<const uint16_t*>(a.residual) + row * a.residual_stride;
-  uint4 v[ITER], r[ITER];
-#pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    const int c = (t + i * kLanes) * 8;
-    v[i] = r[i] = make_uint4(0, 0, 0, 0);
-    if (c < a.hidden) {
-      v[i] = load_once(x + c);
-      if (a.residual) r[i] = load_once(res + c);
+  const auto fetch = [&](int64_t r, int slot) {
+    if (r < a.rows) {
+      ring.fetch(slot, 0, static_cast<const uint16_t*>(a.x) + r * a.x_stride, a.hidden);
+      if (a.residual) ring.fetch(slot, 1, static_cast<const uint16_t*>(a.residual) + r * a.residual_stride, a.hidden);
     }
-  }
-  float sum[1] = {0.0f};
+    cp_async_commit();
+  };
 #pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    float f[8];
-    if (a.residual) {
-      float g[8];
-      unpack8<BF16>(v[i], f);
-      unpack8<BF16>(r[i], g);
+  for (int d = 0; d < DEPTH - 1; ++d) fetch(row + d * step, d);
+  int slot = 0, turn = 0;
+  for (; row < a.rows; row += step, turn ^= 1) {  // a row's warps together
+    const int last = slot ? slot - 1 : DEPTH - 1;  // the slot of the row before, which its lanes have read
+    fetch(row + (DEPTH - 1) * step, last);
+    cp_async_wait<DEPTH - 1>();
+    uint4 v[ITER];
+    float sum[1] = {0.0f};
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] += g[k];
-      v[i] = pack8<BF16>(f);
+    for (int i = 0; i < ITER; ++i) {
       const int c = (t + i * kLanes) * 8;
-      if (a.h && c < a.hidden) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + row * a.h_stride + c) = v[i];
+      v[i] = c < a.hidden ? *ring.at(slot, 0, i) : make_uint4(0, 0, 0, 0);
+      float f[8];
+      unpack8<BF16>(v[i], f);
+      if (a.residual) {
+        float g[8];
+        unpack8<BF16>(c < a.hidden ? *ring.at(slot, 1, i) : make_uint4(0, 0, 0, 0), g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] += g[k];
+        v[i] = pack8<BF16>(f);
+        if (a.h && c < a.hidden) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + row * a.h_stride + c) = v[i];
+        unpack8<BF16>(v[i], f);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[0] += f[k] * f[k];
     }
-    unpack8<BF16>(v[i], f);
+    slot = slot + 1 == DEPTH ? 0 : slot + 1;
+    row_sums<WARPS>(sum, s_sum[turn][sub], sub, t >> 5);
+    const float rstd = rsqrtf(sum[0] / a.hidden + a.eps);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum[0] += f[k] * f[k];
-  }
-  row_sums<WARPS>(sum, s_sum[sub], sub, t >> 5);
-  const float rstd = rsqrtf(sum[0] / a.hidden + a.eps);
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (t + i * kLanes) * 8;
+      const bool in = c < a.hidden;
+      float f[8], g[8];
+      unpack8<BF16>(v[i], f);
+      if (in) gain8<BF16>(a.weight, a.weight_fp32, a.offset, c, g);
 #pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    const int c = (t + i * kLanes) * 8;
-    const bool in = c < a.hidden;
-    float f[8], g[8];
-    unpack8<BF16>(v[i], f);
-    if (in) gain8<BF16>(a.weight, a.weight_fp32, a.offset, c, g);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = in ? f[k] * rstd * g[k] : 0.0f;
-    if (a.y && in) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + row * a.y_stride + c) = pack8<BF16>(f);
-    if (a.codes) {
-      uint32_t byte;
-      const uint2 q = pack8_lane(f, byte);
-      if (in) {
-        *reinterpret_cast<uint2*>(a.codes + row * a.codes_stride + c) = q;
-        if ((t & 3) == 0) a.scales[row * a.scales_stride + c / kBlock8] = static_cast<uint8_t>(byte);
+      for (int k = 0; k < 8; ++k) f[k] = in ? f[k] * rstd * g[k] : 0.0f;
+      if (a.y && in) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + row * a.y_stride + c) = pack8<BF16>(f);
+      if (a.codes) {
+        uint32_t byte;
+        const uint2 q = pack8_lane(f, byte);
+        if (in) {
+          *reinterpret_cast<uint2*>(a.codes + row * a.codes_stride + c) = q;
+          if ((t & 3) == 0) a.scales[row * a.scales_stride + c / kBlock8] = static_cast<uint8_t>(byte);
+        }
       }
     }
   }
@@ -199,46 +240,49 @@ template <bool BF16> __global__ void __launch_bounds__(kNormThreads) norm_any_ke
   }
 }
 
-// Gradients.  Each row's warps of a block take rows in turn, the next row's
-// loads in flight under the sums of this one, and keep their columns' part of
-// dweight in registers; the block's parts meet in shared memory at the end
-// and go to its line of `partial`, which join_kernel adds in block order.
-template <bool BF16, int WARPS, int ITER>
-__global__ void __launch_bounds__(norm_threads<WARPS>()) norm_grad_kernel(const __grid_constant__ NormGradArgs a) {
-  constexpr int kLanes = WARPS * 32, kRows = norm_threads<WARPS>() / kLanes;
+// Gradients.  Each row's warps of a block take rows in turn and keep their
+// columns' part of dweight in registers; the block's parts meet in shared
+// memory at the end and go to its line of `partial`, which norm_join_kernel
+// adds in block order.
+template <bool BF16, int WARPS, int ITER, int DEPTH>
+__global__ void __launch_bounds__(norm_threads<WARPS>(), 512 / norm_threads<WARPS>())
+    norm_grad_kernel(const __grid_constant__ NormGradArgs a) {
+  using Ring = RowRing<WARPS, ITER, DEPTH>;
+  constexpr int kLanes = Ring::kLanes, kRows = Ring::kRows;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ float s_sum[2][kRows][WARPS][2];
   __shared__ __align__(16) float s_part[kRows > 1 ? kLanes * 8 : 1];
   const int sub = threadIdx.x / kLanes, t = threadIdx.x % kLanes;
-  pdl_wait();
-  pdl_launch_dependents();
+  const Ring ring(smem_raw, a.dh ? 3 : 2);
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub;
-  uint4 y[ITER], h[ITER], d[ITER];
-  const auto load = [&](int64_t at) {
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      const int c = (t + i * kLanes) * 8;
-      y[i] = h[i] = d[i] = make_uint4(0, 0, 0, 0);
-      if (c < a.hidden && at < a.rows) {
-        y[i] = load_once(static_cast<const uint16_t*>(a.dy) + at * a.dy_stride + c);
-        h[i] = load_once(static_cast<const uint16_t*>(a.h) + at * a.h_stride + c);
-        if (a.dh) d[i] = load_once(static_cast<const uint16_t*>(a.dh) + at * a.dh_stride + c);
-      }
+  pdl_wait();
+  pdl_launch_dependents();
+  const auto fetch = [&](int64_t r, int slot) {
+    if (r < a.rows) {
+      ring.fetch(slot, 0, static_cast<const uint16_t*>(a.dy) + r * a.dy_stride, a.hidden);
+      ring.fetch(slot, 1, static_cast<const uint16_t*>(a.h) + r * a.h_stride, a.hidden);
+      if (a.dh) ring.fetch(slot, 2, static_cast<const uint16_t*>(a.dh) + r * a.dh_stride, a.hidden);
     }
+    cp_async_commit();
   };
-  load(row);
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) fetch(row + d * step, d);
   float acc[ITER][8] = {};
-  int turn = 0;
+  int slot = 0, turn = 0;
   for (; row < a.rows; row += step, turn ^= 1) {
+    const int last = slot ? slot - 1 : DEPTH - 1;  // the slot of the row before, which its lanes have read
+    fetch(row + (DEPTH - 1) * step, last);
+    cp_async_wait<DEPTH - 1>();
     float sum[2] = {0.0f, 0.0f};
-    uint4 y0[ITER], h0[ITER], d0[ITER];
+    uint4 y[ITER], h[ITER], d[ITER];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (t + i * kLanes) * 8;
-      y0[i] = y[i];
-      h0[i] = h[i];
-      d0[i] = d[i];
       if (c < a.hidden) {
+        y[i] = *ring.at(slot, 0, i);
+        h[i] = *ring.at(slot, 1, i);
+        d[i] = a.dh ? *ring.at(slot, 2, i) : make_uint4(0, 0, 0, 0);
         float fy[8], fh[8], g[8];
         unpack8<BF16>(y[i], fy);
         unpack8<BF16>(h[i], fh);
@@ -250,7 +294,7 @@ __global__ void __launch_bounds__(norm_threads<WARPS>()) norm_grad_kernel(const 
         }
       }
     }
-    load(row + step);
+    slot = slot + 1 == DEPTH ? 0 : slot + 1;
     row_sums<WARPS>(sum, s_sum[turn][sub], sub, t >> 5);
     const float r = rsqrtf(sum[0] / a.hidden + a.eps), m = r * r * (sum[1] / a.hidden);
 #pragma unroll
@@ -258,9 +302,9 @@ __global__ void __launch_bounds__(norm_threads<WARPS>()) norm_grad_kernel(const 
       const int c = (t + i * kLanes) * 8;
       if (c < a.hidden) {
         float fy[8], fh[8], fd[8], g[8];
-        unpack8<BF16>(y0[i], fy);
-        unpack8<BF16>(h0[i], fh);
-        unpack8<BF16>(d0[i], fd);
+        unpack8<BF16>(y[i], fy);
+        unpack8<BF16>(h[i], fh);
+        unpack8<BF16>(d[i], fd);
         gain8<BF16>(a.weight, a.weight_fp32, a.offset, c, g);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -335,42 +379,44 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_any_kernel(const __gri
   }
 }
 
-// dweight = the sum of the blocks' lines: 32 columns a block, its 8 warps
-// every eighth line, then the warps in order.
-template <bool BF16> __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const __grid_constant__ NormGradArgs a) {
-  __shared__ float s_sum[kNormThreads / 32][32];
+// dweight = the sum of the blocks' lines: 32 columns a block, its warps every
+// 32nd line, all their loads in flight together, then the warps in order.
+constexpr int kJoinWarps = 32;
+template <bool BF16> __global__ void __launch_bounds__(kJoinWarps * 32) norm_join_kernel(const __grid_constant__ NormGradArgs a) {
+  __shared__ float s_sum[kJoinWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   pdl_wait();
   pdl_launch_dependents();
   float v = 0.0f;
   if (c < a.hidden) {
     const float* p = a.partial + c;
-    constexpr int kStep = kNormThreads / 32;
-    for (int b = warp; b < a.blocks; b += 8 * kStep) {  // eight loads in flight
-      float t[8];
+    for (int b = warp; b < a.blocks; b += 16 * kJoinWarps) {
+      float t[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = b + i * kStep < a.blocks ? p[static_cast<int64_t>(b + i * kStep) * a.hidden] : 0.0f;
+      for (int i = 0; i < 16; ++i)
+        t[i] = b + i * kJoinWarps < a.blocks ? p[static_cast<int64_t>(b + i * kJoinWarps) * a.hidden] : 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v += t[i];
+      for (int i = 0; i < 16; ++i) v += t[i];
     }
   }
   s_sum[warp][lane] = v;
   __syncthreads();
-  if (warp == 0 && c < a.hidden) {
-    v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kNormThreads / 32; ++w) v += s_sum[w][lane];
-    if (a.weight_fp32) static_cast<float*>(a.dweight)[c] = v;
-    else static_cast<uint16_t*>(a.dweight)[c] = from_f32<BF16>(v);
+  v = warp_sum(s_sum[lane][warp]);  // a warp a column, the lines' 32 sums in its lanes
+  const int col = blockIdx.x * 32 + warp;
+  if (lane == 0 && col < a.hidden) {
+    if (a.weight_fp32) static_cast<float*>(a.dweight)[col] = v;
+    else static_cast<uint16_t*>(a.dweight)[col] = from_f32<BF16>(v);
   }
 }
 
 // ------------------------------------------------------------- host side
 int norm_sm_count() {
+  static int counts[64] = {};  // by device; the same value whoever writes it
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-    n = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && counts[dev] > 0) return counts[dev];
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+  if (dev < 64) counts[dev] = n;
   return n;
 }
 
@@ -382,40 +428,56 @@ bool aligned16(const void* p, int64_t stride, int size = 2) {
 struct NormPlan {
   int warps = 0, iter = 0;
 };
-// few: rows below which more warps take a row
-NormPlan norm_plan(int64_t rows, int hidden, bool aligned, int64_t few) {
+// iter: pieces of a lane that are wanted at most; few: warps below which more take a row
+NormPlan norm_plan(int64_t rows, int hidden, bool aligned, int iter, int64_t few) {
   NormPlan p;
   if (!aligned || hidden % 8 || hidden > kNormWide) return p;
   const int pieces = hidden / 8;
   p.warps = 1;
-  while (p.warps * 32 * kNormIter < pieces) p.warps *= 2;
+  while (p.warps < kNormWarps && p.warps * 32 * iter < pieces) p.warps *= 2;
   while (p.warps < kNormWarps && p.warps * 32 < pieces && rows * p.warps < few) p.warps *= 2;
   p.iter = (pieces + p.warps * 32 - 1) / (p.warps * 32);
   return p;
 }
 
-#define SENMOE_NORM_ITER(KERNEL, B, W)                                                                       \
-  (p.iter == 1 ? KERNEL<B, W, 1> : p.iter == 2 ? KERNEL<B, W, 2> : p.iter == 3 ? KERNEL<B, W, 3> : KERNEL<B, W, 4>)
-#define SENMOE_NORM_PICK(KERNEL, B)                                                                    \
-  (p.warps == 1 ? SENMOE_NORM_ITER(KERNEL, B, 1) : p.warps == 2 ? SENMOE_NORM_ITER(KERNEL, B, 2)       \
-   : p.warps == 4 ? SENMOE_NORM_ITER(KERNEL, B, 4) : p.warps == 8 ? SENMOE_NORM_ITER(KERNEL, B, 8)     \
-                                                   : SENMOE_NORM_ITER(KERNEL, B, 16))
+#define SENMOE_NORM_ITER(KERNEL, B, W, D) \
+  (p.iter == 1 ? KERNEL<B, W, 1, D> : p.iter == 2 ? KERNEL<B, W, 2, D> : p.iter == 3 ? KERNEL<B, W, 3, D> : KERNEL<B, W, 4, D>)
+#define SENMOE_NORM_PICK(KERNEL, B, D)                                                                 \
+  (p.warps == 1 ? SENMOE_NORM_ITER(KERNEL, B, 1, D) : p.warps == 2 ? SENMOE_NORM_ITER(KERNEL, B, 2, D) \
+   : p.warps == 4 ? SENMOE_NORM_ITER(KERNEL, B, 4, D) : p.warps == 8 ? SENMOE_NORM_ITER(KERNEL, B, 8, D) \
+                                                      : SENMOE_NORM_ITER(KERNEL, B, 16, D))
 
 int plan_threads(const NormPlan& p) { return p.warps * 32 > kNormThreads ? p.warps * 32 : kNormThreads; }
 int plan_rows(const NormPlan& p) { return p.warps ? plan_threads(p) / (p.warps * 32) : 1; }
+
+template <typename A>
+cudaError_t launch_rows(void (*kern)(A), const NormPlan& p, int depth, int streams, int64_t grid, const A& a, cudaStream_t st) {
+  const size_t smem = ring_bytes(plan_threads(p), p.iter, depth, streams);
+  const cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(plan_threads(p)), smem, st, a);
+}
 
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
   const bool aligned = aligned16(a.x, a.x_stride) && (!a.residual || aligned16(a.residual, a.residual_stride)) &&
                        (!a.h || aligned16(a.h, a.h_stride)) && (!a.y || aligned16(a.y, a.y_stride)) &&
                        aligned16(a.weight, 0) && (!a.codes || aligned16(a.codes, a.codes_stride, 1));
-  const NormPlan p = norm_plan(a.rows, a.hidden, aligned, 148 * 8);
+  const int64_t sms = norm_sm_count();
+  const NormPlan p = norm_plan(a.rows, a.hidden, aligned, kNormIter, sms * 8);
   if (!p.warps) {
-    const unsigned grid = static_cast<unsigned>(a.rows < 148 * 8 ? a.rows : 148 * 8);
-    return launch_pdl(a.bf16 ? norm_any_kernel<true> : norm_any_kernel<false>, dim3(grid), dim3(kNormThreads), 0, st, a);
+    const int64_t grid = a.rows < sms * 8 ? a.rows : sms * 8;
+    return launch_pdl(a.bf16 ? norm_any_kernel<true> : norm_any_kernel<false>, dim3(static_cast<unsigned>(grid)),
+                      dim3(kNormThreads), 0, st, a);
   }
-  const int per = plan_rows(p);
-  return launch_pdl(a.bf16 ? SENMOE_NORM_PICK(norm_kernel, true) : SENMOE_NORM_PICK(norm_kernel, false),
-                    dim3(static_cast<unsigned>((a.rows + per - 1) / per)), dim3(plan_threads(p)), 0, st, a);
+  const int64_t blocks = (a.rows + plan_rows(p) - 1) / plan_rows(p), streams = a.residual ? 2 : 1;
+  // many rows: the blocks that are resident together
+  const int64_t fit = 200 * 1024 / static_cast<int64_t>(ring_bytes(plan_threads(p), p.iter, kDepth, streams));
+  const int64_t most = kNormBlocks * kNormThreads / plan_threads(p), resident = sms * (fit < most ? fit : most);
+  if (blocks > 4 * resident)
+    return launch_rows(a.bf16 ? SENMOE_NORM_PICK(norm_kernel, true, kDepth) : SENMOE_NORM_PICK(norm_kernel, false, kDepth), p,
+                       kDepth, streams, resident, a, st);
+  return launch_rows(a.bf16 ? SENMOE_NORM_PICK(norm_kernel, true, 1) : SENMOE_NORM_PICK(norm_kernel, false, 1), p, 1,
+                     streams, blocks, a, st);
 }
 
 bool grad_aligned(const NormGradArgs& a) {
@@ -424,9 +486,9 @@ bool grad_aligned(const NormGradArgs& a) {
 }
 // Blocks of a backward pass: as many as are resident together, at most one a
 // row group; by the sizes alone, so that the same call adds in the same order.
-constexpr int kGradBlocksPerSm = 2;
 int grad_blocks(const NormPlan& p, int64_t rows, int sms) {
-  const int64_t groups = (rows + plan_rows(p) - 1) / plan_rows(p), most = static_cast<int64_t>(sms) * kGradBlocksPerSm;
+  const int64_t groups = (rows + plan_rows(p) - 1) / plan_rows(p);
+  const int64_t most = static_cast<int64_t>(sms) * kGradBlocks * kNormThreads / (p.warps ? plan_threads(p) : kNormThreads);
   return static_cast<int>(groups < most ? groups : most);
 }
 
@@ -437,13 +499,13 @@ cudaError_t launch_norm_grad(NormGradArgs a, const NormPlan& p, cudaStream_t st)
       e = launch_pdl(a.bf16 ? norm_grad_any_kernel<true> : norm_grad_any_kernel<false>, dim3(a.blocks),
                      dim3(kNormThreads), 0, st, a);
     else
-      e = launch_pdl(a.bf16 ? SENMOE_NORM_PICK(norm_grad_kernel, true) : SENMOE_NORM_PICK(norm_grad_kernel, false),
-                     dim3(a.blocks), dim3(plan_threads(p)), 0, st, a);
+      e = launch_rows(a.bf16 ? SENMOE_NORM_PICK(norm_grad_kernel, true, kDepth) : SENMOE_NORM_PICK(norm_grad_kernel, false, kDepth), p,
+                      kDepth, a.dh ? 3 : 2, a.blocks, a, st);
     if (e != cudaSuccess || !a.dweight) return e;
   }
   if (!a.dweight) return cudaSuccess;
   return launch_pdl(a.bf16 ? norm_join_kernel<true> : norm_join_kernel<false>, dim3((a.hidden + 31) / 32),
-                    dim3(kNormThreads), 0, st, a);
+                    dim3(kJoinWarps * 32), 0, st, a);
 }
 
 constexpr int64_t kMaxNormRows = (int64_t(1) << 31) - 1024;
@@ -496,7 +558,7 @@ int plan_grad(const char* call, const SenMoeNormGrad* g, NormGradArgs* a, NormPl
   a->eps = g->eps;
   a->offset = g->unit_offset ? 1.0f : 0.0f;
   const int sms = norm_sm_count();
-  *p = norm_plan(g->rows, a->hidden, grad_aligned(*a), sms * 8);
+  *p = norm_plan(g->rows, a->hidden, grad_aligned(*a), kGradIter, sms * 8);
   a->blocks = grad_blocks(*p, g->rows, sms);
   return SENMOE_OK;
 }

@@ -16,7 +16,7 @@ import torch
 
 from . import SenMoeNorm, SenMoeNormGrad, _check, lib
 from .products import _CODES, _DTYPES, _bad, _current_stream, _rows
-from .products8 import _E4M3, _E8M0, Rows8, _blocks, _device_of, _on16
+from .products8 import Rows8, _blocks, _device_of, _empty8, _like, _on16
 
 _FIELD = {**_CODES, C.c_float: "f"}
 _pack_norm = struct.Struct("".join(_FIELD[t] for _, t in SenMoeNorm._fields_)).pack
@@ -31,22 +31,25 @@ class Normed(NamedTuple):
     h: torch.Tensor
 
 
+_F32 = torch.float32
+_c_norm = None  # the library's entry, once it is loaded
+
+
 def _operands(first: torch.Tensor, name: str, weight: torch.Tensor):
-    """(dtype code, device, rows' shape, whether weight is fp32)"""
-    code = _DTYPES.get(first.dtype)
+    """(dtype code, device, whether weight is fp32, row length)"""
+    dtype, shape = first.dtype, first.shape
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise TypeError(f"{name} must be bfloat16 or float16, got {first.dtype}")
+        raise TypeError(f"{name} must be bfloat16 or float16, got {dtype}")
     device = _device_of(first)
-    if not first.dim() or first.shape[-1] < 1:
-        raise _bad(f"{name} {tuple(first.shape)}")
-    fp32 = weight.dtype is torch.float32
-    if not fp32:
-        _on16(weight, device, first.dtype, "weight (or float32)")
-    elif weight.get_device() != device:
-        raise TypeError(f"weight on {weight.device}, {name} on {first.device}")
-    if weight.shape != first.shape[-1:]:
-        raise _bad(f"weight {tuple(weight.shape)} for {name} {tuple(first.shape)}")
-    return code, device, int(fp32)
+    if not shape or shape[-1] < 1:
+        raise _bad(f"{name} {tuple(shape)}")
+    fp32 = weight.dtype is _F32
+    if not fp32 and weight.dtype is not dtype or weight.get_device() != device:
+        raise TypeError(f"weight must be {dtype} or float32 on cuda:{device}, got {weight.dtype} on {weight.device}")
+    if weight.shape != shape[-1:]:
+        raise _bad(f"weight {tuple(weight.shape)} for {name} {tuple(shape)}")
+    return code, device, int(fp32), shape[-1]
 
 
 def _same_rows(t: torch.Tensor, first: torch.Tensor, device: int, name: str):
@@ -68,28 +71,30 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     if stream is not None:
         with torch.cuda.stream(stream):
             return rms_norm(x, weight, eps, residual, unit_offset, sixteen_bit, eight_bit)
-    code, device, fp32 = _operands(x, "x", weight)
+    code, device, fp32, n = _operands(x, "x", weight)
     if not sixteen_bit and not eight_bit:
         raise _bad("rms_norm: neither sixteen_bit nor eight_bit")
-    shape, n = x.shape, x.shape[-1]
     nb = _blocks(n, "8-bit output: row length") if eight_bit else 0
     h, xs = (x, n) if x.is_contiguous() else _rows(x, n)
     ph = pr = rs = py = pc = ps = 0
     px, out_h = h.data_ptr(), x
     if residual is not None:
         residual, rs = _same_rows(residual, x, device, "residual")
-        out_h = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out_h = _like(x)
         pr, ph = residual.data_ptr(), out_h.data_ptr()
-    weight = weight.contiguous()
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
     y = y8 = None
     if sixteen_bit:
-        y = torch.empty(shape, dtype=x.dtype, device=x.device)
+        y = _like(x)
         py = y.data_ptr()
     if eight_bit:
-        y8 = Rows8(torch.empty(shape, dtype=_E4M3, device=x.device),
-                   torch.empty((*shape[:-1], nb), dtype=_E8M0, device=x.device))
-        pc, ps = y8.codes.data_ptr(), y8.scales.data_ptr()
-    status = lib().senmoe_rms_norm(
+        y8 = _empty8(x, x.shape[:-1], n)
+        pc, ps = y8[0].data_ptr(), y8[1].data_ptr()
+    global _c_norm
+    if _c_norm is None:
+        _c_norm = lib().senmoe_rms_norm
+    status = _c_norm(
         _pack_norm(code, fp32, int(unit_offset), eps, x.numel() // n, n, px, xs, pr, rs, weight.data_ptr(), ph, n,
                    py, n, pc, n, ps, nb), _current_stream(device))
     if status:
@@ -106,9 +111,8 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, e
     if stream is not None:
         with torch.cuda.stream(stream):
             return rms_norm_backward(dy, h, weight, eps, dh, unit_offset, need_dx, need_dweight)
-    code, device, fp32 = _operands(h, "h", weight)
-    n = h.shape[-1]
-    shape, rows = h.shape, h.numel() // n
+    code, device, fp32, n = _operands(h, "h", weight)
+    rows = h.numel() // n
     dy, ys = _same_rows(dy, h, device, "dy")
     pd = ds = 0
     if dh is not None:
@@ -116,7 +120,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, e
         pd = dh.data_ptr()
     h, hs = (h, n) if h.is_contiguous() else _rows(h, n)
     weight = weight.contiguous()
-    dx = torch.empty(shape, dtype=h.dtype, device=h.device) if need_dx else None
+    dx = _like(h) if need_dx else None
     dw = torch.empty_like(weight) if need_dweight else None
     args = (code, fp32, int(unit_offset), eps, rows, n, dy.data_ptr(), ys, h.data_ptr(), hs, weight.data_ptr(), pd, ds,
             dx.data_ptr() if need_dx else 0, n, dw.data_ptr() if need_dweight else 0)
@@ -126,7 +130,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, e
         if need < 0:
             _check(-need)
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=h.device)
+            workspace = h.new_empty(need, dtype=torch.uint8)
             pws = workspace.data_ptr()
     status = L.senmoe_rms_norm_backward(_pack_grad(*args, pws, need), _current_stream(device))
     if status:

@@ -38,6 +38,7 @@ from .products import (_CODES, _DTYPES, _GATED, ACTIVATIONS, LINEAR_AUTO, _bad, 
 BLOCK8 = 32  # elements of a scale
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _pack_quantize = struct.Struct("".join(_CODES[t] for _, t in SenMoeQuantize8._fields_)).pack
+_c_quantize = _c_linear8 = None  # the library's entries, once it is loaded
 _pack_linear8 = struct.Struct("".join(_CODES[t] for _, t in SenMoeLinear8._fields_)).pack
 
 
@@ -62,20 +63,48 @@ def _blocks(n: int, what: str) -> int:
     return n // BLOCK8
 
 
-def _check_rows8(r, name: str, device: int) -> None:
-    if not isinstance(r, Rows8):
-        raise TypeError(f"{name} must be Rows8, got {type(r).__name__}")
+def _check_rows8(r, name: str, device: int):
+    """The shape of r's codes."""
     codes, scales = r
     if codes.dtype is not _E4M3 or scales.dtype is not _E8M0:
         raise TypeError(f"{name} must hold float8_e4m3fn codes and float8_e8m0fnu scales, got {codes.dtype} and "
                         f"{scales.dtype}")
     if codes.get_device() != device or scales.get_device() != device:
         raise TypeError(f"{name} on {codes.device} and {scales.device}: tensors must share one device")
-    if not codes.dim():
+    shape = codes.shape
+    if not shape:
         raise _bad(f"{name} has no dimension")
-    b = _blocks(codes.shape[-1], f"{name}: row length")
-    if scales.shape != (*codes.shape[:-1], b):
-        raise _bad(f"{name}: scales {tuple(scales.shape)} for codes {tuple(codes.shape)}")
+    n = shape[-1]
+    if n % BLOCK8 or n < 1:
+        _blocks(n, f"{name}: row length")
+    if scales.shape != (*shape[:-1], n // BLOCK8):
+        raise _bad(f"{name}: scales {tuple(scales.shape)} for codes {tuple(shape)}")
+    return shape
+
+
+def _rows8(r, name: str) -> Rows8:
+    if not isinstance(r, Rows8):
+        raise TypeError(f"{name} must be Rows8, got {type(r).__name__}")
+    return r
+
+
+# A decode step's kernels take a few microseconds, and an allocation two or
+# three on the host: empty_like and empty_strided are the cheapest forms of one.
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _empty(t: torch.Tensor, lead, n: int, dtype) -> torch.Tensor:
+    """An uninitialised contiguous [*lead, n] on t's device."""
+    if len(lead) == 1:
+        return torch.empty_strided((lead[0], n), (n, 1), dtype=dtype, device=t.device)
+    return t.new_empty((*lead, n), dtype=dtype)
+
+
+def _empty8(t: torch.Tensor, lead, n: int) -> Rows8:
+    """Uninitialised rows of n elements on t's device."""
+    return Rows8(_empty(t, lead, n, _E4M3), _empty(t, lead, n // BLOCK8, _E8M0))
 
 
 def _device_of(t: torch.Tensor) -> int:
@@ -136,21 +165,36 @@ def _quantize(x, preact, act: int, device: int) -> Rows8:
     n = x.shape[-1]
     _blocks(n, "row length")
     wide = 2 * n if act >= _GATED else n
-    lead = x.shape[:-1]
-    out = Rows8(torch.empty((*lead, wide), dtype=_E4M3, device=x.device),
-                torch.empty((*lead, wide // BLOCK8), dtype=_E8M0, device=x.device))
-    rows = x.numel() // n
-    x, xs = (x, n) if x.is_contiguous() else _rows(x, n)
-    pz = zs = 0
+    out = _empty8(x, x.shape[:-1], wide)
+    _run_quantize(x, preact, act, n, wide, out[0].data_ptr(), out[1].data_ptr(), device)
+    return out
+
+
+def _run_quantize(x, preact, act, n, wide, codes, scales, device) -> None:
+    xs, zs, pz = n, wide, 0
+    if not x.is_contiguous():
+        x, xs = _rows(x, n)
     if act:
-        preact, zs = (preact, wide) if preact.is_contiguous() else _rows(preact, wide)
+        if not preact.is_contiguous():
+            preact, zs = _rows(preact, wide)
         pz = preact.data_ptr()
-    status = lib().senmoe_quantize8(
-        _pack_quantize(_DTYPES[x.dtype], act, rows, n, x.data_ptr(), xs, pz, zs, out.codes.data_ptr(), wide,
-                       out.scales.data_ptr(), wide // BLOCK8), _current_stream(device))
+    global _c_quantize
+    if _c_quantize is None:
+        _c_quantize = lib().senmoe_quantize8
+    status = _c_quantize(
+        _pack_quantize(_DTYPES[x.dtype], act, x.numel() // n, n, x.data_ptr(), xs, pz, zs, codes, wide, scales,
+                       wide // BLOCK8), _current_stream(device))
     if status:
         _check(status)
-    return out
+
+
+def _run_linear8(*args, device) -> None:
+    global _c_linear8
+    if _c_linear8 is None:
+        _c_linear8 = lib().senmoe_linear8
+    status = _c_linear8(_pack_linear8(*args), _current_stream(device))
+    if status:
+        _check(status)
 
 
 def _check_offsets(offsets: torch.Tensor, experts: int, device: int) -> None:
@@ -170,12 +214,9 @@ def _product8(x, weight, offsets, bias, residual, activation, save_preact, eight
     code = _DTYPES.get(dtype)
     if code is None:
         raise TypeError(f"dtype must be bfloat16 or float16, got {dtype}")
-    if not isinstance(x, Rows8):
-        raise TypeError(f"x must be Rows8, got {type(x).__name__}")
-    device = _device_of(x.codes)
-    _check_rows8(x, "x", device)
-    _check_rows8(weight, "weight", device)
-    wshape, shape = weight.codes.shape, x.codes.shape
+    device = _device_of(_rows8(x, "x")[0])
+    shape = _check_rows8(x, "x", device)
+    wshape = _check_rows8(_rows8(weight, "weight"), "weight", device)
     if len(wshape) != (2 if offsets is None else 3):
         raise _bad(f"weight must be {'[out, in]' if offsets is None else '[experts, out, in]'}, got {tuple(wshape)}")
     wide, k = wshape[-2], wshape[-1]
@@ -215,26 +256,21 @@ def _product8(x, weight, offsets, bias, residual, activation, save_preact, eight
     sw, sws, swg = _stacked(weight.scales, wide, b, 1)
     if eight_bit:
         nb = _blocks(n, "8-bit output: row length")
-        out = Rows8(torch.empty((*lead, n), dtype=_E4M3, device=codes.device),
-                    torch.empty((*lead, nb), dtype=_E8M0, device=codes.device))
-        pc, ps = out.codes.data_ptr(), out.scales.data_ptr()
+        out = _empty8(codes, lead, n)
+        pc, ps = out[0].data_ptr(), out[1].data_ptr()
     else:
         nb = 0
-        out = torch.empty((*lead, n), dtype=dtype, device=codes.device)
+        out = _empty(codes, lead, n, dtype)
         py = out.data_ptr()
     z = None
     if save_preact:
-        z = torch.empty((*lead, wide), dtype=dtype, device=codes.device)
+        z = _empty(codes, lead, wide, dtype)
         pz = z.data_ptr()
     rows = codes.numel() // k
     if rows:
-        status = lib().senmoe_linear8(
-            _pack_linear8(code, act, groups, path, rows, k, n, codes.data_ptr(), xs, scales.data_ptr(), ss,
-                          w.data_ptr(), ws, wg, sw.data_ptr(), sws, swg,
-                          0 if offsets is None else offsets.data_ptr(), pb, pr, rs, py, n, pc, n, ps, nb, pz, wide),
-            _current_stream(device))
-        if status:
-            _check(status)
+        _run_linear8(code, act, groups, path, rows, k, n, codes.data_ptr(), xs, scales.data_ptr(), ss,
+                     w.data_ptr(), ws, wg, sw.data_ptr(), sws, swg, 0 if offsets is None else offsets.data_ptr(), pb,
+                     pr, rs, py, n, pc, n, ps, nb, pz, wide, device=device)
     return (out, z) if save_preact else out
 
 
@@ -272,20 +308,44 @@ def _input_grad(dy, weight_t, offsets, preact, activation, stream, path):
     if dy.dtype not in _DTYPES:
         raise TypeError(f"dy must be bfloat16 or float16, got {dy.dtype}")
     device = _device_of(dy)
-    _check_rows8(weight_t, "weight_t", device)
     if not dy.dim():
         raise _bad("dy has no dimension")
+    wshape = _check_rows8(_rows8(weight_t, "weight_t"), "weight_t", device)
     n = dy.shape[-1]
     wide = 2 * n if act >= _GATED else n
-    if weight_t.codes.shape[-1] != wide:
-        raise _bad(f"dy {tuple(dy.shape)} against weight_t {tuple(weight_t.codes.shape)}")
+    if wshape[-1] != wide:
+        raise _bad(f"dy {tuple(dy.shape)} against weight_t {tuple(wshape)}")
     if act:
         if preact is None or preact.shape != (*dy.shape[:-1], wide):
             raise _bad(f"{activation}: preact {None if preact is None else tuple(preact.shape)}, "
                        f"{(*dy.shape[:-1], wide)} wanted")
         _on16(preact, device, dy.dtype, "preact")
-    dz = _quantize(dy, preact, act, device)
-    return _product8(dz, weight_t, offsets, None, None, "none", False, False, dy.dtype, None, path)
+    _blocks(n, "dy: row length")
+    if len(wshape) != (2 if offsets is None else 3):
+        raise _bad(f"weight_t must be {'[in, out]' if offsets is None else '[experts, in, out]'}, got {tuple(wshape)}")
+    k = wshape[-2]
+    if k < 1:
+        raise _bad(f"weight_t {tuple(wshape)}: in_features={k}")
+    groups = 1
+    if offsets is not None:
+        if dy.dim() != 2:
+            raise _bad(f"dy must be [rows, out], got {tuple(dy.shape)}")
+        groups = wshape[0]
+        _check_offsets(offsets, groups, device)
+        offsets = offsets.contiguous()
+    rows, lead = dy.numel() // n, dy.shape[:-1]
+    dx = _empty(dy, lead, k, dy.dtype)
+    if rows:
+        size = rows * wide  # dz: its elements, then its scales
+        held = _empty(dy, (1,), size + size // BLOCK8, torch.uint8)  # (until both calls are made)
+        dz = held.data_ptr()
+        _run_quantize(dy, preact, act, n, wide, dz, dz + size, device)
+        w, ws, wg = _stacked(weight_t.codes, k, wide, 16)
+        sw, sws, swg = _stacked(weight_t.scales, k, wide // BLOCK8, 1)
+        _run_linear8(_DTYPES[dy.dtype], 0, groups, path, rows, wide, k, dz, wide, dz + size, wide // BLOCK8,
+                     w.data_ptr(), ws, wg, sw.data_ptr(), sws, swg, 0 if offsets is None else offsets.data_ptr(), 0,
+                     0, 0, dx.data_ptr(), k, 0, 0, 0, 0, 0, 0, device=device)
+    return dx
 
 
 def linear8_input_grad(dy: torch.Tensor, weight_t: Rows8, preact: torch.Tensor | None = None,
