@@ -839,6 +839,20 @@ cudaError_t make_tmap_4d(CUtensorMap* map, const void* base, const uint64_t (&di
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t make_tmap_5d(CUtensorMap* map, const void* base, const uint64_t (&dims)[5],
+                         const uint64_t (&stride_bytes)[4], const uint32_t (&box)[5]) {
+  auto enc = tmap_encoder();
+  if (!enc) return cudaErrorNotSupported;
+  const cuuint64_t d[5] = {dims[0], dims[1], dims[2], dims[3], dims[4]};
+  const cuuint64_t s[4] = {stride_bytes[0], stride_bytes[1], stride_bytes[2], stride_bytes[3]};
+  const cuuint32_t x[5] = {box[0], box[1], box[2], box[3], box[4]};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, const_cast<void*>(base), d, s, x, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // Slot-ordered fp16 copy of the token rows (bf16 -> fp16 is exact in range),
 // k-permuted within each block of 8 columns like the dequantised weights
 // (kperm8), or in one of the warp-MMA kernel's orders (kperm256; kperm_g4,

@@ -3,9 +3,9 @@
 //
 // A tile is D[features, w columns] as in linear_tc.cu: M (TMEM lanes) runs
 // along W's rows, N (w <= 224 columns) along the rows of x, so that a ragged
-// group costs MMA time in proportion to its rows.  A stage holds 128 k: the
+// group costs MMA time in proportion to its rows.  A stage holds 256 k: the
 // operands as 128-byte-swizzled boxes by TMA, one byte an element, and their
-// scales, 4 bytes a row.  The tensor core multiplies by the scales itself:
+// scales, 8 bytes a row.  The tensor core multiplies by the scales itself:
 //
 //   D += sum over blocks b of 32 k:  2^(sw[m, b] + sx[n, b])  sum_k W[m, k] x[n, k]
 //
@@ -13,12 +13,11 @@
 // lane r mod 32 (the same in each quarter of the lanes) and column r / 32, the
 // four bytes of a word being four consecutive blocks.  Warps 2 and 3 bring
 // them there: a lane loads the words of rows l, l + 32, l + 64, l + 96 of 128
-// rows (16 bytes of a row, 4 stages, at a time where rows are aligned for it,
-// the next 4 stages' in flight), which side by side are the 16 bytes that
+// rows (the next stage's in flight), which side by side are the 16 bytes that
 // tcgen05.cp 32x128b wants for lane l, and the MMA warp issues the copies
-// ahead of a stage's MMAs.  Copies and MMAs of one thread run in order; two
-// sets of scale columns alternate all the same, so that a copy need not wait
-// for the MMAs before it.
+// ahead of the MMAs.  Copies and MMAs of one thread run in order; two sets of
+// scale columns alternate all the same, so that a copy need not wait for the
+// MMAs before it.
 //
 // Forms of a tile: one CTA (128 features), a pair (cta_group::2, 256 features
 // on two SMs, each holding half of the columns' codes and all of their
@@ -40,15 +39,26 @@
 namespace senmoe {
 namespace {
 
-constexpr int kBK8 = 128;                      // k of a stage: one 128-byte line
-constexpr uint32_t kMBytes8 = 128 * kBK8;      // a CTA's M operand of a stage
+// k of a stage: two pieces of one 128-byte line.  (With one piece a stage took
+// 480 cycles in its barriers alone, whatever its bytes and MMAs.)
+constexpr int kPiece = 128, kPieces = 2, kBK8 = kPiece * kPieces;
+constexpr uint32_t kMPiece = 128 * kPiece;     // a piece of a CTA's M operand
 constexpr int kMaxWidth = 224;                 // columns of a tile: two accumulators and two sets of scales in 512
 constexpr uint32_t kAccColumn = 256;           // from one accumulator to the other
 constexpr uint32_t kScaleColumn = 240;         // of the scales, behind each accumulator
-constexpr uint32_t kAtomBytes = 512;           // 128 rows' scales of a stage
-constexpr uint32_t kScaleBytes = 3 * kAtomBytes;  // W's rows, then up to 256 columns
+constexpr uint32_t kAtomBytes = 512;           // 128 rows' scales of a piece
+constexpr uint32_t kPieceScales = 3 * kAtomBytes;  // W's rows, then up to 256 columns
+constexpr uint32_t kScaleBytes = kPieces * kPieceScales;
+// Warps: 0 the loads, 1 the MMAs, 2 and 3 the scales, the others the epilogue:
+// with 8 of them, two a scheduler, it waited for its own latencies (8192 rows
+// of 2048 -> 8192 gelu 200 us).  20 warps leave 96 registers a thread, one more
+// would leave 80.
+constexpr int kEpi8 = 16, kThreads8 = (kEpiWarp0 + kEpi8) * 32;
+// An epilogue warp's shared memory: where it turns a chunk, and (gated) swaps one before.
+constexpr uint32_t epi_stride(bool gated) { return gated ? kSwapBytes : kTurnBytes; }
+static_assert(kSwapBytes >= kTurnBytes);
 constexpr uint32_t kStaticBytes8 = 9 * 1024 + 1024;
-constexpr uint32_t epilogue_bytes8(bool gated) { return kEpiWarps * (kTurnBytes + (gated ? kSwapBytes : 0)); }
+constexpr uint32_t epilogue_bytes8(bool gated) { return kEpi8 * epi_stride(gated); }
 constexpr uint32_t ring_budget8(bool gated) { return 227 * 1024 - kStaticBytes8 - epilogue_bytes8(gated); }
 
 __device__ int g_linear8_error;  // first device error of these kernels on this device
@@ -58,8 +68,9 @@ struct Tc8Args {
   Linear8Args l;
   int bn, part;          // columns of a tile, and of a CTA's N operand (half of it in a pair)
   int m_tiles, stages, split;
-  uint32_t stage_bytes;  // a stage's operands
-  int w_load, x_load;    // bytes of a scale row in one load: 16, 8, 4 or 1
+  uint32_t stage_bytes;  // a stage's operands: W's pieces, then the columns'
+  int pieces;            // rows are whole pieces, which the maps have as a dimension
+  int w_load, x_load;    // bytes of a scale row in one load: 8, 4 or 1
   long long tile_limit;  // of the wait for a tile's accumulators, cycles
 };
 
@@ -94,6 +105,38 @@ template <bool PAIR> __device__ __forceinline__ void copy_scales(uint32_t taddr,
   if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
   else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
+// TMA load of a box of a 5-d map; PAIR: `bar` may be the other CTA's.
+template <bool PAIR>
+__device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, int c4,
+                                       uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, "
+        "%3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
+        : "memory");
+}
+// Both pieces of stage b of an operand, its rows from `row` on.  Rows of whole
+// pieces: one load (a piece past the last is zeros).  Otherwise two, as the map
+// must know where a row ends.
+template <bool PAIR>
+__device__ __forceinline__ void load_stage(uint32_t dst, uint32_t piece_bytes, const CUtensorMap* map, bool pieces,
+                                           int b, int row, int e, uint32_t bar) {
+  if (pieces) {
+    tma_5d<PAIR>(dst, map, 0, row, 0, b * kPieces, e, bar);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)  // (the maps count pairs of elements)
+      tma_5d<PAIR>(dst + i * piece_bytes, map, (b * kPieces + i) * (kPiece / 2), row, 0, 0, e, bar);
+  }
+}
+
 // ------------------------------------------------------------------ tiles
 struct Tile8 {
   int e;         // group
@@ -127,36 +170,25 @@ __device__ __forceinline__ Tile8 tile_at8(const Tc8Args& a, const int* s_off, co
   return t;
 }
 
-// The scales of a row's blocks 16 q .. 16 q + 15 (four stages), row at p, `have`
+// The scales of a row's blocks from `at` on, a stage's 8, row at p, `have`
 // blocks in all: `load` bytes at a time; what lies past the row reads as 2^0
 // (no MMA takes it).
-__device__ __forceinline__ uint4 load_scales(const uint8_t* p, int q, int have, int load) {
-  uint32_t w[4] = {0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
-  const int at = 16 * q;
+__device__ __forceinline__ uint2 load_scales(const uint8_t* p, int at, int have, int load) {
+  uint32_t w[2] = {0x7f7f7f7fu, 0x7f7f7f7fu};
   p += at;
-  if (load == 16) {
-    if (at < have) return *reinterpret_cast<const uint4*>(p);
-  } else if (load == 8) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (at + 8 * i < have) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p + 8 * i);
-        w[2 * i] = v.x;
-        w[2 * i + 1] = v.y;
-      }
-    }
+  if (load == 8) {
+    if (at < have) return *reinterpret_cast<const uint2*>(p);
   } else if (load == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
       if (at + 4 * i < have) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 8; ++i)
       if (at + i < have) w[i >> 2] = (w[i >> 2] & ~(0xffu << 8 * (i & 3))) | static_cast<uint32_t>(p[i]) << 8 * (i & 3);
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // ---------------------------------------------------------------- epilogue
 // 16 columns x 32 features, a feature a lane -> 8 bits: each column's 32
@@ -224,7 +256,7 @@ template <bool GATED, bool BF16, bool EIGHT> struct Finish8 {
 };
 
 template <bool GATED, bool BF16, bool PAIR, bool EIGHT>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(kThreads8, 1)
     linear8_tc_kernel(const __grid_constant__ CUtensorMap tm_m, const __grid_constant__ CUtensorMap tm_n,
                       const __grid_constant__ CUtensorMap tm_half, const __grid_constant__ Tc8Args a) {
   constexpr int kCtas = PAIR ? 2 : 1;
@@ -244,8 +276,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t scale_base = ring + stages * a.stage_bytes;  // [stage][W's rows, columns 0-127, columns 128 on]
   unsigned char* scale_ptr = ring_ptr + stages * a.stage_bytes;
   unsigned char* epi_ptr = scale_ptr + stages * kScaleBytes;
-  const auto turn_of = [&](int ew) { return reinterpret_cast<uint32_t*>(epi_ptr + ew * kTurnBytes); };
-  const auto swap_of = [&](int ew) { return reinterpret_cast<float*>(epi_ptr + kEpiWarps * kTurnBytes + ew * kSwapBytes); };
+  // (a warp turns its chunk after the swap, when its partner has read)
+  const auto turn_of = [&](int ew) { return reinterpret_cast<uint32_t*>(epi_ptr + ew * epi_stride(GATED)); };
+  const auto swap_of = [&](int ew) { return reinterpret_cast<float*>(turn_of(ew)); };
   const int csize = PAIR ? 2 : a.split;  // CTAs of the cluster
   const int rank = csize > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int unit = blockIdx.x / csize, units = gridDim.x / csize;
@@ -257,7 +290,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_accfull[i], 1);
-      mbar_init(&bar_accempty[i], kCtas * kEpiWarps);
+      mbar_init(&bar_accempty[i], kCtas * kEpi8);
     }
     mbar_init(&bar_drain, 1);
     s_abort = 0;
@@ -294,10 +327,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int part = t.n / kCtas, col = t.c0 + (PAIR ? rank * part : 0);  // this CTA's share of the columns
         // one load of a full part, or of half of one where that holds the columns
         const bool small = 2 * part <= a.part && a.part >= 32;
-        const uint32_t bytes = kMBytes8 + (small ? a.part / 2 : a.part) * kBK8;
+        const uint32_t n_piece = (small ? a.part / 2 : a.part) * kPiece, bytes = kPieces * (kMPiece + n_piece);
         for (int b = t.kb0; b < t.kb1; ++b) {
           if (!(ok = wait_or_abort(&bar_empty[st], ph ^ 1, &s_abort, err))) break;
-          const uint32_t sm = ring + st * a.stage_bytes, sn = sm + kMBytes8;
+          const uint32_t sm = ring + st * a.stage_bytes, sn = sm + kPieces * kMPiece;
           uint32_t full = smem_u32(&bar_full[st]);
           if constexpr (PAIR) {
             if (rank == 0) mbar_arrive_expect_tx(&bar_full[st], 2 * bytes);
@@ -305,9 +338,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           } else {
             mbar_arrive_expect_tx(&bar_full[st], bytes);
           }
-          const int k0 = b * (kBK8 / 2);  // the maps count pairs of elements
-          tma_4d<PAIR>(sm, &tm_m, k0, t.m0, 0, t.e, full);
-          tma_4d<PAIR>(sn, small ? &tm_half : &tm_n, k0, col, 0, 0, full);
+          load_stage<PAIR>(sm, kMPiece, &tm_m, a.pieces, b, t.m0, t.e, full);
+          load_stage<PAIR>(sn, n_piece, small ? &tm_half : &tm_n, a.pieces, b, col, 0, full);
           issued |= 1u << st;
           parity = (parity & ~(1u << st)) | (static_cast<uint32_t>(ph) << st);
           next(st, ph);
@@ -328,7 +360,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const bool leader = elect_one();
     bool ok = true;
     int st = 0, ph = 0, it = 0;
-    uint32_t set = 0;  // of scale columns
     for (int idx = unit; idx < tiles && ok; idx += units, ++it) {
       const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
       const int ab = it & 1, aph = (it >> 1) & 1;
@@ -336,24 +367,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_fence_after();
       const uint32_t d = tmem + ab * kAccColumn;
       const uint32_t idesc = instr_desc8(t.n, 128 * kCtas);
+      const int part = t.n / kCtas;
+      const uint32_t n_piece = (2 * part <= a.part && a.part >= 32 ? a.part / 2 : a.part) * kPiece;  // as loaded
       for (int b = t.kb0; b < t.kb1; ++b) {
         if (!(ok = warp_wait(&bar_full[st], ph, &s_abort, err))) break;
         tc_fence_after();
         if (leader) {
-          const uint32_t sm = ring + st * a.stage_bytes, sc = scale_base + st * kScaleBytes;
-          const uint32_t sa = tmem + kScaleColumn + set * kAccColumn, sb = sa + 4;
-          copy_scales<PAIR>(sa, sc);
-          copy_scales<PAIR>(sb, sc + kAtomBytes);
-          if (t.n > 128) copy_scales<PAIR>(sb + 4, sc + 2 * kAtomBytes);
-          const uint64_t dm = smem_desc<false>(sm), dn = smem_desc<false>(sm + kMBytes8);
-          const int ks = min(kBK8, a.l.k - b * kBK8) / kBlock8;
-          for (int s = 0; s < ks; ++s)  // 32 k: 32 bytes along a line
-            umma_scaled<PAIR>(d, dm + s * (32 >> 4), dn + s * (32 >> 4), idesc | (s << 4) | (s << 29), sa, sb,
-                              (b > t.kb0 || s > 0) ? 1u : 0u);
+          const uint32_t sm = ring + st * a.stage_bytes, sn = sm + kPieces * kMPiece, sc = scale_base + st * kScaleBytes;
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            const int ks = min(kPiece, a.l.k - (b * kPieces + i) * kPiece) / kBlock8;
+            if (ks <= 0) break;
+            const uint32_t sa = tmem + kScaleColumn + i * kAccColumn, sb = sa + 4;
+            copy_scales<PAIR>(sa, sc + i * kPieceScales);
+            copy_scales<PAIR>(sb, sc + i * kPieceScales + kAtomBytes);
+            if (t.n > 128) copy_scales<PAIR>(sb + 4, sc + i * kPieceScales + 2 * kAtomBytes);
+            const uint64_t dm = smem_desc<false>(sm + i * kMPiece), dn = smem_desc<false>(sn + i * n_piece);
+            for (int s = 0; s < ks; ++s)  // 32 k: 32 bytes along a line
+              umma_scaled<PAIR>(d, dm + s * (32 >> 4), dn + s * (32 >> 4), idesc | (s << 4) | (s << 29), sa, sb,
+                                (b > t.kb0 || i > 0 || s > 0) ? 1u : 0u);
+          }
           umma_commit<PAIR>(&bar_empty[st]);
         }
         __syncwarp();
-        set ^= 1;
         next(st, ph);
       }
       if (ok && leader) umma_commit<PAIR>(&bar_accfull[ab]);
@@ -364,77 +400,70 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncwarp();
     volatile int never = 0;
     wait_or_abort(&bar_drain, 0, &never, nullptr);
-  } else if (warp == 2 || warp == 3) {
+  } else if (warp < kEpiWarp0) {
     // ============================================================== scales
-    // warp 2: W's 128 rows of the tile; warp 3: the columns, 128 at a time
+    // 128 rows at a time: W's and the columns from 128 on (warps 2 here and 1
+    // of a pair's second CTA do nothing else), the first 128 columns (warp 3)
     const Linear8Args& l = a.l;
     const int blocks = l.k / kBlock8, cap = static_cast<int>(l.rows) - 1;
-    const int load = warp == 2 ? a.w_load : a.x_load;
     int st = 0, ph = 0;
-    bool ok = true;
+    bool ok = warp >= 2;
     for (int idx = unit; idx < tiles && ok; idx += units) {
       const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
-      const int atoms = warp == 2 ? 1 : (t.n + 127) / 128;
+      const int atoms = warp == 2 && t.n > 128 ? 2 : 1;
       // this lane's rows; past the last one, that one (no result is of it)
       const uint8_t* p[2][4];
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i * 32 + lane;
-          if (warp == 2) {
-            const int half = GATED ? l.n / 2 : l.n, f = GATED ? t.m0 + (r & 63) : t.m0 + r;
-            const int64_t row = min(f, half - 1) + (GATED && r >= 64 ? half : 0);
-            p[g][i] = l.w_scales + t.e * l.w_scales_group_stride + row * l.w_scales_stride;
-          } else {
-            p[g][i] = l.x_scales + static_cast<int64_t>(min(t.c0 + g * 128 + r, cap)) * l.x_scales_stride;
-          }
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 32 + lane, half = GATED ? l.n / 2 : l.n, f = GATED ? t.m0 + (r & 63) : t.m0 + r;
+        const int64_t row = min(f, half - 1) + (GATED && r >= 64 ? half : 0);
+        const auto column = [&](int c) { return l.x_scales + static_cast<int64_t>(min(t.c0 + c, cap)) * l.x_scales_stride; };
+        p[0][i] = warp == 2 ? l.w_scales + t.e * l.w_scales_group_stride + row * l.w_scales_stride : column(r);
+        p[1][i] = column(128 + r);
       }
-      uint4 now[2][4], then[2][4];
-      const auto fetch = [&](uint4 (&v)[2][4], int q) {
+      // a stage's, the next one's on their way
+      uint2 now[2][4], then[2][4];
+      const auto fetch = [&](int b) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          if (g < atoms) {
+          if (g < atoms && b < t.kb1) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[g][i] = load_scales(p[g][i], q, blocks, load);
+            for (int i = 0; i < 4; ++i)
+              then[g][i] = load_scales(p[g][i], b * (kBK8 / kBlock8), blocks, warp == 2 && g == 0 ? a.w_load : a.x_load);
           }
         }
       };
-      const int q0 = t.kb0 / 4, q1 = (t.kb1 + 3) / 4;
-      if (q0 < q1) fetch(now, q0);
-      for (int q = q0; q < q1 && ok; ++q) {
-        if (q + 1 < q1) fetch(then, q + 1);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int b = 4 * q + j;
-          if (b < t.kb0 || b >= t.kb1 || !ok) continue;
-          if (!(ok = warp_wait(&bar_empty[st], ph ^ 1, &s_abort, err))) continue;
-          unsigned char* dst = scale_ptr + st * kScaleBytes + (warp == 2 ? 0 : kAtomBytes) + lane * 16;
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            if (g < atoms)
-              *reinterpret_cast<uint4*>(dst + g * kAtomBytes) = make_uint4(word_of(now[g][0], j), word_of(now[g][1], j),
-                                                                         word_of(now[g][2], j), word_of(now[g][3], j));
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          // (to the other CTA too with the plain arrive: what it guards is this
-          // SM's shared memory, which the proxy fence has ordered; with
-          // .release.cluster a stage took 1600 cycles)
-          if (lane == 0) arrive_at(PAIR ? map_rank(smem_u32(&bar_full[st]), 0) : smem_u32(&bar_full[st]));
-          next(st, ph);
-        }
+      fetch(t.kb0);
+      for (int b = t.kb0; b < t.kb1; ++b) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) now[g][i] = then[g][i];
         }
+        fetch(b + 1);
+        if (!(ok = warp_wait(&bar_empty[st], ph ^ 1, &s_abort, err))) break;
+        unsigned char* dst = scale_ptr + st * kScaleBytes + (warp == 2 ? 0 : kAtomBytes) + lane * 16;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (g < atoms) {
+            *reinterpret_cast<uint4*>(dst + g * 2 * kAtomBytes) = make_uint4(now[g][0].x, now[g][1].x, now[g][2].x, now[g][3].x);
+            *reinterpret_cast<uint4*>(dst + g * 2 * kAtomBytes + kPieceScales) =
+                make_uint4(now[g][0].y, now[g][1].y, now[g][2].y, now[g][3].y);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        // (to the other CTA too with the plain arrive: what it guards is this
+        // SM's shared memory, which the proxy fence has ordered; with
+        // .release.cluster a stage took 1600 cycles)
+        if (lane == 0) arrive_at(PAIR ? map_rank(smem_u32(&bar_full[st]), 0) : smem_u32(&bar_full[st]));
+        next(st, ph);
       }
     }
-  } else if (warp >= kEpiWarp0 && (PAIR || a.split <= 1)) {
+  } else if (PAIR || a.split <= 1) {
     // ============================================================ epilogue
-    // 32 columns at a time, the warps of a lane quarter in turn
+    // 16 columns at a time (gated: 32), the warps of a lane quarter in turn
+    constexpr int kChunk = GATED ? 32 : 16, kStep = kEpi8 / 4 * kChunk;
     const int ew = warp - kEpiWarp0, q = warp & 3, turn2 = ew >> 2;
     const Finish8<GATED, BF16, EIGHT> fin(a.l, turn_of(ew), lane);
     int it = 0;
@@ -453,21 +482,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + ab * kAccColumn;
       const uint32_t release = PAIR ? map_rank(smem_u32(&bar_accempty[ab]), 0) : smem_u32(&bar_accempty[ab]);
       bool released = false;
-      for (int c = turn2 * 32; c < t.w; c += kColStep) {
-        uint32_t r[32];
+      for (int c = turn2 * kChunk; c < t.w; c += kStep) {
+        uint32_t r[kChunk];
         tmem_ld16(acc + c, r);
-        tmem_ld16(acc + c + 16, r + 16);
+        if constexpr (GATED) tmem_ld16(acc + c + 16, r + 16);
         tmem_ld_wait();
-        if (c + kColStep >= t.w) {  // this warp's last read of the accumulator
+        if (c + kStep >= t.w) {  // this warp's last read of the accumulator
           tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_at(release);
           released = true;
         }
         const int64_t row = t.c0 + c;
-        float z[2][16];
+        float z[kChunk / 16][16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) z[i >> 4][i & 15] = __uint_as_float(r[i]) + bias;
+        for (int i = 0; i < kChunk; ++i) z[i >> 4][i & 15] = __uint_as_float(r[i]) + bias;
         if constexpr (GATED) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) fin.keep(z[h], row + 16 * h, up + f0, t.w - c - 16 * h, feats);
@@ -503,14 +532,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int h = gate ? 0 : 16;
           fin.write(y, row + h, f0, t.w - c - h, feats);
         } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int w = t.w - c - 16 * h;
-            if (w <= 0) break;
-            fin.keep(z[h], row + 16 * h, f0, w, feats);
-            act_chunk(a.l.act, z[h]);
-            fin.write(z[h], row + 16 * h, f0, w, feats);
-          }
+          fin.keep(z[0], row, f0, t.w - c, feats);
+          act_chunk(a.l.act, z[0]);
+          fin.write(z[0], row, f0, t.w - c, feats);
         }
       }
       if (!released) {
@@ -519,7 +543,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) arrive_at(release);
       }
     }
-  } else if (warp >= kEpiWarp0) {
+  } else {
     // =========================== K split: this CTA's accumulator is ready
     if (unit < tiles) warp_wait(&bar_accfull[0], 0, &s_abort, err, a.tile_limit);
     tc_fence_after();
@@ -540,7 +564,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (epi) {
         const int q = warp & 3;
         const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16);
-        for (int c = ew >> 2; c < chunks; c += kEpiWarps / 4) {
+        for (int c = ew >> 2; c < chunks; c += kEpi8 / 4) {
           uint32_t r[16];
           if (t.kb1 > t.kb0) {
             tmem_ld16(acc + 16 * c, r);
@@ -562,7 +586,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const Finish8<GATED, BF16, EIGHT> fin(a.l, turn_of(ew), lane);
         constexpr int kQuarters = GATED ? 2 : 4;
         const int mine = chunks > rank ? (chunks - rank + csize - 1) / csize : 0;  // chunks rank, rank + csize, ...
-        for (int i = ew; i < mine * kQuarters; i += kEpiWarps) {
+        for (int i = ew; i < mine * kQuarters; i += kEpi8) {
           const int q = i % kQuarters, slot = i / kQuarters, c = (slot * csize + rank) * 16, w = t.w - c;
           const int f0 = t.m0 + q * 32, feats = min(32, fin.cols - f0);
           const float b0 = fin.bias(t.e, f0, feats, 0), b1 = GATED ? fin.bias(t.e, f0, feats, fin.cols) : 0.0f;
@@ -603,13 +627,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
       const int64_t r = i < head ? i : tail + (i - head);
       if constexpr (EIGHT) {
-        for (int f = first; f < cols; f += kEpiWarps * 32) l.codes[r * l.codes_stride + f] = 0;
-        for (int f = first; f < cols / kBlock8; f += kEpiWarps * 32) l.scales[r * l.scales_stride + f] = 0;
+        for (int f = first; f < cols; f += kEpi8 * 32) l.codes[r * l.codes_stride + f] = 0;
+        for (int f = first; f < cols / kBlock8; f += kEpi8 * 32) l.scales[r * l.scales_stride + f] = 0;
       } else {
-        for (int f = first; f < cols; f += kEpiWarps * 32) out[r * l.y_stride + f] = 0;
+        for (int f = first; f < cols; f += kEpi8 * 32) out[r * l.y_stride + f] = 0;
       }
       if (pre)
-        for (int f = first; f < l.n; f += kEpiWarps * 32) pre[r * l.preact_stride + f] = 0;
+        for (int f = first; f < l.n; f += kEpi8 * 32) pre[r * l.preact_stride + f] = 0;
     }
   }
 
@@ -645,7 +669,7 @@ int tc8_sm_count() {
   return n;
 }
 
-constexpr uint32_t stage_bytes8(int part) { return kMBytes8 + part * kBK8; }
+constexpr uint32_t stage_bytes8(int part) { return kPieces * (kMPiece + part * kPiece); }
 constexpr int stages8(bool gated, int part) {
   const int fit = static_cast<int>(ring_budget8(gated) / (stage_bytes8(part) + kScaleBytes));
   return fit < kMaxStages ? fit : kMaxStages;
@@ -664,8 +688,8 @@ static_assert(one_cta_an_sm8(), "tcgen05.alloc would wait for the CTA beside");
 // Bytes of scale rows that one load may take: the rows' alignment allows it,
 // and rows are whole loads, so that none passes the last row's end.
 int scale_load(const void* p, int64_t stride, int64_t group_stride, int k) {
-  for (int n = 16; n > 1; n /= 2)
-    if (n != 2 && reinterpret_cast<uintptr_t>(p) % n == 0 && stride % n == 0 && group_stride % n == 0 &&
+  for (int n = 8; n > 2; n /= 2)
+    if (reinterpret_cast<uintptr_t>(p) % n == 0 && stride % n == 0 && group_stride % n == 0 &&
         k / kBlock8 % n == 0)
       return n;
   return 1;
@@ -684,7 +708,7 @@ cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorM
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kTcThreads);
+  cfg.blockDim = dim3(kThreads8);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -700,8 +724,7 @@ struct Plan8 {
   double cycles = 0;
 };
 
-// As in linear_tc.cu, with a k block of 128: the same bytes and MMA cycles as
-// 64 16-bit k.
+// As in linear_tc.cu, with a k block of 256: the bytes and MMA cycles of 128 16-bit k.
 constexpr double kL2Bytes8 = 57, kTileCycles8 = 900, kSplitCycles8 = 2000, kSplitColumn8 = 20;
 
 Plan8 make_plan8(const Linear8Args& l, bool gated, int sms, bool pair, int bn, int split) {
@@ -723,8 +746,9 @@ Plan8 make_plan8(const Linear8Args& l, bool gated, int sms, bool pair, int bn, i
   }
   const int step = pair ? 32 : 16;
   const double n = (static_cast<int64_t>(width + step - 1) / step) * step;
-  const double blocks = (l.k + kBK8 - 1) / kBK8;
-  const double mma = 2.0 * n > 128 ? 2.0 * n : 128, load = 128.0 * (128 + (pair ? n / 2 : n)) / kL2Bytes8;
+  const double blocks = static_cast<double>((l.k + kPiece - 1) / kPiece) / kPieces;
+  const double mma = kPieces * (2.0 * n > 128 ? 2.0 * n : 128);
+  const double load = kBK8 * (128 + (pair ? n / 2 : n)) / kL2Bytes8;
   const double per = mma > load ? mma : load;
   const double slots = static_cast<double>(sms / ((pair ? 2 : 1) * split));
   double waves = chunks * m_tiles / slots;
@@ -784,16 +808,22 @@ cudaError_t launch_linear8_tc(const Linear8Args& l, int form, cudaStream_t st) {
   const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
   const size_t smem = smem8(gated, a.part);
 
-  // two elements a 16-bit unit of the maps
+  // two elements a 16-bit unit of the maps: [unit, row, gate or up, piece, group]
   CUtensorMap tm{}, tn{}, half{};
-  const uint64_t w_row = l.w_stride, x_row = l.x_stride, n = features, k2 = l.k / 2, rows = l.rows;
+  a.pieces = l.k % kPiece == 0;
+  const uint64_t w_row = l.w_stride, x_row = l.x_stride, n = features, rows = l.rows;
+  const uint64_t units = a.pieces ? kPiece / 2 : l.k / 2, pieces = a.pieces ? l.k / kPiece : 1;
+  const uint32_t box = a.pieces ? kPieces : 1;
   const uint64_t gs = l.groups > 1 ? l.w_group_stride : w_row * l.n;
-  cudaError_t e = make_tmap_4d(&tm, l.w, {k2, n, gated ? 2u : 1u, uint64_t(l.groups)}, {w_row, n * w_row, gs},
-                               {64, gated ? 64u : 128u, gated ? 2u : 1u, 1});
-  if (e == cudaSuccess) e = make_tmap_4d(&tn, l.x, {k2, rows, 1, 1}, {x_row, x_row, x_row}, {64, uint32_t(a.part), 1, 1});
+  cudaError_t e = make_tmap_5d(&tm, l.w, {units, n, gated ? 2u : 1u, pieces, uint64_t(l.groups)},
+                               {w_row, n * w_row, kPiece, gs}, {kPiece / 2, gated ? 64u : 128u, gated ? 2u : 1u, box, 1});
+  const auto columns = [&](CUtensorMap* map, int part) {
+    return make_tmap_5d(map, l.x, {units, rows, 1, pieces, 1}, {x_row, x_row, kPiece, x_row},
+                        {kPiece / 2, uint32_t(part), 1, box, 1});
+  };
+  if (e == cudaSuccess) e = columns(&tn, a.part);
   half = tn;
-  if (e == cudaSuccess && a.part >= 32)
-    e = make_tmap_4d(&half, l.x, {k2, rows, 1, 1}, {x_row, x_row, x_row}, {64, uint32_t(a.part / 2), 1, 1});
+  if (e == cudaSuccess && a.part >= 32) e = columns(&half, a.part / 2);
   if (e != cudaSuccess) return e;
   if (plan.pair)
     return l.codes ? launch_form<true, true>(gated, l.bf16, tm, tn, half, a, grid, smem, st)
