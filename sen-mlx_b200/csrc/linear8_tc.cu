@@ -30,6 +30,7 @@
 
 #include <cuda.h>
 
+#include <cmath>
 #include <mutex>
 
 #include "kernels.h"
@@ -739,16 +740,23 @@ Plan8 make_plan8(const Linear8Args& l, bool gated, int sms, bool pair, int bn, i
   const int64_t upper = (l.rows + bn - 1) / bn + (l.offsets ? l.groups : 0);
   q.tiles = (upper < l.rows ? upper : l.rows) * m_tiles;
   double chunks = static_cast<double>((l.rows + bn - 1) / bn), width = l.rows / chunks;
-  if (l.offsets) {  // counts spread about the mean: a group near a multiple of bn takes one chunk more half the time
-    const double used = mean < 1 ? l.rows : l.groups;  // groups with rows, about
-    chunks = used * (mean < 1 ? 1.0 : static_cast<int64_t>(mean / bn + 0.5) < 1 ? 1.0 : mean / bn + 0.5);
-    width = mean < 1 ? 1 : l.rows / chunks;
+  if (l.offsets) {
+    if (mean < 1) {  // groups with rows, about
+      chunks = static_cast<double>(l.rows);
+    } else {  // counts spread about the mean as random routing's do: a chunk more for each multiple of bn below a count
+      const double sd = std::sqrt(mean);
+      double each = 1.0;
+      for (double at = bn; at < mean + 4 * sd; at += bn) each += 0.5 * std::erfc((at - mean) / (1.4142136 * sd));
+      chunks = each * l.groups;
+    }
+    width = l.rows / chunks;
   }
   const int step = pair ? 32 : 16;
   const double n = (static_cast<int64_t>(width + step - 1) / step) * step;
   const double blocks = static_cast<double>((l.k + kPiece - 1) / kPiece) / kPieces;
   const double mma = kPieces * (2.0 * n > 128 ? 2.0 * n : 128);
-  const double load = kBK8 * (128 + (pair ? n / 2 : n)) / kL2Bytes8;
+  const double loaded = 2 * n <= bn && bn >= 32 ? bn / 2 : bn;  // columns: a whole box, or half of one
+  const double load = kBK8 * (128 + (pair ? loaded / 2 : loaded)) / kL2Bytes8;
   const double per = mma > load ? mma : load;
   const double slots = static_cast<double>(sms / ((pair ? 2 : 1) * split));
   double waves = chunks * m_tiles / slots;
