@@ -13,9 +13,8 @@
 // lane r mod 32 (the same in each quarter of the lanes) and column r / 32, the
 // four bytes of a word being four consecutive blocks.  Warps 2 and 3 bring
 // them there: a lane loads the words of rows l, l + 32, l + 64, l + 96 of 128
-// rows (the next stage's in flight), which side by side are the 16 bytes that
-// tcgen05.cp 32x128b wants for lane l, and the MMA warp issues the copies
-// ahead of the MMAs.  Copies and MMAs of one thread run in order; two sets of
+// rows, which side by side are the 16 bytes that tcgen05.cp 32x128b wants for
+// lane l, and the MMA warp issues the copies ahead of the MMAs.  Copies and MMAs of one thread run in order; two sets of
 // scale columns alternate all the same, so that a copy need not wait for the
 // MMAs before it.
 //
@@ -50,17 +49,26 @@ constexpr uint32_t kScaleColumn = 240;         // of the scales, behind each acc
 constexpr uint32_t kAtomBytes = 512;           // 128 rows' scales of a piece
 constexpr uint32_t kPieceScales = 3 * kAtomBytes;  // W's rows, then up to 256 columns
 constexpr uint32_t kScaleBytes = kPieces * kPieceScales;
-// Warps: 0 the loads, 1 the MMAs, 2 and 3 the scales, the others the epilogue:
-// with 8 of them, two a scheduler, it waited for its own latencies (8192 rows
-// of 2048 -> 8192 gelu 200 us).  20 warps leave 96 registers a thread, one more
-// would leave 80.
-constexpr int kEpi8 = 16, kThreads8 = (kEpiWarp0 + kEpi8) * 32;
+// Scales on their way: units of two stages, 16 bytes a row, 128 rows three times.
+constexpr int kUnits = 2;
+constexpr uint32_t kUnitAtom = 128 * 16, kUnitBytes = kUnits * 3 * kUnitAtom;
+// Warps: 0 the loads, 1 the MMAs, 2 to 7 the scales, the others the epilogue.
+// With 8 epilogue warps, two a scheduler, it waited for its own latencies
+// (8192 rows of 2048 -> 8192 gelu 200 us); with 2 warps for the scales, whose
+// gathered loads take 200 cycles an instruction, the MMAs waited for them.  20
+// warps leave 96 registers a thread, one more would leave 80.
+constexpr int kScaleWarp0 = 2, kScaleWarps = 6, kEpi0 = kScaleWarp0 + kScaleWarps;
+constexpr int kEpi8 = 12, kThreads8 = (kEpi0 + kEpi8) * 32;
+static_assert(kEpi0 % 4 == 0);  // an epilogue warp's number gives its quarter of the lanes
 // An epilogue warp's shared memory: where it turns a chunk, and (gated) swaps one before.
 constexpr uint32_t epi_stride(bool gated) { return gated ? kSwapBytes : kTurnBytes; }
 static_assert(kSwapBytes >= kTurnBytes);
-constexpr uint32_t kStaticBytes8 = 9 * 1024 + 1024;
+constexpr uint32_t kStaticBytes8 = 1024 + 1024;  // barriers; the ring's alignment
+constexpr uint32_t table_bytes(int groups) { return (2 * (groups + 1) * 4 + 15) & ~15; }  // row groups' offsets and chunks
 constexpr uint32_t epilogue_bytes8(bool gated) { return kEpi8 * epi_stride(gated); }
-constexpr uint32_t ring_budget8(bool gated) { return 227 * 1024 - kStaticBytes8 - epilogue_bytes8(gated); }
+constexpr uint32_t ring_budget8(bool gated, int groups) {
+  return 227 * 1024 - kStaticBytes8 - table_bytes(groups) - epilogue_bytes8(gated) - kUnitBytes;
+}
 
 __device__ int g_linear8_error;  // first device error of these kernels on this device
 __device__ int g_linear8_taken;  // what the last check found there
@@ -71,7 +79,7 @@ struct Tc8Args {
   int m_tiles, stages, split;
   uint32_t stage_bytes;  // a stage's operands: W's pieces, then the columns'
   int pieces;            // rows are whole pieces, which the maps have as a dimension
-  int w_load, x_load;    // bytes of a scale row in one load: 8, 4 or 1
+  int w_load, x_load;    // bytes of a scale row in one copy: 16, 8, 4 or 1
   long long tile_limit;  // of the wait for a tile's accumulators, cycles
 };
 
@@ -171,24 +179,25 @@ __device__ __forceinline__ Tile8 tile_at8(const Tc8Args& a, const int* s_off, co
   return t;
 }
 
-// The scales of a row's blocks from `at` on, a stage's 8, row at p, `have`
-// blocks in all: `load` bytes at a time; what lies past the row reads as 2^0
-// (no MMA takes it).
-__device__ __forceinline__ uint2 load_scales(const uint8_t* p, int at, int have, int load) {
-  uint32_t w[2] = {0x7f7f7f7fu, 0x7f7f7f7fu};
-  p += at;
-  if (load == 8) {
-    if (at < have) return *reinterpret_cast<const uint2*>(p);
+// The 16 scales from p on, of which `have` are in the row, into shared memory
+// with `load` bytes a copy; bytes (1) are there at once.  What lies past the row
+// stays as it is: no MMA takes it.
+__device__ __forceinline__ void fetch_scales(unsigned char* dst, const uint8_t* p, int have, int load) {
+  if (load == 16) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(p) : "memory");
+  } else if (load == 8) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+      if (i < have) cp_async_8(smem_u32(dst + i), p + i);
   } else if (load == 4) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (at + 4 * i < have) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+    for (int i = 0; i < 16; i += 4)
+      if (i < have) cp_async_4(smem_u32(dst + i), p + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (at + i < have) w[i >> 2] = (w[i >> 2] & ~(0xffu << 8 * (i & 3))) | static_cast<uint32_t>(p[i]) << 8 * (i & 3);
+    for (int i = 0; i < 16; ++i)
+      if (i < have) dst[i] = p[i];
   }
-  return make_uint2(w[0], w[1]);
 }
 
 // ---------------------------------------------------------------- epilogue
@@ -264,7 +273,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kMaxStages], bar_empty[kMaxStages], bar_accfull[2], bar_accempty[2],
       bar_drain;
-  __shared__ int s_off[kMaxGroups + 1], s_pre[kMaxGroups + 1], s_tot[64];
+  __shared__ int s_tot[64];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
 
@@ -276,7 +285,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
   const int stages = a.stages;
   const uint32_t scale_base = ring + stages * a.stage_bytes;  // [stage][W's rows, columns 0-127, columns 128 on]
   unsigned char* scale_ptr = ring_ptr + stages * a.stage_bytes;
-  unsigned char* epi_ptr = scale_ptr + stages * kScaleBytes;
+  unsigned char* unit_ptr = scale_ptr + stages * kScaleBytes;
+  unsigned char* epi_ptr = unit_ptr + kUnitBytes;
+  int* const s_off = reinterpret_cast<int*>(epi_ptr + epilogue_bytes8(GATED));
+  int* const s_pre = s_off + a.l.groups + 1;
   // (a warp turns its chunk after the swap, when its partner has read)
   const auto turn_of = [&](int ew) { return reinterpret_cast<uint32_t*>(epi_ptr + ew * epi_stride(GATED)); };
   const auto swap_of = [&](int ew) { return reinterpret_cast<float*>(turn_of(ew)); };
@@ -286,7 +298,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
 
   if (tid == 0) {
     for (int i = 0; i < stages; ++i) {
-      mbar_init(&bar_full[i], 1 + 2 * kCtas);  // the loads, and the scale warps of both CTAs
+      mbar_init(&bar_full[i], 1 + kScaleWarps * kCtas);  // the loads, and the scale warps of both CTAs
       mbar_init(&bar_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -401,56 +413,78 @@ __global__ void __launch_bounds__(kThreads8, 1)
     __syncwarp();
     volatile int never = 0;
     wait_or_abort(&bar_drain, 0, &never, nullptr);
-  } else if (warp < kEpiWarp0) {
+  } else if (warp >= kScaleWarp0 && warp < kEpi0) {
     // ============================================================== scales
-    // 128 rows at a time: W's and the columns from 128 on (warps 2 here and 1
-    // of a pair's second CTA do nothing else), the first 128 columns (warp 3)
+    // Half of an atom a warp (atom: W's 128 rows, the first 128 columns, the
+    // others).  A lane's two rows come as 16 bytes, two stages' worth, with
+    // cp.async into its own places, one such unit ahead (also of the next
+    // tile); with each stage their words go side by side to where tcgen05.cp
+    // takes them.
     const Linear8Args& l = a.l;
     const int blocks = l.k / kBlock8, cap = static_cast<int>(l.rows) - 1;
-    int st = 0, ph = 0;
-    bool ok = warp >= 2;
+    const int atom = (warp - kScaleWarp0) >> 1, half = (warp - kScaleWarp0) & 1, load = atom == 0 ? a.w_load : a.x_load;
+    unsigned char* const own = unit_ptr + (warp - kScaleWarp0) * kUnits * 1024 + lane * 16;
+    const auto place = [&](int slot, int i) { return own + (slot * 2 + i) * 512; };
+    const auto some = [&](const Tile8& t) { return atom < 2 || t.n > 128; };
+    const uint8_t* p[2];  // rows of the tile being fetched
+    int f_idx = unit, f_unit = 0, f_end = 0, f_slot = 0;
+    bool f_some = false;
+    const auto f_tile = [&]() {
+      if (f_idx >= tiles) return;
+      const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, f_idx, rank);
+      f_unit = t.kb0 / 2;
+      f_end = (t.kb1 + 1) / 2;
+      f_some = some(t);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // past the last row, that one: no result is of it
+        const int r = (half * 2 + i) * 32 + lane;
+        if (atom == 0) {
+          const int up = GATED ? l.n / 2 : l.n, f = GATED ? t.m0 + (r & 63) : t.m0 + r;
+          const int64_t row = min(f, up - 1) + (GATED && r >= 64 ? up : 0);
+          p[i] = l.w_scales + t.e * l.w_scales_group_stride + row * l.w_scales_stride;
+        } else {
+          p[i] = l.x_scales + static_cast<int64_t>(min(t.c0 + (atom - 1) * 128 + r, cap)) * l.x_scales_stride;
+        }
+      }
+    };
+    const auto fetch = [&]() {  // the next unit, if there is one
+      while (f_idx < tiles && f_unit >= f_end) {
+        f_idx += units;
+        f_tile();
+      }
+      if (f_idx < tiles) {
+        const int at = f_unit * 16;
+        if (f_some) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) fetch_scales(place(f_slot, i), p[i] + at, blocks - at, load);
+        }
+        ++f_unit;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      f_slot = f_slot + 1 == kUnits ? 0 : f_slot + 1;
+    };
+    f_tile();
+#pragma unroll
+    for (int i = 0; i < kUnits - 1; ++i) fetch();
+    int st = 0, ph = 0, slot = kUnits - 1;
+    bool ok = true;
     for (int idx = unit; idx < tiles && ok; idx += units) {
       const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
-      const int atoms = warp == 2 && t.n > 128 ? 2 : 1;
-      // this lane's rows; past the last one, that one (no result is of it)
-      const uint8_t* p[2][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 32 + lane, half = GATED ? l.n / 2 : l.n, f = GATED ? t.m0 + (r & 63) : t.m0 + r;
-        const int64_t row = min(f, half - 1) + (GATED && r >= 64 ? half : 0);
-        const auto column = [&](int c) { return l.x_scales + static_cast<int64_t>(min(t.c0 + c, cap)) * l.x_scales_stride; };
-        p[0][i] = warp == 2 ? l.w_scales + t.e * l.w_scales_group_stride + row * l.w_scales_stride : column(r);
-        p[1][i] = column(128 + r);
-      }
-      // a stage's, the next one's on their way
-      uint2 now[2][4], then[2][4];
-      const auto fetch = [&](int b) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (g < atoms && b < t.kb1) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              then[g][i] = load_scales(p[g][i], b * (kBK8 / kBlock8), blocks, warp == 2 && g == 0 ? a.w_load : a.x_load);
-          }
-        }
-      };
-      fetch(t.kb0);
+      const bool mine = some(t);
       for (int b = t.kb0; b < t.kb1; ++b) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) now[g][i] = then[g][i];
+        if (b == t.kb0 || b % 2 == 0) {  // the next unit
+          fetch();
+          asm volatile("cp.async.wait_group %0;" ::"n"(kUnits - 1) : "memory");
+          slot = slot + 1 == kUnits ? 0 : slot + 1;
         }
-        fetch(b + 1);
+        // a stage's scales of the two rows
+        const uint2 v0 = *reinterpret_cast<const uint2*>(place(slot, 0) + b % 2 * 8);
+        const uint2 v1 = *reinterpret_cast<const uint2*>(place(slot, 1) + b % 2 * 8);
         if (!(ok = warp_wait(&bar_empty[st], ph ^ 1, &s_abort, err))) break;
-        unsigned char* dst = scale_ptr + st * kScaleBytes + (warp == 2 ? 0 : kAtomBytes) + lane * 16;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (g < atoms) {
-            *reinterpret_cast<uint4*>(dst + g * 2 * kAtomBytes) = make_uint4(now[g][0].x, now[g][1].x, now[g][2].x, now[g][3].x);
-            *reinterpret_cast<uint4*>(dst + g * 2 * kAtomBytes + kPieceScales) =
-                make_uint4(now[g][0].y, now[g][1].y, now[g][2].y, now[g][3].y);
-          }
+        if (mine) {
+          unsigned char* dst = scale_ptr + st * kScaleBytes + atom * kAtomBytes + lane * 16 + half * 8;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(v0.x, v1.x);
+          *reinterpret_cast<uint2*>(dst + kPieceScales) = make_uint2(v0.y, v1.y);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -461,11 +495,12 @@ __global__ void __launch_bounds__(kThreads8, 1)
         next(st, ph);
       }
     }
-  } else if (PAIR || a.split <= 1) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (warp >= kEpi0 && (PAIR || a.split <= 1)) {
     // ============================================================ epilogue
     // 16 columns at a time (gated: 32), the warps of a lane quarter in turn
     constexpr int kChunk = GATED ? 32 : 16, kStep = kEpi8 / 4 * kChunk;
-    const int ew = warp - kEpiWarp0, q = warp & 3, turn2 = ew >> 2;
+    const int ew = warp - kEpi0, q = warp & 3, turn2 = ew >> 2;
     const Finish8<GATED, BF16, EIGHT> fin(a.l, turn_of(ew), lane);
     int it = 0;
     for (int idx = unit; idx < tiles; idx += units, ++it) {
@@ -544,7 +579,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
         if (lane == 0) arrive_at(release);
       }
     }
-  } else {
+  } else if (warp >= kEpi0) {
     // =========================== K split: this CTA's accumulator is ready
     if (unit < tiles) warp_wait(&bar_accfull[0], 0, &s_abort, err, a.tile_limit);
     tc_fence_after();
@@ -557,8 +592,8 @@ __global__ void __launch_bounds__(kThreads8, 1)
       // its share of a chunk to the chunk's owner, whose ring is free by then,
       // and the owner adds the shares in rank order: [its chunk][rank][column][lane].
       cluster_sync();
-      const bool epi = warp >= kEpiWarp0 && unit < tiles;
-      const int ew = warp - kEpiWarp0;
+      const bool epi = warp >= kEpi0 && unit < tiles;
+      const int ew = warp - kEpi0;
       Tile8 t{};
       if (epi) t = tile_at8<GATED, PAIR>(a, s_off, s_pre, unit, rank);
       const int chunks = (t.w + 15) / 16;
@@ -620,10 +655,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
       __syncwarp();
     }
   }
-  if (a.l.offsets && warp >= kEpiWarp0) {  // rows of no group: zero
+  if (a.l.offsets && warp >= kEpi0) {  // rows of no group: zero
     const Linear8Args& l = a.l;
     uint16_t *out = static_cast<uint16_t*>(l.y), *pre = static_cast<uint16_t*>(l.preact);
-    const int cols = l.n / (GATED ? 2 : 1), first = tid - kEpiWarp0 * 32;
+    const int cols = l.n / (GATED ? 2 : 1), first = tid - kEpi0 * 32;
     const int64_t head = s_off[0], tail = s_off[l.groups], n = head + (l.rows - tail);
     for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
       const int64_t r = i < head ? i : tail + (i - head);
@@ -671,17 +706,20 @@ int tc8_sm_count() {
 }
 
 constexpr uint32_t stage_bytes8(int part) { return kPieces * (kMPiece + part * kPiece); }
-constexpr int stages8(bool gated, int part) {
-  const int fit = static_cast<int>(ring_budget8(gated) / (stage_bytes8(part) + kScaleBytes));
+constexpr int stages8(bool gated, int part, int groups) {
+  const int fit = static_cast<int>(ring_budget8(gated, groups) / (stage_bytes8(part) + kScaleBytes));
   return fit < kMaxStages ? fit : kMaxStages;
 }
-constexpr size_t smem8(bool gated, int part) {
-  return 1024 + static_cast<size_t>(stages8(gated, part)) * (stage_bytes8(part) + kScaleBytes) + epilogue_bytes8(gated);
+constexpr size_t smem8(bool gated, int part, int groups) {
+  return 1024 + static_cast<size_t>(stages8(gated, part, groups)) * (stage_bytes8(part) + kScaleBytes) + kUnitBytes +
+         epilogue_bytes8(gated) + table_bytes(groups);
 }
-// As in linear_tc.cu: no two CTAs that use TMEM share an SM.
+// As in linear_tc.cu: no two CTAs that use TMEM share an SM.  (Forms with less than two stages are not taken.)
 constexpr bool one_cta_an_sm8() {
   for (int part = 16; part <= kMaxWidth; part += 16)
-    if (smem8(false, part) < 120 * 1024 || smem8(true, part) < 120 * 1024) return false;
+    for (int groups : {1, kMaxGroups})
+      for (bool gated : {false, true})
+        if (stages8(gated, part, groups) >= 2 && smem8(gated, part, groups) < 120 * 1024) return false;
   return true;
 }
 static_assert(one_cta_an_sm8(), "tcgen05.alloc would wait for the CTA beside");
@@ -689,7 +727,7 @@ static_assert(one_cta_an_sm8(), "tcgen05.alloc would wait for the CTA beside");
 // Bytes of scale rows that one load may take: the rows' alignment allows it,
 // and rows are whole loads, so that none passes the last row's end.
 int scale_load(const void* p, int64_t stride, int64_t group_stride, int k) {
-  for (int n = 8; n > 2; n /= 2)
+  for (int n = 16; n > 2; n /= 2)
     if (reinterpret_cast<uintptr_t>(p) % n == 0 && stride % n == 0 && group_stride % n == 0 &&
         k / kBlock8 % n == 0)
       return n;
@@ -772,6 +810,7 @@ Plan8 choose_plan8(const Linear8Args& l, bool gated, int sms, int form) {
   for (int w : kWidths) {
     for (int pair = 0; pair < 2; ++pair) {
       if (pair && w < 64) continue;  // a pair's CTAs hold at least 32 columns each
+      if (stages8(gated, pair ? w / 2 : w, l.groups) < 2) continue;
       if (form == (pair ? kFormOne : kFormPair)) continue;
       const Plan8 q = make_plan8(l, gated, sms, pair, w, 1);
       if (form != kFormSplit && (best.cycles == 0 || q.cycles < best.cycles)) best = q;
@@ -811,10 +850,10 @@ cudaError_t launch_linear8_tc(const Linear8Args& l, int form, cudaStream_t st) {
   a.w_load = scale_load(l.w_scales, l.w_scales_stride, l.groups > 1 ? l.w_scales_group_stride : 0, l.k);
   a.x_load = scale_load(l.x_scales, l.x_scales_stride, 0, l.k);
   a.tile_limit = kWaitLimitCycles + 2048ll * ((l.k + kBK8 - 1) / kBK8);
-  a.stages = stages8(gated, a.part);
+  a.stages = stages8(gated, a.part, l.groups);
   const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
   const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
-  const size_t smem = smem8(gated, a.part);
+  const size_t smem = smem8(gated, a.part, l.groups);
 
   // two elements a 16-bit unit of the maps: [unit, row, gate or up, piece, group]
   CUtensorMap tm{}, tn{}, half{};
