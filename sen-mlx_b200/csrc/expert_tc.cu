@@ -839,6 +839,20 @@ cudaError_t make_tmap_4d(CUtensorMap* map, const void* base, const uint64_t (&di
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t make_tmap_bytes_4d(CUtensorMap* map, const void* base, const uint64_t (&dims)[4],
+                               const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4]) {
+  auto enc = tmap_encoder();
+  if (!enc) return cudaErrorNotSupported;
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+  const cuuint64_t s[3] = {stride_bytes[0], stride_bytes[1], stride_bytes[2]};
+  const cuuint32_t x[4] = {box[0], box[1], box[2], box[3]};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), d, s, x, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 cudaError_t make_tmap_5d(CUtensorMap* map, const void* base, const uint64_t (&dims)[5],
                          const uint64_t (&stride_bytes)[4], const uint32_t (&box)[5]) {
   auto enc = tmap_encoder();

@@ -216,6 +216,9 @@ cudaError_t make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType
 // A 4-D tensor map of 16-bit elements with SWIZZLE_128B, innermost dimension first.
 cudaError_t make_tmap_4d(CUtensorMap* map, const void* base, const uint64_t (&dims)[4],
                          const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4]);
+// bytes, not swizzled
+cudaError_t make_tmap_bytes_4d(CUtensorMap* map, const void* base, const uint64_t (&dims)[4],
+                               const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4]);
 cudaError_t make_tmap_5d(CUtensorMap* map, const void* base, const uint64_t (&dims)[5],
                          const uint64_t (&stride_bytes)[4], const uint32_t (&box)[5]);
 // x_sorted[s - s0, :] = fp16(x[perm[s] / k_div, :]) for s < num_slots (x bf16, rows of

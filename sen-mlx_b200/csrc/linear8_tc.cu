@@ -51,7 +51,7 @@ constexpr uint32_t kPieceScales = 3 * kAtomBytes;  // W's rows, then up to 256 c
 constexpr uint32_t kScaleBytes = kPieces * kPieceScales;
 // Scales on their way: units of two stages, 16 bytes a row, 128 rows three times.
 constexpr int kUnits = 2;
-constexpr uint32_t kUnitAtom = 128 * 16, kUnitBytes = kUnits * 3 * kUnitAtom;
+constexpr uint32_t kUnitAtom = 128 * 16, kUnitBytes = kUnits * 3 * kUnitAtom;  // [unit][W, columns 0-127, 128 on][row]
 // Warps: 0 the loads, 1 the MMAs, 2 to 7 the scales, the others the epilogue.
 // With 8 epilogue warps, two a scheduler, it waited for its own latencies
 // (8192 rows of 2048 -> 8192 gelu 200 us); with 2 warps for the scales, whose
@@ -60,18 +60,22 @@ constexpr uint32_t kUnitAtom = 128 * 16, kUnitBytes = kUnits * 3 * kUnitAtom;
 constexpr int kScaleWarp0 = 2, kScaleWarps = 6, kEpi0 = kScaleWarp0 + kScaleWarps;
 constexpr int kEpi8 = 12, kThreads8 = (kEpi0 + kEpi8) * 32;
 static_assert(kEpi0 % 4 == 0);  // an epilogue warp's number gives its quarter of the lanes
-// An epilogue warp's shared memory: where it turns a chunk, and (gated) swaps one before.
-constexpr uint32_t epi_stride(bool gated) { return gated ? kSwapBytes : kTurnBytes; }
-static_assert(kSwapBytes >= kTurnBytes);
-constexpr uint32_t kStaticBytes8 = 1024 + 1024;  // barriers; the ring's alignment
+// An epilogue warp's shared memory: 16 columns of 32 features in fp32 where a
+// gated pair swaps them or 8 bits are made of them, else a turning buffer.
+constexpr uint32_t epi_stride(bool words) { return words ? kSwapBytes : kTurnBytes; }
+static_assert(kSwapBytes == 16 * 32 * 4 && kSwapBytes >= kTurnBytes);
+constexpr int kTileCache = 64;  // of a CTA's tiles in shared memory
+constexpr uint32_t kStaticBytes8 = kTileCache * 32 + 1024 + 1024;  // tiles and barriers; the ring's alignment
 constexpr uint32_t table_bytes(int groups) { return (2 * (groups + 1) * 4 + 15) & ~15; }  // row groups' offsets and chunks
-constexpr uint32_t epilogue_bytes8(bool gated) { return kEpi8 * epi_stride(gated); }
-constexpr uint32_t ring_budget8(bool gated, int groups) {
-  return 227 * 1024 - kStaticBytes8 - table_bytes(groups) - epilogue_bytes8(gated) - kUnitBytes;
+constexpr uint32_t epilogue_bytes8(bool words) { return kEpi8 * epi_stride(words); }
+constexpr uint32_t ring_budget8(bool words, int groups) {
+  return 227 * 1024 - kStaticBytes8 - table_bytes(groups) - epilogue_bytes8(words) - kUnitBytes;
 }
 
 __device__ int g_linear8_error;  // first device error of these kernels on this device
 __device__ int g_linear8_taken;  // what the last check found there
+
+constexpr int kScaleMap = 0;
 
 struct Tc8Args {
   Linear8Args l;
@@ -79,7 +83,7 @@ struct Tc8Args {
   int m_tiles, stages, split;
   uint32_t stage_bytes;  // a stage's operands: W's pieces, then the columns'
   int pieces;            // rows are whole pieces, which the maps have as a dimension
-  int w_load, x_load;    // bytes of a scale row in one copy: 16, 8, 4 or 1
+  int w_load, x_load;    // bytes of a scale row in one copy: 16, 8, 4 or 1; kScaleMap: by TMA
   long long tile_limit;  // of the wait for a tile's accumulators, cycles
 };
 
@@ -146,16 +150,26 @@ __device__ __forceinline__ void load_stage(uint32_t dst, uint32_t piece_bytes, c
   }
 }
 
+// TMA load of scale rows into this CTA's shared memory.
+__device__ __forceinline__ void tma_scales(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // ------------------------------------------------------------------ tiles
-struct Tile8 {
+struct __align__(16) Tile8 {
   int e;         // group
   int m0;        // this CTA's first feature
   int c0, w, n;  // first column (a row of x), columns, columns of the MMA
   int kb0, kb1;  // this CTA's k blocks
+  int unused;
 };
 
 template <bool GATED, bool PAIR>
-__device__ __forceinline__ Tile8 tile_at8(const Tc8Args& a, const int* s_off, const int* s_pre, int idx, int rank) {
+__device__ __forceinline__ Tile8 find_tile8(const Tc8Args& a, const int* s_off, const int* s_pre, int idx, int rank) {
   constexpr int kFeat = GATED ? 64 : 128, kStep = PAIR ? 32 : 16;
   Tile8 t;
   const int mt = idx % a.m_tiles, rest = idx / a.m_tiles;
@@ -202,23 +216,38 @@ __device__ __forceinline__ void fetch_scales(unsigned char* dst, const uint8_t* 
 
 // ---------------------------------------------------------------- epilogue
 // 16 columns x 32 features, a feature a lane -> 8 bits: each column's 32
-// values are one block of a row of y.
+// values are one block of a row of y.  They are turned in shared memory (16-byte
+// pieces of a column in an order of its own, against bank conflicts), after
+// which a lane has 16 features of a column.  (With a warp reduction a column the
+// block's largest cost three times the instructions.)
 __device__ __forceinline__ void store_chunk8(const float (&v)[16], uint32_t* turn, uint8_t* codes, int64_t stride,
                                              uint8_t* scales, int64_t scales_stride, int w, int lane) {
-  uint8_t* t8 = reinterpret_cast<uint8_t*>(turn);
-  uint32_t mine = 0;
+  float* t = reinterpret_cast<float*>(turn);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    uint32_t byte;
-    t8[i * 32 + lane] = pack8_warp(v[i], byte);
-    if (lane == i) mine = byte;
-  }
+  for (int i = 0; i < 16; ++i) t[i * 32 + ((lane >> 2) ^ (i & 7)) * 4 + (lane & 3)] = v[i];
   __syncwarp();
   const int c = lane >> 1, half = lane & 1;
-  const uint4 q = *reinterpret_cast<const uint4*>(t8 + c * 32 + half * 16);
+  float f[16];
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float4 q = *reinterpret_cast<const float4*>(t + c * 32 + ((half * 4 + k) ^ (c & 7)) * 4);
+    f[4 * k] = q.x; f[4 * k + 1] = q.y; f[4 * k + 2] = q.z; f[4 * k + 3] = q.w;
+  }
   __syncwarp();
-  if (c < w) *reinterpret_cast<uint4*>(codes + c * stride + half * 16) = q;
-  if (lane < w && lane < 16) scales[lane * scales_stride] = static_cast<uint8_t>(mine);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max(m, magnitude(f[i]));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  const uint32_t byte = scale_byte(m);
+  const float inv = scale_inverse(byte);
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = to_e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv);
+  if (c < w) {
+    *reinterpret_cast<uint4*>(codes + c * stride + half * 16) =
+        make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+    if (half == 0) scales[c * scales_stride] = static_cast<uint8_t>(byte);
+  }
 }
 
 // What a warp needs to finish a tile's accumulators.
@@ -268,12 +297,14 @@ template <bool GATED, bool BF16, bool EIGHT> struct Finish8 {
 template <bool GATED, bool BF16, bool PAIR, bool EIGHT>
 __global__ void __launch_bounds__(kThreads8, 1)
     linear8_tc_kernel(const __grid_constant__ CUtensorMap tm_m, const __grid_constant__ CUtensorMap tm_n,
-                      const __grid_constant__ CUtensorMap tm_half, const __grid_constant__ Tc8Args a) {
+                      const __grid_constant__ CUtensorMap tm_half, const __grid_constant__ CUtensorMap tm_sw,
+                      const __grid_constant__ CUtensorMap tm_sx, const __grid_constant__ Tc8Args a) {
   constexpr int kCtas = PAIR ? 2 : 1;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kMaxStages], bar_empty[kMaxStages], bar_accfull[2], bar_accempty[2],
-      bar_drain;
+      bar_ufull[2][kUnits], bar_uempty[2][kUnits], bar_drain;
   __shared__ int s_tot[64];
+  __shared__ Tile8 s_tile[kTileCache];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
 
@@ -287,10 +318,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
   unsigned char* scale_ptr = ring_ptr + stages * a.stage_bytes;
   unsigned char* unit_ptr = scale_ptr + stages * kScaleBytes;
   unsigned char* epi_ptr = unit_ptr + kUnitBytes;
-  int* const s_off = reinterpret_cast<int*>(epi_ptr + epilogue_bytes8(GATED));
+  int* const s_off = reinterpret_cast<int*>(epi_ptr + epilogue_bytes8(GATED || EIGHT));
   int* const s_pre = s_off + a.l.groups + 1;
   // (a warp turns its chunk after the swap, when its partner has read)
-  const auto turn_of = [&](int ew) { return reinterpret_cast<uint32_t*>(epi_ptr + ew * epi_stride(GATED)); };
+  const auto turn_of = [&](int ew) { return reinterpret_cast<uint32_t*>(epi_ptr + ew * epi_stride(GATED || EIGHT)); };
   const auto swap_of = [&](int ew) { return reinterpret_cast<float*>(turn_of(ew)); };
   const int csize = PAIR ? 2 : a.split;  // CTAs of the cluster
   const int rank = csize > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -304,6 +335,12 @@ __global__ void __launch_bounds__(kThreads8, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_accfull[i], 1);
       mbar_init(&bar_accempty[i], kCtas * kEpi8);
+    }
+    for (int i = 0; i < kUnits; ++i) {  // W's scales, the columns'
+      mbar_init(&bar_ufull[0][i], 1);
+      mbar_init(&bar_ufull[1][i], 1);
+      mbar_init(&bar_uempty[0][i], 2);
+      mbar_init(&bar_uempty[1][i], 4);
     }
     mbar_init(&bar_drain, 1);
     s_abort = 0;
@@ -324,6 +361,15 @@ __global__ void __launch_bounds__(kThreads8, 1)
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int tiles = a.m_tiles * s_pre[a.l.groups];
+  // The CTA's first tiles, found by a thread each: a search and three divisions
+  // that every role would otherwise make for itself, between a tile and the next.
+  if (tid < kTileCache && unit + tid * units < tiles)
+    s_tile[tid] = find_tile8<GATED, PAIR>(a, s_off, s_pre, unit + tid * units, rank);
+  __syncthreads();
+  const int mine = unit < tiles ? (tiles - unit + units - 1) / units : 0;
+  const auto tile = [&](int it) {
+    return it < kTileCache ? s_tile[it] : find_tile8<GATED, PAIR>(a, s_off, s_pre, unit + it * units, rank);
+  };
   // shared by all roles: the tile's k blocks walk the ring in order
   auto next = [stages](int& st, int& ph) {
     if (++st == stages) { st = 0; ph ^= 1; }
@@ -335,8 +381,8 @@ __global__ void __launch_bounds__(kThreads8, 1)
       uint32_t issued = 0, parity = 0;  // by stage: loaded at least once, parity of the last load
       int st = 0, ph = 0;
       bool ok = true;
-      for (int idx = unit; idx < tiles && ok; idx += units) {
-        const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
+      for (int it = 0; it < mine && ok; ++it) {
+        const Tile8 t = tile(it);
         const int part = t.n / kCtas, col = t.c0 + (PAIR ? rank * part : 0);  // this CTA's share of the columns
         // one load of a full part, or of half of one where that holds the columns
         const bool small = 2 * part <= a.part && a.part >= 32;
@@ -372,9 +418,9 @@ __global__ void __launch_bounds__(kThreads8, 1)
     // ========================================================== MMA issuer
     const bool leader = elect_one();
     bool ok = true;
-    int st = 0, ph = 0, it = 0;
-    for (int idx = unit; idx < tiles && ok; idx += units, ++it) {
-      const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
+    int st = 0, ph = 0;
+    for (int it = 0; it < mine && ok; ++it) {
+      const Tile8 t = tile(it);
       const int ab = it & 1, aph = (it >> 1) & 1;
       if (!(ok = warp_wait(&bar_accempty[ab], aph ^ 1, &s_abort, err))) break;
       tc_fence_after();
@@ -416,72 +462,86 @@ __global__ void __launch_bounds__(kThreads8, 1)
   } else if (warp >= kScaleWarp0 && warp < kEpi0) {
     // ============================================================== scales
     // Half of an atom a warp (atom: W's 128 rows, the first 128 columns, the
-    // others).  A lane's two rows come as 16 bytes, two stages' worth, with
-    // cp.async into its own places, one such unit ahead (also of the next
-    // tile); with each stage their words go side by side to where tcgen05.cp
-    // takes them.
+    // others).  Rows come as 16 bytes, two stages' worth, one such unit ahead
+    // (also of the next tile): by TMA where their strides allow a map (a.maps),
+    // else each lane its two rows with cp.async.  With each stage a lane lays
+    // its rows' words side by side to where tcgen05.cp takes them.
     const Linear8Args& l = a.l;
     const int blocks = l.k / kBlock8, cap = static_cast<int>(l.rows) - 1;
-    const int atom = (warp - kScaleWarp0) >> 1, half = (warp - kScaleWarp0) & 1, load = atom == 0 ? a.w_load : a.x_load;
-    unsigned char* const own = unit_ptr + (warp - kScaleWarp0) * kUnits * 1024 + lane * 16;
-    const auto place = [&](int slot, int i) { return own + (slot * 2 + i) * 512; };
+    const int atom = (warp - kScaleWarp0) >> 1, half = (warp - kScaleWarp0) & 1, side = atom > 0;
+    const bool maps = side ? a.x_load == kScaleMap : a.w_load == kScaleMap;
+    const bool lead = lane == 0 && (warp == kScaleWarp0 || warp == kScaleWarp0 + 2);  // issues a side's loads
+    const auto place = [&](int slot, int i) {
+      return unit_ptr + (slot * 3 + atom) * kUnitAtom + ((half * 2 + i) * 32 + lane) * 16;
+    };
     const auto some = [&](const Tile8& t) { return atom < 2 || t.n > 128; };
-    const uint8_t* p[2];  // rows of the tile being fetched
-    int f_idx = unit, f_unit = 0, f_end = 0, f_slot = 0;
-    bool f_some = false;
-    const auto f_tile = [&]() {
-      if (f_idx >= tiles) return;
-      const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, f_idx, rank);
-      f_unit = t.kb0 / 2;
-      f_end = (t.kb1 + 1) / 2;
-      f_some = some(t);
+    bool ok = true;
+    Tile8 f{};               // the tile being fetched
+    const uint8_t* p[2];     // cp.async: this lane's rows of it
+    int f_it = -1, f_unit = 0, f_end = 0, f_count = 0;
+    const auto fetch = [&]() {  // the next unit, if there is one
+      while (f_unit >= f_end && f_it < mine) {
+        if (++f_it == mine) break;
+        f = tile(f_it);
+        f_unit = f.kb0 / 2;
+        f_end = (f.kb1 + 1) / 2;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {  // past the last row, that one: no result is of it
-        const int r = (half * 2 + i) * 32 + lane;
-        if (atom == 0) {
-          const int up = GATED ? l.n / 2 : l.n, f = GATED ? t.m0 + (r & 63) : t.m0 + r;
-          const int64_t row = min(f, up - 1) + (GATED && r >= 64 ? up : 0);
-          p[i] = l.w_scales + t.e * l.w_scales_group_stride + row * l.w_scales_stride;
-        } else {
-          p[i] = l.x_scales + static_cast<int64_t>(min(t.c0 + (atom - 1) * 128 + r, cap)) * l.x_scales_stride;
+        for (int i = 0; i < 2; ++i) {  // past the last row, that one: no result is of it
+          const int r = (half * 2 + i) * 32 + lane;
+          if (atom == 0) {
+            const int up = GATED ? l.n / 2 : l.n, row = min(GATED ? f.m0 + (r & 63) : f.m0 + r, up - 1) + (GATED && r >= 64 ? up : 0);
+            p[i] = l.w_scales + f.e * l.w_scales_group_stride + row * l.w_scales_stride;
+          } else {
+            p[i] = l.x_scales + static_cast<int64_t>(min(f.c0 + (atom - 1) * 128 + r, cap)) * l.x_scales_stride;
+          }
         }
       }
-    };
-    const auto fetch = [&]() {  // the next unit, if there is one
-      while (f_idx < tiles && f_unit >= f_end) {
-        f_idx += units;
-        f_tile();
-      }
-      if (f_idx < tiles) {
-        const int at = f_unit * 16;
-        if (f_some) {
+      if (f_it < mine) {
+        const int slot = f_count % kUnits, at = f_unit * 16;
+        if (!maps) {
+          if (some(f)) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) fetch_scales(place(f_slot, i), p[i] + at, blocks - at, load);
+            for (int i = 0; i < 2; ++i) fetch_scales(place(slot, i), p[i] + at, blocks - at, side ? a.x_load : a.w_load);
+          }
+        } else if (lead && ok) {
+          uint64_t* full = &bar_ufull[side][slot];
+          ok = wait_or_abort(&bar_uempty[side][slot], (f_count / kUnits & 1) ^ 1, &s_abort, err);
+          if (ok) {
+            unsigned char* dst = unit_ptr + (slot * 3 + side) * kUnitAtom;
+            mbar_arrive_expect_tx(full, side ? a.bn * 16 : kUnitAtom);
+            if (side) tma_scales(dst, &tm_sx, at, f.c0, 0, 0, full);
+            else tma_scales(dst, &tm_sw, at, f.m0, 0, f.e, full);
+          }
         }
         ++f_unit;
+        ++f_count;
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      f_slot = f_slot + 1 == kUnits ? 0 : f_slot + 1;
+      if (!maps) asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    f_tile();
 #pragma unroll
     for (int i = 0; i < kUnits - 1; ++i) fetch();
-    int st = 0, ph = 0, slot = kUnits - 1;
-    bool ok = true;
-    for (int idx = unit; idx < tiles && ok; idx += units) {
-      const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
-      const bool mine = some(t);
+    int st = 0, ph = 0, count = -1;
+    for (int it = 0; it < mine && ok; ++it) {
+      const Tile8 t = tile(it);
+      const bool used = some(t);
       for (int b = t.kb0; b < t.kb1; ++b) {
-        if (b == t.kb0 || b % 2 == 0) {  // the next unit
+        const bool first = b == t.kb0 || b % 2 == 0, last = b + 1 == t.kb1 || b % 2 == 1;  // of a unit
+        if (first) {
+          ++count;
           fetch();
-          asm volatile("cp.async.wait_group %0;" ::"n"(kUnits - 1) : "memory");
-          slot = slot + 1 == kUnits ? 0 : slot + 1;
+          if (!maps) asm volatile("cp.async.wait_group %0;" ::"n"(kUnits - 1) : "memory");
+          else ok = warp_wait(&bar_ufull[side][count % kUnits], count / kUnits & 1, &s_abort, err) && __all_sync(0xffffffffu, ok);
+          if (!ok) break;
         }
         // a stage's scales of the two rows
-        const uint2 v0 = *reinterpret_cast<const uint2*>(place(slot, 0) + b % 2 * 8);
-        const uint2 v1 = *reinterpret_cast<const uint2*>(place(slot, 1) + b % 2 * 8);
+        const uint2 v0 = *reinterpret_cast<const uint2*>(place(count % kUnits, 0) + b % 2 * 8);
+        const uint2 v1 = *reinterpret_cast<const uint2*>(place(count % kUnits, 1) + b % 2 * 8);
+        if (last && maps) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_uempty[side][count % kUnits]);
+        }
         if (!(ok = warp_wait(&bar_empty[st], ph ^ 1, &s_abort, err))) break;
-        if (mine) {
+        if (used) {
           unsigned char* dst = scale_ptr + st * kScaleBytes + atom * kAtomBytes + lane * 16 + half * 8;
           *reinterpret_cast<uint2*>(dst) = make_uint2(v0.x, v1.x);
           *reinterpret_cast<uint2*>(dst + kPieceScales) = make_uint2(v0.y, v1.y);
@@ -495,16 +555,19 @@ __global__ void __launch_bounds__(kThreads8, 1)
         next(st, ph);
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!maps) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (lead && maps && !ok) {  // gave up: loads already issued get a bounded chance to land
+      volatile int never = 0;
+      for (int i = max(count, 0); i < f_count; ++i) wait_or_abort(&bar_ufull[side][i % kUnits], i / kUnits & 1, &never, nullptr);
+    }
   } else if (warp >= kEpi0 && (PAIR || a.split <= 1)) {
     // ============================================================ epilogue
     // 16 columns at a time (gated: 32), the warps of a lane quarter in turn
     constexpr int kChunk = GATED ? 32 : 16, kStep = kEpi8 / 4 * kChunk;
     const int ew = warp - kEpi0, q = warp & 3, turn2 = ew >> 2;
     const Finish8<GATED, BF16, EIGHT> fin(a.l, turn_of(ew), lane);
-    int it = 0;
-    for (int idx = unit; idx < tiles; idx += units, ++it) {
-      const Tile8 t = tile_at8<GATED, PAIR>(a, s_off, s_pre, idx, rank);
+    for (int it = 0; it < mine; ++it) {
+      const Tile8 t = tile(it);
       const int ab = it & 1, aph = (it >> 1) & 1;
       // a gated pair: quarters 0, 1 hold the gate of features 32 (q & 1) on, 2, 3 the up
       const int f0 = t.m0 + (GATED ? q & 1 : q) * 32, feats = min(32, fin.cols - f0);
@@ -581,7 +644,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
     }
   } else if (warp >= kEpi0) {
     // =========================== K split: this CTA's accumulator is ready
-    if (unit < tiles) warp_wait(&bar_accfull[0], 0, &s_abort, err, a.tile_limit);
+    if (mine > 0) warp_wait(&bar_accfull[0], 0, &s_abort, err, a.tile_limit);
     tc_fence_after();
   }
 
@@ -592,10 +655,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
       // its share of a chunk to the chunk's owner, whose ring is free by then,
       // and the owner adds the shares in rank order: [its chunk][rank][column][lane].
       cluster_sync();
-      const bool epi = warp >= kEpi0 && unit < tiles;
+      const bool epi = warp >= kEpi0 && mine > 0;
       const int ew = warp - kEpi0;
       Tile8 t{};
-      if (epi) t = tile_at8<GATED, PAIR>(a, s_off, s_pre, unit, rank);
+      if (epi) t = tile(0);
       const int chunks = (t.w + 15) / 16;
       if (epi) {
         const int q = warp & 3;
@@ -706,20 +769,20 @@ int tc8_sm_count() {
 }
 
 constexpr uint32_t stage_bytes8(int part) { return kPieces * (kMPiece + part * kPiece); }
-constexpr int stages8(bool gated, int part, int groups) {
-  const int fit = static_cast<int>(ring_budget8(gated, groups) / (stage_bytes8(part) + kScaleBytes));
+constexpr int stages8(bool words, int part, int groups) {
+  const int fit = static_cast<int>(ring_budget8(words, groups) / (stage_bytes8(part) + kScaleBytes));
   return fit < kMaxStages ? fit : kMaxStages;
 }
-constexpr size_t smem8(bool gated, int part, int groups) {
-  return 1024 + static_cast<size_t>(stages8(gated, part, groups)) * (stage_bytes8(part) + kScaleBytes) + kUnitBytes +
-         epilogue_bytes8(gated) + table_bytes(groups);
+constexpr size_t smem8(bool words, int part, int groups) {
+  return 1024 + static_cast<size_t>(stages8(words, part, groups)) * (stage_bytes8(part) + kScaleBytes) + kUnitBytes +
+         epilogue_bytes8(words) + table_bytes(groups);
 }
 // As in linear_tc.cu: no two CTAs that use TMEM share an SM.  (Forms with less than two stages are not taken.)
 constexpr bool one_cta_an_sm8() {
   for (int part = 16; part <= kMaxWidth; part += 16)
     for (int groups : {1, kMaxGroups})
-      for (bool gated : {false, true})
-        if (stages8(gated, part, groups) >= 2 && smem8(gated, part, groups) < 120 * 1024) return false;
+      for (bool words : {false, true})
+        if (stages8(words, part, groups) >= 2 && smem8(words, part, groups) < 120 * 1024) return false;
   return true;
 }
 static_assert(one_cta_an_sm8(), "tcgen05.alloc would wait for the CTA beside");
@@ -734,9 +797,12 @@ int scale_load(const void* p, int64_t stride, int64_t group_stride, int k) {
   return 1;
 }
 
+struct Maps8 {
+  CUtensorMap w, x, half, sw, sx;
+};
+
 template <bool GATED, bool BF16, bool PAIR, bool EIGHT>
-cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorMap& half, const Tc8Args& a, int grid,
-                     size_t smem, cudaStream_t st) {
+cudaError_t launch_t(const Maps8& m, const Tc8Args& a, int grid, size_t smem, cudaStream_t st) {
   auto kern = linear8_tc_kernel<GATED, BF16, PAIR, EIGHT>;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
@@ -752,7 +818,7 @@ cudaError_t launch_t(const CUtensorMap& m, const CUtensorMap& n, const CUtensorM
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = PAIR || a.split > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, m, n, half, a);
+  return cudaLaunchKernelEx(&cfg, kern, m.w, m.x, m.half, m.sw, m.sx, a);
 }
 
 // The form of a product's tiles and its estimated time in SM cycles.
@@ -810,7 +876,7 @@ Plan8 choose_plan8(const Linear8Args& l, bool gated, int sms, int form) {
   for (int w : kWidths) {
     for (int pair = 0; pair < 2; ++pair) {
       if (pair && w < 64) continue;  // a pair's CTAs hold at least 32 columns each
-      if (stages8(gated, pair ? w / 2 : w, l.groups) < 2) continue;
+      if (stages8(gated || l.codes, pair ? w / 2 : w, l.groups) < 2) continue;
       if (form == (pair ? kFormOne : kFormPair)) continue;
       const Plan8 q = make_plan8(l, gated, sms, pair, w, 1);
       if (form != kFormSplit && (best.cycles == 0 || q.cycles < best.cycles)) best = q;
@@ -847,36 +913,50 @@ cudaError_t launch_linear8_tc(const Linear8Args& l, int form, cudaStream_t st) {
   a.m_tiles = (features + feat - 1) / feat;
   a.part = plan.pair ? a.bn / 2 : a.bn;
   a.stage_bytes = stage_bytes8(a.part);
-  a.w_load = scale_load(l.w_scales, l.w_scales_stride, l.groups > 1 ? l.w_scales_group_stride : 0, l.k);
+  const int64_t sgs = l.groups > 1 ? l.w_scales_group_stride : 0;
+  a.w_load = scale_load(l.w_scales, l.w_scales_stride, sgs, l.k);
   a.x_load = scale_load(l.x_scales, l.x_scales_stride, 0, l.k);
   a.tile_limit = kWaitLimitCycles + 2048ll * ((l.k + kBK8 - 1) / kBK8);
-  a.stages = stages8(gated, a.part, l.groups);
+  a.stages = stages8(gated || l.codes, a.part, l.groups);
   const int csize = plan.pair ? 2 : plan.split, most = sms / csize;
   const int grid = static_cast<int>(plan.tiles < 1 ? 1 : plan.tiles < most ? plan.tiles : most) * csize;
-  const size_t smem = smem8(gated, a.part, l.groups);
+  const size_t smem = smem8(gated || l.codes, a.part, l.groups);
 
   // two elements a 16-bit unit of the maps: [unit, row, gate or up, piece, group]
-  CUtensorMap tm{}, tn{}, half{};
+  Maps8 m{};
   a.pieces = l.k % kPiece == 0;
   const uint64_t w_row = l.w_stride, x_row = l.x_stride, n = features, rows = l.rows;
   const uint64_t units = a.pieces ? kPiece / 2 : l.k / 2, pieces = a.pieces ? l.k / kPiece : 1;
   const uint32_t box = a.pieces ? kPieces : 1;
   const uint64_t gs = l.groups > 1 ? l.w_group_stride : w_row * l.n;
-  cudaError_t e = make_tmap_5d(&tm, l.w, {units, n, gated ? 2u : 1u, pieces, uint64_t(l.groups)},
+  cudaError_t e = make_tmap_5d(&m.w, l.w, {units, n, gated ? 2u : 1u, pieces, uint64_t(l.groups)},
                                {w_row, n * w_row, kPiece, gs}, {kPiece / 2, gated ? 64u : 128u, gated ? 2u : 1u, box, 1});
   const auto columns = [&](CUtensorMap* map, int part) {
     return make_tmap_5d(map, l.x, {units, rows, 1, pieces, 1}, {x_row, x_row, kPiece, x_row},
                         {kPiece / 2, uint32_t(part), 1, box, 1});
   };
-  if (e == cudaSuccess) e = columns(&tn, a.part);
-  half = tn;
-  if (e == cudaSuccess && a.part >= 32) e = columns(&half, a.part / 2);
+  if (e == cudaSuccess) e = columns(&m.x, a.part);
+  m.half = m.x;
+  if (e == cudaSuccess && a.part >= 32) e = columns(&m.half, a.part / 2);
+  // scales: 16 bytes of each row
+  const uint64_t s_row = l.w_scales_stride, blocks = l.k / kBlock8;
+  if (e == cudaSuccess && a.w_load == 16) {
+    e = make_tmap_bytes_4d(&m.sw, l.w_scales, {blocks, n, gated ? 2u : 1u, uint64_t(l.groups)},
+                           {s_row, n * s_row, l.groups > 1 ? uint64_t(sgs) : s_row * l.n},
+                           {16, gated ? 64u : 128u, gated ? 2u : 1u, 1});
+    a.w_load = kScaleMap;
+  }
+  if (e == cudaSuccess && a.x_load == 16) {
+    const uint64_t xs = l.x_scales_stride;
+    e = make_tmap_bytes_4d(&m.sx, l.x_scales, {blocks, rows, 1, 1}, {xs, xs, xs}, {16, uint32_t(a.bn), 1, 1});
+    a.x_load = kScaleMap;
+  }
   if (e != cudaSuccess) return e;
   if (plan.pair)
-    return l.codes ? launch_form<true, true>(gated, l.bf16, tm, tn, half, a, grid, smem, st)
-                   : launch_form<true, false>(gated, l.bf16, tm, tn, half, a, grid, smem, st);
-  return l.codes ? launch_form<false, true>(gated, l.bf16, tm, tn, half, a, grid, smem, st)
-                 : launch_form<false, false>(gated, l.bf16, tm, tn, half, a, grid, smem, st);
+    return l.codes ? launch_form<true, true>(gated, l.bf16, m, a, grid, smem, st)
+                   : launch_form<true, false>(gated, l.bf16, m, a, grid, smem, st);
+  return l.codes ? launch_form<false, true>(gated, l.bf16, m, a, grid, smem, st)
+                 : launch_form<false, false>(gated, l.bf16, m, a, grid, smem, st);
 }
 
 cudaError_t linear8_device_error(cudaStream_t st, int* error) {
