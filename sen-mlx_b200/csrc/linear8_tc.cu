@@ -442,8 +442,9 @@ __global__ void __launch_bounds__(kThreads8, 1)
             copy_scales<PAIR>(sb, sc + i * kPieceScales + kAtomBytes);
             if (t.n > 128) copy_scales<PAIR>(sb + 4, sc + i * kPieceScales + 2 * kAtomBytes);
             const uint64_t dm = smem_desc<false>(sm + i * kMPiece), dn = smem_desc<false>(sn + i * n_piece);
-            for (int s = 0; s < ks; ++s)  // 32 k: 32 bytes along a line
-              umma_scaled<PAIR>(d, dm + s * (32 >> 4), dn + s * (32 >> 4), idesc | (s << 4) | (s << 29), sa, sb,
+#pragma unroll
+            for (int s = 0; s < 4; ++s)  // 32 k: 32 bytes along a line
+              if (s < ks) umma_scaled<PAIR>(d, dm + s * (32 >> 4), dn + s * (32 >> 4), idesc | (s << 4) | (s << 29), sa, sb,
                                 (b > t.kb0 || i > 0 || s > 0) ? 1u : 0u);
           }
           umma_commit<PAIR>(&bar_empty[st]);
