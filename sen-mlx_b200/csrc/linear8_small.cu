@@ -6,11 +6,12 @@
 // rows over their 8 up rows) for one chunk of up to 8 * NT rows of one group;
 // KWARPS warps a tile take runs of kSteps scale blocks (32 k each) in turn.
 // Of a block, thread 4g + t of a warp loads 8 consecutive columns, 8t .. 8t + 7,
-// of W's rows g and g + 8 and of the chunk's rows g, g + 8, ...; an m16n8k32 MMA
-// wants 4 and 4 of them, and as a contraction does not depend on the order of
-// k, what is loaded is the fragment.  Each MMA starts from zero and its sums
-// are added with their scale, 2^(sw + sx), in fp32.  The warps' sums meet in
-// shared memory and are added in warp order: the same bits every time.
+// of W's rows g and g + 8 and of the chunk's rows g, g + 8, ...; as fp16, which
+// holds e4m3, they are the fragments of two m16n8k16 MMAs, since a contraction
+// does not depend on the order of k.  (The m16n8k32 MMA of e4m3 itself took
+// longer: one token's 8 experts 18.3 us against 13.6.)  A scale block's sums
+// start from zero and are added times 2^(sw + sx), in fp32.  The warps' sums
+// meet in shared memory and are added in warp order: the same bits every time.
 //
 // With an 8-bit output a block has 32 features, one scale block of a row of y.
 
@@ -19,13 +20,17 @@
 namespace senmoe {
 namespace {
 
-// D = A B from zero, e4m3 x e4m3, fp32 sums
-__device__ __forceinline__ void mma16832(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+// 4 e4m3 as 2 x 2 fp16 (exact)
+__device__ __forceinline__ void to_f16(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(static_cast<uint16_t>(v)));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(static_cast<uint16_t>(v >> 16)));
+}
+// D += A B, fp16 x fp16, fp32 sums
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-               "{%10,%10,%10,%10};"
-               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // 8 bytes at p, or zeros; W is read once and passes L1 by.
@@ -37,13 +42,11 @@ __device__ __forceinline__ uint2 load_w(const uint8_t* p, bool live) {
 __device__ __forceinline__ uint2 load_x(const uint8_t* p, bool live) {
   return live ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
 }
-// N scales from block b on, `have` blocks in all, one a byte; past the last: 2^0.
+// N scales (4 or 2) from block b on, `have` blocks in all, one a byte; past the last: 2^0.
 template <int N> __device__ __forceinline__ uint32_t load_scales(const uint8_t* p, int b, int have, bool words, bool live) {
   uint32_t v = 0x7f7f7f7fu;
   if (!live || b >= have) return v;
-  if constexpr (N == 4) {
-    if (words) return *reinterpret_cast<const uint32_t*>(p + b);
-  }
+  if (words) return N == 4 ? *reinterpret_cast<const uint32_t*>(p + b) : *reinterpret_cast<const uint16_t*>(p + b);
 #pragma unroll
   for (int i = 0; i < N; ++i)
     if (b + i < have) v = (v & ~(0xffu << 8 * i)) | static_cast<uint32_t>(p[b + i]) << 8 * i;
@@ -59,11 +62,12 @@ template <bool BF16, bool GATED, bool EIGHT, int NT> struct Shape {
   static constexpr int kWarpsK = EIGHT && GATED ? 4 : 8;
   static constexpr int kThreads = 32 * kTiles * kWarpsK;
   static constexpr int kFeat = 16 * kTiles / (GATED ? 2 : 1);  // features of a block
-  static constexpr int kSteps = NT > 2 ? 2 : 4;  // scale blocks whose loads are in flight together
+  static constexpr int kSteps = NT > 4 ? 2 : 4;  // scale blocks whose loads are in flight together
+  static constexpr int kBlocks = NT > 1 ? 1 : 2;  // an SM, at least
 };
 
 template <bool BF16, bool GATED, bool EIGHT, int NT>
-__global__ void __launch_bounds__(Shape<BF16, GATED, EIGHT, NT>::kThreads)
+__global__ void __launch_bounds__(Shape<BF16, GATED, EIGHT, NT>::kThreads, Shape<BF16, GATED, EIGHT, NT>::kBlocks)
     linear8_small_kernel(const __grid_constant__ Linear8Args a, const bool words) {
   using S = Shape<BF16, GATED, EIGHT, NT>;
   constexpr int kWarps = S::kThreads / 32, kFeat = S::kFeat, kSteps = S::kSteps, kChunk = 8 * NT;
@@ -180,10 +184,19 @@ __global__ void __launch_bounds__(Shape<BF16, GATED, EIGHT, NT>::kThreads)
     for (int s = 0; s < kSteps; ++s) {
       if (b + s >= blocks) break;
       const float v0 = scale_value(sw[0], s), v1 = scale_value(sw[1], s);
+      uint32_t a0[4], a1[4];  // rows g and g + 8, in fp16 pairs
+      to_f16(wa[s][0].x, a0[0], a0[1]);
+      to_f16(wa[s][0].y, a0[2], a0[3]);
+      to_f16(wa[s][1].x, a1[0], a1[1]);
+      to_f16(wa[s][1].y, a1[2], a1[3]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float d[4];
-        mma16832(d, wa[s][0].x, wa[s][1].x, wa[s][0].y, wa[s][1].y, xb[s][n].x, xb[s][n].y);
+        uint32_t x[4];
+        to_f16(xb[s][n].x, x[0], x[1]);
+        to_f16(xb[s][n].y, x[2], x[3]);
+        float d[4] = {};
+        mma16816(d, a0[0], a1[0], a0[1], a1[1], x[0], x[1]);
+        mma16816(d, a0[2], a1[2], a0[3], a1[3], x[2], x[3]);
         const float u0 = scale_value(sx[n][0], s), u1 = scale_value(sx[n][1], s);
         acc[n][0] += d[0] * (v0 * u0);
         acc[n][1] += d[1] * (v0 * u1);
