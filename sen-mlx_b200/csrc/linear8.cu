@@ -44,12 +44,20 @@ int check_type(const char* call, int32_t dtype, int32_t epilogue) {
   return SENMOE_OK;
 }
 
+// Whether the few-row kernel is the faster one.  Measured against the tcgen05
+// tiles (us, W from HBM):
+//   dense 2048 x 2048    8 rows 5.4 / 9.6    16 rows 6.4 / 9.6    64 rows 15.1 / 10.0
+//   dense 2816 x 2112    8 rows 6.8 / 9.8    16 rows 8.4 / 9.9    32 rows 11.8 / 9.9
+//   dense 512 x 2048     8 rows 2.7 / 6.2    64 rows 5.6 / 6.5    96 rows 9.6 / 6.6
+//   dense 2048 x 8192    8 rows 12.0 / 11.6  8192 x 2048  1 row 14.8 / 12.6
+// It reads W in pieces of 64 bytes a row, which bounds it at 2 TB/s, and all
+// rows for every 16 features.  Grouped, by what the touched experts hold:
+//   8 x 768 x 2048       14.6 / 9.9    8 x 2048 x 1536  14.7 / 12.7
+//   4 x 2048 x 1536      11.2 / 12.7   8 x 2048 x 512   7.2 / 9.5
 bool few_rows8(const Linear8Args& a) {
-  if (!a.offsets)
-    return a.rows <= 8 || (a.rows <= 64 && static_cast<int64_t>(a.n) * a.k * a.rows <= 400000000);
-  if (a.rows > 64 && a.rows > 4 * a.groups) return false;
-  const int64_t chunks = a.rows < a.groups ? a.rows : a.groups;
-  return chunks * ((a.n + 15) / 16) <= (a.k >= 1024 ? 148 * 40 : 148 * 8);
+  const int64_t weight = static_cast<int64_t>(a.n) * a.k;
+  if (!a.offsets) return a.rows <= 64 && weight * (a.rows > 8 ? a.rows : 8) <= 100000000;
+  return a.rows <= 64 && weight * (a.rows < a.groups ? a.rows : a.groups) <= 10000000;
 }
 
 }  // namespace
