@@ -549,8 +549,8 @@ class GemmaRouter:
     __call__ = forward
 
 
-def dispatch(topk_ids: torch.Tensor, num_experts: int, stream=None):
-    """Expert-contiguous permutation: returns (perm, inverse, offsets, active_list)."""
+def _dispatch(topk_ids: torch.Tensor, num_experts: int, stream=None):
+    """(perm, inverse, offsets, scratch) of senmoe_dispatch, without waiting for it."""
     ids = topk_ids.to(torch.int32).contiguous()
     T, K = ids.shape
     dev = ids.device
@@ -560,6 +560,12 @@ def dispatch(topk_ids: torch.Tensor, num_experts: int, stream=None):
     scratch = torch.zeros(num_experts + 2, dtype=torch.int32, device=dev)
     _check(lib().senmoe_dispatch(_ptr(ids), T, K, num_experts, _ptr(perm), _ptr(inv), _ptr(offs), _ptr(scratch),
                                  _stream(stream)))
+    return perm, inv, offs, scratch
+
+
+def dispatch(topk_ids: torch.Tensor, num_experts: int, stream=None):
+    """Expert-contiguous permutation: returns (perm, inverse, offsets, active_list)."""
+    perm, inv, offs, scratch = _dispatch(topk_ids, num_experts, stream)
     n = int(scratch[num_experts].item())
     if int(scratch[num_experts + 1].item()):
         raise SenMoeError(ERR_DEVICE, f"dispatch saw an expert id outside [0, {num_experts})")
