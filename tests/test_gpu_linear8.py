@@ -397,3 +397,46 @@ def test_linear8_large(senmoe, torch):
         y = senmoe.linear8(s["x"], s["w"], path=path)
         L.assert_within(y[part], ref, R.rounded(ref, d, y.dtype), "y")
     senmoe.linear_check()
+
+
+def test_refusals(senmoe, torch):
+    """What does not fit together raises before a launch, with the package's errors."""
+    s = _make(senmoe, torch, 8, 64, 48, experts=2)
+    x, w3 = s["x"], s["w"]
+    w = senmoe.Rows8(w3.codes[0], w3.scales[0])
+    x16 = torch.zeros(8, 64, dtype=torch.bfloat16, device="cuda")
+    off = _offsets(torch, [4, 4])
+    bad = [lambda: senmoe.linear8(x, w3), lambda: senmoe.grouped_linear8(x, w, off),
+           lambda: senmoe.linear8(senmoe.Rows8(x.codes, x.scales[:, :1]), w),
+           lambda: senmoe.linear8(senmoe.Rows8(x.codes[:, :32], x.scales[:, :1]), w),
+           lambda: senmoe.linear8(x, senmoe.Rows8(w.codes[:47], w.scales[:47]), activation="swiglu"),
+           lambda: senmoe.linear8(x, w, bias=x16[0]), lambda: senmoe.linear8(x, w, residual=x16),
+           lambda: senmoe.grouped_linear8(x, w3, off[:2]), lambda: senmoe.linear8_input_grad(x16, w, activation="silu"),
+           lambda: senmoe.linear8_input_grad(x16, w, preact=x16[:4], activation="silu"),
+           lambda: senmoe.linear8_input_grad(x16, w3), lambda: senmoe.linear8_input_grad(x16[:, :32], w),
+           lambda: senmoe.grouped_linear8_input_grad(x16, w3, off[:2]), lambda: senmoe.linear8(x, w, path=9),
+           lambda: senmoe.rms_norm(x16, x16[0, :32]), lambda: senmoe.rms_norm(x16, x16[0], residual=x16[:4]),
+           lambda: senmoe.rms_norm(x16, x16[0], sixteen_bit=False), lambda: senmoe.rms_norm(x16, x16[0], eps=-1.0),
+           lambda: senmoe.rms_norm_backward(x16[:4], x16, x16[0])]
+    for i, call in enumerate(bad):
+        with pytest.raises(senmoe.SenMoeError) as e:
+            call()
+        assert e.value.status == 1, i
+    unsupported = [lambda: senmoe.quantize8(x16[:, :40]), lambda: senmoe.linear8(x, w, eight_bit=True),
+                   lambda: senmoe.rms_norm(x16[:, :40], x16[0, :40], eight_bit=True),
+                   lambda: senmoe.linear8(x, w, path=senmoe.LINEAR_ANY),
+                   lambda: senmoe.linear8_input_grad(x16[:, :40], w)]
+    for i, call in enumerate(unsupported):
+        with pytest.raises(senmoe.SenMoeError) as e:
+            call()
+        assert e.value.status in (1, 5), i
+    wrong = [lambda: senmoe.linear8(senmoe.Rows8(x.codes.view(torch.uint8), x.scales), w),
+             lambda: senmoe.linear8(senmoe.Rows8(x.codes.cpu(), x.scales.cpu()), w),
+             lambda: senmoe.linear8(x, senmoe.Rows8(w.codes.cpu(), w.scales.cpu())),
+             lambda: senmoe.linear8(x, w, bias=s["b"][0].half()), lambda: senmoe.linear8(x, w, dtype=torch.float32),
+             lambda: senmoe.grouped_linear8(x, w3, off.long()), lambda: senmoe.grouped_linear8(x, w3, off.cpu()),
+             lambda: senmoe.rms_norm(x16, x16[0].half()), lambda: senmoe.rms_norm(x16, x16[0], residual=x16.half())]
+    for i, call in enumerate(wrong):
+        with pytest.raises(TypeError):
+            call()
+    torch.cuda.synchronize()
