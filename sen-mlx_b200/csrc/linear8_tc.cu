@@ -831,7 +831,9 @@ struct Plan8 {
 };
 
 // As in linear_tc.cu, with a k block of 256: the bytes and MMA cycles of 128 16-bit k.
-constexpr double kL2Bytes8 = 57, kTileCycles8 = 900, kSplitCycles8 = 2000, kSplitColumn8 = 20;
+// A K split pays from K about 4096 on: 16 rows of 8192 -> 2048 20.0 us without,
+// 12.5 over four CTAs; 64 rows of 2048 -> 2048 9.4 without, 10.1 over four.
+constexpr double kL2Bytes8 = 57, kTileCycles8 = 900, kSplitCycles8 = 6500, kSplitColumn8 = 20;
 
 Plan8 make_plan8(const Linear8Args& l, bool gated, int sms, bool pair, int bn, int split) {
   Plan8 q;
