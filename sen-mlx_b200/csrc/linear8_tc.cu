@@ -83,7 +83,7 @@ struct Tc8Args {
   int m_tiles, stages, split;
   uint32_t stage_bytes;  // a stage's operands: W's pieces, then the columns'
   int pieces;            // rows are whole pieces, which the maps have as a dimension
-  int w_load, x_load;    // bytes of a scale row in one copy: 16, 8, 4 or 1; kScaleMap: by TMA
+  int w_load, x_load;    // bytes of a scale row in one copy: 8, 4 or 1; kScaleMap: by TMA
   long long tile_limit;  // of the wait for a tile's accumulators, cycles
 };
 
@@ -197,9 +197,7 @@ __device__ __forceinline__ Tile8 find_tile8(const Tc8Args& a, const int* s_off, 
 // with `load` bytes a copy; bytes (1) are there at once.  What lies past the row
 // stays as it is: no MMA takes it.
 __device__ __forceinline__ void fetch_scales(unsigned char* dst, const uint8_t* p, int have, int load) {
-  if (load == 16) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(p) : "memory");
-  } else if (load == 8) {
+  if (load == 8) {
 #pragma unroll
     for (int i = 0; i < 16; i += 8)
       if (i < have) cp_async_8(smem_u32(dst + i), p + i);

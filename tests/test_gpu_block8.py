@@ -132,3 +132,13 @@ def test_block_capture_and_requantize(senmoe, torch):
     assert torch.equal(block.forward(x, residual=r), x + r)
     with pytest.raises(ValueError):
         block.backward(x, None)
+
+
+def test_block_without_a_shared_expert_or_residual(senmoe, torch):
+    block, x, _ = _block(senmoe, torch, 9, 256, 64, 8, 2, 0)
+    out, saved = block.forward(x, train=True)
+    assert saved[0].h is x and torch.equal(out, block.forward(x))
+    dx, grads = block.backward(out, saved)
+    assert dx.shape == x.shape and sorted(grads) == ["down", "gate_up", "norm"]
+    with pytest.raises(senmoe.SenMoeError):
+        _block(senmoe, torch, 4, 256, 48, 8, 2, 0)  # 48 columns: not whole blocks of 32

@@ -440,3 +440,48 @@ def test_refusals(senmoe, torch):
         with pytest.raises(TypeError):
             call()
     torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits(senmoe, torch):
+    """Rows some 2^23 elements apart, in all over 2^32 bytes: norm, quantization and product of the last rows."""
+    import rows8_ref as R
+    rows, n, far = 300, 256, 1 << 23
+    g = torch.Generator(device="cuda").manual_seed(3)
+    buf = torch.empty(rows * far, dtype=torch.bfloat16, device="cuda")
+    x = buf.as_strided((rows, n), (far, 1))
+    x.copy_(torch.randn(rows, n, generator=g, device="cuda"))
+    w = R.rows8(senmoe, torch.randn(96, n, generator=g, device="cuda"))
+    near = x.contiguous()
+    gain = torch.rand(n, generator=g, device="cuda").bfloat16()
+    a, b = senmoe.rms_norm(x, gain, residual=x, eight_bit=True), senmoe.rms_norm(near, gain, residual=near, eight_bit=True)
+    assert torch.equal(a.y, b.y) and torch.equal(a.h, b.h) and _same8(torch, a.y8, b.y8)
+    assert all(torch.equal(p, q) for p, q in zip(senmoe.rms_norm_backward(x, x, gain, dh=x), senmoe.rms_norm_backward(near, near, gain, dh=near)))
+    x8 = senmoe.quantize8(x)
+    assert _same8(torch, x8, senmoe.quantize8(near))
+    raw = buf.view(torch.uint8)
+    codes = raw.as_strided((rows, n), (2 * far, 1)).view(torch.float8_e4m3fn)
+    scales = raw.as_strided((rows, n // 32), (2 * far, 1), 4096).view(torch.float8_e8m0fnu)
+    codes.view(torch.uint8).copy_(x8.codes.view(torch.uint8))
+    scales.view(torch.uint8).copy_(x8.scales.view(torch.uint8))
+    for path in (senmoe.LINEAR_SMALL, senmoe.LINEAR_TCGEN05_ONE, senmoe.LINEAR_TCGEN05_PAIR):
+        assert torch.equal(senmoe.linear8(senmoe.Rows8(codes, scales), w, path=path), senmoe.linear8(x8, w, path=path))
+
+
+def test_beside_the_16_bit_products(senmoe, torch):
+    """8-bit and 16-bit tcgen05 kernels, every form, in turn and side by side on two streams: the same bits as alone."""
+    s = _make(senmoe, torch, 700, 512, 768)
+    x16, w16 = s["x"].dequantize(torch.bfloat16), s["w"].dequantize(torch.bfloat16)
+    forms = (senmoe.LINEAR_TCGEN05_ONE, senmoe.LINEAR_TCGEN05_PAIR, senmoe.LINEAR_AUTO)
+    want8 = [senmoe.linear8(s["x"], s["w"], path=p) for p in forms]
+    want16 = [senmoe.linear(x16, w16, path=p) for p in forms]
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for side in (a, b):
+        side.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i in range(30):
+        got.append((want8[i % 3], senmoe.linear8(s["x"], s["w"], path=forms[i % 3], stream=a)))
+        got.append((want16[i % 3], senmoe.linear(x16, w16, path=forms[i % 3], stream=b if i % 2 else a)))
+        got.append((want8[(i + 1) % 3], senmoe.linear8(s["x"], s["w"], path=forms[(i + 1) % 3], stream=b)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in got)
+    senmoe.linear_check()
