@@ -42,15 +42,15 @@ __device__ __forceinline__ uint2 load_w(const uint8_t* p, bool live) {
 __device__ __forceinline__ uint2 load_x(const uint8_t* p, bool live) {
   return live ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
 }
-// N scales (4 or 2) from block b on, `have` blocks in all, one a byte; past the last: 2^0.
-template <int N> __device__ __forceinline__ uint32_t load_scales(const uint8_t* p, int b, int have, bool words, bool live) {
-  uint32_t v = 0x7f7f7f7fu;
-  if (!live || b >= have) return v;
+// N scales (4 or 2) from block b on, `have` blocks in all, one a byte; words: rows
+// lie on a 4-byte grid and are whole words.
+template <int N> __device__ __forceinline__ uint32_t load_scales(const uint8_t* p, int b, int have, bool words, bool live,
+                                                                 const uint8_t* begin, const uint8_t* end) {
+  if (!live || b >= have) return 0x7f7f7f7fu;
   if (words) return N == 4 ? *reinterpret_cast<const uint32_t*>(p + b) : *reinterpret_cast<const uint16_t*>(p + b);
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (b + i < have) v = (v & ~(0xffu << 8 * i)) | static_cast<uint32_t>(p[b + i]) << 8 * i;
-  return v;
+  uint32_t v[1];
+  scale_words<1>(p + b, min(N, have - b), begin, end, v);
+  return v[0];
 }
 __device__ __forceinline__ float scale_value(uint32_t word, int i) {
   const uint32_t byte = word >> 8 * i & 0xffu;
@@ -158,6 +158,8 @@ __global__ void __launch_bounds__(Shape<BF16, GATED, EIGHT, NT>::kThreads, Shape
   const uint8_t* x0 = a.x + static_cast<int64_t>(row0 + g) * a.x_stride + 8 * t4;
   const uint8_t* sx0 = a.x_scales + static_cast<int64_t>(row0 + 2 * t4) * a.x_scales_stride;
   const int blocks = a.k / kBlock8;
+  const uint8_t* const w_end = a.w_scales + (a.groups - 1) * a.w_scales_group_stride + (a.n - 1) * a.w_scales_stride + blocks;
+  const uint8_t* const x_end = a.x_scales + (a.rows - 1) * a.x_scales_stride + blocks;
   float acc[NT][4] = {};
   for (int b = kw * kSteps; b < blocks; b += S::kWarpsK * kSteps) {
     uint2 wa[kSteps][2], xb[kSteps][NT];
@@ -169,8 +171,8 @@ __global__ void __launch_bounds__(Shape<BF16, GATED, EIGHT, NT>::kThreads, Shape
       wa[s][0] = load_w(w0 + c, live0 && in);
       wa[s][1] = load_w(w1 + c, live1 && in);
     }
-    sw[0] = load_scales<kSteps>(sw0, b, blocks, words, live0);
-    sw[1] = load_scales<kSteps>(sw1, b, blocks, words, live1);
+    sw[0] = load_scales<kSteps>(sw0, b, blocks, words, live0, a.w_scales, w_end);
+    sw[1] = load_scales<kSteps>(sw1, b, blocks, words, live1, a.w_scales, w_end);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -178,7 +180,8 @@ __global__ void __launch_bounds__(Shape<BF16, GATED, EIGHT, NT>::kThreads, Shape
         xb[s][n] = load_x(x0 + n * 8 * a.x_stride + (b + s) * kBlock8, n * 8 + g < rows && b + s < blocks);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        sx[n][j] = load_scales<kSteps>(sx0 + (n * 8 + j) * a.x_scales_stride, b, blocks, words, n * 8 + 2 * t4 + j < rows);
+        sx[n][j] = load_scales<kSteps>(sx0 + (n * 8 + j) * a.x_scales_stride, b, blocks, words, n * 8 + 2 * t4 + j < rows,
+                                       a.x_scales, x_end);
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {

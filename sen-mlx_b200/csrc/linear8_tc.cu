@@ -83,7 +83,7 @@ struct Tc8Args {
   int m_tiles, stages, split;
   uint32_t stage_bytes;  // a stage's operands: W's pieces, then the columns'
   int pieces;            // rows are whole pieces, which the maps have as a dimension
-  int w_load, x_load;    // bytes of a scale row in one copy: 8, 4 or 1; kScaleMap: by TMA
+  int w_load, x_load;    // bytes of a scale row in one copy: 8, 4, or 1 (rows on no grid); kScaleMap: by TMA
   long long tile_limit;  // of the wait for a tile's accumulators, cycles
 };
 
@@ -194,9 +194,10 @@ __device__ __forceinline__ Tile8 find_tile8(const Tc8Args& a, const int* s_off, 
 }
 
 // The 16 scales from p on, of which `have` are in the row, into shared memory
-// with `load` bytes a copy; bytes (1) are there at once.  What lies past the row
-// stays as it is: no MMA takes it.
-__device__ __forceinline__ void fetch_scales(unsigned char* dst, const uint8_t* p, int have, int load) {
+// with `load` bytes a copy; those of rows on no grid (1) are there at once.  What
+// lies past the row is of no meaning: no MMA takes it.
+__device__ __forceinline__ void fetch_scales(unsigned char* dst, const uint8_t* p, int have, int load,
+                                             const uint8_t* begin, const uint8_t* end) {
   if (load == 8) {
 #pragma unroll
     for (int i = 0; i < 16; i += 8)
@@ -206,9 +207,9 @@ __device__ __forceinline__ void fetch_scales(unsigned char* dst, const uint8_t* 
     for (int i = 0; i < 16; i += 4)
       if (i < have) cp_async_4(smem_u32(dst + i), p + i);
   } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < have) dst[i] = p[i];
+    uint32_t w[4];
+    scale_words<4>(p, have, begin, end, w);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -474,6 +475,10 @@ __global__ void __launch_bounds__(kThreads8, 1)
       return unit_ptr + (slot * 3 + atom) * kUnitAtom + ((half * 2 + i) * 32 + lane) * 16;
     };
     const auto some = [&](const Tile8& t) { return atom < 2 || t.n > 128; };
+    // all scales of a side, for rows on no grid
+    const uint8_t* const begin = side ? l.x_scales : l.w_scales;
+    const uint8_t* const end = side ? begin + cap * l.x_scales_stride + blocks
+                                    : begin + (l.groups - 1) * l.w_scales_group_stride + (l.n - 1) * l.w_scales_stride + blocks;
     bool ok = true;
     Tile8 f{};               // the tile being fetched
     const uint8_t* p[2];     // cp.async: this lane's rows of it
@@ -500,7 +505,8 @@ __global__ void __launch_bounds__(kThreads8, 1)
         if (!maps) {
           if (some(f)) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) fetch_scales(place(slot, i), p[i] + at, blocks - at, side ? a.x_load : a.w_load);
+            for (int i = 0; i < 2; ++i)
+              fetch_scales(place(slot, i), p[i] + at, blocks - at, side ? a.x_load : a.w_load, begin, end);
           }
         } else if (lead && ok) {
           uint64_t* full = &bar_ufull[side][slot];

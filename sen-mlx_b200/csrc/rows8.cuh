@@ -59,4 +59,26 @@ __device__ __forceinline__ uint8_t pack8_warp(float v, uint32_t& byte) {
   return static_cast<uint8_t>(to_e4m3x2(v * scale_inverse(byte), 0.0f));
 }
 
+// N * 4 scale bytes from p on, p anywhere, in aligned words: begin and end are
+// those of all scales, outside of which nothing is read.  `have` bytes belong to
+// the row; what lies behind them is of no meaning.
+template <int N> __device__ __forceinline__ void scale_words(const uint8_t* p, int have, const uint8_t* begin,
+                                                             const uint8_t* end, uint32_t (&w)[N]) {
+  const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3);
+  const uint8_t* a = p - skew;
+  if (a >= begin && a + 4 * (N + 1) <= end) {
+    uint32_t v[N + 1];
+#pragma unroll
+    for (int i = 0; i <= N; ++i) v[i] = reinterpret_cast<const uint32_t*>(a)[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __funnelshift_r(v[i], v[i + 1], 8 * skew);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i)
+      if (i < have) w[i >> 2] |= static_cast<uint32_t>(p[i]) << 8 * (i & 3);
+  }
+}
+
 }  // namespace senmoe
