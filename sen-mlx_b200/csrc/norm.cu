@@ -34,13 +34,14 @@ constexpr int kNormThreads = 256;
 constexpr int kNormIter = 4;    // most pieces of 8 elements a lane holds
 constexpr int kGradIter = 2;    // wanted at most in the backward pass: 8 sums for dweight a piece
 constexpr int kNormWarps = 16;  // most warps of a row
+constexpr int kOddIter = 16, kOddWide = kNormWarps * 32 * kOddIter;  // elements of a lane where rows are on no 16-byte grid
 constexpr int kNormWide = kNormIter * kNormWarps * 32 * 8;  // longest row held in registers
 // With many rows: rows of a row's warps in shared memory, and blocks of 256
 // threads an SM.  32767 rows of 2816 fp16 (369 MB) forward 64.7 us with 2 rows,
 // 66.2 with 3, 70.9 with 4; 80.7 us with 2 blocks, 79.2 with 3, 67.8 with 6.
 // 32768 rows of 2048 backward (537 MB) 90 us with 2 rows, 104 with 3, 108 with
 // 4; 158 us with 1 block, 110 with 3; 104 with 4 pieces a lane, 116 with 1.
-constexpr int kDepth = 2, kNormBlocks = 4, kGradBlocks = 2;
+constexpr int kDepth = 2, kNormBlocks = 4, kGradBlocks = 2, kOddBlocks = 4;
 
 struct NormArgs {
   const void *x, *residual, *weight;
@@ -205,6 +206,51 @@ __global__ void __launch_bounds__(norm_threads<WARPS>(), 1024 / norm_threads<WAR
   }
 }
 
+// Rows on no 16-byte grid of at most 32 * kOddIter elements: a warp a row, an
+// element a lane and load.
+template <bool BF16> __global__ void __launch_bounds__(kNormThreads) norm_odd_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int kLanes = 32, kRows = kNormThreads / kLanes;
+  const int sub = threadIdx.x / kLanes, t = threadIdx.x % kLanes;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  pdl_wait();
+  pdl_launch_dependents();
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub; row < a.rows; row += step) {
+    const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.x_stride;
+    const uint16_t* res = static_cast<const uint16_t*>(a.residual) + row * a.residual_stride;
+    uint16_t v[kOddIter], r[kOddIter];
+#pragma unroll
+    for (int i = 0; i < kOddIter; ++i) {
+      const int c = t + i * kLanes;
+      v[i] = c < a.hidden ? x[c] : uint16_t(0);
+      r[i] = a.residual && c < a.hidden ? res[c] : uint16_t(0);
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kOddIter; ++i) {
+      const int c = t + i * kLanes;
+      if (a.residual) {
+        v[i] = from_f32<BF16>(to_f32<BF16>(v[i]) + to_f32<BF16>(r[i]));
+        if (a.h && c < a.hidden) (static_cast<uint16_t*>(a.h) + row * a.h_stride)[c] = v[i];
+      }
+      const float f = to_f32<BF16>(v[i]);
+      sum += f * f;
+    }
+    const float rstd = rsqrtf(warp_sum(sum) / a.hidden + a.eps);
+#pragma unroll
+    for (int i = 0; i < kOddIter; ++i) {
+      const int c = t + i * kLanes;
+      if (c >= a.hidden) break;  // (8 bits: hidden is in whole blocks, a warp has one)
+      const float f = to_f32<BF16>(v[i]) * rstd * gain<BF16>(a.weight, a.weight_fp32, a.offset, c);
+      if (a.y) (static_cast<uint16_t*>(a.y) + row * a.y_stride)[c] = from_f32<BF16>(f);
+      if (a.codes) {
+        uint32_t byte;
+        a.codes[row * a.codes_stride + c] = pack8_warp(f, byte);
+        if (t == 0) a.scales[row * a.scales_stride + c / kBlock8] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+}
+
 // Any width, stride and alignment: a block a row, element by element, the row
 // read twice (the second time mostly from L1).
 template <bool BF16> __global__ void __launch_bounds__(kNormThreads) norm_any_kernel(const __grid_constant__ NormArgs a) {
@@ -347,6 +393,68 @@ __global__ void __launch_bounds__(norm_threads<WARPS>(), 512 / norm_threads<WARP
   }
 }
 
+// Rows on no 16-byte grid of at most kOddWide elements: an element a lane and load
+// (14251 x 1467 with dh 94 us, with a block a row 266).
+template <bool BF16, int WARPS>
+__global__ void __launch_bounds__(norm_threads<WARPS>()) norm_grad_odd_kernel(const __grid_constant__ NormGradArgs a) {
+  constexpr int kLanes = WARPS * 32, kRows = norm_threads<WARPS>() / kLanes;
+  __shared__ float s_sum[2][kRows][WARPS][2];
+  __shared__ float s_part[kRows > 1 ? kLanes : 1];
+  const int sub = threadIdx.x / kLanes, t = threadIdx.x % kLanes;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  pdl_wait();
+  pdl_launch_dependents();
+  float acc[kOddIter] = {};
+  int turn = 0;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub; row < a.rows; row += step, turn ^= 1) {
+    const uint16_t* dy = static_cast<const uint16_t*>(a.dy) + row * a.dy_stride;
+    const uint16_t* h = static_cast<const uint16_t*>(a.h) + row * a.h_stride;
+    const uint16_t* dh = static_cast<const uint16_t*>(a.dh) + row * a.dh_stride;
+    uint16_t y[kOddIter], v[kOddIter], d[kOddIter];
+#pragma unroll
+    for (int i = 0; i < kOddIter; ++i) {
+      const int c = t + i * kLanes;
+      y[i] = c < a.hidden ? dy[c] : uint16_t(0);
+      v[i] = c < a.hidden ? h[c] : uint16_t(0);
+      d[i] = a.dh && c < a.hidden ? dh[c] : uint16_t(0);
+    }
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kOddIter; ++i) {
+      const int c = t + i * kLanes;
+      if (c >= a.hidden) break;
+      const float fh = to_f32<BF16>(v[i]);
+      sum[0] += fh * fh;
+      sum[1] += to_f32<BF16>(y[i]) * gain<BF16>(a.weight, a.weight_fp32, a.offset, c) * fh;
+    }
+    row_sums<WARPS>(sum, s_sum[turn][sub], sub, t >> 5);
+    const float r = rsqrtf(sum[0] / a.hidden + a.eps), m = r * r * (sum[1] / a.hidden);
+#pragma unroll
+    for (int i = 0; i < kOddIter; ++i) {
+      const int c = t + i * kLanes;
+      if (c >= a.hidden) break;
+      const float fh = to_f32<BF16>(v[i]), fy = to_f32<BF16>(y[i]);
+      acc[i] += fy * (fh * r);
+      if (a.dx)
+        (static_cast<uint16_t*>(a.dx) + row * a.dx_stride)[c] = from_f32<BF16>(
+            to_f32<BF16>(d[i]) + r * (fy * gain<BF16>(a.weight, a.weight_fp32, a.offset, c) - fh * m));
+    }
+  }
+  if (!a.partial) return;
+  float* part = a.partial + static_cast<int64_t>(blockIdx.x) * a.hidden;
+#pragma unroll
+  for (int i = 0; i < kOddIter; ++i) {
+    const int c = t + i * kLanes;
+    if constexpr (kRows > 1) {  // row group by row group, one after the other
+      for (int s = 0; s < kRows; ++s) {
+        __syncthreads();
+        if (sub == s) s_part[t] = acc[i] = (s > 0 ? s_part[t] : 0.0f) + acc[i];
+      }
+    }
+    if (sub == kRows - 1 && c < a.hidden) part[c] = acc[i];
+  }
+}
+
 // Any width, stride and alignment; a block adds to its line of `partial` row by row.
 template <bool BF16>
 __global__ void __launch_bounds__(kNormThreads) norm_grad_any_kernel(const __grid_constant__ NormGradArgs a) {
@@ -424,14 +532,19 @@ bool aligned16(const void* p, int64_t stride, int size = 2) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0;
 }
 
-// Warps of a row and pieces of a lane; warps 0: the kernels for any width.
+// Warps of a row and pieces of a lane; iter 0: an element a lane and load; warps
+// 0: a block a row.
 struct NormPlan {
   int warps = 0, iter = 0;
 };
 // iter: pieces of a lane that are wanted at most; few: warps below which more take a row
 NormPlan norm_plan(int64_t rows, int hidden, bool aligned, int iter, int64_t few) {
   NormPlan p;
-  if (!aligned || hidden % 8 || hidden > kNormWide) return p;
+  if (!aligned || hidden % 8 || hidden > kNormWide) {
+    if (hidden <= kOddWide)
+      for (p.warps = 1; p.warps * 32 * kOddIter < hidden;) p.warps *= 4;
+    return p;
+  }
   const int pieces = hidden / 8;
   p.warps = 1;
   while (p.warps < kNormWarps && p.warps * 32 * iter < pieces) p.warps *= 2;
@@ -440,6 +553,7 @@ NormPlan norm_plan(int64_t rows, int hidden, bool aligned, int iter, int64_t few
   return p;
 }
 
+#define SENMOE_NORM_ODD(KERNEL, B) (p.warps == 1 ? KERNEL<B, 1> : p.warps == 4 ? KERNEL<B, 4> : KERNEL<B, 16>)
 #define SENMOE_NORM_ITER(KERNEL, B, W, D) \
   (p.iter == 1 ? KERNEL<B, W, 1, D> : p.iter == 2 ? KERNEL<B, W, 2, D> : p.iter == 3 ? KERNEL<B, W, 3, D> : KERNEL<B, W, 4, D>)
 #define SENMOE_NORM_PICK(KERNEL, B, D)                                                                 \
@@ -464,12 +578,17 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
                        aligned16(a.weight, 0) && (!a.codes || aligned16(a.codes, a.codes_stride, 1));
   const int64_t sms = norm_sm_count();
   const NormPlan p = norm_plan(a.rows, a.hidden, aligned, kNormIter, sms * 8);
-  if (!p.warps) {
+  // on no grid: a warp a row, or a block (with a residual, a warp a row: 21461 x 223 17.6 us, a
+  // block a row 42.9; 4 warps a row: 6191 x 820 50.7, a block a row 22.0)
+  if (!p.warps || (!p.iter && p.warps > 1)) {
     const int64_t grid = a.rows < sms * 8 ? a.rows : sms * 8;
     return launch_pdl(a.bf16 ? norm_any_kernel<true> : norm_any_kernel<false>, dim3(static_cast<unsigned>(grid)),
                       dim3(kNormThreads), 0, st, a);
   }
   const int64_t blocks = (a.rows + plan_rows(p) - 1) / plan_rows(p), streams = a.residual ? 2 : 1;
+  if (!p.iter)
+    return launch_pdl(a.bf16 ? norm_odd_kernel<true> : norm_odd_kernel<false>,
+                      dim3(static_cast<unsigned>(blocks < sms * 32 ? blocks : sms * 32)), dim3(plan_threads(p)), 0, st, a);
   // many rows: the blocks that are resident together
   const int64_t fit = 200 * 1024 / static_cast<int64_t>(ring_bytes(plan_threads(p), p.iter, kDepth, streams));
   const int64_t most = kNormBlocks * kNormThreads / plan_threads(p), resident = sms * (fit < most ? fit : most);
@@ -488,14 +607,18 @@ bool grad_aligned(const NormGradArgs& a) {
 // row group; by the sizes alone, so that the same call adds in the same order.
 int grad_blocks(const NormPlan& p, int64_t rows, int sms) {
   const int64_t groups = (rows + plan_rows(p) - 1) / plan_rows(p);
-  const int64_t most = static_cast<int64_t>(sms) * kGradBlocks * kNormThreads / (p.warps ? plan_threads(p) : kNormThreads);
+  const int resident = p.warps && !p.iter ? kOddBlocks : kGradBlocks;
+  const int64_t most = static_cast<int64_t>(sms) * resident * kNormThreads / (p.warps ? plan_threads(p) : kNormThreads);
   return static_cast<int>(groups < most ? groups : most);
 }
 
 cudaError_t launch_norm_grad(NormGradArgs a, const NormPlan& p, cudaStream_t st) {
   if (a.rows > 0) {
     cudaError_t e;
-    if (!p.warps)
+    if (p.warps && !p.iter)
+      e = launch_pdl(a.bf16 ? SENMOE_NORM_ODD(norm_grad_odd_kernel, true) : SENMOE_NORM_ODD(norm_grad_odd_kernel, false),
+                     dim3(a.blocks), dim3(plan_threads(p)), 0, st, a);
+    else if (!p.warps)
       e = launch_pdl(a.bf16 ? norm_grad_any_kernel<true> : norm_grad_any_kernel<false>, dim3(a.blocks),
                      dim3(kNormThreads), 0, st, a);
     else
