@@ -11,12 +11,12 @@
 //
 // with fp32 sums.  It reads the scales from TMEM, where row r of an operand is
 // lane r mod 32 (the same in each quarter of the lanes) and column r / 32, the
-// four bytes of a word being four consecutive blocks.  Warps 2 and 3 bring
-// them there: a lane loads the words of rows l, l + 32, l + 64, l + 96 of 128
-// rows, which side by side are the 16 bytes that tcgen05.cp 32x128b wants for
-// lane l, and the MMA warp issues the copies ahead of the MMAs.  Copies and MMAs of one thread run in order; two sets of
-// scale columns alternate all the same, so that a copy need not wait for the
-// MMAs before it.
+// four bytes of a word being four consecutive blocks.  Six warps bring them
+// there: the words of rows l, l + 32, l + 64, l + 96 of 128 rows, laid side by
+// side, are the 16 bytes that tcgen05.cp 32x128b wants for lane l, and the MMA
+// warp issues the copies ahead of the MMAs.  Copies and MMAs of one thread run
+// in order; two sets of scale columns alternate all the same, so that a copy
+// need not wait for the MMAs before it.
 //
 // Forms of a tile: one CTA (128 features), a pair (cta_group::2, 256 features
 // on two SMs, each holding half of the columns' codes and all of their
@@ -25,7 +25,16 @@
 // need none, as in linear_tc.cu.
 //
 // 8-bit output: a warp's 32 lanes are 32 consecutive features, one block of a
-// row of y, so the block's largest is one warp reduction a column.
+// row of y, which is finished where it stands (store_chunk8).
+//
+// What bounds it, and what it measured (one B200, a graph of launches on cold
+// inputs): power first, as SM clocks fall to 1.2 to 1.6 GHz under it, and shared
+// memory, which takes an 8-bit tile's bytes in half of a 16-bit tile's MMA time.
+// 8192 x 2048 -> 8192 gelu 144 us = 1900 TFLOP/s (110 without the epilogue, 131
+// without the scales, 89 without either), 50 % tensor pipe.  4096 tokens of 128
+// experts, 2048 -> 2 x 768 swiglu to 8 bits with z kept, 140 to 158 us for 0.61 GB
+// and 206 GFLOP; every group of more than 224 rows is two chunks, each with its
+// trip of W from L2.
 
 #include <cuda.h>
 
@@ -75,7 +84,7 @@ constexpr uint32_t ring_budget8(bool words, int groups) {
 __device__ int g_linear8_error;  // first device error of these kernels on this device
 __device__ int g_linear8_taken;  // what the last check found there
 
-constexpr int kScaleMap = 0;
+constexpr int kScaleMap = 0;     // see Tc8Args
 
 struct Tc8Args {
   Linear8Args l;
@@ -442,9 +451,11 @@ __global__ void __launch_bounds__(kThreads8, 1)
             if (t.n > 128) copy_scales<PAIR>(sb + 4, sc + i * kPieceScales + 2 * kAtomBytes);
             const uint64_t dm = smem_desc<false>(sm + i * kMPiece), dn = smem_desc<false>(sn + i * n_piece);
 #pragma unroll
-            for (int s = 0; s < 4; ++s)  // 32 k: 32 bytes along a line
-              if (s < ks) umma_scaled<PAIR>(d, dm + s * (32 >> 4), dn + s * (32 >> 4), idesc | (s << 4) | (s << 29), sa, sb,
-                                (b > t.kb0 || i > 0 || s > 0) ? 1u : 0u);
+            for (int s = 0; s < kPiece / kBlock8; ++s) {  // 32 k: 32 bytes along a line
+              if (s < ks)
+                umma_scaled<PAIR>(d, dm + s * (32 >> 4), dn + s * (32 >> 4), idesc | (s << 4) | (s << 29), sa, sb,
+                                  (b > t.kb0 || i > 0 || s > 0) ? 1u : 0u);
+            }
           }
           umma_commit<PAIR>(&bar_empty[st]);
         }
@@ -463,7 +474,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
     // ============================================================== scales
     // Half of an atom a warp (atom: W's 128 rows, the first 128 columns, the
     // others).  Rows come as 16 bytes, two stages' worth, one such unit ahead
-    // (also of the next tile): by TMA where their strides allow a map (a.maps),
+    // (also of the next tile): by TMA where their strides allow a map,
     // else each lane its two rows with cp.async.  With each stage a lane lays
     // its rows' words side by side to where tcgen05.cp takes them.
     const Linear8Args& l = a.l;
