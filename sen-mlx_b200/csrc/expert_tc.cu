@@ -750,17 +750,6 @@ bool tc_supported(int rows, int kdim, int bits, int nproj, int bn) {
          tc_smem_bytes(bits, nproj, bn, kdim) + 2048 <= 227 * 1024;
 }
 
-static int sm_count() {
-  static int n = 0;
-  if (n == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-      n = 148;
-  }
-  return n;
-}
-
 template <int BITS, int NPROJ, int BN>
 static cudaError_t launch_tc_t(const CUtensorMap& tA0, const CUtensorMap& tA1, const CUtensorMap& tB,
                                const TcGemmArgs& a, int tiles_upper, cudaStream_t st) {

@@ -371,6 +371,17 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// SMs of the current device.
+inline int sm_count() {
+  static int counts[64] = {};  // by device; the same value whoever writes it
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && counts[dev] > 0) return counts[dev];
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+  if (dev < 64) counts[dev] = n;
+  return n;
+}
+
 // Raises a kernel's dynamic shared-memory limit to at least `bytes` on the
 // current device.  Only the first call per (kernel, device, size) reaches the
 // driver, so launches inside a CUDA-graph capture after a warm-up call make

@@ -774,16 +774,6 @@ __global__ void __launch_bounds__(kThreads8, 1)
 __global__ void take_error8_kernel() { g_linear8_taken = atomicExch(&g_linear8_error, 0); }
 
 // ------------------------------------------------------------- host side
-int tc8_sm_count() {
-  static int counts[64] = {};  // by device; the same value whoever writes it
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (dev < 64 && counts[dev] > 0) return counts[dev];
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-  if (dev < 64) counts[dev] = n;
-  return n;
-}
-
 constexpr uint32_t stage_bytes8(int part) { return kPieces * (kMPiece + part * kPiece); }
 constexpr int stages8(bool words, int part, int groups) {
   const int fit = static_cast<int>(ring_budget8(words, groups) / (stage_bytes8(part) + kScaleBytes));
@@ -920,7 +910,7 @@ cudaError_t launch_form(bool gated, bool bf16, const A&... args) {
 
 cudaError_t launch_linear8_tc(const Linear8Args& l, int form, cudaStream_t st) {
   const bool gated = act_gated(l.act);
-  const int sms = tc8_sm_count();
+  const int sms = sm_count();
   const Plan8 plan = choose_plan8(l, gated, sms, form);
   if (plan.cycles == 0) return cudaErrorNotSupported;  // too many tiles for the K split asked for
   Tc8Args a{};

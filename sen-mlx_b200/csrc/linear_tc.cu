@@ -723,16 +723,6 @@ __global__ void selftest_wait_kernel() {
 }
 
 // ------------------------------------------------------------- host side
-int tc_sm_count() {
-  static int counts[64] = {};  // by device; the same value whoever writes it
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (dev < 64 && counts[dev] > 0) return counts[dev];
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-  if (dev < 64) counts[dev] = n;
-  return n;
-}
-
 bool tma_ok(const void* p, int64_t stride, int64_t group_stride, int groups) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 8 == 0 && stride < (int64_t(1) << 36) &&
          (groups <= 1 || (group_stride % 8 == 0 && group_stride < (int64_t(1) << 38)));
@@ -880,7 +870,7 @@ bool linear_tc_supported(const LinearArgs& a, LinearProduct p) {
 cudaError_t launch_linear_tc(const LinearArgs& l, LinearProduct p, int form, const BiasJoin* bias, bool* summed,
                              cudaStream_t st) {
   const bool gated = p == kProdForward && act_gated(l.act);
-  const int sms = tc_sm_count();
+  const int sms = sm_count();
   const Plan plan = choose_plan(l, p, gated, sms, form);
   if (plan.cycles == 0) return cudaErrorNotSupported;  // too many tiles for the K split asked for
   TcArgs a{};

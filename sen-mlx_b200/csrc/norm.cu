@@ -518,16 +518,6 @@ template <bool BF16> __global__ void __launch_bounds__(kJoinWarps * 32) norm_joi
 }
 
 // ------------------------------------------------------------- host side
-int norm_sm_count() {
-  static int counts[64] = {};  // by device; the same value whoever writes it
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (dev < 64 && counts[dev] > 0) return counts[dev];
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-  if (dev < 64) counts[dev] = n;
-  return n;
-}
-
 bool aligned16(const void* p, int64_t stride, int size = 2) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0;
 }
@@ -576,7 +566,7 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
   const bool aligned = aligned16(a.x, a.x_stride) && (!a.residual || aligned16(a.residual, a.residual_stride)) &&
                        (!a.h || aligned16(a.h, a.h_stride)) && (!a.y || aligned16(a.y, a.y_stride)) &&
                        aligned16(a.weight, 0) && (!a.codes || aligned16(a.codes, a.codes_stride, 1));
-  const int64_t sms = norm_sm_count();
+  const int64_t sms = sm_count();
   const NormPlan p = norm_plan(a.rows, a.hidden, aligned, kNormIter, sms * 8);
   // on no grid: a warp a row, or a block (with a residual, a warp a row: 21461 x 223 17.6 us, a
   // block a row 42.9; 4 warps a row: 6191 x 820 50.7, a block a row 22.0)
@@ -680,7 +670,7 @@ int plan_grad(const char* call, const SenMoeNormGrad* g, NormGradArgs* a, NormPl
   a->bf16 = g->dtype == SENMOE_BF16;
   a->eps = g->eps;
   a->offset = g->unit_offset ? 1.0f : 0.0f;
-  const int sms = norm_sm_count();
+  const int sms = sm_count();
   *p = norm_plan(g->rows, a->hidden, grad_aligned(*a), kGradIter, sms * 8);
   a->blocks = grad_blocks(*p, g->rows, sms);
   return SENMOE_OK;
