@@ -51,13 +51,17 @@ int check_type(const char* call, int32_t dtype, int32_t epilogue) {
 //   dense 512 x 2048     8 rows 2.7 / 6.2    64 rows 5.6 / 6.5    96 rows 9.6 / 6.6
 //   dense 2048 x 8192    8 rows 12.0 / 11.6  8192 x 2048  1 row 14.8 / 12.6
 // It reads W in pieces of 64 bytes a row, which bounds it at 2 TB/s, and all
-// rows for every 16 features.  Grouped, by what the touched experts hold:
-//   8 x 768 x 2048       14.6 / 9.9    8 x 2048 x 1536  14.7 / 12.7
-//   4 x 2048 x 1536      11.2 / 12.7   8 x 2048 x 512   7.2 / 9.5
+// rows for every 16 features; and its blocks, short ones, should be resident
+// together.  Grouped, by what the touched experts hold, and blocks:
+//   8 x 768 x 2048    1024 blocks 14.6 / 9.9    8 x 2048 x 1536 (8 bits) 192 blocks 14.7 / 12.7
+//   4 x 2048 x 1536 (8 bits)  96 blocks 11.2 / 12.7    8 x 512 x 1024  512 blocks 6.9 / 8.2
+//   16 x 96 x 512     512 blocks 7.3 / 8.1      32 x 256 x 512   1024 blocks 11.6 / 8.4
 bool few_rows8(const Linear8Args& a) {
   const int64_t weight = static_cast<int64_t>(a.n) * a.k;
-  if (!a.offsets) return a.rows <= 64 && weight * (a.rows > 8 ? a.rows : 8) <= 100000000;
-  return a.rows <= 64 && weight * (a.rows < a.groups ? a.rows : a.groups) <= 10000000;
+  const int64_t chunks = !a.offsets ? (a.rows + 63) / 64 : a.rows < a.groups ? a.rows : a.groups;
+  const int rows_of_w = !a.codes ? 16 : act_gated(a.act) ? 64 : 32;  // of a block
+  if (a.rows > 64 || chunks * ((a.n + rows_of_w - 1) / rows_of_w) > 148 * 4) return false;
+  return a.offsets ? weight * chunks <= 13000000 : weight * (a.rows > 8 ? a.rows : 8) <= 100000000;
 }
 
 }  // namespace
