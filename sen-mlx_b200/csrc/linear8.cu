@@ -50,6 +50,8 @@ int check_type(const char* call, int32_t dtype, int32_t epilogue) {
 //   dense 2816 x 2112    8 rows 6.8 / 9.8    16 rows 8.4 / 9.9    32 rows 11.8 / 9.9
 //   dense 512 x 2048     8 rows 2.7 / 6.2    64 rows 5.6 / 6.5    96 rows 9.6 / 6.6
 //   dense 2048 x 8192    8 rows 12.0 / 11.6  8192 x 2048  1 row 14.8 / 12.6
+//   dense 1024 x 512     64 rows 8.8 / 7.3   4096 x 512   8 rows 8.3 / 9.7   16 rows 10.4 / 9.7
+// A block walks the whole of K for all rows, whatever the number of blocks.
 // It reads W in pieces of 64 bytes a row, which bounds it at 2 TB/s, and all
 // rows for every 16 features; and its blocks, short ones, should be resident
 // together.  Grouped, by what the touched experts hold, and blocks:
@@ -61,7 +63,8 @@ bool few_rows8(const Linear8Args& a) {
   const int64_t chunks = !a.offsets ? (a.rows + 63) / 64 : a.rows < a.groups ? a.rows : a.groups;
   const int rows_of_w = !a.codes ? 16 : act_gated(a.act) ? 64 : 32;  // of a block
   if (a.rows > 64 || chunks * ((a.n + rows_of_w - 1) / rows_of_w) > 148 * 4) return false;
-  return a.offsets ? weight * chunks <= 13000000 : weight * (a.rows > 8 ? a.rows : 8) <= 100000000;
+  const int64_t each = a.rows > 8 ? a.rows : 8;
+  return a.offsets ? weight * chunks <= 13000000 : weight * each <= 100000000 && a.k * each <= 50000;
 }
 
 }  // namespace
