@@ -556,7 +556,7 @@ def _dispatch(topk_ids: torch.Tensor, num_experts: int, stream=None):
     dev = ids.device
     perm = torch.empty(T * K, dtype=torch.int32, device=dev)
     inv = torch.empty(T * K, dtype=torch.int32, device=dev)
-    offs = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
+    offs = (torch.empty if T else torch.zeros)(num_experts + 1, dtype=torch.int32, device=dev)
     scratch = torch.zeros(num_experts + 2, dtype=torch.int32, device=dev)
     _check(lib().senmoe_dispatch(_ptr(ids), T, K, num_experts, _ptr(perm), _ptr(inv), _ptr(offs), _ptr(scratch),
                                  _stream(stream)))

@@ -22,7 +22,7 @@ from .block16 import Moe16Weights
 class Moe8:
     """x [T, H] bf16; norm [H] bf16 or fp32.  ``train`` also keeps the weights'
     transposes in 8 bits, for ``backward``; after a change of the 16-bit weights
-    ``requantize`` makes the 8-bit ones again.
+    ``requantize`` makes the 8-bit ones again, in the same memory.
 
     Nothing here waits for the device, so ``forward`` can be captured into a CUDA
     graph (once run before): call ``senmoe.linear_check`` where the
@@ -32,17 +32,22 @@ class Moe8:
                  norm_topk_prob: bool = True, train: bool = False):
         self.w, self.norm, self.top_k, self.eps, self.norm_topk = weights, norm, top_k, eps, norm_topk_prob
         self.train = train
+        self.w8: dict[str, Rows8] = {}
         self.requantize()
 
     def requantize(self) -> None:
-        w = self.w
-        self.w8: dict[str, Rows8] = {}
         for name in ("gate_up", "down", "shared_gate_up", "shared_down"):
-            m = getattr(w, name)
+            m = getattr(self.w, name)
             if m is not None:
-                self.w8[name] = quantize8(m)
+                self._keep(name, quantize8(m))
                 if self.train:
-                    self.w8[name + "_t"] = quantize8(m.transpose(-1, -2).contiguous())
+                    self._keep(name + "_t", quantize8(m.transpose(-1, -2).contiguous()))
+
+    def _keep(self, name: str, new: Rows8) -> None:
+        """new, where a captured ``forward`` reads it: in the place of the one before."""
+        for kept, part in zip(self.w8.setdefault(name, new), new):
+            if kept is not part:
+                kept.view(torch.uint8).copy_(part.view(torch.uint8))
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, train: bool = False):
         """out, or with ``train`` (out, what ``backward`` needs)."""
@@ -55,7 +60,7 @@ class Moe8:
                             save_preact=train)
         a, z = a if train else (a, None)
         d = grouped_linear8(a, w8["down"], offsets)
-        rows = d[inverse.long()].view(x.shape[0], K, -1)
+        rows = d[inverse.long()].view(x.shape[0], K, x.shape[1])
         out = (n.h.float() + (rows.float() * prob[..., None]).sum(1)).to(x.dtype)
         b = zb = None
         if w.shared_gate_up is not None:

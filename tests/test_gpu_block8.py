@@ -134,6 +134,39 @@ def test_block_capture_and_requantize(senmoe, torch):
         block.backward(x, None)
 
 
+def test_block_replay_after_requantize(senmoe, torch):
+    """A captured step reads the weights that requantize made, not the ones it was captured with."""
+    block, x, r = _block(senmoe, torch, 4, 256, 64, 8, 2, 64)
+    block.forward(x, residual=r)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = block.forward(x, residual=r)
+    g.replay()
+    before = out.clone()
+    for m in (block.w.gate_up, block.w.down, block.w.shared_gate_up, block.w.shared_down):
+        m.mul_(0.5)
+    block.requantize()
+    other = senmoe.quantize8(block.w.gate_up.flip(0))  # (what was freed is written by others)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, block.forward(x, residual=r)) and not torch.equal(out, before)
+    same = senmoe.quantize8(block.w.down.transpose(-1, -2).contiguous())
+    assert torch.equal(block.w8["down_t"].codes.view(torch.uint8), same.codes.view(torch.uint8)) and other.codes.numel()
+    assert torch.equal(block.w8["down_t"].scales.view(torch.uint8), same.scales.view(torch.uint8))
+
+
+def test_block_without_tokens(senmoe, torch):
+    block, x, r = _block(senmoe, torch, 4, 256, 64, 8, 2, 64)
+    out, saved = block.forward(x[:0], residual=r[:0], train=True)
+    assert out.shape == (0, 256) and not saved[2].any()
+    dx, grads = block.backward(out, saved)
+    torch.cuda.synchronize()
+    assert dx.shape == (0, 256)
+    for name, grad in grads.items():
+        assert not grad.any(), name
+
+
 def test_block_without_a_shared_expert_or_residual(senmoe, torch):
     block, x, _ = _block(senmoe, torch, 9, 256, 64, 8, 2, 0)
     out, saved = block.forward(x, train=True)
