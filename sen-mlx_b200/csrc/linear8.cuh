@@ -42,6 +42,19 @@ struct Linear8Args {
   void* preact;                // or null
   int64_t preact_stride;
 };
+// [begin, end) in k blocks (stages of linear8_tc.cu) of CTA `rank` of a K split
+// over `split`; empty for some where there are fewer blocks than CTAs.
+struct KRange {
+  int begin, end;
+};
+__host__ __device__ inline KRange k_share(int blocks, int rank, int split) {
+  return {static_cast<int>(static_cast<int64_t>(blocks) * rank / split),
+          static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / split)};
+}
+// The units of two blocks in which their scales come; none without blocks.
+__host__ __device__ inline KRange scale_units(int kb0, int kb1) {
+  return {kb0 / 2, kb1 > kb0 ? (kb1 + 1) / 2 : kb0 / 2};
+}
 // Few rows (linear8_small.cu).
 bool linear8_small_supported(const Linear8Args& a);
 cudaError_t launch_linear8_small(const Linear8Args& a, cudaStream_t st);

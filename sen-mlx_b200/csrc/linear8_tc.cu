@@ -195,8 +195,9 @@ __device__ __forceinline__ Tile8 find_tile8(const Tc8Args& a, const int* s_off, 
   t.kb1 = kb;
   if constexpr (!PAIR) {
     if (a.split > 1) {
-      t.kb0 = static_cast<int>(static_cast<int64_t>(kb) * rank / a.split);
-      t.kb1 = static_cast<int>(static_cast<int64_t>(kb) * (rank + 1) / a.split);
+      const KRange r = k_share(kb, rank, a.split);
+      t.kb0 = r.begin;
+      t.kb1 = r.end;
     }
   }
   return t;
@@ -498,8 +499,9 @@ __global__ void __launch_bounds__(kThreads8, 1)
       while (f_unit >= f_end && f_it < mine) {
         if (++f_it == mine) break;
         f = tile(f_it);
-        f_unit = f.kb0 / 2;
-        f_end = (f.kb1 + 1) / 2;
+        const KRange u = scale_units(f.kb0, f.kb1);
+        f_unit = u.begin;
+        f_end = u.end;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {  // past the last row, that one: no result is of it
           const int r = (half * 2 + i) * 32 + lane;
@@ -572,7 +574,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
       }
     }
     if (!maps) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (lead && maps && !ok) {  // gave up: loads already issued get a bounded chance to land
+    if (lead && maps) {  // every load issued has landed (after giving up: gets a bounded chance to)
       volatile int never = 0;
       for (int i = max(count, 0); i < f_count; ++i) wait_or_abort(&bar_ufull[side][i % kUnits], i / kUnits & 1, &never, nullptr);
     }
