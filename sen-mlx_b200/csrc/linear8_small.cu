@@ -52,10 +52,16 @@ template <int N> __device__ __forceinline__ uint32_t load_scales(const uint8_t* 
   scale_words<1>(p + b, min(N, have - b), begin, end, v);
   return v[0];
 }
-__device__ __forceinline__ float scale_value(uint32_t word, int i) {
-  const uint32_t byte = word >> 8 * i & 0xffu;
-  return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
+// d times two scales 2^(w - 127), 2^(x - 127), given by their bytes (up to 254).
+// The scales' product can leave fp32 where the result is in range, or zero.  So d
+// is multiplied by 2^(floor(s / 2) - 127), then by 2^(ceil(s / 2) - 127), s = w + x:
+// within a factor of two of one another, they leave fp32 only with the result.
+// (The first is 0 in place of 2^-127, where the result is under 2^-229.)
+__device__ __forceinline__ float scaled(float d, uint32_t w, uint32_t x) {
+  const uint32_t s = w + x, half = s << 22 & 0x7f800000u;
+  return d * __uint_as_float(half) * __uint_as_float((s << 23) - half);
 }
+__device__ __forceinline__ uint32_t scale_of(uint32_t word, int i) { return word >> 8 * i & 0xffu; }
 
 template <bool BF16, bool GATED, bool EIGHT, int NT> struct Shape {
   static constexpr int kTiles = !EIGHT ? 1 : GATED ? 4 : 2;
@@ -186,7 +192,7 @@ __global__ void __launch_bounds__(Shape<BF16, GATED, EIGHT, NT>::kThreads, Shape
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       if (b + s >= blocks) break;
-      const float v0 = scale_value(sw[0], s), v1 = scale_value(sw[1], s);
+      const uint32_t v0 = scale_of(sw[0], s), v1 = scale_of(sw[1], s);
       uint32_t a0[4], a1[4];  // rows g and g + 8, in fp16 pairs
       to_f16(wa[s][0].x, a0[0], a0[1]);
       to_f16(wa[s][0].y, a0[2], a0[3]);
@@ -200,11 +206,18 @@ __global__ void __launch_bounds__(Shape<BF16, GATED, EIGHT, NT>::kThreads, Shape
         float d[4] = {};
         mma16816(d, a0[0], a1[0], a0[1], a1[1], x[0], x[1]);
         mma16816(d, a0[2], a1[2], a0[3], a1[3], x[2], x[3]);
-        const float u0 = scale_value(sx[n][0], s), u1 = scale_value(sx[n][1], s);
-        acc[n][0] += d[0] * (v0 * u0);
-        acc[n][1] += d[1] * (v0 * u1);
-        acc[n][2] += d[2] * (v1 * u0);
-        acc[n][3] += d[3] * (v1 * u1);
+        const uint32_t u0 = scale_of(sx[n][0], s), u1 = scale_of(sx[n][1], s);
+        acc[n][0] += scaled(d[0], v0, u0);
+        acc[n][1] += scaled(d[1], v0, u1);
+        acc[n][2] += scaled(d[2], v1, u0);
+        acc[n][3] += scaled(d[3], v1, u1);
+        if (max(max(v0, v1), max(u0, u1)) == 255u) {  // a scale that is NaN: so are its rows' sums, from here on
+          const float nan = __uint_as_float(0x7fc00000u);
+          if (max(v0, u0) == 255u) acc[n][0] = nan;
+          if (max(v0, u1) == 255u) acc[n][1] = nan;
+          if (max(v1, u0) == 255u) acc[n][2] = nan;
+          if (max(v1, u1) == 255u) acc[n][3] = nan;
+        }
       }
     }
   }

@@ -45,3 +45,43 @@ def test_split_over_few_blocks(senmoe, torch, k, activation):
     ref, d, _, _ = R.product(R.values(g["x"]), R.values(g["w"]), off, g["b"], None, activation)
     L.assert_within(y, ref, R.rounded(ref, d, y.dtype), "y grouped")
     senmoe.linear_check()
+
+
+@pytest.fixture(params=["small", "one", "pair", "split", "auto"])
+def path(request, senmoe):
+    return {"small": senmoe.LINEAR_SMALL, "one": senmoe.LINEAR_TCGEN05_ONE, "pair": senmoe.LINEAR_TCGEN05_PAIR,
+            "split": senmoe.LINEAR_TCGEN05_SPLIT, "auto": senmoe.LINEAR_AUTO}[request.param]
+
+
+@pytest.mark.parametrize("rows", [1, 9, 40])
+def test_scales_over_their_whole_range(senmoe, torch, path, rows):
+    """Scales from 2^-127 to 2^127 on both sides, one element of each row of x: the product of two scales leaves fp32
+    in every direction, while the result is zero, or in range, or not.  One product each, so exact."""
+    k, out = 256, 96
+    g = torch.Generator(device="cuda").manual_seed(rows)
+
+    def whole(lo, hi, *shape):
+        return torch.randint(lo, hi, shape, generator=g, device="cuda")
+    col = whole(0, k, rows)
+    x = torch.zeros(rows, k, device="cuda")
+    x[torch.arange(rows, device="cuda"), col] = whole(1, 8, rows).float()
+    w = whole(-7, 8, out, k).float()
+    xs, ws = whole(0, 255, rows, k // 32).to(torch.uint8), whole(0, 255, out, k // 32).to(torch.uint8)
+    e4m3, e8m0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+    y = senmoe.linear8(senmoe.Rows8(x.to(e4m3), xs.view(e8m0)), senmoe.Rows8(w.to(e4m3), ws.view(e8m0)), path=path)
+    wide = lambda v, s: v.double() * torch.exp2(s.double() - 127).repeat_interleave(32, -1)  # noqa: E731
+    want = wide(x, xs) @ wide(w, ws).t()
+    assert not bool(y.isnan().any())
+    near = (want == 0) | (want.abs() >= 2.0 ** -120)  # (what rounds to subnormals, or below them, is small)
+    assert torch.equal(y[near], want.to(y.dtype)[near])
+    assert bool((y[~near].abs() <= 2.0 ** -119).all())
+    assert bool((want.abs() > 1e39).any()) or rows == 1
+
+
+def test_zero_times_large_scales(senmoe, torch, path):
+    """2^110 in a column of x, 2^40 in another one of W: the product is 0."""
+    import rows8_ref as R
+    x, w = torch.zeros(4, 64, device="cuda"), torch.zeros(32, 64, device="cuda")
+    x[:, 0], w[:, 1] = 2.0 ** 110, 2.0 ** 40
+    y = senmoe.linear8(R.rows8(senmoe, x), R.rows8(senmoe, w), path=path)
+    assert torch.equal(y, torch.zeros_like(y))
