@@ -118,9 +118,9 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, e
     if dh is not None:
         dh, ds = _same_rows(dh, h, device, "dh")
         pd = dh.data_ptr()
+    dx = _like(h) if need_dx else None
     h, hs = (h, n) if h.is_contiguous() else _rows(h, n)
     weight = weight.contiguous()
-    dx = _like(h) if need_dx else None
     dw = torch.empty_like(weight) if need_dweight else None
     args = (code, fp32, int(unit_offset), eps, rows, n, dy.data_ptr(), ys, h.data_ptr(), hs, weight.data_ptr(), pd, ds,
             dx.data_ptr() if need_dx else 0, n, dw.data_ptr() if need_dweight else 0)
