@@ -175,9 +175,9 @@ __global__ void __launch_bounds__(norm_threads<WARPS>(), 1024 / norm_threads<WAR
 #pragma unroll
         for (int k = 0; k < 8; ++k) f[k] += g[k];
         v[i] = pack8<BF16>(f);
-        if (a.h && c < a.hidden) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + row * a.h_stride + c) = v[i];
         unpack8<BF16>(v[i], f);
       }
+      if (a.h && c < a.hidden) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + row * a.h_stride + c) = v[i];
 #pragma unroll
       for (int k = 0; k < 8; ++k) sum[0] += f[k] * f[k];
     }
@@ -228,10 +228,8 @@ template <bool BF16> __global__ void __launch_bounds__(kNormThreads) norm_odd_ke
 #pragma unroll
     for (int i = 0; i < kOddIter; ++i) {
       const int c = t + i * kLanes;
-      if (a.residual) {
-        v[i] = from_f32<BF16>(to_f32<BF16>(v[i]) + to_f32<BF16>(r[i]));
-        if (a.h && c < a.hidden) (static_cast<uint16_t*>(a.h) + row * a.h_stride)[c] = v[i];
-      }
+      if (a.residual) v[i] = from_f32<BF16>(to_f32<BF16>(v[i]) + to_f32<BF16>(r[i]));
+      if (a.h && c < a.hidden) (static_cast<uint16_t*>(a.h) + row * a.h_stride)[c] = v[i];
       const float f = to_f32<BF16>(v[i]);
       sum += f * f;
     }
@@ -262,20 +260,18 @@ template <bool BF16> __global__ void __launch_bounds__(kNormThreads) norm_any_ke
     const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.x_stride;
     const uint16_t* res = static_cast<const uint16_t*>(a.residual) + row * a.residual_stride;
     uint16_t* h = static_cast<uint16_t*>(a.h) + row * a.h_stride;
-    const auto value = [&](int c) {
-      const float f = to_f32<BF16>(x[c]);
-      return a.residual ? to_f32<BF16>(from_f32<BF16>(f + to_f32<BF16>(res[c]))) : f;
-    };
+    const auto value = [&](int c) { return a.residual ? from_f32<BF16>(to_f32<BF16>(x[c]) + to_f32<BF16>(res[c])) : x[c]; };
     float sum[1] = {0.0f};
     for (int c = threadIdx.x; c < a.hidden; c += kNormThreads) {
-      const float f = value(c);
+      const float f = to_f32<BF16>(value(c));
       sum[0] += f * f;
     }
     row_sums<kNormThreads / 32>(sum, s_sum[turn], 0, threadIdx.x >> 5);
     const float rstd = rsqrtf(sum[0] / a.hidden + a.eps);
     for (int c = threadIdx.x; c < a.hidden; c += kNormThreads) {  // (8 bits: hidden is in whole blocks, a warp has one)
-      const float f = value(c), v = f * rstd * gain<BF16>(a.weight, a.weight_fp32, a.offset, c);
-      if (a.residual && a.h) h[c] = from_f32<BF16>(f);
+      const uint16_t hc = value(c);
+      const float v = to_f32<BF16>(hc) * rstd * gain<BF16>(a.weight, a.weight_fp32, a.offset, c);
+      if (a.h) h[c] = hc;
       if (a.y) (static_cast<uint16_t*>(a.y) + row * a.y_stride)[c] = from_f32<BF16>(v);
       if (a.codes) {
         uint32_t byte;
@@ -692,7 +688,7 @@ int senmoe_rms_norm(const SenMoeNorm* n, senmoe_stream_t stream) {
   if (n->codes && n->hidden % kBlock8)
     return reject(SENMOE_ERR_UNSUPPORTED, "%s: hidden=%lld in 8 bits (a multiple of %d)", call, (long long)n->hidden, kBlock8);
   if (n->rows == 0) return SENMOE_OK;
-  if (!n->y && !n->codes && !(n->residual && n->h)) return reject(SENMOE_ERR_BAD_ARG, "%s: no output", call);
+  if (!n->y && !n->codes && !n->h) return reject(SENMOE_ERR_BAD_ARG, "%s: no output", call);
   if (!n->weight) return reject(SENMOE_ERR_BAD_ARG, "%s: weight is NULL", call);
   if ((rc = check_rows(call, "x", n->x, n->x_stride, n->hidden, n->rows, 2))) return rc;
   if (n->residual && (rc = check_rows(call, "residual", n->residual, n->residual_stride, n->hidden, n->rows, 2))) return rc;
@@ -708,7 +704,7 @@ int senmoe_rms_norm(const SenMoeNorm* n, senmoe_stream_t stream) {
   a.residual = n->residual;
   a.residual_stride = n->residual_stride;
   a.weight = n->weight;
-  a.h = n->residual ? n->h : nullptr;
+  a.h = n->h;
   a.h_stride = n->h_stride;
   a.y = n->y;
   a.y_stride = n->y_stride;
