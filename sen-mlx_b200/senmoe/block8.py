@@ -19,6 +19,12 @@ from . import (Rows8, _dispatch, grouped_linear8, grouped_linear8_input_grad, gr
 from .block16 import Moe16Weights
 
 
+class Saved(tuple):
+    """What ``backward`` needs of a ``forward``; ``slots`` [T, K]: the rows, in
+    expert order, of each token's experts."""
+    slots: torch.Tensor
+
+
 class Moe8:
     """x [T, H] bf16; norm [H] bf16 or fp32.  ``train`` also keeps the weights'
     transposes in 8 bits, for ``backward``; after a change of the 16-bit weights
@@ -60,14 +66,19 @@ class Moe8:
                             save_preact=train)
         a, z = a if train else (a, None)
         d = grouped_linear8(a, w8["down"], offsets)
-        rows = d[inverse.long()].view(x.shape[0], K, x.shape[1])
+        slots = inverse.long().view(x.shape[0], K)
+        rows = d[slots]
         out = (n.h.float() + (rows.float() * prob[..., None]).sum(1)).to(x.dtype)
         b = zb = None
         if w.shared_gate_up is not None:
             b = linear8(n.y8, w8["shared_gate_up"], activation="swiglu", eight_bit=True, save_preact=train)
             b, zb = b if train else (b, None)
             out = linear8(b, w8["shared_down"], residual=out)
-        return (out, (n, token, offsets, prob.flatten()[perm.long()], a, z, b, zb)) if train else out
+        if not train:
+            return out
+        saved = Saved((n, token, offsets, prob.flatten()[perm.long()], a, z, b, zb))
+        saved.slots = slots
+        return out, saved
 
     def backward(self, dout: torch.Tensor, saved):
         """(dx, gradients by name) from dout [T, H]; dx is the residual's as well;
@@ -90,6 +101,7 @@ class Moe8:
         dxs = grouped_linear8_input_grad(da, w8["gate_up_t"], offsets, preact=z, activation="swiglu")
         _, grads["gate_up"], _ = grouped_linear_backward(da, n.y[token], w.gate_up, offsets, preact=z,
                                                          activation="swiglu", need_dx=False)
-        dy = dy.index_add(0, token, dxs.float()).to(dout.dtype)
+        # a token's K rows in one order: the same bits every time, as atomic additions would not give
+        dy = (dy + dxs[saved.slots].sum(1, dtype=torch.float32)).to(dout.dtype)
         dx, grads["norm"] = rms_norm_backward(dy, n.h, self.norm, self.eps, dh=dout)
         return dx, grads

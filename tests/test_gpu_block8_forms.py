@@ -1,0 +1,44 @@
+"""The layer half over 8-bit rows (senmoe.block8): that a step's gradients are
+the same bits every time, and what it refuses."""
+import pytest
+from test_gpu_block8 import _block
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def senmoe():
+    import build as b
+    b.build()
+    import senmoe as s
+    return s
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+    t.cuda.set_device(0)
+    return t
+
+
+def test_gradients_repeat(senmoe, torch):
+    """Rows of eight experts meet in a token's gradient, in one order: equal bits, and no step of it that adds by
+    atomics, whose order shows in few of the rounded results."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        names = set()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.add(func.overloadpacket.__name__)
+            return func(*args, **(kwargs or {}))
+    block, x, r = _block(senmoe, torch, 1031, 512, 96, 32, 8, 64)
+    out, saved = block.forward(x, residual=r, train=True)
+    with Seen() as seen:
+        dx, grads = block.backward(out, saved)
+    assert "sum" in seen.names  # (it does see them)
+    assert not {n for n in seen.names if "index_add" in n or "scatter_add" in n or "index_put" in n or "bincount" in n}
+    for _ in range(20):
+        again, g = block.backward(out, saved)
+        assert torch.equal(again, dx)
+        assert all(torch.equal(g[k], v) for k, v in grads.items())
