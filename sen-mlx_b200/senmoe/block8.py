@@ -17,6 +17,7 @@ import torch
 from . import (Rows8, _dispatch, grouped_linear8, grouped_linear8_input_grad, grouped_linear_backward, linear8,
                linear8_input_grad, linear_backward, quantize8, rms_norm, rms_norm_backward, router)
 from .block16 import Moe16Weights
+from .products import _bad
 
 
 class Saved(tuple):
@@ -58,6 +59,11 @@ class Moe8:
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, train: bool = False):
         """out, or with ``train`` (out, what ``backward`` needs)."""
         w, w8, K = self.w, self.w8, self.top_k
+        for name, t in (("x", x), ("the router's weight", w.router)):  # (the router reads bf16 whatever it is given)
+            if t.dtype is not torch.bfloat16:
+                raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+            if t.dim() != 2 or t.shape[1] != w.router.shape[1]:
+                raise _bad(f"{name} {tuple(t.shape)}: x is [tokens, hidden], the router's weight [experts, hidden]")
         n = rms_norm(x, self.norm, self.eps, residual=residual, eight_bit=True)
         ids, prob = router(n.y, w.router, K, self.norm_topk)
         perm, inverse, offsets, _ = _dispatch(ids, w.router.shape[0])  # (the router's ids are in range)

@@ -42,3 +42,18 @@ def test_gradients_repeat(senmoe, torch):
         again, g = block.backward(out, saved)
         assert torch.equal(again, dx)
         assert all(torch.equal(g[k], v) for k, v in grads.items())
+
+
+def test_block_refuses(senmoe, torch):
+    """Rows and router weights of another type, which the router would read as bf16, and of other dimensions."""
+    block, x, r = _block(senmoe, torch, 6, 256, 96, 8, 2, 0)
+    for dtype in (torch.float16, torch.float32):
+        with pytest.raises(TypeError):
+            block.forward(x.to(dtype), residual=r.to(dtype))
+    for bad in (x.view(2, 3, 256), x[0], x[:, :128]):
+        with pytest.raises(senmoe.SenMoeError):
+            block.forward(bad)
+    block.w.router = block.w.router.half()
+    with pytest.raises(TypeError):
+        block.forward(x, residual=r)
+    torch.cuda.synchronize()
