@@ -857,10 +857,18 @@ Plan8 make_plan8(const Linear8Args& l, bool gated, int sms, bool pair, int bn, i
   if (l.offsets) {
     if (mean < 1) {  // groups with rows, about
       chunks = static_cast<double>(l.rows);
-    } else {  // counts spread about the mean as random routing's do: a chunk more for each multiple of bn below a count
+    } else {
+      // Counts spread about the mean as random routing's do: a chunk more for each
+      // multiple of bn below a count.  Multiples 8 sd below the mean are below every
+      // count; where the spread is wider than bn, the mean of that many is as below to
+      // 2^-28 (both keep the host's time the same for any rows).
       const double sd = std::sqrt(mean);
-      double each = 1.0;
-      for (double at = bn; at < mean + 4 * sd; at += bn) each += 0.5 * std::erfc((at - mean) / (1.4142136 * sd));
+      double each = mean / bn + 0.5;
+      if (sd < bn) {
+        const double sure = mean > 8 * sd + bn ? std::floor((mean - 8 * sd) / bn) : 0.0;
+        each = 1.0 + sure;
+        for (double at = (sure + 1) * bn; at < mean + 4 * sd; at += bn) each += 0.5 * std::erfc((at - mean) / (1.4142136 * sd));
+      }
       chunks = each * l.groups;
     }
     width = l.rows / chunks;

@@ -42,3 +42,25 @@ def test_k_blocks_are_dealt_out_once(ranges):
 def test_scale_units_are_those_of_the_blocks(ranges):
     for blocks, split, rank, k0, k1, u0, u1 in ranges:
         assert list(range(u0, u1)) == sorted({b // 2 for b in range(k0, k1)}), (blocks, split, rank)
+
+
+def test_planning_takes_no_longer_with_more_rows():
+    """The choice of tiles for a grouped product, on the host before every launch.  The K split is refused for so many
+    tiles, after the choice and before anything is launched."""
+    import ctypes as C
+    import time
+
+    import build
+    build.build()
+    import senmoe
+    P = 0x10000  # never read
+    q = senmoe.SenMoeLinear8(dtype=0, epilogue=0, num_groups=2, path=senmoe.LINEAR_TCGEN05_SPLIT, rows=(1 << 31) - 1024,
+                             in_features=64, out_features=16, x=P, x_stride=64, x_scales=P, x_scales_stride=2, weight=P,
+                             weight_stride=64, weight_group_stride=1024, weight_scales=P, weight_scales_stride=2,
+                             weight_scales_group_stride=32, offsets=P, y=P, y_stride=16)
+    took = []
+    for _ in range(3):
+        start = time.perf_counter()
+        assert senmoe.lib().senmoe_linear8(C.byref(q), None) == 5
+        took.append(time.perf_counter() - start)
+    assert min(took) < 0.01, took  # (a few microseconds; seconds where every chunk of 2^30 rows is counted)
