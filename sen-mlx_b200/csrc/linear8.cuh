@@ -55,7 +55,11 @@ __host__ __device__ inline KRange k_share(int blocks, int rank, int split) {
 __host__ __device__ inline KRange scale_units(int kb0, int kb1) {
   return {kb0 / 2, kb1 > kb0 ? (kb1 + 1) / 2 : kb0 / 2};
 }
-// Few rows (linear8_small.cu).
+// Few rows (linear8_small.cu), in chunks of 8, 16, 32 or 64 by the mean group.
+inline int linear8_small_chunk(const Linear8Args& a) {
+  const int64_t mean = a.rows / a.groups;
+  return mean <= 8 ? 8 : mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+}
 bool linear8_small_supported(const Linear8Args& a);
 cudaError_t launch_linear8_small(const Linear8Args& a, cudaStream_t st);
 // tcgen05 (linear8_tc.cu); form: a LinearForm, kFormAuto by estimated time.

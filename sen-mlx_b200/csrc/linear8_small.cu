@@ -276,12 +276,12 @@ template <bool BF16, bool GATED, bool EIGHT, int NT> cudaError_t launch_t(const 
   return launch_pdl(linear8_small_kernel<BF16, GATED, EIGHT, NT>, grid, dim3(S::kThreads), 0, st, a, words);
 }
 template <bool BF16, bool GATED, bool EIGHT> cudaError_t launch_n(const Linear8Args& a, bool words, cudaStream_t st) {
-  // rows of a chunk: those of the mean group that has any
-  const int64_t mean = a.rows / a.groups;
-  return mean <= 8    ? launch_t<BF16, GATED, EIGHT, 1>(a, words, st)
-         : mean <= 16 ? launch_t<BF16, GATED, EIGHT, 2>(a, words, st)
-         : mean <= 32 ? launch_t<BF16, GATED, EIGHT, 4>(a, words, st)
-                      : launch_t<BF16, GATED, EIGHT, 8>(a, words, st);
+  switch (linear8_small_chunk(a)) {
+    case 8: return launch_t<BF16, GATED, EIGHT, 1>(a, words, st);
+    case 16: return launch_t<BF16, GATED, EIGHT, 2>(a, words, st);
+    case 32: return launch_t<BF16, GATED, EIGHT, 4>(a, words, st);
+    default: return launch_t<BF16, GATED, EIGHT, 8>(a, words, st);
+  }
 }
 template <bool EIGHT> cudaError_t launch_e(const Linear8Args& a, bool words, cudaStream_t st) {
   if (act_gated(a.act)) return a.bf16 ? launch_n<true, true, EIGHT>(a, words, st) : launch_n<false, true, EIGHT>(a, words, st);
