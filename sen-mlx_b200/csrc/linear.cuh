@@ -98,9 +98,13 @@ template <bool BF16> __device__ __forceinline__ uint4 pack8(const float (&f)[8])
   return make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
 }
 
-// Activations in fp32, rounded once, to 16 bits.  The intrinsics' error (a few
-// units in the last place, __expf one more for every unit of its argument: below
-// 2^-15 of the value down to z = -12) is far below a 16-bit unit.  Where its
+// Activations in fp32, rounded once, to 16 bits or (FINE) to 8.  The intrinsics'
+// error (a few units in the last place, __expf one more for every unit of its
+// argument: below 2^-15 of the value down to z = -12) is far below a 16-bit unit.
+// In 8 bits it decides which side of a border a value next to one falls on: of
+// silu's and gelu's tanh form, and of their slopes, as many fall on the other side
+// as with exact exponentials and divisions (2, 3 and 9 against 3, 5 and 10 of 1.4,
+// 12.6 and 8.4 million slopes); gelu's Phi is fitted closer there.  Where its
 // exponential nears overflow (z < -87, gelu's tanh form z < -10), a value under
 // 1e-35 comes out as 0.
 // gelu's tanh form 0.5 z (1 + tanh(a)) equals z / (1 + exp(-2a)), which has
@@ -114,24 +118,34 @@ __device__ __forceinline__ float gelu_arg2(float z) {  // 2a, a = sqrt(2/pi) (z 
 // Stegun, 7.1.26), which bound the absolute error only.  P is fitted for the
 // least maximum of the *relative* error over |z| <= 15 (linear program over
 // 4000 points), 1.3e-6 in fp32, so that the lower tail is as exact as the rest.
-__device__ __forceinline__ float normal_cdf(float z, float e) {
+// FINE: two degrees more, 1e-8, in fp32 4e-7 and 7e-8 on average (gelu's slopes in
+// 8 bits: 240 of 8.4 million were on the other side of a border, now none; 8192 x
+// 2048 -> 8192 gelu to 8 bits 155.4 -> 158.0 us, the slopes' kernel the same).
+template <bool FINE> __device__ __forceinline__ float normal_cdf(float z, float e) {
+  if constexpr (FINE) {
+    const float t = __fdividef(1.0f, 1.0f + 0.35f * fabsf(z));
+    const float p = 0.139619693f + t * (0.139894828f + t * (0.119570084f + t * (0.106644519f + t * (-0.0260373186f + t * (0.163785264f +
+                    t * (-0.260060489f + t * (0.146217644f + t * -0.0296342336f)))))));
+    const float q = t * p * e;
+    return z < 0.0f ? q : 1.0f - q;
+  }
   const float t = __fdividef(1.0f, 1.0f + 0.365f * fabsf(z));
   const float p = 0.14567815f + t * (0.14424385f + t * (0.13795274f + t * (0.03523802f +
                   t * (0.16542687f + t * (-0.17671363f + t * 0.04817444f)))));
   const float q = t * p * e;
   return z < 0.0f ? q : 1.0f - q;
 }
-__device__ __forceinline__ float act_value(int act, float z) {
+template <bool FINE = false> __device__ __forceinline__ float act_value(int act, float z) {
   switch (act) {
     case kActRelu: return z > 0.0f ? z : (z != z ? z : 0.0f);
     case kActSilu: case kActSwiglu: return __fdividef(z, 1.0f + __expf(-z));
-    case kActGelu: return z * normal_cdf(z, __expf(-0.5f * z * z));
+    case kActGelu: return z * normal_cdf<FINE>(z, __expf(-0.5f * z * z));
     case kActGeluTanh: case kActGeglu: return __fdividef(z, 1.0f + __expf(-gelu_arg2(z)));
     default: return z;
   }
 }
 // act'(z), and act(z) in `value` (the two share their exponential).
-__device__ __forceinline__ float act_both(int act, float z, float& value) {
+template <bool FINE = false> __device__ __forceinline__ float act_both(int act, float z, float& value) {
   switch (act) {
     case kActRelu:
       value = z > 0.0f ? z : 0.0f;
@@ -142,7 +156,7 @@ __device__ __forceinline__ float act_both(int act, float z, float& value) {
       return s * (1.0f + z * (1.0f - s));
     }
     case kActGelu: {  // Phi(z) + z phi(z)
-      const float e = __expf(-0.5f * z * z), c = normal_cdf(z, e);
+      const float e = __expf(-0.5f * z * z), c = normal_cdf<FINE>(z, e);
       value = z * c;
       return c + z * 0.3989422804014327f * e;
     }

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(Shape<BF16, GATED, EIGHT, NT>::kThreads, Shape
 #pragma unroll
     for (int w = 0; w < kHalf; ++w) z += s_part[w][i0][r];
     if (pre) pre[row * a.preact_stride + f] = from_f32<BF16>(z);
-    float y = act_value(a.act, z);
+    float y = act_value<EIGHT>(a.act, z);
     if constexpr (GATED) {
       float u = b1;
 #pragma unroll

@@ -643,14 +643,14 @@ __global__ void __launch_bounds__(kThreads8, 1)
             }
           }
           asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory");
-          act_chunk(a.l.act, y);
+          act_chunk<EIGHT>(a.l.act, y);
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i] *= u[i];
           const int h = gate ? 0 : 16;
           fin.write(y, row + h, f0, t.w - c - h, feats);
         } else {
           fin.keep(z[0], row, f0, t.w - c, feats);
-          act_chunk(a.l.act, z[0]);
+          act_chunk<EIGHT>(a.l.act, z[0]);
           fin.write(z[0], row, f0, t.w - c, feats);
         }
       }
@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
           const int64_t row = t.c0 + c;
           fin.keep(z, row, f0, w, feats);
           if constexpr (GATED) fin.keep(u, row, fin.cols + f0, w, feats);
-          act_chunk(a.l.act, z);
+          act_chunk<EIGHT>(a.l.act, z);
           if constexpr (GATED) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) z[k] *= u[k];

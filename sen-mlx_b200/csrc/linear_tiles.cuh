@@ -132,16 +132,16 @@ __device__ __forceinline__ bool both_warps(int id, bool mine) {
 }
 
 // ---------------------------------------------------------------- epilogue
-template <int ACT> __device__ __forceinline__ void act_chunk(float (&z)[16]) {
+template <int ACT, bool FINE> __device__ __forceinline__ void act_chunk(float (&z)[16]) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) z[i] = act_value(ACT, z[i]);
+  for (int i = 0; i < 16; ++i) z[i] = act_value<FINE>(ACT, z[i]);
 }
-__device__ __forceinline__ void act_chunk(int act, float (&z)[16]) {
+template <bool FINE = false> __device__ __forceinline__ void act_chunk(int act, float (&z)[16]) {
   switch (act) {  // one uniform branch a chunk
-    case kActRelu: act_chunk<kActRelu>(z); break;
-    case kActSilu: case kActSwiglu: act_chunk<kActSilu>(z); break;
-    case kActGelu: act_chunk<kActGelu>(z); break;
-    case kActGeluTanh: case kActGeglu: act_chunk<kActGeluTanh>(z); break;
+    case kActRelu: act_chunk<kActRelu, FINE>(z); break;
+    case kActSilu: case kActSwiglu: act_chunk<kActSilu, FINE>(z); break;
+    case kActGelu: act_chunk<kActGelu, FINE>(z); break;
+    case kActGeluTanh: case kActGeglu: act_chunk<kActGeluTanh, FINE>(z); break;
     default: break;
   }
 }

@@ -39,7 +39,7 @@ template <bool BF16, int V, int ACT> struct Piece {
       for (int i = 0; i < V; ++i) {
         float value;
         const float d = g[i];
-        g[i] = d * act_both(ACT, zf[i], value);
+        g[i] = d * act_both<true>(ACT, zf[i], value);
         if constexpr (kGated) {
           g[i] *= up[i];
           up[i] = d * value;
