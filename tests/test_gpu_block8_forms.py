@@ -57,3 +57,11 @@ def test_block_refuses(senmoe, torch):
     with pytest.raises(TypeError):
         block.forward(x, residual=r)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("T,shared", [(1, 0), (37, 64), (300, 128)])
+def test_inference_gives_what_training_does(senmoe, torch, T, shared):
+    """The products choose their kernels by sizes alone, whether or not pre-activations are kept."""
+    block, x, r = _block(senmoe, torch, T, 512, 96, 16, 4, shared)
+    out, _ = block.forward(x, residual=r, train=True)
+    assert torch.equal(block.forward(x, residual=r), out)

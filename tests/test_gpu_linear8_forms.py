@@ -126,3 +126,108 @@ def test_gelu_falls_on_the_right_side_of_a_border(senmoe, torch, path):
     codes, scales = R.quantize(L.act("gelu", R.values(xr) @ R.values(wr).t() + b.double()))
     off = int((y.codes.double() != codes).sum())
     assert off <= max(1, codes.numel() * 2.0 ** -17) and torch.equal(y.scales.double(), scales), off
+
+
+def _grouped(senmoe, torch, *args, **kw):
+    try:
+        return senmoe.grouped_linear8(*args, **kw)
+    except senmoe.SenMoeError as e:
+        assert kw["path"] == senmoe.LINEAR_TCGEN05_SPLIT and e.status == 5, e
+        pytest.skip("too many tiles for a K split")
+
+
+# scale rows by TMA (K 512, 2048, 3584), in words of 8 (768) and 4 bytes (1408), and byte by byte (704)
+@pytest.mark.parametrize("activation,eight", [("none", False), ("swiglu", True), ("geglu", False)])
+@pytest.mark.parametrize("k", [512, 704, 768, 1408, 2048, 3584])
+@pytest.mark.parametrize("counts,first", [([5, 0, 33, 1, 3], 0), ([300, 0, 161, 225, 17], 3)])
+def test_grouped_scale_rows(senmoe, torch, path, counts, first, k, activation, eight):
+    """Grouped calls whose scales come in several units, by each way, over ragged and empty groups."""
+    import linear_ref as L
+    import rows8_ref as R
+    rows, out = first + sum(counts) + 5, 160
+    s = _make(senmoe, torch, rows, k, _wide(activation, out), experts=len(counts))
+    off = _offsets(torch, counts, first)
+    y, z = _grouped(senmoe, torch, s["x"], s["w"], off, bias=s["b"], activation=activation, save_preact=True, eight_bit=eight,
+                    path=path)
+    ref, d, zr, zd = R.product(R.values(s["x"]), R.values(s["w"]), off, s["b"], None, activation)
+    L.assert_within(z, zr, R.rounded(zr, zd, z.dtype), "preact")
+    if eight:
+        R.assert_rows8(y, ref, d, "y8")
+        y = y.codes.view(torch.uint8)
+    else:
+        L.assert_within(y, ref, R.rounded(ref, d, y.dtype), "y")
+    for part in (slice(0, first), slice(rows - 5, rows)):
+        assert not bool(y[part].any()) and not bool(z[part].any())
+    senmoe.linear_check()
+
+
+@pytest.mark.parametrize("activation,eight", [("none", False), ("swiglu", True)])
+@pytest.mark.parametrize("k", [96, 512])
+def test_more_tiles_than_a_cta_keeps(senmoe, torch, k, activation, eight):
+    """1024 experts with one to three rows: more than 64 tiles for each CTA, or pair of them."""
+    import linear_ref as L
+    import rows8_ref as R
+    out = 1408 if activation == "none" else 704
+    g = torch.Generator(device="cuda").manual_seed(5)
+    counts = torch.randint(1, 4, (1024,), generator=g, device="cuda").tolist()
+    s = _make(senmoe, torch, sum(counts), k, _wide(activation, out), experts=1024)
+    off = _offsets(torch, counts)
+    ref, d, _, _ = R.product(R.values(s["x"]), R.values(s["w"]), off, s["b"], None, activation)
+    for path in (senmoe.LINEAR_TCGEN05_ONE, senmoe.LINEAR_TCGEN05_PAIR, senmoe.LINEAR_AUTO):
+        y = senmoe.grouped_linear8(s["x"], s["w"], off, bias=s["b"], activation=activation, eight_bit=eight, path=path)
+        if eight:
+            R.assert_rows8(y, ref, d, "y8")
+        else:
+            L.assert_within(y, ref, R.rounded(ref, d, y.dtype), "y")
+    senmoe.linear_check()
+
+
+def test_weights_past_32_bits(senmoe, torch):
+    """Experts' weights and scales some 2^31 bytes apart."""
+    import rows8_ref as R
+    rows, k, out, far = 60, 512, 160, (1 << 31) + 16
+    s = _make(senmoe, torch, rows, k, out, experts=3)
+    off = _offsets(torch, [11, 40, 9])
+    raw = torch.empty(3 * far, dtype=torch.uint8, device="cuda")
+    codes, scales = raw.as_strided((3, out, k), (far, k, 1)), raw.as_strided((3, out, k // 32), (far, 16, 1), out * k)
+    codes.copy_(s["w"].codes.view(torch.uint8))
+    scales.copy_(s["w"].scales.view(torch.uint8))
+    w = senmoe.Rows8(codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu))
+    for path in (senmoe.LINEAR_SMALL, senmoe.LINEAR_TCGEN05_ONE, senmoe.LINEAR_TCGEN05_PAIR):
+        want = senmoe.grouped_linear8(s["x"], s["w"], off, path=path)
+        assert torch.equal(senmoe.grouped_linear8(s["x"], w, off, path=path), want)
+        assert bool(R.values(s["x"]).any()) and bool(want[-1].any())
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("values", [[0, 30, 10, 40], [-5, 10, 20, 400], [50, 60, 70, 80], [2 ** 31 - 1, 0, -2 ** 31, 7],
+                                    [3, 9, 9, 31]])
+def test_offsets_of_any_value_leave_the_buffers_around(senmoe, torch, values, eight):
+    """Through the C entry, with outputs inside larger buffers: whatever the offsets hold, nothing else is written."""
+    from senmoe import products8
+    rows, k, out, pad = 40, 64, 32, 7
+    wide = 2 * out
+    s = _make(senmoe, torch, rows, k, wide, experts=3)
+    off = torch.tensor(values, dtype=torch.int32, device="cuda")
+
+    def around(cols, dtype, step):
+        """[rows, cols] inside a wider and longer buffer of bytes 165, and what of it lies outside."""
+        buf = torch.zeros(rows + 2 * pad, cols + step, dtype=dtype, device="cuda")
+        buf.view(torch.uint8).fill_(165)
+        outside = torch.ones(buf.shape, dtype=torch.bool, device="cuda")
+        outside[pad:pad + rows, :cols] = False
+        return buf, buf[pad:pad + rows, :cols], outside
+    for path in (senmoe.LINEAR_SMALL, senmoe.LINEAR_TCGEN05_ONE, senmoe.LINEAR_TCGEN05_PAIR):
+        held = [around(wide, torch.bfloat16, 8)]  # preact
+        held += [around(out, torch.uint8, 16), around(1, torch.uint8, 3)] if eight else [around(out, torch.bfloat16, 8)]
+        z, y, *scales = (t for _, t, _ in held)
+        py = (0, 0, y.data_ptr(), y.stride(0), scales[0].data_ptr(), scales[0].stride(0)) if eight else \
+            (y.data_ptr(), y.stride(0), 0, 0, 0, 0)
+        w = s["w"]
+        products8._run_linear8(0, 5, 3, path, rows, k, out, s["x"].codes.data_ptr(), k, s["x"].scales.data_ptr(), 2,
+                               w.codes.data_ptr(), k, wide * k, w.scales.data_ptr(), 2, wide * 2, off.data_ptr(), 0, 0, 0,
+                               *py, z.data_ptr(), z.stride(0), device=0)
+        torch.cuda.synchronize()
+        for buf, _, outside in held:
+            assert bool((buf[outside].view(torch.uint8) == 165).all())
+    senmoe.linear_check()
