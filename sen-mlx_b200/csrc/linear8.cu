@@ -46,26 +46,28 @@ int check_type(const char* call, int32_t dtype, int32_t epilogue) {
 
 // Whether the few-row kernel is the faster one.  Measured against the tcgen05
 // tiles (us, W from HBM):
-//   dense 2048 x 2048    8 rows 5.4 / 9.6    16 rows 6.4 / 9.6    64 rows 15.1 / 10.0
-//   dense 2816 x 2112    8 rows 6.8 / 9.8    16 rows 8.4 / 9.9    32 rows 11.8 / 9.9
-//   dense 512 x 2048     8 rows 2.7 / 6.2    64 rows 5.6 / 6.5    96 rows 9.6 / 6.6
-//   dense 2048 x 8192    8 rows 12.0 / 11.6  8192 x 2048  1 row 14.8 / 12.6
-//   dense 1024 x 512     64 rows 8.8 / 7.3   4096 x 512   8 rows 8.3 / 9.7   16 rows 10.4 / 9.7
+//   dense 2048 x 2048    8 rows 4.7 / 8.9    16 rows 5.8 / 9.3    64 rows 13.9 / 9.5
+//   dense 2816 x 2112    8 rows 5.8 / 10.7   16 rows 7.4 / 10.7   32 rows 10.7 / 10.8
+//   dense 512 x 2048     8 rows 2.4 / 6.1    64 rows 5.9 / 6.3    96 rows 10.2 / 6.4
+//   dense 2048 x 8192    8 rows 10.9 / 10.0  8192 x 2048  1 row 12.6 / 12.6
+//   dense 1024 x 512     64 rows 8.1 / 7.2   4096 x 512   8 rows 7.0 / 9.7   16 rows 9.3 / 9.7
 // A block walks the whole of K for all rows, whatever the number of blocks.
 // It reads W in pieces of 32 bytes a row, which bounds it at 2 TB/s, and all
 // rows for every 16 features; and its blocks, short ones, should be resident
-// together.  Grouped, by what the touched experts hold, and blocks:
-//   8 x 768 x 2048    1024 blocks 14.6 / 9.9    8 x 2048 x 1536 (8 bits) 192 blocks 14.7 / 12.7
-//   4 x 2048 x 1536 (8 bits)  96 blocks 11.2 / 12.7    8 x 512 x 1024  512 blocks 6.9 / 8.2
-//   16 x 96 x 512     512 blocks 7.3 / 8.1      32 x 256 x 512   1024 blocks 11.6 / 8.4
+// together.  Grouped (touched experts x K x rows of W), by what the experts hold,
+// and blocks:
+//   8 x 768 x 2048    1024 blocks 12.9 / 9.4    8 x 2048 x 1536 (8 bits) 192 blocks 14.0 / 13.0
+//   4 x 2048 x 1536 (8 bits)  96 blocks 10.4 / 11.8    8 x 512 x 1024  512 blocks 6.4 / 8.3
+//   16 x 96 x 512     512 blocks 6.3 / 7.7      32 x 256 x 512   1024 blocks 10.6 / 8.4
 // and with more than 8 rows a group, where an SM has one block (two of 16 rows
 // with a 16-bit output) and K times a chunk's rows counts, twice with an 8-bit
 // output's larger blocks, four times with a gated pair's, half as many warps of
 // which share K:
-//   2 x 2048 x 1536  16 rows 8.4 / 11.2  21 rows (192 blocks) 15.6 / 11.3   2 x 4096 x 512  16 rows 10.4 / 11.6  32 rows 14.4 / 11.7
-//   2 x 2816 x 352 geglu  32 rows 10.6 / 12.5   4 x 768 x 2048  16 rows (512 blocks) 10.0 / 9.2
+//   2 x 2048 x 1536  16 rows 8.4 / 11.2  21 rows (192 blocks) 15.6 / 11.3
+//   2 x 4096 x 512   16 rows 10.4 / 11.6  32 rows 14.4 / 11.7
+//   2 x 2816 x 704 geglu  32 rows 10.6 / 12.5   4 x 768 x 2048  16 rows (512 blocks) 10.0 / 9.2
 //   8 bits: 2 x 1024 x 1536  32 rows 8.3 / 9.5  2 x 2048 x 1024  16 rows 8.8 / 11.2  32 rows 12.8 / 11.4
-//   8 bits, swiglu: 3 x 1024 x 512  16 rows 8.4 / 9.7  21 rows 11.3 / 9.8  2 x 2048 x 768  12 rows 13.6 / 11.9
+//   8 bits, swiglu: 3 x 1024 x 1024  16 rows 8.4 / 9.7  21 rows 11.3 / 9.8  2 x 2048 x 1536  12 rows 13.6 / 11.9
 bool few_rows8(const Linear8Args& a) {
   const int64_t weight = static_cast<int64_t>(a.n) * a.k;
   const int64_t chunks = !a.offsets ? (a.rows + 63) / 64 : a.rows < a.groups ? a.rows : a.groups;

@@ -32,9 +32,12 @@
 // memory, which takes an 8-bit tile's bytes in half of a 16-bit tile's MMA time.
 // 8192 x 2048 -> 8192 gelu 144 us = 1900 TFLOP/s (110 without the epilogue, 131
 // without the scales, 89 without either), 50 % tensor pipe.  4096 tokens of 128
-// experts, 2048 -> 2 x 768 swiglu to 8 bits with z kept, 140 to 158 us for 0.61 GB
-// and 206 GFLOP; every group of more than 224 rows is two chunks, each with its
-// trip of W from L2.
+// experts, 2048 -> 2 x 768 swiglu to 8 bits with z kept, 140 to 160 us for 0.61 GB
+// and 206 GFLOP; in pairs of 160 columns the groups, 256 rows on average, are two
+// chunks or three, each with its trip of W from L2.
+//
+// The sums round towards zero: z is off by 1.5e-7 of its root mean square at K
+// 2816 and smaller by 1.1e-7 on average, where fp32 products are off by 0.7e-7.
 
 #include <cuda.h>
 
