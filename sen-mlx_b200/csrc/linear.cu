@@ -272,11 +272,9 @@ int senmoe_linear_backward(const SenMoeLinearGrad* g, senmoe_stream_t stream) {
 
 int senmoe_linear_check(senmoe_stream_t stream) {
   clear_failure();
-  int error = 0, error8 = 0;
-  int rc = cuda_status("linear_check", linear_device_error(stream, &error));
-  if (rc) return rc;
-  if ((rc = cuda_status("linear_check", linear8_device_error(stream, &error8)))) return rc;
-  if (!error) error = error8;
+  int error = 0, *word8 = nullptr;
+  int rc = cuda_status("linear_check", linear8_error_word(&word8));
+  if (rc || (rc = cuda_status("linear_check", linear_device_error(stream, &error, word8)))) return rc;
   if (error == kDevWaitTimeout) return reject(SENMOE_ERR_TIMEOUT, "linear: a bounded wait on the device ran out");
   return error ? reject(SENMOE_ERR_DEVICE, "linear: device error %d", error) : SENMOE_OK;
 }

@@ -268,8 +268,8 @@ enum LinearForm : int { kFormAuto = 0, kFormOne = 1, kFormPair = 2, kFormSplit =
 cudaError_t launch_linear_tc(const LinearArgs& a, LinearProduct p, int form, const BiasJoin* bias, bool* summed,
                              cudaStream_t st);
 // Waits for `st`, returns and clears the device error that the tcgen05
-// kernels recorded on the current device (DeviceError).
-cudaError_t linear_device_error(cudaStream_t st, int* error);
+// kernels recorded on the current device (DeviceError), here or at `also`.
+cudaError_t linear_device_error(cudaStream_t st, int* error, int* also);
 // A kernel whose only wait runs out (about 2 s) and is recorded.
 cudaError_t selftest_linear_wait(cudaStream_t st);
 

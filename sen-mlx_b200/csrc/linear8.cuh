@@ -64,7 +64,7 @@ bool linear8_small_supported(const Linear8Args& a);
 cudaError_t launch_linear8_small(const Linear8Args& a, cudaStream_t st);
 // tcgen05 (linear8_tc.cu); form: a LinearForm, kFormAuto by estimated time.
 cudaError_t launch_linear8_tc(const Linear8Args& a, int form, cudaStream_t st);
-// As linear_device_error, for these kernels.
-cudaError_t linear8_device_error(cudaStream_t st, int* error);
+// Where these kernels record their device error, on the current device (for linear_device_error).
+cudaError_t linear8_error_word(int** word);
 
 }  // namespace senmoe

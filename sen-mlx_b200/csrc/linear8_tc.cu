@@ -42,7 +42,6 @@
 #include <cuda.h>
 
 #include <cmath>
-#include <mutex>
 
 #include "kernels.h"
 #include "linear8.cuh"
@@ -85,7 +84,6 @@ constexpr uint32_t ring_budget8(bool words, int groups) {
 }
 
 __device__ int g_linear8_error;  // first device error of these kernels on this device
-__device__ int g_linear8_taken;  // what the last check found there
 
 constexpr int kScaleMap = 0;     // see Tc8Args
 
@@ -776,8 +774,6 @@ __global__ void __launch_bounds__(kThreads8, 1)
   if constexpr (PAIR) cluster_sync();
 }
 
-__global__ void take_error8_kernel() { g_linear8_taken = atomicExch(&g_linear8_error, 0); }
-
 // ------------------------------------------------------------- host side
 constexpr uint32_t stage_bytes8(int part) { return kPieces * (kMPiece + part * kPiece); }
 constexpr int stages8(bool words, int part, int groups) {
@@ -980,14 +976,11 @@ cudaError_t launch_linear8_tc(const Linear8Args& l, int form, cudaStream_t st) {
                  : launch_form<false, false>(gated, l.bf16, m, a, grid, smem, st);
 }
 
-cudaError_t linear8_device_error(cudaStream_t st, int* error) {
-  static std::mutex once;  // g_linear8_taken is one word a device
-  const std::lock_guard<std::mutex> hold(once);
-  *error = 0;
-  cudaError_t e = cudaLaunchKernel(reinterpret_cast<const void*>(take_error8_kernel), dim3(1), dim3(1), nullptr, 0, st);
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(error, g_linear8_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
-  const cudaError_t done = cudaStreamSynchronize(st);
-  return e != cudaSuccess ? e : done;
+cudaError_t linear8_error_word(int** word) {
+  void* p = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&p, g_linear8_error);
+  *word = static_cast<int*>(p);
+  return e;
 }
 
 }  // namespace senmoe

@@ -710,7 +710,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 // Reads and clears in one step: an error that a kernel on another stream
 // records meanwhile is this check's or the next one's.
-__global__ void take_error_kernel() { g_linear_taken = atomicExch(&g_linear_error, 0); }
+__global__ void take_error_kernel(int* also) {
+  const int first = atomicExch(&g_linear_error, 0), other = atomicExch(also, 0);
+  g_linear_taken = first ? first : other;
+}
 
 // A wait that nothing ends, through its limit.
 __global__ void selftest_wait_kernel() {
@@ -938,11 +941,12 @@ cudaError_t selftest_linear_wait(cudaStream_t st) {
   return cudaLaunchKernel(reinterpret_cast<const void*>(selftest_wait_kernel), dim3(1), dim3(1), nullptr, 0, st);
 }
 
-cudaError_t linear_device_error(cudaStream_t st, int* error) {
+cudaError_t linear_device_error(cudaStream_t st, int* error, int* also) {
   static std::mutex once;  // g_linear_taken is one word a device
   const std::lock_guard<std::mutex> hold(once);
   *error = 0;
-  cudaError_t e = cudaLaunchKernel(reinterpret_cast<const void*>(take_error_kernel), dim3(1), dim3(1), nullptr, 0, st);
+  void* args[] = {&also};
+  cudaError_t e = cudaLaunchKernel(reinterpret_cast<const void*>(take_error_kernel), dim3(1), dim3(1), args, 0, st);
   if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(error, g_linear_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
   const cudaError_t done = cudaStreamSynchronize(st);
   return e != cudaSuccess ? e : done;
