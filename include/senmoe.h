@@ -480,7 +480,7 @@ typedef struct SenMoeNorm {
   const void* residual;  /* [rows, hidden], or NULL */
   int64_t residual_stride;
   const void* weight;    /* [hidden] */
-  void* h;               /* x + residual (without one x), or NULL */
+  void* h;               /* x + residual (without one x, beside another output), or NULL */
   int64_t h_stride;
   void* y;               /* or NULL */
   int64_t y_stride;

@@ -688,7 +688,7 @@ int senmoe_rms_norm(const SenMoeNorm* n, senmoe_stream_t stream) {
   if (n->codes && n->hidden % kBlock8)
     return reject(SENMOE_ERR_UNSUPPORTED, "%s: hidden=%lld in 8 bits (a multiple of %d)", call, (long long)n->hidden, kBlock8);
   if (n->rows == 0) return SENMOE_OK;
-  if (!n->y && !n->codes && !n->h) return reject(SENMOE_ERR_BAD_ARG, "%s: no output", call);
+  if (!n->y && !n->codes && !(n->residual && n->h)) return reject(SENMOE_ERR_BAD_ARG, "%s: no output", call);
   if (!n->weight) return reject(SENMOE_ERR_BAD_ARG, "%s: weight is NULL", call);
   if ((rc = check_rows(call, "x", n->x, n->x_stride, n->hidden, n->rows, 2))) return rc;
   if (n->residual && (rc = check_rows(call, "residual", n->residual, n->residual_stride, n->hidden, n->rows, 2))) return rc;

@@ -49,18 +49,19 @@ def test_backward_of_strided_rows_keeps_their_shape(senmoe, torch, n):
 
 @pytest.mark.parametrize("rows,n,stride", [(9, 2048, 2048), (9, 2048, 2051), (40, 333, 333), (40, 96, 101), (2, 17000, 17000)])
 def test_h_without_a_residual_is_x(senmoe, torch, rows, n, stride):
-    """The C entry's h is what was normed: x itself where there is no residual, also as the call's only output."""
+    """The C entry's h is what was normed: beside another output x itself where there is no residual."""
     from senmoe import norm
     s = _make(torch, rows, n, "float16")
     want = senmoe.rms_norm(s["x"], s["w"], EPS)
-    for y in (torch.zeros_like(s["x"]), None):
-        h = torch.zeros(rows, stride, dtype=torch.float16, device="cuda")
-        assert senmoe.lib().senmoe_rms_norm(
-            norm._pack_norm(1, 0, 0, EPS, rows, n, s["x"].data_ptr(), n, 0, 0, s["w"].data_ptr(), h.data_ptr(), stride,
-                            0 if y is None else y.data_ptr(), n, 0, 0, 0, 0), torch.cuda.current_stream().cuda_stream) == 0
-        assert torch.equal(h[:, :n], s["x"]) and not bool(h[:, n:].any())
-        if y is not None and stride == n:  # (else the rows are on another grid: another kernel's sums)
-            assert torch.equal(y, want.y)
+    h, y = torch.zeros(rows, stride, dtype=torch.float16, device="cuda"), torch.zeros_like(s["x"])
+    call = lambda py: senmoe.lib().senmoe_rms_norm(  # noqa: E731
+        norm._pack_norm(1, 0, 0, EPS, rows, n, s["x"].data_ptr(), n, 0, 0, s["w"].data_ptr(), h.data_ptr(), stride, py, n,
+                        0, 0, 0, 0), torch.cuda.current_stream().cuda_stream)
+    assert call(0) == 1 and not bool(h.any())  # (a copy alone is refused)
+    assert call(y.data_ptr()) == 0
+    assert torch.equal(h[:, :n], s["x"]) and not bool(h[:, n:].any())
+    if stride == n:  # (else the rows are on another grid: another kernel's sums)
+        assert torch.equal(y, want.y)
 
 
 # rows past which a warp's next row is on its way, with ragged last rounds: 1 to 16 warps a row, 1 to 4 pieces a lane
